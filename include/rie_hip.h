@@ -207,6 +207,91 @@ int32_t rie_hip_k_argmax(const float *x, int32_t n, uint32_t *out_idx);
  * overlap on one GPU (several streams or host threads) share that array and race. */
 int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, void *stream, char *err, size_t err_len);
 
+/* ---- batched serving: a cache of pages, attention over it and over packed prompts,
+ * token log probabilities.  No counterpart in the reference, whose backends hold one
+ * sequence each.  Everything but the structs themselves is device memory; nothing of it
+ * is read by the host, so a call can be captured into a graph and replayed over new
+ * contents.
+ *
+ * Types are ggml ids: 0 f32, 1 f16, 30 bf16.  Strides count elements.  Pointers and
+ * strides of q, k, v, the pages and the outputs have to keep every row (of head_dim
+ * consecutive values) 16-byte aligned.  head_dim: 32, 64, 96, 128 or 256.
+ *
+ * stream: a hipStream_t of any device (NULL: the current device's null stream); the call
+ * queues its kernels there and returns.  Pointers of host memory, or of another device
+ * than the stream's, are refused.
+ * No call allocates: ws is the caller's, of at least the bytes that the matching _ws
+ * function names; two calls that may run at the same time (on two streams, or in two
+ * graphs) need a workspace each. */
+
+/* The sequences of a batch.  Rows starts[i]..starts[i+1] (ascending, starts[n_seq] ≤
+ * n_rows) of the tensors hold sequence i's new tokens, which are the last of its lens[i]
+ * positions; rows behind starts[n_seq] are neither read nor written.  A sequence may
+ * bring no token; a token before position 0 (more new tokens than positions) is not
+ * written to the cache and attends to nothing.  max_new and max_len bound the new tokens
+ * and the positions of any one sequence: they choose kernels and splits, and of a
+ * sequence that exceeds max_new only some rows may be computed. */
+typedef struct rie_hip_seqs {
+    int32_t n_seq, n_rows, max_new, max_len;
+    const int32_t *starts; /* [n_seq + 1] */
+    const int32_t *lens;   /* [n_seq] (packed attention ignores it) */
+} rie_hip_seqs;
+
+/* A layer's keys and values in pages: position p of sequence i lies in page
+ * table[i*table_stride + p/page_size], slot p%page_size, and head h's values start at
+ * page*page_stride + slot*slot_stride + h*head_stride of k and of v.  page_size: a power
+ * of two, 16 to 4096.  Positions at and past table_cols*page_size do not exist, and
+ * those of a page id outside 0..n_pages-1 are neither written nor seen. */
+typedef struct rie_hip_pages {
+    int32_t ty, head_dim, n_kv, n_pages, page_size, table_cols;
+    void *k, *v;
+    int64_t page_stride, slot_stride, head_stride;
+    const int32_t *table;
+    int64_t table_stride;
+} rie_hip_pages;
+
+/* Queries and outputs of an attention call, of the keys' type: row r, head h at
+ * r*row_stride + h*head_stride.  Query head h reads KV head h / (n_head/n_kv).  scale:
+ * positive.  window > 0: a token sees its own position and the window-1 before it.
+ * softcap > 0: scores become softcap·tanh(score/softcap). */
+typedef struct rie_hip_attn {
+    int32_t n_head, window;
+    float scale, softcap;
+    const void *q;
+    int64_t q_row_stride, q_head_stride;
+    void *out;
+    int64_t out_row_stride, out_head_stride;
+} rie_hip_attn;
+
+/* Writes the new tokens' keys and values (src_ty: f32, rounded to nearest, or the pages'
+ * own type) to their pages. */
+int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *seqs, int32_t src_ty, const void *k, const void *v,
+                               int64_t row_stride, int64_t head_stride, void *stream, char *err, size_t err_len);
+/* Causal attention of every sequence's new tokens over its pages, which already hold them:
+ * chunks of prompts and single tokens in one batch.  A token that sees nothing gets zeros.
+ * An infinite or NaN key or value reaches only the tokens that see it. */
+size_t rie_hip_k_paged_attention_ws(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn);
+int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn, void *ws,
+                                  size_t ws_bytes, void *stream, char *err, size_t err_len);
+/* Causal attention within whole prompts packed one behind the other: keys and values are
+ * rows beside the queries' (n_kv heads; slices of a fused projection, say). */
+size_t rie_hip_k_packed_attention_ws(const rie_hip_seqs *seqs, int32_t ty, int32_t head_dim, int32_t n_kv, const rie_hip_attn *attn);
+int32_t rie_hip_k_packed_attention(const rie_hip_seqs *seqs, int32_t ty, int32_t head_dim, int32_t n_kv, const void *k, const void *v,
+                                   int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                                   const rie_hip_attn *attn, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len);
+
+/* Of n rows of n_vocab logits (row_stride elements apart, any alignment of their type):
+ * logprob[i] = ln p(targets[i]) (NaN for a target outside 0..n_vocab-1), the entropy of
+ * the distribution in nats, and the n_top (≤ 64) most likely tokens in order, the lowest
+ * index first among equals, with their log probabilities ([n][n_top]).  logprob with
+ * targets, entropy, and top_ids with top_logprobs may be NULL.  −inf logits have
+ * probability 0.  A row with a NaN or +inf logit, or nothing above −inf, has NaN for all
+ * of its numbers (its top_ids rank NaN as −inf).  n_vocab ≤ 2^21. */
+size_t rie_hip_k_token_logprobs_ws(int32_t n, int32_t n_vocab);
+int32_t rie_hip_k_token_logprobs(int32_t ty, const void *logits, int32_t n, int32_t n_vocab, int64_t row_stride,
+                                 const int32_t *targets, float *logprob, float *entropy, int32_t n_top, int32_t *top_ids,
+                                 float *top_logprobs, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

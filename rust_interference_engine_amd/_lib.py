@@ -29,6 +29,25 @@ class Config(C.Structure):
                 ("use_graph", C.c_int32)]
 
 
+class Seqs(C.Structure):
+    """rie_hip_seqs"""
+    _fields_ = [(n, C.c_int32) for n in ("n_seq", "n_rows", "max_new", "max_len")] + [("starts", C.c_void_p), ("lens", C.c_void_p)]
+
+
+class Pages(C.Structure):
+    """rie_hip_pages"""
+    _fields_ = [(n, C.c_int32) for n in ("ty", "head_dim", "n_kv", "n_pages", "page_size", "table_cols")] + [
+        ("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in ("page_stride", "slot_stride", "head_stride")] + [
+        ("table", C.c_void_p), ("table_stride", C.c_int64)]
+
+
+class Attn(C.Structure):
+    """rie_hip_attn"""
+    _fields_ = [("n_head", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float),
+                ("q", C.c_void_p), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64)]
+
+
 def build(jobs: int = 8) -> None:
     """Compile librie_hip.so for gfx950 (hipcc cross-compiles without a GPU)."""
     subprocess.run(["make", "-s", f"-j{jobs}", "-C", os.path.join(PKG, "csrc")], check=True)
@@ -46,6 +65,7 @@ def lib():
     L = C.CDLL(LIB_PATH)
     P, S, I, F, D = C.c_void_p, C.c_size_t, C.c_int32, C.c_float, C.c_double
     CP, U8P = C.c_char_p, C.POINTER(C.POINTER(C.c_uint8))
+    I64, PG, SQ, AT = C.c_int64, C.POINTER(Pages), C.POINTER(Seqs), C.POINTER(Attn)
     sig = {
         "rie_hip_default_config": (Config, []),
         "rie_hip_create": (P, [P, S, C.POINTER(Config), C.POINTER(I), CP, S]),
@@ -76,6 +96,13 @@ def lib():
         "rie_hip_k_moe_route": (I, [P, I, I, I, I, I, P, P]),
         "rie_hip_k_argmax": (I, [P, I, P]),
         "rie_hip_k_argmax_noalloc": (I, [P, I, P, P, CP, S]),
+        "rie_hip_k_paged_append": (I, [PG, SQ, I, P, P, I64, I64, P, CP, S]),
+        "rie_hip_k_paged_attention_ws": (S, [PG, SQ, AT]),
+        "rie_hip_k_paged_attention": (I, [PG, SQ, AT, P, S, P, CP, S]),
+        "rie_hip_k_packed_attention_ws": (S, [SQ, I, I, I, AT]),
+        "rie_hip_k_packed_attention": (I, [SQ, I, I, I, P, P, I64, I64, I64, I64, AT, P, S, P, CP, S]),
+        "rie_hip_k_token_logprobs_ws": (S, [I, I]),
+        "rie_hip_k_token_logprobs": (I, [I, P, I, I, I64, P, P, P, I, P, P, P, S, P, CP, S]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -5,6 +5,7 @@
 
 #include "../kernels.hpp"
 #include "backend.hpp"
+#include "guard.hpp"
 #include "synth.hpp"
 
 #include <algorithm>
@@ -14,35 +15,13 @@
 #include <vector>
 
 using rie::Error;
+using rie::guarded;
 using rie::HipBackend;
+using rie::write_err;
 
 struct rie_hip_backend {
     HipBackend *b;
 };
-
-static void write_err(char *err, size_t len, const std::string &m) {
-    if (!err || !len) return;
-    size_t n = std::min(len - 1, m.size());
-    std::memcpy(err, m.data(), n);
-    err[n] = 0;
-}
-
-template <class F>
-static int32_t guarded(char *err, size_t err_len, F &&f) {
-    try {
-        f();
-        return RIE_HIP_OK;
-    } catch (const Error &e) {
-        write_err(err, err_len, e.msg);
-        return e.code;
-    } catch (const std::exception &e) {
-        write_err(err, err_len, std::string("internal error: ") + e.what());
-        return RIE_HIP_ERR_RUNTIME;
-    } catch (...) {
-        write_err(err, err_len, "internal error");
-        return RIE_HIP_ERR_RUNTIME;
-    }
-}
 
 extern "C" {
 

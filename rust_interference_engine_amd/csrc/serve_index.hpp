@@ -1,0 +1,82 @@
+// serve_index.hpp — where the sequences of a serving batch lie: their rows, positions
+// and pages, the blocks of query rows that workgroups take, and the splits of long
+// caches.  The starts, lengths and page tables are device memory that the host never
+// reads, so everything taken from them is clamped here before it is used as an index;
+// the same functions compile for the host, where tests check them.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#ifdef __HIPCC__
+#define RIE_HD __host__ __device__ __forceinline__
+#else
+#define RIE_HD inline
+#endif
+
+namespace rie {
+
+RIE_HD int iclamp(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+RIE_HD int imin(int a, int b) { return a < b ? a : b; }
+RIE_HD int imax(int a, int b) { return a > b ? a : b; }
+
+// One sequence of a batch: rows [row0, row0 + n_new) hold its new tokens, the last of
+// its len positions.  Token t is at position len − n_new + t (negative: before the
+// sequence's first position, a token that sees nothing).
+struct SeqView {
+    int row0, n_new, len;
+};
+// starts[i], starts[i + 1] and lens[i] as the device memory has them; n_rows rows exist,
+// cap positions can be addressed
+RIE_HD SeqView seq_view(int start, int end, int len, int n_rows, int cap) {
+    SeqView s;
+    s.row0 = iclamp(start, 0, n_rows);
+    s.n_new = iclamp(end, s.row0, n_rows) - s.row0;
+    s.len = iclamp(len, 0, cap);
+    return s;
+}
+
+// First of the block ids that belong to the sequence starting at row `start`, number i
+// of the batch, where a block is M consecutive query rows (token · G + head of the
+// group).  Sequence i owns the ids up to the next one's first: at least ⌈n_new·G/M⌉, so
+// that no list of blocks has to be made before the launch.
+RIE_HD int block_base(int start, int i, int G, int M) { return (int)((int64_t)start * G / M) + i; }
+inline int64_t block_count(int n_rows, int n_seq, int G, int M) { return (int64_t)n_rows * G / M + n_seq; }
+
+// Positions [lo, hi) that at least one of tokens t0..t1 of s sees (window 0: all up to its own)
+struct KeyRange {
+    int lo, hi;
+};
+RIE_HD KeyRange key_range(const SeqView &s, int t0, int t1, int window) {
+    KeyRange r;
+    const int p0 = s.len - s.n_new + t0, p1 = s.len - s.n_new + t1;
+    r.hi = imax(p1 + 1, 0);
+    r.lo = window > 0 ? imax(imax(p0, 0) + 1 - window, 0) : 0;
+    if (r.lo > r.hi) r.lo = r.hi;
+    return r;
+}
+// tiles of KT positions that hold [lo, hi): the first one, and how many
+RIE_HD int first_tile(const KeyRange &r, int KT) { return r.lo / KT; }
+RIE_HD int tile_count(const KeyRange &r, int KT) { return r.hi > r.lo ? (r.hi + KT - 1) / KT - r.lo / KT : 0; }
+// splits of nt tiles when a split takes C of them and the last of S all that are left
+RIE_HD int split_count(int nt, int C, int S) { return imax(1, imin(S, (nt + C - 1) / C)); }
+
+// How a launch divides the positions of a block: every split takes C tiles, S at most.
+struct SplitPlan {
+    int C, S;
+};
+// wgs: workgroups without splits; tiles: those of the longest block; want: workgroups
+// that fill the card; least: tiles that a split is worth
+inline SplitPlan split_plan(int64_t wgs, int tiles, int want, int least, int most) {
+    SplitPlan p{tiles > 0 ? tiles : 1, 1};
+    if (wgs >= want || tiles < 2 * least) return p;
+    int64_t s = (want + wgs - 1) / wgs;
+    if (s > tiles / least) s = tiles / least;
+    if (s > most) s = most;
+    if (s < 2) return p;
+    p.C = (int)((tiles + s - 1) / s);
+    p.S = (tiles + p.C - 1) / p.C;
+    return p;
+}
+
+}  // namespace rie

@@ -1,0 +1,393 @@
+"""The batched serving operators on the GPU against plain float64 forms: appended rows, attention over pages and
+over packed prompts, token log probabilities; sizes, masks and layouts where they can go wrong."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import serving_ref as S  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+GPU = "cuda:0"
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "needs the MI355X"
+    from rust_interference_engine_amd import ops
+    return ops
+
+
+def paged(ops, b, window=0, softcap=0.0, scale=None, max_new=None, max_len=None, fill=7.0):
+    """outputs of the paged call on the CPU; rows outside the sequences keep `fill`"""
+    k, v = b.k_pages.to(GPU), b.v_pages.to(GPU)
+    kv = ops.PagedKv(b.paged(k), b.paged(v), b.table.to(GPU))
+    seqs = ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=max_new or b.max_new(), max_len=max_len or b.max_len())
+    out = torch.full((b.rows, b.H, b.hd), fill, dtype=b.dtype, device=GPU)
+    call = ops.PagedAttention(kv, seqs, b.q.to(GPU), out, scale=scale, window=window, softcap=softcap)
+    call()
+    first = out.cpu()
+    call()
+    assert torch.equal(out.cpu().nan_to_num(5.0), first.nan_to_num(5.0))  # the same bits again
+    return first
+
+
+def check(b, out, window=0, softcap=0.0, scale=None, fill=7.0):
+    scale = 1 / math.sqrt(b.hd) if scale is None else scale
+    for i, (n, L) in enumerate(b.lens):
+        r = int(b.starts[i])
+        q = b.q[r:r + n]
+        o, a, size = S.attend(q, b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, scale, window, softcap)
+        tol = S.tolerance(o, a, size, L, b.hd, b.dtype, softcap)
+        err = (out[r:r + n].double() - o).abs()
+        assert bool((err <= tol).all()), (i, n, L, float((err / tol).max()))
+    assert bool((out[int(b.starts[-1]):] == fill).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,KV,hd", [(4, 1, 32), (15, 5, 64), (14, 2, 64), (6, 6, 96), (8, 2, 128), (8, 1, 128), (4, 1, 256), (3, 1, 256)])
+def test_single_tokens(ops, H, KV, hd, dtype):
+    b = S.Batch([(1, 1), (1, 17), (1, 32), (1, 33), (1, 0), (1, 500), (0, 64), (1, 129)], H, KV, hd, dtype=dtype, extra_rows=2, extra_cols=1)
+    check(b, paged(ops, b))
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 128), (4, 1, 256), (8, 8, 64)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (40, 0.0), (0, 5.0), (1, 2.0)])
+def test_a_few_tokens_of_each_sequence(ops, H, KV, hd, page, window, softcap):
+    b = S.Batch([(3, 3), (2, 100), (4, 515), (1, 40), (3, 2), (4, 4)], H, KV, hd, page=page, dtype=BF16, seed=1)
+    check(b, paged(ops, b, window, softcap), window, softcap)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,KV,hd,page", [(4, 1, 32, 16), (15, 5, 64, 32), (6, 3, 96, 16), (8, 2, 128, 128), (8, 1, 128, 16), (4, 1, 256, 16), (7, 7, 128, 64)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (70, 0.0), (0, 3.0)])
+def test_chunks_and_single_tokens_in_one_batch(ops, H, KV, hd, page, dtype, window, softcap):
+    b = S.Batch([(1, 300), (37, 37), (65, 400), (0, 9), (1, 1), (130, 131), (5, 2)], H, KV, hd, page=page, dtype=dtype, seed=2, extra_rows=3)
+    check(b, paged(ops, b, window, softcap), window, softcap)
+
+
+@pytest.mark.parametrize("lens", [[(1, 5000)], [(2, 4097), (1, 3)], [(40, 6000)], [(1, 4096)] * 3])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_long_caches_in_splits(ops, lens, hd):
+    b = S.Batch(lens, 8, 2, hd, page=64, dtype=F16, seed=3)
+    check(b, paged(ops, b))
+    check(b, paged(ops, b, 1500), 1500)
+    check(b, paged(ops, b, max_len=6000))
+
+
+def test_rows_of_pages_in_either_order_and_a_scale(ops):
+    b = S.Batch([(9, 90), (1, 33)], 8, 4, 64, page=32, seed=4, order="slots")
+    check(b, paged(ops, b, scale=0.31), scale=0.31)
+
+
+def test_large_scores_and_a_moving_maximum(ops):
+    b = S.Batch([(1, 700), (60, 700)], 4, 2, 64, seed=5)
+    t = b.table[1, :44].long()
+    ramp = torch.linspace(0.1, 6.0, 44)[:, None, None, None]  # later keys are ever larger
+    b.k_pages[t] = (b.k_pages[t].float() * ramp).half()
+    check(b, paged(ops, b))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("H,KV,hd,new", [(8, 2, 128, 60), (8, 2, 64, 3), (4, 1, 256, 40), (4, 1, 256, 2)])
+def test_infinite_and_nan_rows_stay_with_the_tokens_that_see_them(ops, H, KV, hd, new, bad):
+    L = 200
+    b = S.Batch([(new, L), (1, 70)], H, KV, hd, dtype=BF16, seed=6)
+    clean = paged(ops, b)
+    at = L - 2  # the last two tokens see it
+    page, slot = int(b.table[0, at // 16]), at % 16
+    b.v_pages[page, 0, slot, 5] = bad
+    out = paged(ops, b)
+    G = H // KV
+    assert torch.equal(out[new:], clean[new:]) and torch.equal(out[:new - 2], clean[:new - 2])
+    hit = out[new - 2:new, :G]
+    assert bool((~torch.isfinite(hit[..., 5])).all())
+    keep = torch.ones(hd, dtype=torch.bool)
+    keep[5] = False
+    assert torch.equal(hit[..., keep], clean[new - 2:new, :G][..., keep]) and torch.equal(out[:, G:], clean[:, G:])
+    b.v_pages[page, 0, slot, 5] = 0
+    b.k_pages[page, 0, slot, 3] = float("nan")  # a key: every number of the tokens that see it
+    out = paged(ops, b)
+    assert torch.equal(out[:new - 2], clean[:new - 2]) and bool(out[new - 2:new, :G].isnan().all())
+
+
+def test_slots_behind_the_last_position_may_hold_anything(ops):
+    b = S.Batch([(1, 37), (20, 50), (2, 33)], 4, 2, 64, seed=7)
+    clean = paged(ops, b)
+    for i, (_, L) in enumerate(b.lens):
+        page = int(b.table[i, (L - 1) // 16])
+        b.k_pages[page, :, (L - 1) % 16 + 1:] = float("nan")
+        b.v_pages[page, :, (L - 1) % 16 + 1:] = float("inf")
+    assert torch.equal(paged(ops, b), clean)
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_positions_of_pages_that_are_none_are_not_seen(ops, new):
+    b = S.Batch([(new, 210), (1, 60)], 8, 2, 128, seed=8)
+    good = b.table.clone()
+    for bad in (-1, b.n_pages, 2 ** 31 - 1, -2 ** 31):
+        b.table[0, 3] = bad
+        out = paged(ops, b)
+        k = torch.cat([b.cached(b.k_pages, 0, 48), b.k_pages.transpose(1, 2)[good[0, 4:].long()].reshape(-1, 2, 128)])[:194]
+        v = torch.cat([b.cached(b.v_pages, 0, 48), b.v_pages.transpose(1, 2)[good[0, 4:].long()].reshape(-1, 2, 128)])[:194]
+        o, a, size = S.attend(b.q[:new], k, v, 194 - new, 1 / math.sqrt(128))
+        tol = S.tolerance(o, a, size, 210, 128, F16)
+        assert bool(((out[:new].double() - o).abs() <= tol).all())
+        b.table.copy_(good)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 32), (15, 5, 64), (4, 4, 96), (8, 2, 128), (8, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (50, 0.0), (0, 4.0)])
+def test_packed_prompts(ops, H, KV, hd, dtype, window, softcap):
+    lens = [1, 64, 0, 129, 33, 300, 2, 128]
+    g = torch.Generator().manual_seed(9)
+    n = sum(lens)
+    qkv = torch.randn(n + 2, H + 2 * KV, hd, generator=g).to(dtype)
+    dev = qkv.to(GPU)
+    starts = torch.tensor([0] + lens).cumsum(0).int()
+    out = torch.full((n + 2, H + 1, hd), 3.0, dtype=dtype, device=GPU)[:, :H]
+    call = ops.PackedAttention(ops.Seqs(starts.to(GPU), max_new=max(lens), max_len=max(lens)), dev[:, :H], dev[:, H:H + KV], dev[:, H + KV:],
+                               out, window=window, softcap=softcap)
+    call()
+    got = out.cpu()
+    for i, L in enumerate(lens):
+        r = int(starts[i])
+        if not L:
+            continue
+        o, a, size = S.attend(qkv[r:r + L, :H], qkv[r:r + L, H:H + KV], qkv[r:r + L, H + KV:], 0, 1 / math.sqrt(hd), window, softcap)
+        tol = S.tolerance(o, a, size, L, hd, dtype, softcap)
+        assert bool(((got[r:r + L].double() - o).abs() <= tol).all()), (i, L)
+    assert bool((got[n:] == 3).all())
+
+
+def test_one_long_prompt_in_splits(ops):
+    g = torch.Generator().manual_seed(10)
+    L, H, KV, hd = 1500, 4, 1, 128
+    q, k, v = (torch.randn(L, x, hd, generator=g).half() for x in (H, KV, KV))
+    out = torch.empty(L, H, hd, dtype=F16, device=GPU)
+    ops.PackedAttention(ops.Seqs(torch.tensor([0, L], dtype=torch.int32, device=GPU), max_new=L, max_len=L), q.to(GPU), k.to(GPU), v.to(GPU), out)()
+    o, a, size = S.attend(q, k, v, 0, 1 / math.sqrt(hd))
+    assert bool(((out.cpu().double() - o).abs() <= S.tolerance(o, a, size, L, hd, F16)).all())
+
+
+@pytest.mark.parametrize("n_seq", [1, 63, 64, 65, 200, 4100])
+def test_many_sequences(ops, n_seq):
+    lens = [(i % 3, max(1, i % 40)) for i in range(n_seq)]
+    b = S.Batch(lens, 2, 1, 32, seed=11, extra_rows=1)  # one sequence, no token: a batch of none is refused
+    out = paged(ops, b)
+    got = paged(ops, b, max_new=40)  # the tile kernel's way
+    for i in list(range(0, n_seq, max(1, n_seq // 50))) + [n_seq - 1]:
+        n, L = lens[i]
+        r = int(b.starts[i])
+        o, a, size = S.attend(b.q[r:r + n], b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, 1 / math.sqrt(32))
+        tol = S.tolerance(o, a, size, L, 32, F16)
+        assert bool(((out[r:r + n].double() - o).abs() <= tol).all()) and bool(((got[r:r + n].double() - o).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("src", [F32, F16, BF16])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("order", ["heads", "slots"])
+def test_append(ops, src, dtype, order):
+    if src not in (F32, dtype):
+        pytest.skip("refused: another 16-bit type")
+    lens = [(1, 1), (20, 20), (3, 200), (0, 17), (5, 3), (1, 64)]
+    b = S.Batch(lens, 4, 3, 64, dtype=dtype, order=order, extra_rows=2, seed=12)
+    g = torch.Generator().manual_seed(13)
+    new = torch.randn(b.rows, 6, 64, generator=g).to(src)
+    dev, k, v = new.to(GPU), b.k_pages.to(GPU), b.v_pages.to(GPU)
+    kv = ops.PagedKv(b.paged(k), b.paged(v), b.table.to(GPU))
+    ops.PagedAppend(kv, ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=20, max_len=200), dev[:, :3], dev[:, 3:])()
+    want_k, want_v = b.paged(b.k_pages).clone(), b.paged(b.v_pages).clone()
+    for i, (n, L) in enumerate(lens):
+        for t in range(n):
+            p = L - n + t
+            if p >= 0:
+                at = (int(b.table[i, p // 16]), p % 16)
+                want_k[at], want_v[at] = new[int(b.starts[i]) + t, :3].to(dtype), new[int(b.starts[i]) + t, 3:].to(dtype)
+    assert torch.equal(b.paged(k.cpu()), want_k) and torch.equal(b.paged(v.cpu()), want_v)
+
+
+def test_append_leaves_pages_that_are_none_alone(ops):
+    b = S.Batch([(40, 40)], 2, 1, 32, seed=14)
+    b.table[0, 1] = -5
+    k, v = b.k_pages.to(GPU), b.v_pages.to(GPU)
+    new = torch.randn(40, 1, 32, device=GPU)
+    ops.PagedAppend(ops.PagedKv(b.paged(k), b.paged(v), b.table.to(GPU)), ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=40, max_len=40), new, new)()
+    want = b.k_pages.clone()
+    want[int(b.table[0, 0]), 0] = new[:16, 0].half().cpu()
+    want[int(b.table[0, 2]), 0, :8] = new[32:, 0].half().cpu()
+    assert torch.equal(k.cpu(), want)
+
+
+# ln p of f32 logits, all within R of each other: x − m and the two subtractions round to 2^-24 of at most R each, ln S is
+# off by the sum's n·2^-24 at most (chains are far shorter), an exponential by 2^-22 + R·2^-23
+def logprob_tol(x, V):
+    fin = x[torch.isfinite(x)]
+    R = float(fin.max() - fin.min()) if fin.numel() else 0.0
+    return 3 * (R + math.log(V) + 1) * 2.0 ** -24 + (V / 64 + 40) * 2.0 ** -24 + 2.0 ** -21 + min(R, 40.0) * 2.0 ** -22
+
+
+def run_logprobs(ops, x, targets, top):
+    n, V = x.shape
+    lp, h = torch.full((n,), 9.0, device=GPU), torch.full((n,), 9.0, device=GPU)
+    ids = torch.full((n, top), -9, dtype=torch.int32, device=GPU) if top else None
+    tops = torch.full((n, top), 9.0, device=GPU) if top else None
+    ops.TokenLogprobs(x, targets=targets.to(GPU), logprob=lp, entropy=h, top_ids=ids, top_logprobs=tops)()
+    return lp.cpu().double(), h.cpu().double(), ids.cpu() if top else None, tops.cpu().double() if top else None
+
+
+def check_logprobs(ops, x, dev, targets, top):
+    lp, h, ids, tops = run_logprobs(ops, dev, targets, top)
+    wl, wh, wi, wt = S.logprobs(x, targets, top)
+    tol = logprob_tol(x.double(), x.shape[1])
+
+    def near(a, b, t):
+        fine = torch.isfinite(b)
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[~fine].nan_to_num(1.0, 2.0, 3.0), b[~fine].nan_to_num(1.0, 2.0, 3.0))
+        assert bool(((a - b).abs()[fine] <= t).all()), float((a - b).abs()[fine].max() / t)
+
+    near(lp, wl, tol)
+    near(h, wh, tol * (1 + 2 * math.log(x.shape[1])))  # ln S, and a mean of x − m over the same probabilities
+    if top:
+        assert torch.equal(ids.long(), wi)
+        near(tops, wt, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("V,n,top", [(1, 2, 1), (5, 3, 5), (511, 4, 3), (512, 3, 20), (513, 2, 64), (1100, 3, 64), (40007, 5, 20), (49152, 9, 1), (151936, 2, 5)])
+def test_logprobs(ops, V, n, top, dtype):
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(n, V, generator=g) * 3).to(dtype)
+    t = torch.randint(0, V, (n,), generator=g).int()
+    t[0] = V if n > 2 else t[0]  # no token
+    check_logprobs(ops, x, x.to(GPU), t, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("off", [1, 3, 7])
+def test_logprobs_of_rows_at_any_place(ops, dtype, off):
+    g = torch.Generator().manual_seed(off)
+    x = torch.randn(3, 3001, generator=g).to(dtype)
+    dev = torch.full((3, 3100), 50.0, dtype=dtype, device=GPU)  # its neighbours would win
+    dev[:, off:off + 3001] = x.to(GPU)
+    check_logprobs(ops, x, dev[:, off:off + 3001], torch.tensor([0, 3000, -1], dtype=torch.int32), 20)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_logprobs_of_odd_rows(ops, dtype):
+    inf, nan, low = math.inf, math.nan, torch.finfo(dtype).min
+    V = 5000
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(10, V, generator=g)
+    x[0] = 2.5                     # all equal: the lowest indices
+    x[1, :4990] = -inf             # nearly all masked
+    x[2] = -inf                    # nothing
+    x[3, 77] = nan
+    x[4, 4000] = inf
+    x[5, 100:] = low               # masks of the lowest value
+    x[6] = -inf
+    x[6, 3] = 0                    # one token
+    x[7] = 0
+    x[7, 10:3000] = 1              # more ties than are ranked at once
+    x[8] = nan
+    x[9] = low
+    x = x.to(dtype)
+    t = torch.tensor([0, 4995, 1, 2, 4000, 200, 3, 10, 0, 9], dtype=torch.int32)
+    lp, h, ids, tops = run_logprobs(ops, x.to(GPU), t, 20)
+    wl, wh, wi, wt = S.logprobs(x, t, 20)
+    wi = wi.long()
+    for r in range(10):
+        assert torch.equal(ids[r].long(), wi[r]), r
+        tol = 2.0 ** -18 * (1 + math.log(V)) ** 2
+        for a, b in ((lp[r:r + 1], wl[r:r + 1]), (h[r:r + 1], wh[r:r + 1]), (tops[r], wt[r])):
+            assert torch.equal(a.isnan(), b.isnan()), r
+            fine = torch.isfinite(b)
+            big = fine & (b.abs() > 1e4)  # a masked token's own: the difference of two logits, to a step
+            assert bool(((a - b).abs()[fine & ~big] <= tol).all()), r
+            assert bool(((a - b).abs()[big] <= b.abs()[big] * 2.0 ** -22).all()), r
+            assert torch.equal(a[~fine & ~b.isnan()], b[~fine & ~b.isnan()]), r
+
+
+def test_logprobs_of_a_nearly_certain_token(ops):
+    x = torch.zeros(1, 4000)
+    x[0, 1234] = 30.0
+    lp, h, _, _ = run_logprobs(ops, x.to(GPU), torch.tensor([1234], dtype=torch.int32), 0)
+    rest = 3999 * math.exp(-30)  # −ln p = ln(1 + rest), H = ln(1 + rest) + 30 rest / (1 + rest): 3.7e-10 and 1.2e-8 keep their digits
+    assert abs(float(lp[0]) / -math.log1p(rest) - 1) < 1e-5 and abs(float(h[0]) / (math.log1p(rest) + 30 * rest / (1 + rest)) - 1) < 1e-5
+
+
+def test_a_step_of_a_batch_captured_and_replayed(ops):
+    """append, attention over the pages, log probabilities of rows made from its outputs: as one graph over buffers
+    that change between the replays, on a stream of its own"""
+    b = S.Batch([(1, 90), (7, 60), (1, 1), (1, 2100)], 8, 2, 64, seed=15)
+    g = torch.Generator().manual_seed(16)
+    k, v = b.k_pages.to(GPU), b.v_pages.to(GPU)
+    kv = ops.PagedKv(b.paged(k), b.paged(v), b.table.to(GPU))
+    seqs = ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=7, max_len=2100)
+    new = torch.empty(b.rows, 4, 64, device=GPU)
+    q, out = torch.empty(b.rows, 8, 64, dtype=F16, device=GPU), torch.empty(b.rows, 8, 64, dtype=F16, device=GPU)
+    logits = out.view(b.rows, 512)
+    t = torch.arange(b.rows, dtype=torch.int32, device=GPU)
+    lp, h = torch.empty(b.rows, device=GPU), torch.empty(b.rows, device=GPU)
+    calls = [ops.PagedAppend(kv, seqs, new[:, :2], new[:, 2:]), ops.PagedAttention(kv, seqs, q, out), ops.TokenLogprobs(logits, targets=t, logprob=lp, entropy=h)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for c in calls:
+            c()
+    for rep in range(4):
+        new.copy_(torch.randn(b.rows, 4, 64, generator=g))
+        q.copy_(torch.randn(b.rows, 8, 64, generator=g))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.cpu().clone(), lp.cpu().clone(), h.cpu().clone(), k.cpu().clone()
+        for x in (out, lp, h):
+            x.zero_()
+        for c in calls:
+            c(stream=side if rep % 2 else None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y.cpu()) for x, y in zip(got, (out, lp, h, k)))
+        b.k_pages, b.v_pages, b.q = k.cpu(), v.cpu(), q.cpu()
+        r, n, L = int(b.starts[1]), 7, 60
+        assert torch.equal(b.cached(b.k_pages, 1)[L - n:], new[r:r + n, :2].half().cpu())
+        check(b, out.cpu())
+
+
+def test_two_calls_at_once_on_two_streams(ops):
+    a = S.Batch([(1, 3000), (1, 500)], 8, 2, 128, seed=17)
+    b = S.Batch([(2, 2500)], 8, 2, 128, seed=18)
+    alone = [paged(ops, x) for x in (a, b)]
+    made = []
+    for x in (a, b):
+        kv = ops.PagedKv(x.paged(x.k_pages.to(GPU)), x.paged(x.v_pages.to(GPU)), x.table.to(GPU))
+        out = torch.zeros(x.rows, 8, 128, dtype=F16, device=GPU)
+        made.append((ops.PagedAttention(kv, ops.Seqs(x.starts.to(GPU), x.L.to(GPU), max_new=x.max_new(), max_len=x.max_len()), x.q.to(GPU), out), out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for call, out, st in made:
+            call(stream=st)
+    torch.cuda.synchronize()
+    for (_, out, _), want in zip(made, alone):
+        assert torch.equal(out.cpu(), want)
+
+
+def test_refused_on_the_gpu(ops):
+    from rust_interference_engine_amd import RieError, _lib
+    import ctypes as C
+
+    x = torch.zeros(4, 100, device=GPU)
+    ent = torch.zeros(4)  # host memory
+    err = C.create_string_buffer(256)
+    ws = torch.empty(4096, dtype=torch.uint8, device=GPU)
+    f = _lib.lib().rie_hip_k_token_logprobs
+    assert f(0, x.data_ptr(), 4, 100, 100, None, None, ent.data_ptr(), 0, None, None, ws.data_ptr(), 4096, None, err, 256) == -5
+    assert b"entropy is not device memory" in err.value
+    assert f(0, ent.data_ptr(), 4, 1, 1, None, None, None, 0, None, None, ws.data_ptr(), 4096, None, err, 256) == -5
+    with pytest.raises(RieError, match="on one GPU"):
+        ops.TokenLogprobs(x, entropy=ent)
