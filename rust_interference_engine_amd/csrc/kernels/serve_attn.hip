@@ -150,8 +150,6 @@ constexpr int HDP = HD <= 64 ? 64 : HD <= 128 ? 128 : HD;  // values between row
 // 16-byte chunk c of row r goes to chunk c ^ swz(r), so that the lanes of a read, which
 // take the same chunk of many rows (keys) or 4 chunks of 4 rows (values), use all banks
 template <int HD>
-__device__ __forceinline__ int swz_k(int r) { return HDP<HD> >= 128 ? r & 15 : (r >> 1) & 7; }
-template <int HD>
 __device__ __forceinline__ int swz_v(int r) { return HDP<HD> >= 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
 
 // score → exponent in log2 units, where the softcap makes it one already
@@ -162,16 +160,56 @@ __device__ __forceinline__ float cap_score(float s, float in, float out) {
     return out * (1.0f - 2.0f / (e + 1.0f));
 }
 
+// 16 bytes per lane from global memory (base + off) to LDS: lane l's go to dst + 16·l, with base
+// and dst the same for the wave.  Written as the instruction, since the compiler waits for the
+// builtin's copies before it reads any LDS, also of the buffers that they do not write; it has
+// no result register, and the callers wait (wait_vmem) before the barrier behind which the
+// copy is read.  Nothing else here uses m0.  Loads return in order, so waits that count without these wait longer at most.
+__device__ __forceinline__ void copy_lds(const uint8_t *base, int off, const uint8_t *dst) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(from) : "memory");
+}
+
 constexpr int TILE_M = 128;  // query rows of a workgroup
+// A tile in LDS.  A wave copies 1 KB at a time, its lanes' 16-byte chunks side by side, which
+// is RPI whole rows in an order of their own choice: keys by chunk, then row, so that the 32
+// rows' chunks of a read lie in all banks and a row's chunks at fixed distances; values by 64
+// bytes of a row (32 dims), then row, for the same reasons of the transposed read.  Blocks are
+// PAD bytes further apart than 1 KB where the next block's rows would meet the same banks.
+// Rows shorter than their place (head sizes 32 and 96) leave the chunks behind them unused.
+template <int HD>
+struct TileLds {
+    static constexpr int CPR = HDP<HD> / 8, RPI = 64 / CPR;  // chunks per row, rows per block
+    static constexpr int K_BLOCK = 1024 + RPI * 16, V_BLOCK = 1024 + (RPI == 2 ? 128 : 0);
+    static __device__ __forceinline__ int key(int r, int chunk) { return r / RPI * K_BLOCK + chunk * (RPI * 16) + r % RPI * 16; }
+    static __device__ __forceinline__ int value(int r, int chunk) { return r / RPI * V_BLOCK + chunk / 4 * (RPI * 64) + r % RPI * 64 + chunk % 4 * 16; }
+    // row and chunk of a lane's place in a block
+    static __device__ __forceinline__ int key_row(int lane) { return lane % RPI; }
+    static __device__ __forceinline__ int key_chunk(int lane) { return lane / RPI; }
+    static __device__ __forceinline__ int value_row(int lane) { return lane / 4 % RPI; }
+    static __device__ __forceinline__ int value_chunk(int lane) { return lane / (4 * RPI) * 4 + lane % 4; }
+};
+
 template <int HD>
 constexpr int TILE_KT = HD <= 128 ? 64 : 32;  // positions of a tile
 
+// A tile's work is cut into groups of 32 positions (KB to a tile), and the three steps of a
+// group run in three places: while the vector units make the probabilities of group h, the
+// matrix units form the outputs of h − 1 and the scores of h + 1, so that neither waits for
+// the other within a wave.  K and V tiles go from global memory straight to LDS, two buffers
+// each, one barrier per tile: at tile t's barrier the loads of K(t + 1) and V(t + KB − 2) are
+// complete, K(t) and V(t + KB − 3) have been read, and K(t + 2) and V(t + KB − 1) are
+// requested into their places.
 template <int HD, bool BF, bool CAP>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(ServeAttnArgs a) {
-    constexpr int KT = TILE_KT<HD>, RW = KT / 4, NLD = RW * HD / 8 / 64, ROWB = HDP<HD> * 2, KS = HD / 16, DB = HD / 32, KB = KT / 32;
-    __shared__ __align__(16) uint8_t s_k[2][KT * ROWB];
-    __shared__ __align__(16) uint8_t s_v[2][KT * ROWB];
-    __shared__ __align__(16) int s_flag[2][4];
+    constexpr int KT = TILE_KT<HD>, KB = KT / 32, RW = KT / 4, KS = HD / 16, DB = HD / 32;
+    using Lds = TileLds<HD>;
+    constexpr int RPI = Lds::RPI, NLD = RW / RPI, KBYTES = KT / RPI * Lds::K_BLOCK, VBYTES = KT / RPI * Lds::V_BLOCK;
+    constexpr int NG = KT / 16;                                     // groups of 16 positions, which lie in one page
+    __shared__ __align__(16) uint8_t s_k0[KBYTES], s_k1[KBYTES], s_v0[VBYTES], s_v1[VBYTES];
+    __shared__ __align__(16) int s_nf[4];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int G = a.G, kvh = blockIdx.x % a.n_kv;
     const int blk = a.n_blocks - 1 - (int)(blockIdx.x / a.n_kv);  // a sequence's longest rows first
@@ -195,7 +233,6 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const int lo_q = a.window > 0 ? p_q - a.window : -1;  // sees j in (lo_q, p_q]
     const bool wave_live = r0 + w * 32 <= r1;
     const int w_t0 = imin(r0 + w * 32, r1) / G, w_t1 = imin(r0 + w * 32 + 31, r1) / G;
-    const KeyRange wr = key_range(sv, w_t0, w_t1, a.window);
     const int all_hi = pos0 + w_t0, all_lo = a.window > 0 ? pos0 + w_t1 - a.window : -1;  // every row of the wave sees (all_lo, all_hi]
     const int wg_hi = pos0 + r0 / G, wg_lo = a.window > 0 ? pos0 + r1 / G - a.window : -1;  // and of the workgroup
     u32x4 qf[KS];
@@ -205,57 +242,40 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         for (int i = 0; i < KS; i++) qf[i] = live ? *(const u32x4 *)(qp + i * 32) : u32x4{0, 0, 0, 0};
     }
 
-    // staging: wave w holds rows w·RW .. of the tile, which lie in one page
+    // ---- copies: wave w's are rows w·RW .. of a tile, which lie in one page ----
     const int *trow = a.kv.table ? a.kv.table + (int64_t)si * a.kv.table_stride : nullptr;
     const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
-    int st_r[NLD], st_ch[NLD];
-#pragma unroll
-    for (int i = 0; i < NLD; i++) {
-        st_r[i] = (i * 64 + lane) / (HD / 8);
-        st_ch[i] = (i * 64 + lane) % (HD / 8);
-    }
-    u32x4 rk[NLD], rv[NLD];
-    bool r_ok = true;  // the group's page exists
-    auto load = [&](int t) {
-        const int g0 = t * KT + w * RW;
-        const uint8_t *kp = kbase, *vp = vbase;
-        r_ok = true;
-        if (g0 < kr.hi) {
-            if (trow) {
-                int page;
-                r_ok = page_of(a.kv, trow, g0, page);
-                const int slot = g0 & ((1 << a.kv.page_shift) - 1);
-                kp += page * a.kv.page + slot * a.kv.k_row;
-                vp += page * a.kv.page + slot * a.kv.v_row;
-            } else {
-                kp += (int64_t)(sv.row0 + g0) * a.kv.k_row;
-                vp += (int64_t)(sv.row0 + g0) * a.kv.v_row;
-            }
-        }
-        const int n = r_ok ? kr.hi - g0 : 0;  // rows that some token sees: the others are not read
-#pragma unroll
-        for (int i = 0; i < NLD; i++) {
-            rk[i] = rv[i] = u32x4{0, 0, 0, 0};
-            if (st_r[i] < n) {
-                rk[i] = *(const u32x4 *)(kp + st_r[i] * (int)a.kv.k_row + st_ch[i] * 16);
-                rv[i] = *(const u32x4 *)(vp + st_r[i] * (int)a.kv.v_row + st_ch[i] * 16);
-            }
-        }
+    const int k_r = Lds::key_row(lane), k_c = imin(Lds::key_chunk(lane), HD / 8 - 1) * 16;
+    const int v_r = Lds::value_row(lane), v_c = imin(Lds::value_chunk(lane), HD / 8 - 1) * 16;
+    // page ids of the groups of a tile, a lane each: requested a tile ahead of their use
+    auto request_pages = [&](int t) { return trow && t < t_end ? trow[imin(t * KT + imin(lane, NG - 1) * 16, kr.hi - 1) >> a.kv.page_shift] : 0; };
+    struct Tile {
+        int page, bad;  // the wave's own page; bit g: the page of group g is none
     };
-    // bit 0: rows of a page that is none; bit 1: infinite or NaN values
-    auto stage = [&](int t, int buf) {
-        const bool part = (t + 1) * KT - 1 > wg_hi || t * KT <= wg_lo;  // some row does not see all of the tile
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < NLD; i++) {
-            const int r = w * RW + st_r[i];
-            *(u32x4 *)(s_k[buf] + r * ROWB + ((st_ch[i] ^ swz_k<HD>(r)) << 4)) = rk[i];
-            *(u32x4 *)(s_v[buf] + r * ROWB + ((st_ch[i] ^ swz_v<HD>(r)) << 4)) = rv[i];
-            if (part) bad = bad || nonfinite8<BF>(rv[i]);
+    auto tile_of = [&](int ids) {
+        Tile x{0, 0};
+        if (trow) {
+            const bool ok = (unsigned)ids < (unsigned)a.kv.n_pages;
+            x.bad = (int)(__ballot(!ok) & ((1u << NG) - 1));
+            x.page = __builtin_amdgcn_readlane(ok ? ids : 0, w * RW / 16);  // a page that is none: any that exists, whose values nobody sees
         }
-        const int f = (r_ok ? 0 : 1) | (part && __any(bad) ? 2 : 0);
-        if (lane == 0) s_flag[buf][w] = f;
+        return x;
     };
+    auto copy = [&](auto is_v, int t, int page, uint8_t *dst) __attribute__((always_inline)) {
+        if (t >= t_end) return;
+        constexpr bool V = decltype(is_v)::value;
+        const int64_t rs = V ? a.kv.v_row : a.kv.k_row;
+        const int g0 = imin(t * KT + w * RW, (kr.hi - 1) & ~(RW - 1)), n = kr.hi - g0;  // rows behind the last one seen: copies of it
+        const uint8_t *src = V ? vbase : kbase;
+        if (trow) src += page * a.kv.page + (g0 & ((1 << a.kv.page_shift) - 1)) * rs;
+        else src += (sv.row0 + g0) * rs;
+        const int cr = V ? v_r : k_r, cc = V ? v_c : k_c;
+        uint8_t *d = dst + w * NLD * (V ? Lds::V_BLOCK : Lds::K_BLOCK);
+#pragma unroll
+        for (int i = 0; i < NLD; i++) copy_lds(src, imin(i * RPI + cr, n - 1) * (int)rs + cc, d + i * (V ? Lds::V_BLOCK : Lds::K_BLOCK));
+    };
+    using K_ = std::false_type;
+    using V_ = std::true_type;
 
     f32x16 o[DB];
 #pragma unroll
@@ -263,117 +283,204 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     float m = -FLT_MAX, l = 0;
     // exponent of a score in log2 units is s · c
     const float c = CAP ? 1.0f : a.scale * LOG2E_F, cap_in = CAP ? 2.0f * LOG2E_F * a.scale / a.softcap : 0.0f, cap_out = CAP ? a.softcap * LOG2E_F : 0.0f;
-    // addresses within a tile: keys row-wise, values transposed
-    const int ka = (lane & 31) * ROWB, kx = h ^ swz_k<HD>(lane & 31);
-    const int vr = 4 * h + ((lane & 15) >> 2);
-    const int va = vr * ROWB + (lane & 1) * 8, vx = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swz_v<HD>(vr);
+    // the lane's places in a tile: keys row-wise, values transposed
+    const int k_at = Lds::key(lane & 31, h), v_at = Lds::value(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
+
+    f32x16 s[2];
+    u32x4 pf[2][2];
+    auto scores = [&](const uint8_t *kt, int kb, f32x16 &d) __attribute__((always_inline)) {
+        d = f32x16{};
+#pragma unroll
+        for (int i = 0; i < KS; i++) d = mfma32<BF>(*(const u32x4 *)(kt + k_at + Lds::key(kb * 32, 2 * i)), qf[i], d);
+    };
+    auto outputs = [&](const uint8_t *vt, int kb, const u32x4 (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const uint8_t *vp = vt + v_at + Lds::value(kb * 32 + st * 16, 4 * d);
+                const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
+                o[d] = mfma32<BF>(u32x4{v0[0], v0[1], v1[0], v1[1]}, p[st], o[d]);
+            }
+    };
+    // group (t, kb): probabilities of its scores x → p; outputs of the group before from values
+    // (vt, vkb) and probabilities po; scores of the group behind from keys (kt, nkb) → y
+    auto group = [&](int key0, int bad2, f32x16 &x, u32x4 (&p)[2], const u32x4 (&po)[2], f32x16 &y, const uint8_t *vt, int vkb, const uint8_t *kt, int nkb) __attribute__((always_inline)) {
+        if constexpr (CAP) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = cap_score<CAP>(x[e], cap_in, cap_out);
+        }
+        // positions of the lane's scores: key0 + 4 h + (8 (e / 4) + e % 4)
+        if (key0 + 31 > all_hi) {
+            const int d = p_q - key0 - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 <= d ? x[e] : -INFINITY;
+        }
+        if (key0 <= all_lo) {
+            const int d = lo_q - key0 - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 > d ? x[e] : -INFINITY;
+        }
+        if (bad2) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = bad2 >> (e / 8) & 1 ? -INFINITY : x[e];
+        }
+        float mx = fmaxf(fmaxf(x[0], x[1]), x[2]);
+#pragma unroll
+        for (int e = 3; e < 15; e += 2) mx = fmaxf(fmaxf(mx, x[e]), x[e + 1]);
+        mx = fmaxf(mx, x[15]) * c;
+        const bool moved = __any(mx > m + M_SLACK);
+        float al = 1;
+        if (moved) {
+            float a0, a1;
+            pair_f<32>(mx, a0, a1);
+            const float mn = fmaxf(m, fmaxf(a0, a1));
+            al = exp2_hw(m - mn);
+            m = mn;
+            l *= al;
+        }
+        // Eight rounds of an output product and a score product, operands read two rounds ahead,
+        // with a share of the probabilities after each: the fences keep the order.
+        constexpr int NV = 2 * DB, NR = NV > KS ? NV : KS;
+        y = f32x16{};
+        const float ref = P_SHIFT<BF> - m;
+        u32x4 kf[KS], vf[NV];
+        auto read_v = [&](int u) {
+            const uint8_t *vp = vt + v_at + Lds::value(vkb * 32 + u / DB * 16, u % DB * 4);
+            const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
+            vf[u] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        };
+        auto read_k = [&](int u) { kf[u] = *(const u32x4 *)(kt + k_at + Lds::key(nkb * 32, 2 * u)); };
+        float ex[16];
+        auto exps = [&](int i) {
+            ex[2 * i] = exp2_hw(fmaf(x[2 * i], c, ref));
+            ex[2 * i + 1] = exp2_hw(fmaf(x[2 * i + 1], c, ref));
+        };
+        auto pack = [&](int i) { p[i / 4][i % 4] = pack2<BF>(ex[2 * i], ex[2 * i + 1]); };
+        auto add = [&](int i) { l = add2<BF>(p[i / 4][i % 4], l); };
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            read_v(i);
+            read_k(i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            if (i < NV) o[i % DB] = mfma32<BF>(vf[i], po[i / DB], o[i % DB]);
+            if (i + 2 < NV) read_v(i + 2);
+#pragma unroll
+            for (int u = i * 8 / NR; u < (i + 1) * 8 / NR; u++) exps(u);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i < KS) y = mfma32<BF>(kf[i], qf[i], y);
+            if (i + 2 < KS) read_k(i + 2);
+#pragma unroll
+            for (int u = i * 8 / NR; u < (i + 1) * 8 / NR; u++) {
+                pack(u);
+                if (u) add(u - 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        add(7);
+        // all three belong into this block: the compiler would move the probabilities to where
+        // they are used, and make two copies of the block
+        asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l));
+        int after = __builtin_amdgcn_readfirstlane(moved);
+        asm volatile("" : "+s"(after));
+        if (after) {  // the outputs so far were formed with the maximum before
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= al;
+        }
+    };
+    // Infinite and NaN values of tile t, some of whose positions some row does not see: added
+    // to the outputs of the rows that see them, then replaced by zeros.  All waves call this.
+    auto apart = [&](int t, int bad, uint8_t *vt) __attribute__((always_inline)) {
+        if ((t + 1) * KT - 1 <= wg_hi && t * KT > wg_lo && !bad) return;
+        bool nf = false;
+#pragma unroll
+        for (int i = 0; i < NLD; i++) nf = nf || nonfinite8<BF>(*(const u32x4 *)(vt + (w * NLD + i) * Lds::V_BLOCK + lane * 16));
+        const int f = __any(nf);
+        if (lane == 0) s_nf[w] = f;
+        lds_barrier();
+        if (!__builtin_amdgcn_readfirstlane(s_nf[0] | s_nf[1] | s_nf[2] | s_nf[3])) return;
+        for (int r = 0; r < KT; r++) {
+            const int j = t * KT + r;
+            const bool see = j <= p_q && j > lo_q && !(bad >> (r / 16) & 1);
+            if (!__any(see)) continue;
+            const uint8_t *vp = vt + Lds::value(r, 0) + 8 * h;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {  // dim 32 d + 8 (e / 4) + 4 h + e % 4
+                    const float v = value16<BF>(*(const uint16_t *)(vp + Lds::value(0, 4 * d + e / 4) + e % 4 * 2));
+                    o[d][e] += (see & !(fabsf(v) <= FLT_MAX)) ? v : 0.0f;
+                }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < NLD; i++) {
+            u32x4 *p = (u32x4 *)(vt + (w * NLD + i) * Lds::V_BLOCK + lane * 16);
+            u32x4 v = *p;
+            for (int e = 0; e < 4; e++) v[e] = finite2<BF>(v[e]);
+            *p = v;
+        }
+        lds_barrier();
+    };
 
     if (t_begin < t_end) {
-        load(t_begin);
-        stage(t_begin, t_begin & 1);
-    }
-    for (int t = t_begin; t < t_end; t++) {
-        const int buf = t & 1;
+        Tile cur = tile_of(request_pages(t_begin)), nxt = tile_of(request_pages(t_begin + 1));
+        int ids = request_pages(t_begin + 2);
+        int prev_bad = 0;  // KB = 1: of tile t − 1
+        copy(K_{}, t_begin, cur.page, s_k0);
+        copy(K_{}, t_begin + 1, nxt.page, s_k1);
+        if constexpr (KB == 2) copy(V_{}, t_begin, cur.page, s_v0);
+        // the first group's outputs before it: zeros
+        for (int i = w; i < 32 / RPI; i += 4) *(u32x4 *)(s_v1 + Lds::value((KB - 1) * 32 + i * RPI, 0) + lane * 16) = u32x4{0, 0, 0, 0};
+        pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
+        wait_vmem();
         lds_barrier();
-        if (t + 1 < t_end) load(t + 1);
-        int fl[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) fl[i] = __builtin_amdgcn_readfirstlane(s_flag[buf][i]);
-        const int any = fl[0] | fl[1] | fl[2] | fl[3];
-        const int key0 = t * KT;
-        auto sees = [&](int r) {  // whether this lane's row sees row r of the tile
-            const int j = key0 + r;
-            return j <= p_q && j > lo_q && !(fl[r / RW] & 1);
+        if (wave_live) scores(s_k0, 0, s[0]);
+        auto tile = [&](int t, uint8_t *k_t, uint8_t *k_n, uint8_t *v_t, uint8_t *v_n, f32x16 &x0, f32x16 &x1, u32x4 (&p0)[2], u32x4 (&p1)[2]) __attribute__((always_inline)) {
+            if constexpr (KB == 2)
+                if (wave_live) group(t * KT, cur.bad & 3, x0, p0, p1, x1, v_n, 1, k_t, 1);
+            wait_vmem();
+            lds_barrier();
+            const Tile third = tile_of(ids);
+            copy(K_{}, t + 2, third.page, k_t);
+            if constexpr (KB == 2) copy(V_{}, t + 1, nxt.page, v_n);
+            else copy(V_{}, t, cur.page, v_t);
+            ids = request_pages(t + 3);
+            if constexpr (KB == 2) {
+                apart(t, cur.bad, v_t);
+                if (wave_live) group(t * KT + 32, cur.bad >> 2, x1, p1, p0, x0, v_t, 0, k_n, 0);
+            } else {
+                if (t > t_begin) apart(t - 1, prev_bad, v_n);
+                if (wave_live) group(t * KT, cur.bad, x0, p0, p1, x1, v_n, 0, k_n, 0);
+                prev_bad = cur.bad;
+            }
+            cur = nxt;
+            nxt = third;
         };
-        if (any & 2) {  // rare: infinite or NaN values in a tile that is not everybody's
-            for (int r = 0; r < KT; r++) {
-                const bool see = sees(r);
-                if (!__any(see)) continue;
-                const uint8_t *vp = s_v[buf] + r * ROWB;
-#pragma unroll
-                for (int d = 0; d < DB; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int dim = d * 32 + 8 * (e / 4) + 4 * h + e % 4;
-                        const float x = value16<BF>(*(const uint16_t *)(vp + (((dim >> 3) ^ swz_v<HD>(r)) << 4) + (dim & 7) * 2));
-                        if (see && !(fabsf(x) <= FLT_MAX)) o[d][e] += x;
-                    }
-            }
-            lds_barrier();
-#pragma unroll
-            for (int i = 0; i < NLD; i++) {
-                const int r = w * RW + st_r[i];
-                u32x4 *p = (u32x4 *)(s_v[buf] + r * ROWB + ((st_ch[i] ^ swz_v<HD>(r)) << 4));
-                u32x4 x = *p;
-                for (int e = 0; e < 4; e++) x[e] = finite2<BF>(x[e]);
-                *p = x;
-            }
-            lds_barrier();
+        int t = t_begin;
+        for (; t < t_end; t += 2) {
+            if constexpr (KB == 2) tile(t, s_k0, s_k1, s_v0, s_v1, s[0], s[1], pf[0], pf[1]);
+            else tile(t, s_k0, s_k1, s_v0, s_v1, s[0], s[1], pf[0], pf[1]);
+            if (t + 1 >= t_end) break;
+            if constexpr (KB == 2) tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[0], s[1], pf[0], pf[1]);
+            else tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[1], s[0], pf[1], pf[0]);
         }
-        if (wave_live && key0 < wr.hi && key0 + KT > wr.lo) {
-            f32x16 s[KB];
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                s[kb] = f32x16{};
-#pragma unroll
-                for (int i = 0; i < KS; i++) {
-                    const u32x4 kf = *(const u32x4 *)(s_k[buf] + ka + kb * 32 * ROWB + ((kx ^ (2 * i)) << 4));
-                    s[kb] = mfma32<BF>(kf, qf[i], s[kb]);
-                }
-            }
-            if constexpr (CAP) {
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) s[kb][e] = cap_score<CAP>(s[kb][e], cap_in, cap_out);
-            }
-            if (key0 + KT - 1 > all_hi || key0 <= all_lo || (any & 1)) {
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int r = kb * 32 + 8 * (e / 4) + 4 * h + e % 4;
-                        const int j = key0 + r;
-                        const bool gone = fl[(kb * 32 + 8 * (e / 4)) / RW] & 1;
-                        if (j > p_q || j <= lo_q || gone) s[kb][e] = -INFINITY;
-                    }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[kb][e]);
-            mx *= c;
-            if (__any(mx > m + M_SLACK)) {
-                float a0, a1;
-                pair_f<32>(mx, a0, a1);
-                const float mn = fmaxf(m, fmaxf(a0, a1)), al = exp2_hw(m - mn);
-                m = mn;
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < DB; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] *= al;
-            }
-            const float ref = P_SHIFT<BF> - m;
-#pragma unroll
-            for (int st = 0; st < KT / 16; st++) {
-                u32x4 pf;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int x = (st & 1) * 8 + 2 * e;
-                    pf[e] = pack2<BF>(exp2_hw(fmaf(s[st / 2][x], c, ref)), exp2_hw(fmaf(s[st / 2][x + 1], c, ref)));
-                    l = add2<BF>(pf[e], l);
-                }
-#pragma unroll
-                for (int d = 0; d < DB; d++) {
-                    const uint8_t *vp = s_v[buf] + va + st * 16 * ROWB + ((vx ^ (4 * d)) << 4);
-                    const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + 8 * ROWB);
-                    o[d] = mfma32<BF>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf, o[d]);
-                }
-            }
+        // the last group's outputs
+        const bool odd = (t_end - t_begin) & 1;
+        if constexpr (KB == 1) {
+            wait_vmem();
+            lds_barrier();
+            apart(t_end - 1, prev_bad, odd ? s_v0 : s_v1);
         }
-        if (t + 1 < t_end) stage(t + 1, buf ^ 1);
+        if (wave_live) {
+            if (odd) outputs(s_v0, KB - 1, pf[KB == 2 ? 1 : 0]);
+            else outputs(s_v1, KB - 1, pf[1]);
+        }
     }
 
     float l0, l1;
