@@ -3,7 +3,7 @@
 //
 //   m = max x, S = Σ e^(x − m):  ln p_t = x_t − m − ln S,  H = ln S + Σ e^(x − m) (m − x) / S
 //
-// The logits are read once.  logprob_part_kernel takes groups of 512 consecutive logits, a
+// The logits are read once.  logprob_part_kernel takes groups of 1024 consecutive logits, a
 // wave per run of groups, with the running maximum, the sum and the weighted sum in f32, and
 // keeps every group's maximum; logprob_row_kernel joins a row's runs.  The k most likely
 // tokens lie in the k groups with the largest maxima (by value, then by place: a group ahead
@@ -29,8 +29,8 @@ namespace rie {
 
 namespace {
 
-constexpr int GROUP = 512;     // logits of a group: 8 per lane
-constexpr float D_MIN = -200;  // e^-200 is 0 in f32: the weighted sum's factor is cut there, so that 0 · -inf is not NaN
+constexpr int R = 16, GROUP = 64 * R;  // logits of a lane and of a group
+constexpr float D_MIN = -200;          // e^-200 is 0 in f32: the weighted sum's factor is cut there, so that 0 · -inf is not NaN
 
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
@@ -41,33 +41,34 @@ __device__ __forceinline__ float logit(const void *x, int64_t i) {
     return TY == T_BF16 ? __uint_as_float((uint32_t)b << 16) : h2f(b);
 }
 
-// Place of a lane's value j of a group: two runs of 4 (f32) or one of 8, each 16 bytes
+// Place of a lane's value j of a group: runs of 16 bytes, the lanes' side by side
 template <int TY>
 __device__ __forceinline__ int place(int lane, int j) {
-    return TY == T_F32 ? (j >> 2) * 256 + lane * 4 + (j & 3) : lane * 8 + j;
+    constexpr int N = TY == T_F32 ? 4 : 8;
+    return j / N * (64 * N) + lane * N + j % N;
 }
 
-// The lane's 8 values of the group that starts at element e0 of the row; −inf behind the
-// row's ends (e0 is negative in the first group of a row that is not 16-byte aligned)
+// The lane's values of the group that starts at element e0 of the row; −inf behind the row's
+// ends (e0 is negative in the first group of a row that is not 16-byte aligned)
 template <int TY>
-__device__ __forceinline__ void load_group(const void *x, int e0, int V, int lane, float (&v)[8]) {
+__device__ __forceinline__ void load_group(const void *x, int e0, int V, int lane, float (&v)[R]) {
     if (e0 >= 0 && e0 + GROUP <= V) {
         if constexpr (TY == T_F32) {
-            const float *p = (const float *)x + e0;
-            const f32x4 a = *(const f32x4 *)(p + lane * 4), b = *(const f32x4 *)(p + 256 + lane * 4);
+            f32x4 a[R / 4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[j] = a[j];
-                v[4 + j] = b[j];
-            }
+            for (int i = 0; i < R / 4; i++) a[i] = *(const f32x4 *)((const float *)x + e0 + place<TY>(lane, 4 * i));
+#pragma unroll
+            for (int j = 0; j < R; j++) v[j] = a[j / 4][j % 4];
         } else {
-            const u16x8 a = *(const u16x8 *)((const uint16_t *)x + e0 + lane * 8);
+            u16x8 a[R / 8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = TY == T_BF16 ? __uint_as_float((uint32_t)a[j] << 16) : h2f(a[j]);
+            for (int i = 0; i < R / 8; i++) a[i] = *(const u16x8 *)((const uint16_t *)x + e0 + place<TY>(lane, 8 * i));
+#pragma unroll
+            for (int j = 0; j < R; j++) v[j] = TY == T_BF16 ? __uint_as_float((uint32_t)a[j / 8][j % 8] << 16) : h2f(a[j / 8][j % 8]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < R; j++) {
             const int e = e0 + place<TY>(lane, j);
             v[j] = e >= 0 && e < V ? logit<TY>(x, e) : -INFINITY;
         }
@@ -109,11 +110,14 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
     const void *x = (const uint8_t *)a.x + row * a.ld * (TY == T_F32 ? 4 : 2);
     const int off = misplaced<TY>(x), g0 = part * per, g1 = min(g0 + per, n_groups);
     float M = -FLT_MAX, s = 0, t = 0, cnt = 0;  // M is the wave's; s, t and cnt are the lane's
-    float v[8], nx[8];
+    float v[R], nx[R];
     load_group<TY>(x, g0 * GROUP - off, a.V, lane, v);
     for (int g = g0; g < g1; g++) {
         if (g + 1 < g1) load_group<TY>(x, (g + 1) * GROUP - off, a.V, lane, nx);
-        float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+        float mx = v[0];
+#pragma unroll
+        for (int j = 1; j < R - 1; j += 2) mx = fmaxf(fmaxf(mx, v[j]), v[j + 1]);
+        mx = fmaxf(mx, v[R - 1]);
         mx = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(xmax_f<64>(mx))));
         mx = mx == mx ? mx : -INFINITY;  // nothing but NaN
         if (lane == 0) gmax[(int64_t)row * n_groups + g] = mx;
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
                 M = mx;
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < R; j++) {
                 const bool eq = v[j] == M;
                 const float d = v[j] - M, e = eq ? 0.0f : exp2_hw(d * LOG2E_F);
                 cnt += eq ? 1.0f : 0.0f;
@@ -135,14 +139,14 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < R; j++) {
                 const float d = v[j] - M, e = exp2_hw(d * LOG2E_F);
                 s += e;
                 t = fmaf(e, fmaxf(d, D_MIN), t);
             }
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = nx[j];
+        for (int j = 0; j < R; j++) v[j] = nx[j];
     }
     s = xsum_f<64>(s);
     t = xsum_f<64>(t);
@@ -185,30 +189,57 @@ __global__ __launch_bounds__(256) void logprob_row_kernel(LogprobArgs a, int n_g
     const int k = a.n_top;
     if (!k) return;
 
-    // the k groups with the largest maxima
+    // The k groups with the largest maxima: the first wave takes them out one by one, a lane
+    // holding the maxima of every 64th group in LDS and the best of them (the lowest group among
+    // equals) in registers.
     const int kg = min(k, n_groups);
-    for (int i = tid; i < n_groups; i += 256) {
-        const float v = s_gmax[i];
-        int ahead = 0;
-        for (int j = 0; j < n_groups; j++) ahead += s_gmax[j] > v || (s_gmax[j] == v && j < i);
-        if (ahead < kg) s_group[ahead] = i;
-        if (ahead == k - 1) s_thr = v;
+    if (w == 0) {
+        float best = -INFINITY;
+        int at = INT32_MAX;
+        auto look = [&] {
+            best = -INFINITY;
+            at = INT32_MAX;
+#pragma unroll 4
+            for (int i = lane; i < n_groups; i += 64) {
+                const float v = s_gmax[i];
+                if (v > best || (at == INT32_MAX && v == best)) {
+                    best = v;
+                    at = i;
+                }
+            }
+        };
+        look();
+        float thr = -INFINITY;
+        for (int r = 0; r < kg; r++) {
+            // at < INT32_MAX with the largest best: −inf is a value like others here
+            const float top = xmax_f<64>(at == INT32_MAX ? -INFINITY : best);
+            const int first = xreduce<64>(best == top ? at : INT32_MAX, [](int x, int y) { return x < y ? x : y; });
+            if (lane == 0) s_group[r] = first;
+            thr = top;
+            if (at == first) {
+                s_gmax[at] = NAN;  // compares with nothing
+                look();
+            }
+        }
+        if (lane == 0) s_thr = n_groups < k ? -INFINITY : thr;
     }
-    if (n_groups < k && tid == 0) s_thr = -INFINITY;
     __syncthreads();
     // their logits that may be among the first k
     const float thr = s_thr;
     const int off = misplaced<TY>(x);
-    for (int i = tid; i < kg * GROUP; i += 256) {
-        const int e = s_group[i / GROUP] * GROUP - off + i % GROUP;
-        if (e < 0 || e >= a.V) continue;
-        float v = logit<TY>(x, e);
-        v = v != v ? -INFINITY : v;
-        if (v >= thr) {
-            const int at = atomicAdd(&s_n, 1);
-            if (at < CAND) {
-                s_val[at] = v;
-                s_idx[at] = e;
+    for (int i = w; i < kg; i += 4) {
+        const int e0 = s_group[i] * GROUP - off;
+        float v[R];
+        load_group<TY>(x, e0, a.V, lane, v);
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            const int e = e0 + place<TY>(lane, j);
+            if (e >= 0 && e < a.V && (v[j] >= thr || (v[j] != v[j] && thr == -INFINITY))) {
+                const int c = atomicAdd(&s_n, 1);
+                if (c < CAND) {
+                    s_val[c] = v[j] != v[j] ? -INFINITY : v[j];
+                    s_idx[c] = e;
+                }
             }
         }
     }
@@ -219,7 +250,8 @@ __global__ __launch_bounds__(256) void logprob_row_kernel(LogprobArgs a, int n_g
             const float v = s_val[i];
             const int e = s_idx[i];
             int ahead = 0;
-            for (int j = 0; j < n; j++) ahead += s_val[j] > v || (s_val[j] == v && s_idx[j] < e);
+#pragma unroll 8
+            for (int j = 0; j < n; j++) ahead += (s_val[j] > v) | ((s_val[j] == v) & (s_idx[j] < e));
             if (ahead < k) {
                 a.top_ids[(int64_t)row * k + ahead] = e;
                 a.top_logprobs[(int64_t)row * k + ahead] = v - p.m - log_s;

@@ -107,32 +107,39 @@ template <bool BF>
 constexpr float P_SHIFT = BF ? 0.0f : 6.0f;
 constexpr float M_SLACK = 8.0f;  // how far a score may pass the maximum that is subtracted
 
-// The largest i in [0, n) with key(starts[i], i) ≤ x, for keys that rise with i (0 where
-// there is none): 64 candidates at a time, one per lane.
+__device__ __forceinline__ SeqView uniform(const SeqView &v) {
+    return SeqView{__builtin_amdgcn_readfirstlane(v.row0), __builtin_amdgcn_readfirstlane(v.n_new), __builtin_amdgcn_readfirstlane(v.len)};
+}
+// x, the same for the whole wave, where the compiler cannot see it (behind divisions, say):
+// kept in a scalar register, with branches on it that are no masks
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// positions that a sequence can have (packed rows: as many as it has rows)
+__device__ __forceinline__ SeqView view_at(const BatchView &b, const KvView &kv, int start, int end, int len) {
+    SeqView v = seq_view(start, end, len, b.n_rows, kv.table ? kv.cap : INT32_MAX);
+    if (!kv.table) v.len = v.n_new;
+    return uniform(v);
+}
+__device__ __forceinline__ SeqView view_of(const BatchView &b, const KvView &kv, int i) {
+    return view_at(b, kv, b.starts[i], b.starts[i + 1], b.lens ? b.lens[i] : 0);
+}
+// The sequence with the largest number i that has key(starts[i], i) ≤ x, for keys that rise
+// with i (0 where there is none): 63 candidates at a time, one per lane, whose starts, ends
+// and lengths are there at once when so few are left.
 template <class F>
-__device__ __forceinline__ int wave_find(const int *starts, int n, int x, F key) {
-    int lo = 0;
-    while (true) {
-        const int w = (n + 63) >> 6;
-        const int i = (int)(threadIdx.x & 63) * w;
-        const bool le = i < n && key(starts[lo + imin(i, n - 1)], lo + i) <= x;
+__device__ __forceinline__ SeqView find_seq(const BatchView &b, const KvView &kv, int x, int &si, F key) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = b.n_seq;
+    while (n > 63) {
+        const int w = (n + 62) / 63, i = lane * w;
+        const bool le = lane < 63 && i < n && key(b.starts[lo + imin(i, n - 1)], lo + imin(i, n - 1)) <= x;
         const int c = imax((int)__popcll(__ballot(le)) - 1, 0);
         lo += c * w;
         n = imin(w, n - c * w);
-        if (w == 1) break;
     }
-    return __builtin_amdgcn_readfirstlane(lo);
-}
-
-__device__ __forceinline__ SeqView view_of(const BatchView &b, const KvView &kv, int i) {
-    const int s = b.starts[i], e = b.starts[i + 1];
-    // packed rows: as many positions as rows
-    SeqView v = seq_view(s, e, b.lens ? b.lens[i] : INT32_MAX, b.n_rows, kv.table ? kv.cap : INT32_MAX);
-    if (!kv.table) v.len = v.n_new;
-    v.row0 = __builtin_amdgcn_readfirstlane(v.row0);
-    v.n_new = __builtin_amdgcn_readfirstlane(v.n_new);
-    v.len = __builtin_amdgcn_readfirstlane(v.len);
-    return v;
+    const int i = lo + imin(lane, n), start = b.starts[i], len = b.lens ? b.lens[imin(i, b.n_seq - 1)] : 0;
+    const int c = __builtin_amdgcn_readfirstlane(imax((int)__popcll(__ballot(lane < n && key(start, i) <= x)) - 1, 0));
+    si = lo + c;
+    return view_at(b, kv, __builtin_amdgcn_readlane(start, c), __builtin_amdgcn_readlane(start, c + 1), __builtin_amdgcn_readlane(len, c));
 }
 
 // Offset in bytes of position g's row (the same for a group of up to 16 positions that
@@ -147,11 +154,6 @@ __device__ __forceinline__ bool page_of(const KvView &kv, const int *trow, int g
 
 template <int HD>
 constexpr int HDP = HD <= 64 ? 64 : HD <= 128 ? 128 : HD;  // values between rows of a tile in LDS
-// 16-byte chunk c of row r goes to chunk c ^ swz(r), so that the lanes of a read, which
-// take the same chunk of many rows (keys) or 4 chunks of 4 rows (values), use all banks
-template <int HD>
-__device__ __forceinline__ int swz_v(int r) { return HDP<HD> >= 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
-
 // score → exponent in log2 units, where the softcap makes it one already
 template <bool CAP>
 __device__ __forceinline__ float cap_score(float s, float in, float out) {
@@ -211,19 +213,19 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     __shared__ __align__(16) uint8_t s_k0[KBYTES], s_k1[KBYTES], s_v0[VBYTES], s_v1[VBYTES];
     __shared__ __align__(16) int s_nf[4];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-    const int G = a.G, kvh = blockIdx.x % a.n_kv;
-    const int blk = a.n_blocks - 1 - (int)(blockIdx.x / a.n_kv);  // a sequence's longest rows first
-    const int si = wave_find(a.b.starts, a.b.n_seq, blk, [&](int s, int i) { return block_base(iclamp(s, 0, a.b.n_rows), i, G, TILE_M); });
-    const SeqView sv = view_of(a.b, a.kv, si);
-    const int lb = blk - block_base(sv.row0, si, G, TILE_M);
+    // the splits of a block side by side, and a KV head's workgroups on one XCD where there are 8 of them
+    const int G = a.G, kvh = blockIdx.x % a.n_kv, sp = blockIdx.x / a.n_kv % a.S, blk = blockIdx.x / a.n_kv / a.S;
+    int si;
+    const SeqView sv = find_seq(a.b, a.kv, blk, si, [&](int s, int i) { return block_base(iclamp(s, 0, a.b.n_rows), i, G, TILE_M); });
     const int n_rows = sv.n_new * G;
+    const int lb = (n_rows + TILE_M - 1) / TILE_M - 1 - (blk - block_base(sv.row0, si, G, TILE_M));  // a sequence's longest rows first
     if (lb < 0 || lb >= (n_rows + TILE_M - 1) / TILE_M) return;
-    const int r0 = lb * TILE_M, r1 = imin(r0 + TILE_M, n_rows) - 1;
+    const int r0 = same(lb * TILE_M), r1 = same(imin(r0 + TILE_M, n_rows) - 1), tok0 = same(r0 / G), tok1 = same(r1 / G);
     const int pos0 = sv.len - sv.n_new;  // position of token 0
-    const KeyRange kr = key_range(sv, r0 / G, r1 / G, a.window);
-    const int nt = tile_count(kr, KT), ns = split_count(nt, a.C, a.S), sp = blockIdx.y;
+    const KeyRange kr = key_range(sv, tok0, tok1, a.window);
+    const int hi = same(kr.hi), nt = same(tile_count(kr, KT)), ns = same(split_count(nt, a.C, a.S));
     if (sp >= ns) return;
-    const int t_begin = first_tile(kr, KT) + sp * a.C, t_end = sp == ns - 1 ? first_tile(kr, KT) + nt : t_begin + a.C;
+    const int t_first = same(first_tile(kr, KT)), t_begin = t_first + sp * a.C, t_end = sp == ns - 1 ? t_first + nt : t_begin + a.C;
 
     // this lane's query row, and what the rows of its wave see
     const int row = r0 + w * 32 + (lane & 31);
@@ -232,9 +234,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const int p_q = live ? pos0 + tok : -1;
     const int lo_q = a.window > 0 ? p_q - a.window : -1;  // sees j in (lo_q, p_q]
     const bool wave_live = r0 + w * 32 <= r1;
-    const int w_t0 = imin(r0 + w * 32, r1) / G, w_t1 = imin(r0 + w * 32 + 31, r1) / G;
+    const int w_t0 = same(imin(r0 + w * 32, r1) / G), w_t1 = same(imin(r0 + w * 32 + 31, r1) / G);
     const int all_hi = pos0 + w_t0, all_lo = a.window > 0 ? pos0 + w_t1 - a.window : -1;  // every row of the wave sees (all_lo, all_hi]
-    const int wg_hi = pos0 + r0 / G, wg_lo = a.window > 0 ? pos0 + r1 / G - a.window : -1;  // and of the workgroup
+    const int wg_hi = pos0 + tok0, wg_lo = a.window > 0 ? pos0 + tok1 - a.window : -1;    // and of the workgroup
     u32x4 qf[KS];
     {
         const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + h * 16;
@@ -247,32 +249,49 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
     const int k_r = Lds::key_row(lane), k_c = imin(Lds::key_chunk(lane), HD / 8 - 1) * 16;
     const int v_r = Lds::value_row(lane), v_c = imin(Lds::value_chunk(lane), HD / 8 - 1) * 16;
-    // page ids of the groups of a tile, a lane each: requested a tile ahead of their use
-    auto request_pages = [&](int t) { return trow && t < t_end ? trow[imin(t * KT + imin(lane, NG - 1) * 16, kr.hi - 1) >> a.kv.page_shift] : 0; };
-    struct Tile {
-        int page, bad;  // the wave's own page; bit g: the page of group g is none
+    const int k_row = (int)a.kv.k_row, v_row = (int)a.kv.v_row, k_off = k_r * k_row + k_c, v_off = v_r * v_row + v_c;
+    // Page ids of a tile's groups of 16 positions, a lane each, requested a tile ahead of their
+    // use (ids that stay in a register for several tiles, 64 pages at once, made the compiler
+    // wait for all copies where their loads join the loop: 424 to 461 us for four packed prompts).
+    const int page_mask = (1 << a.kv.page_shift) - 1;
+    auto request_pages = [&](int t) __attribute__((always_inline)) {
+        return trow && t < t_end ? trow[imin(t * KT + imin(lane, NG - 1) * 16, hi - 1) >> a.kv.page_shift] : 0;
     };
-    auto tile_of = [&](int ids) {
-        Tile x{0, 0};
+    // a tile's place in memory for this wave's rows, and (bit g) which of its groups of 16
+    // positions lie in a page that is none (one that exists is read, and nobody sees its values)
+    struct Tile {
+        int64_t k, v;
+        int rows, bad;  // rows: how many of the wave's are seen by some token
+    };
+    auto tile_of = [&](int t, int ids) __attribute__((always_inline)) {
+        const int g0 = imin(t * KT + w * RW, (hi - 1) & ~(RW - 1));  // rows behind the last one seen: copies of it
+        Tile x;
+        x.rows = hi - g0;
+        x.bad = 0;
         if (trow) {
             const bool ok = (unsigned)ids < (unsigned)a.kv.n_pages;
-            x.bad = (int)(__ballot(!ok) & ((1u << NG) - 1));
-            x.page = __builtin_amdgcn_readlane(ok ? ids : 0, w * RW / 16);  // a page that is none: any that exists, whose values nobody sees
+            x.bad = same((int)(__ballot(!ok) & ((1u << NG) - 1)));
+            const int64_t page = __builtin_amdgcn_readlane(ok ? ids : 0, w * RW / 16), slot = g0 & page_mask;
+            x.k = page * a.kv.page + slot * a.kv.k_row;
+            x.v = page * a.kv.page + slot * a.kv.v_row;
+        } else {
+            x.k = (int64_t)(sv.row0 + g0) * a.kv.k_row;
+            x.v = (int64_t)(sv.row0 + g0) * a.kv.v_row;
         }
         return x;
     };
-    auto copy = [&](auto is_v, int t, int page, uint8_t *dst) __attribute__((always_inline)) {
-        if (t >= t_end) return;
+    auto copy = [&](auto is_v, const uint8_t *src, int rows, uint8_t *dst) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
-        const int64_t rs = V ? a.kv.v_row : a.kv.k_row;
-        const int g0 = imin(t * KT + w * RW, (kr.hi - 1) & ~(RW - 1)), n = kr.hi - g0;  // rows behind the last one seen: copies of it
-        const uint8_t *src = V ? vbase : kbase;
-        if (trow) src += page * a.kv.page + (g0 & ((1 << a.kv.page_shift) - 1)) * rs;
-        else src += (sv.row0 + g0) * rs;
-        const int cr = V ? v_r : k_r, cc = V ? v_c : k_c;
-        uint8_t *d = dst + w * NLD * (V ? Lds::V_BLOCK : Lds::K_BLOCK);
+        constexpr int BLOCK = V ? Lds::V_BLOCK : Lds::K_BLOCK;
+        const int rs = V ? v_row : k_row;
+        uint8_t *d = dst + w * NLD * BLOCK;
+        if (rows >= RW) {
 #pragma unroll
-        for (int i = 0; i < NLD; i++) copy_lds(src, imin(i * RPI + cr, n - 1) * (int)rs + cc, d + i * (V ? Lds::V_BLOCK : Lds::K_BLOCK));
+            for (int i = 0; i < NLD; i++) copy_lds(src + i * RPI * rs, V ? v_off : k_off, d + i * BLOCK);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NLD; i++) copy_lds(src, imin(i * RPI + (V ? v_r : k_r), rows - 1) * rs + (V ? v_c : k_c), d + i * BLOCK);
+        }
     };
     using K_ = std::false_type;
     using V_ = std::true_type;
@@ -280,7 +299,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
-    float m = -FLT_MAX, l = 0;
+    float m = -FLT_MAX, l = 0, ym = 0;  // ym: largest score of the group whose turn is next
     // exponent of a score in log2 units is s · c
     const float c = CAP ? 1.0f : a.scale * LOG2E_F, cap_in = CAP ? 2.0f * LOG2E_F * a.scale / a.softcap : 0.0f, cap_out = CAP ? a.softcap * LOG2E_F : 0.0f;
     // the lane's places in a tile: keys row-wise, values transposed
@@ -292,6 +311,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         d = f32x16{};
 #pragma unroll
         for (int i = 0; i < KS; i++) d = mfma32<BF>(*(const u32x4 *)(kt + k_at + Lds::key(kb * 32, 2 * i)), qf[i], d);
+    };
+    auto max16 = [&](const f32x16 &x) __attribute__((always_inline)) {
+        float v = fmaxf(fmaxf(x[0], x[1]), x[2]);
+#pragma unroll
+        for (int e = 3; e < 15; e += 2) v = fmaxf(fmaxf(v, x[e]), x[e + 1]);
+        return fmaxf(v, x[15]);
     };
     auto outputs = [&](const uint8_t *vt, int kb, const u32x4 (&p)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -306,29 +331,31 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     // group (t, kb): probabilities of its scores x → p; outputs of the group before from values
     // (vt, vkb) and probabilities po; scores of the group behind from keys (kt, nkb) → y
     auto group = [&](int key0, int bad2, f32x16 &x, u32x4 (&p)[2], const u32x4 (&po)[2], f32x16 &y, const uint8_t *vt, int vkb, const uint8_t *kt, int nkb) __attribute__((always_inline)) {
-        if constexpr (CAP) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = cap_score<CAP>(x[e], cap_in, cap_out);
-        }
         // positions of the lane's scores: key0 + 4 h + (8 (e / 4) + e % 4)
-        if (key0 + 31 > all_hi) {
-            const int d = p_q - key0 - 4 * h;
+        float mx = ym;
+        const bool late = key0 + 31 > all_hi, early = key0 <= all_lo;
+        if (CAP || late || early || bad2) {
+            if constexpr (CAP) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 <= d ? x[e] : -INFINITY;
+                for (int e = 0; e < 16; e++) x[e] = cap_score<CAP>(x[e], cap_in, cap_out);
+            }
+            if (late) {
+                const int d = p_q - key0 - 4 * h;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 <= d ? x[e] : -INFINITY;
+            }
+            if (early) {
+                const int d = lo_q - key0 - 4 * h;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 > d ? x[e] : -INFINITY;
+            }
+            if (bad2) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = bad2 >> (e / 8) & 1 ? -INFINITY : x[e];
+            }
+            mx = max16(x);
         }
-        if (key0 <= all_lo) {
-            const int d = lo_q - key0 - 4 * h;
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 > d ? x[e] : -INFINITY;
-        }
-        if (bad2) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = bad2 >> (e / 8) & 1 ? -INFINITY : x[e];
-        }
-        float mx = fmaxf(fmaxf(x[0], x[1]), x[2]);
-#pragma unroll
-        for (int e = 3; e < 15; e += 2) mx = fmaxf(fmaxf(mx, x[e]), x[e + 1]);
-        mx = fmaxf(mx, x[15]) * c;
+        mx *= c;
         const bool moved = __any(mx > m + M_SLACK);
         float al = 1;
         if (moved) {
@@ -339,51 +366,70 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
             m = mn;
             l *= al;
         }
-        // Eight rounds of an output product and a score product, operands read two rounds ahead,
-        // with a share of the probabilities after each: the fences keep the order.
-        constexpr int NV = 2 * DB, NR = NV > KS ? NV : KS;
+        // Eight rounds of matrix products, first the scores', then the outputs', operands read two
+        // products ahead, with a share of the probabilities after each; the next group's maximum
+        // at the end, so that its own round begins with it.  The fences keep the order.
+        constexpr int NV = 2 * DB, NM = KS + NV;
         y = f32x16{};
         const float ref = P_SHIFT<BF> - m;
-        u32x4 kf[KS], vf[NV];
-        auto read_v = [&](int u) {
-            const uint8_t *vp = vt + v_at + Lds::value(vkb * 32 + u / DB * 16, u % DB * 4);
-            const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
-            vf[u] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        u32x4 fr[NM];
+        auto read = [&](int u) __attribute__((always_inline)) {
+            if (u < KS) {
+                fr[u] = *(const u32x4 *)(kt + k_at + Lds::key(nkb * 32, 2 * u));
+            } else if (u < NM) {
+                const uint8_t *vp = vt + v_at + Lds::value(vkb * 32 + (u - KS) / DB * 16, (u - KS) % DB * 4);
+                const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
+                fr[u] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+            }
         };
-        auto read_k = [&](int u) { kf[u] = *(const u32x4 *)(kt + k_at + Lds::key(nkb * 32, 2 * u)); };
         float ex[16];
-        auto exps = [&](int i) {
+        auto exps = [&](int i) __attribute__((always_inline)) {
             ex[2 * i] = exp2_hw(fmaf(x[2 * i], c, ref));
             ex[2 * i + 1] = exp2_hw(fmaf(x[2 * i + 1], c, ref));
         };
-        auto pack = [&](int i) { p[i / 4][i % 4] = pack2<BF>(ex[2 * i], ex[2 * i + 1]); };
-        auto add = [&](int i) { l = add2<BF>(p[i / 4][i % 4], l); };
+        auto pack = [&](int i) __attribute__((always_inline)) { p[i / 4][i % 4] = pack2<BF>(ex[2 * i], ex[2 * i + 1]); };
+        auto add = [&](int i) __attribute__((always_inline)) { l = add2<BF>(p[i / 4][i % 4], l); };
+        auto product = [&](int u) __attribute__((always_inline)) {
+            if (u < KS) y = mfma32<BF>(fr[u], qf[u], y);
+            else o[(u - KS) % DB] = mfma32<BF>(fr[u], po[(u - KS) / DB], o[(u - KS) % DB]);
+        };
+        constexpr int AHEAD = 3;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            read_v(i);
-            read_k(i);
-        }
+        for (int u = 0; u < AHEAD; u++) read(u);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-            if (i < NV) o[i % DB] = mfma32<BF>(vf[i], po[i / DB], o[i % DB]);
-            if (i + 2 < NV) read_v(i + 2);
-#pragma unroll
-            for (int u = i * 8 / NR; u < (i + 1) * 8 / NR; u++) exps(u);
-            __builtin_amdgcn_sched_barrier(0);
-            if (i < KS) y = mfma32<BF>(kf[i], qf[i], y);
-            if (i + 2 < KS) read_k(i + 2);
-#pragma unroll
-            for (int u = i * 8 / NR; u < (i + 1) * 8 / NR; u++) {
-                pack(u);
-                if (u) add(u - 1);
+        for (int i = 0; i < 8; i++) {
+            const int u0 = i * NM / 8, u1 = (i + 1) * NM / 8;
+            if (u0 < u1) {
+                product(u0);
+                read(u0 + AHEAD);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            exps(i);
+            if (u0 < u1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = u0 + 1; u < u1; u++) {
+                product(u);
+                read(u + AHEAD);
+                if (u < u1 - 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            pack(i);
+            if (i) add(i - 1);
+            if (u0 + 1 < u1) __builtin_amdgcn_sched_barrier(0);
+            if (i == 6) {
+                ym = fmaxf(fmaxf(y[0], y[1]), y[2]);
+#pragma unroll
+                for (int e = 3; e < 9; e += 2) ym = fmaxf(fmaxf(ym, y[e]), y[e + 1]);
+            }
+            if (i == 7) {
+#pragma unroll
+                for (int e = 9; e < 15; e += 2) ym = fmaxf(fmaxf(ym, y[e]), y[e + 1]);
+                ym = fmaxf(ym, y[15]);
+            }
         }
         add(7);
         // all three belong into this block: the compiler would move the probabilities to where
         // they are used, and make two copies of the block
-        asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l));
+        asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l), "+v"(ym));
         int after = __builtin_amdgcn_readfirstlane(moved);
         asm volatile("" : "+s"(after));
         if (after) {  // the outputs so far were formed with the maximum before
@@ -429,35 +475,42 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     };
 
     if (t_begin < t_end) {
-        Tile cur = tile_of(request_pages(t_begin)), nxt = tile_of(request_pages(t_begin + 1));
+        const int ids0 = request_pages(t_begin), ids1 = request_pages(t_begin + 1);
         int ids = request_pages(t_begin + 2);
-        int prev_bad = 0;  // KB = 1: of tile t − 1
-        copy(K_{}, t_begin, cur.page, s_k0);
-        copy(K_{}, t_begin + 1, nxt.page, s_k1);
-        if constexpr (KB == 2) copy(V_{}, t_begin, cur.page, s_v0);
+        Tile cur = tile_of(t_begin, ids0), nxt = tile_of(t_begin + 1, ids1);
+        int bad_before = 0;  // KB = 1: of tile t − 1
+        copy(K_{}, kbase + cur.k, cur.rows, s_k0);
+        if (t_begin + 1 < t_end) copy(K_{}, kbase + nxt.k, nxt.rows, s_k1);
+        if constexpr (KB == 2) copy(V_{}, vbase + cur.v, cur.rows, s_v0);
         // the first group's outputs before it: zeros
         for (int i = w; i < 32 / RPI; i += 4) *(u32x4 *)(s_v1 + Lds::value((KB - 1) * 32 + i * RPI, 0) + lane * 16) = u32x4{0, 0, 0, 0};
         pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
         wait_vmem();
         lds_barrier();
-        if (wave_live) scores(s_k0, 0, s[0]);
+        if (wave_live) {
+            scores(s_k0, 0, s[0]);
+            ym = max16(s[0]);
+        }
         auto tile = [&](int t, uint8_t *k_t, uint8_t *k_n, uint8_t *v_t, uint8_t *v_n, f32x16 &x0, f32x16 &x1, u32x4 (&p0)[2], u32x4 (&p1)[2]) __attribute__((always_inline)) {
             if constexpr (KB == 2)
                 if (wave_live) group(t * KT, cur.bad & 3, x0, p0, p1, x1, v_n, 1, k_t, 1);
             wait_vmem();
             lds_barrier();
-            const Tile third = tile_of(ids);
-            copy(K_{}, t + 2, third.page, k_t);
-            if constexpr (KB == 2) copy(V_{}, t + 1, nxt.page, v_n);
-            else copy(V_{}, t, cur.page, v_t);
+            Tile third{};
+            if (t + 2 < t_end) {
+                third = tile_of(t + 2, ids);
+                copy(K_{}, kbase + third.k, third.rows, k_t);
+            }
             ids = request_pages(t + 3);
             if constexpr (KB == 2) {
+                if (t + 1 < t_end) copy(V_{}, vbase + nxt.v, nxt.rows, v_n);
                 apart(t, cur.bad, v_t);
                 if (wave_live) group(t * KT + 32, cur.bad >> 2, x1, p1, p0, x0, v_t, 0, k_n, 0);
             } else {
-                if (t > t_begin) apart(t - 1, prev_bad, v_n);
+                copy(V_{}, vbase + cur.v, cur.rows, v_t);
+                if (t > t_begin) apart(t - 1, bad_before, v_n);
                 if (wave_live) group(t * KT, cur.bad, x0, p0, p1, x1, v_n, 0, k_n, 0);
-                prev_bad = cur.bad;
+                bad_before = cur.bad;
             }
             cur = nxt;
             nxt = third;
@@ -475,7 +528,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         if constexpr (KB == 1) {
             wait_vmem();
             lds_barrier();
-            apart(t_end - 1, prev_bad, odd ? s_v0 : s_v1);
+            apart(t_end - 1, bad_before, odd ? s_v0 : s_v1);
         }
         if (wave_live) {
             if (odd) outputs(s_v0, KB - 1, pf[KB == 2 ? 1 : 0]);
@@ -510,14 +563,26 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
 
 // At most 16·NB query rows of a sequence and KV head: each of the workgroup's 4 waves takes
 // every fourth tile of 32 positions, and the waves' results are added up at the end.  Keys go
-// from global memory straight to operand registers, values through the wave's own LDS; both
-// are requested a tile ahead, so no barrier lies between the reading and the arithmetic.
+// from global memory straight to operand registers, values to the wave's own part of LDS, so no
+// barrier lies between the reading and the arithmetic; each is requested as soon as its place
+// is free, and the other waves of the CU (16 at head size 128) keep the memory busy meanwhile.
+// The matrix units being idle, a probability is two values of the tensors' type (value and
+// remainder), and the outputs are as exact as their own rounding.
 constexpr int FEW_KT = 32, FEW_STEP = 4 * FEW_KT;
+template <int HD, int NB>
+constexpr int FEW_WAVES = NB == 1 ? (HD <= 128 ? 4 : 2) : (HD <= 64 ? 3 : HD <= 128 ? 2 : 1);  // of a SIMD, as registers allow
+
+// the 16-bit value nearest to a, as f32
+template <bool BF>
+__device__ __forceinline__ float low16(uint32_t w) { return BF ? __uint_as_float(w << 16) : h2f(w & 0xFFFF); }
+template <bool BF>
+__device__ __forceinline__ float high16(uint32_t w) { return BF ? __uint_as_float(w & 0xFFFF0000u) : h2f(w >> 16); }
 
 template <int HD, bool BF, bool CAP, int NB>
-__global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
-    constexpr int KT = FEW_KT, NLD = KT * HD / 8 / 64, ROWB = HDP<HD> * 2, KS = HD / 32, DB = HD / 16;
-    constexpr int VB = KT * ROWB, OB = 16 * NB * HD * 4;  // a wave's values, and its outputs at the end
+__global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(ServeAttnArgs a) {
+    using Lds = TileLds<HD>;
+    constexpr int KT = FEW_KT, RPI = Lds::RPI, NLD = KT / RPI, KS = HD / 32, DB = HD / 16;
+    constexpr int VB = NLD * Lds::V_BLOCK, OB = 16 * NB * HD * 4;  // a wave's values, and its outputs at the end
     constexpr int WB = VB > OB ? VB : OB;
     __shared__ __align__(16) uint8_t s_buf[4][WB];
     __shared__ float s_ml[4][16 * NB][2];
@@ -526,11 +591,11 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
     const SeqView sv = view_of(a.b, a.kv, si);
     const int n_rows = imin(sv.n_new * G, 16 * NB);
     if (n_rows == 0) return;
-    const int n_tok = (n_rows + G - 1) / G, pos0 = sv.len - sv.n_new;
+    const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.len - sv.n_new;
     const KeyRange kr = key_range(sv, 0, n_tok - 1, a.window);
-    const int t0 = first_tile(kr, FEW_STEP), nt = tile_count(kr, FEW_STEP), ns = split_count(nt, a.C, a.S), sp = blockIdx.y;
+    const int hi = same(kr.hi), t0 = same(first_tile(kr, FEW_STEP)), nt = same(tile_count(kr, FEW_STEP)), ns = same(split_count(nt, a.C, a.S)), sp = blockIdx.y;
     if (sp >= ns) return;
-    const int begin = (t0 + sp * a.C) * 4 + w, end = imin((sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * 4, (kr.hi + KT - 1) / KT);
+    const int begin = (t0 + sp * a.C) * 4 + w, end = imin((sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * 4, (hi + KT - 1) / KT);
 
     int p_q[NB], lo_q[NB];
     u32x4 qf[NB][KS];
@@ -546,38 +611,45 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
     }
     const int all_hi = pos0, all_lo = a.window > 0 ? pos0 + n_tok - 1 - a.window : -1;
 
-    const int *trow = a.kv.table ? a.kv.table + (int64_t)si * a.kv.table_stride : nullptr;
+    const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
     const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
-    uint8_t *sv_t = s_buf[w];
-    u32x4 rk[2][KS], rv[NLD];
-    int r_bad = 0;  // bit b: the tile's 16 positions b lie in a page that is none
-    auto load = [&](int t) {
-        r_bad = 0;
+    uint8_t *vt = s_buf[w];
+    const int k_row = (int)a.kv.k_row, v_row = (int)a.kv.v_row;
+    const int v_r = Lds::value_row(lane), v_c = imin(Lds::value_chunk(lane), HD / 8 - 1) * 16;
+    // Page ids of a tile's two groups of 16 positions (lanes 0 and 1), requested a tile ahead.
+    // Positions behind the last one seen are read as copies of it.
+    auto first_of = [&](int t, int b) { return imin(t * KT + b * 16, (hi - 1) & ~15); };
+    auto request_pages = [&](int t) { return t < end ? trow[first_of(t, lane & 1) >> a.kv.page_shift] : 0; };
+    struct Pages {
+        int id[2], bad;  // bad bit b: the page of group b is none (any that exists is read, and nobody sees it)
+    };
+    auto pages_of = [&](int ids) {
+        const bool ok = (unsigned)ids < (unsigned)a.kv.n_pages;
+        const int id = ok ? ids : 0;
+        Pages x;
+        x.bad = (int)(__ballot(!ok) & 3);
+        x.id[0] = __builtin_amdgcn_readlane(id, 0);
+        x.id[1] = __builtin_amdgcn_readlane(id, 1);
+        return x;
+    };
+    u32x4 rk[2][KS];
+    auto load_keys = [&](int t, const Pages &pg) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const int g0 = t * KT + b * 16;
-            const uint8_t *kp = kbase, *vp = vbase;
-            bool ok = true;
-            if (g0 < kr.hi) {
-                int page;
-                ok = page_of(a.kv, trow, g0, page);
-                const int slot = g0 & ((1 << a.kv.page_shift) - 1);
-                kp += page * a.kv.page + slot * a.kv.k_row;
-                vp += page * a.kv.page + slot * a.kv.v_row;
-            }
-            if (!ok) r_bad |= 1 << b;
-            const int n = ok ? kr.hi - g0 : 0;
+            const int g0 = first_of(t, b), slot = g0 & ((1 << a.kv.page_shift) - 1);
+            const uint8_t *kp = kbase + pg.id[b] * a.kv.page + slot * a.kv.k_row;
+            const int off = imin(col, hi - 1 - g0) * k_row + g * 16;
 #pragma unroll
-            for (int i = 0; i < KS; i++) {
-                rk[b][i] = u32x4{0, 0, 0, 0};
-                if (col < n) rk[b][i] = *(const u32x4 *)(kp + col * (int)a.kv.k_row + i * 64 + g * 16);
-            }
+            for (int i = 0; i < KS; i++) rk[b][i] = *(const u32x4 *)(kp + off + i * 64);
+        }
+    };
+    auto copy_values = [&](int t, const Pages &pg) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < NLD / 2; i++) {
-                const int r = (i * 64 + lane) / (HD / 8), ch = (i * 64 + lane) % (HD / 8);
-                rv[b * (NLD / 2) + i] = u32x4{0, 0, 0, 0};
-                if (r < n) rv[b * (NLD / 2) + i] = *(const u32x4 *)(vp + r * (int)a.kv.v_row + ch * 16);
-            }
+        for (int b = 0; b < 2; b++) {
+            const int g0 = first_of(t, b), slot = g0 & ((1 << a.kv.page_shift) - 1), last = hi - 1 - g0;
+            const uint8_t *vp = vbase + pg.id[b] * a.kv.page + slot * a.kv.v_row;
+#pragma unroll
+            for (int i = 0; i < NLD / 2; i++) copy_lds(vp, imin(i * RPI + v_r, last) * v_row + v_c, vt + (b * (NLD / 2) + i) * Lds::V_BLOCK);
         }
     };
 
@@ -591,13 +663,20 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
         for (int d = 0; d < DB; d++) o[b][d] = f32x4{};
     }
     const float c = CAP ? 1.0f : a.scale * LOG2E_F, cap_in = CAP ? 2.0f * LOG2E_F * a.scale / a.softcap : 0.0f, cap_out = CAP ? a.softcap * LOG2E_F : 0.0f;
-    const int vr = 4 * g + (col >> 2);
-    const int va = vr * ROWB + (lane & 1) * 8, vx = ((lane & 3) >> 1) ^ swz_v<HD>(vr);
+    const int v_at = Lds::value(4 * g + (col >> 2), (lane & 3) >> 1) + (lane & 1) * 8;
 
-    if (begin < end) load(begin);
+    Pages pg{};
+    int ids = 0;
+    if (begin < end) {
+        pg = pages_of(request_pages(begin));
+        load_keys(begin, pg);
+        copy_values(begin, pg);
+        ids = request_pages(begin + 4);
+    }
     for (int t = begin; t < end; t += 4) {
-        const int key0 = t * KT, bad = r_bad;
+        const int key0 = t * KT, bad = pg.bad;
         const bool part = key0 + KT - 1 > all_hi || key0 <= all_lo || bad;  // some row does not see all of the tile
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         f32x4 s[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -607,45 +686,44 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < KS; i++) s[b][kb] = mfma16<BF>(rk[kb][i], qf[b][i], s[b][kb]);
             }
-        bool nf = false;
-#pragma unroll
-        for (int i = 0; i < NLD; i++) {
-            const int r = i / (NLD / 2) * 16 + (i % (NLD / 2) * 64 + lane) / (HD / 8), ch = (i % (NLD / 2) * 64 + lane) % (HD / 8);
-            *(u32x4 *)(sv_t + r * ROWB + ((ch ^ swz_v<HD>(r)) << 4)) = rv[i];
-            if (part) nf = nf || nonfinite8<BF>(rv[i]);
+        if (t + 4 < end) {
+            pg = pages_of(ids);
+            load_keys(t + 4, pg);
+            ids = request_pages(t + 8);
         }
-        wave_sync();
-        if (t + 4 < end) load(t + 4);
-        if (part && __any(nf)) {  // rare
-            for (int r = 0; r < KT; r++) {
-                const int j = key0 + r;
-                const uint8_t *vp = sv_t + r * ROWB;
+        if (part) {
+            bool nf = false;
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const bool see = j <= p_q[b] && j > lo_q[b] && !(bad >> (r / 16) & 1);
-                    if (!__any(see)) continue;
+            for (int i = 0; i < NLD; i++) nf = nf || nonfinite8<BF>(*(const u32x4 *)(vt + i * Lds::V_BLOCK + lane * 16));
+            if (__any(nf)) {  // rare: added one by one for the rows that see them, then zeros
+                for (int r = 0; r < KT; r++) {
+                    const int j = key0 + r;
+                    const uint8_t *vp = vt + Lds::value(r, 0) + 8 * (g & 1);
 #pragma unroll
-                    for (int d = 0; d < DB; d++)
+                    for (int b = 0; b < NB; b++) {
+                        const bool see = j <= p_q[b] && j > lo_q[b] && !(bad >> (r / 16) & 1);
+                        if (!__any(see)) continue;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int dim = d * 16 + 4 * g + e;
-                            const float x = value16<BF>(*(const uint16_t *)(vp + (((dim >> 3) ^ swz_v<HD>(r)) << 4) + (dim & 7) * 2));
-                            if (see && !(fabsf(x) <= FLT_MAX)) o[b][d][e] += x;
-                        }
+                        for (int d = 0; d < DB; d++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {  // dim 16 d + 4 g + e
+                                const float x = value16<BF>(*(const uint16_t *)(vp + Lds::value(0, 2 * d) + (g >> 1) * 16 + e * 2));
+                                o[b][d][e] += (see & !(fabsf(x) <= FLT_MAX)) ? x : 0.0f;
+                            }
+                    }
                 }
-            }
-            wave_sync();
+                wave_sync();
 #pragma unroll
-            for (int i = 0; i < NLD; i++) {
-                const int r = i / (NLD / 2) * 16 + (i % (NLD / 2) * 64 + lane) / (HD / 8), ch = (i % (NLD / 2) * 64 + lane) % (HD / 8);
-                u32x4 *p = (u32x4 *)(sv_t + r * ROWB + ((ch ^ swz_v<HD>(r)) << 4));
-                u32x4 x = *p;
-                for (int e = 0; e < 4; e++) x[e] = finite2<BF>(x[e]);
-                *p = x;
+                for (int i = 0; i < NLD; i++) {
+                    u32x4 *p = (u32x4 *)(vt + i * Lds::V_BLOCK + lane * 16);
+                    u32x4 x = *p;
+                    for (int e = 0; e < 4; e++) x[e] = finite2<BF>(x[e]);
+                    *p = x;
+                }
+                wave_sync();
             }
-            wave_sync();
         }
-        u32x4 pf[NB];
+        u32x4 pf[NB][2];  // probabilities, and what their rounding left
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             float mx = -INFINITY;
@@ -656,7 +734,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
                     if constexpr (CAP) s[b][kb][e] = cap_score<CAP>(s[b][kb][e], cap_in, cap_out);
                     if (part) {
                         const int j = key0 + kb * 16 + 4 * g + e;
-                        if (j > p_q[b] || j <= lo_q[b] || (bad >> kb & 1)) s[b][kb][e] = -INFINITY;
+                        s[b][kb][e] = (j > p_q[b]) | (j <= lo_q[b]) | (bad >> kb & 1) ? -INFINITY : s[b][kb][e];
                     }
                     mx = fmaxf(mx, s[b][kb][e]);
                 }
@@ -674,27 +752,36 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
             const float ref = P_SHIFT<BF> - m[b];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                pf[b][e] = pack2<BF>(exp2_hw(fmaf(s[b][e / 2][2 * (e & 1)], c, ref)), exp2_hw(fmaf(s[b][e / 2][2 * (e & 1) + 1], c, ref)));
-                l[b] = add2<BF>(pf[b][e], l[b]);
+                const float p0 = exp2_hw(fmaf(s[b][e / 2][2 * (e & 1)], c, ref)), p1 = exp2_hw(fmaf(s[b][e / 2][2 * (e & 1) + 1], c, ref));
+                const uint32_t near = pack2<BF>(p0, p1);
+                pf[b][0][e] = near;
+                pf[b][1][e] = pack2<BF>(p0 - low16<BF>(near), p1 - high16<BF>(near));
+                l[b] += p0 + p1;
             }
         }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
-            const uint8_t *vp = sv_t + va + ((vx ^ (2 * d)) << 4);
-            const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + 16 * ROWB);
+            const uint8_t *vp = vt + v_at + Lds::value(0, 2 * d);
+            const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(16, 0));
+            const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
-            for (int b = 0; b < NB; b++) o[b][d] = mfma16<BF>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[b], o[b][d]);
+            for (int b = 0; b < NB; b++) {
+                o[b][d] = mfma16<BF>(vf, pf[b][1], o[b][d]);
+                o[b][d] = mfma16<BF>(vf, pf[b][0], o[b][d]);
+            }
         }
-        wave_sync();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values have been read: their place is free
+        if (t + 4 < end) copy_values(t + 4, pg);
     }
 
     // the four waves' results
+    wave_sync();
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         float x0, x1, y0, y1;
         pair_f<16>(l[b], x0, x1);
         pair_f<32>(x0 + x1, y0, y1);
-        float *po = (float *)sv_t + (b * 16 + col) * HD + 4 * g;
+        float *po = (float *)vt + (b * 16 + col) * HD + 4 * g;
 #pragma unroll
         for (int d = 0; d < DB; d++) *(f32x4 *)(po + d * 16) = o[b][d];
         if (g == 0) {
@@ -730,34 +817,82 @@ __global__ __launch_bounds__(256) void attn_few_kernel(ServeAttnArgs a) {
     }
 }
 
-// The splits of each (row, head), added up: a wave takes one, lane l the values l·HD/64 …
-// M rows per block and KT positions per tile are those of the kernel that made the partials.
-template <bool BF>
+// The splits of each (row, head), added up by W waves: HD / 4 lanes hold a split's values, and
+// the groups of so many lanes take the splits in turn.  W = 4 where there are few rows, whose
+// time is that of the loads behind one another, W = 1 (4 rows to a workgroup) where there are
+// many: one token over 100003 positions (32 heads, 61 splits) 19.9 us with a wave that read its
+// splits one by one.  M rows per block and KT positions per tile are those of the kernel that
+// made the partials.
+template <bool BF, int W>
 __global__ __launch_bounds__(256) void serve_combine_kernel(ServeAttnArgs a, int M, int KT) {
-    const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ float s_f[4][SERVE_MAX_SPLIT];
+    __shared__ f32x4 s_o[W == 1 ? 1 : 256];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = W == 1 ? blockIdx.x * 4 + w : blockIdx.x;
     const int row = id / a.n_head, head = id - row * a.n_head, G = a.G;
     if (row >= a.b.n_rows) return;
-    const int si = wave_find(a.b.starts, a.b.n_seq, row, [&](int s, int) { return iclamp(s, 0, a.b.n_rows); });
-    const SeqView sv = view_of(a.b, a.kv, si);
+    int si;
+    const SeqView sv = find_seq(a.b, a.kv, row, si, [&](int s, int) { return iclamp(s, 0, a.b.n_rows); });
     if (row < sv.row0 || row >= sv.row0 + sv.n_new) return;
     const int r = (row - sv.row0) * G + head % G, n_rows = sv.n_new * G, r0 = r / M * M, r1 = imin(r0 + M, n_rows) - 1;
     const int ns = split_count(tile_count(key_range(sv, r0 / G, r1 / G, a.window), KT), a.C, a.S);
     if (ns == 1) return;
     const int64_t at = ((int64_t)row * a.n_head + head) * a.S;
-    const f32x2 ml = lane < ns ? *(const f32x2 *)(a.ml + (at + lane) * 2) : f32x2{-FLT_MAX, 0};
-    const float mm = xmax_f<64>(ml[0]), f = exp2_hw(ml[0] - mm);
-    const float L = xsum_f<64>(lane < ns ? f * ml[1] : 0.0f);
+    const int lpr = a.hd / 4, per = 64 / lpr, g = lane / lpr, d = lane - g * lpr;  // lanes of a split, splits of a wave
+    // the first splits' values are requested before the maxima that weigh them are known
+    constexpr int FIRST = W == 1 ? 2 : 8;
+    const float *p = a.part + at * a.hd + d * 4;
+    const int s0 = g < per ? w % W * per + g : ns;
+    f32x4 x[FIRST];
+#pragma unroll
+    for (int k = 0; k < FIRST; k++) x[k] = s0 + k * W * per < ns ? *(const f32x4 *)(p + (int64_t)(s0 + k * W * per) * a.hd) : f32x4{};
+    float m0 = -FLT_MAX, l0 = 0, m1 = -FLT_MAX, l1 = 0;
+    if (lane < ns) {
+        m0 = a.ml[(at + lane) * 2];
+        l0 = a.ml[(at + lane) * 2 + 1];
+    }
+    if (lane + 64 < ns) {
+        m1 = a.ml[(at + lane + 64) * 2];
+        l1 = a.ml[(at + lane + 64) * 2 + 1];
+    }
+    const float mm = xmax_f<64>(fmaxf(m0, m1)), f0 = exp2_hw(m0 - mm), f1 = exp2_hw(m1 - mm);
+    const float L = xsum_f<64>(f0 * l0 + f1 * l1);
     const float inv = L > 0 || L != L ? 1.0f / L : 0.0f;
-    uint8_t *op = a.out + (int64_t)row * a.o_row + head * a.o_head;
-    for (int d = lane * 2; d < a.hd; d += 128) {
-        f32x2 acc = f32x2{};
-        for (int s = 0; s < ns; s++) {
-            const f32x2 x = *(const f32x2 *)(a.part + (at + s) * a.hd + d);
-            const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
-            acc[0] = fmaf(fs, x[0], acc[0]);
-            acc[1] = fmaf(fs, x[1], acc[1]);
+    s_f[w][lane] = f0 * inv;
+    s_f[w][lane + 64] = f1 * inv;
+    wave_sync();
+    f32x4 acc = f32x4{};
+#pragma unroll
+    for (int k = 0; k < FIRST; k++)
+        if (s0 + k * W * per < ns) {
+            const float f = s_f[w][s0 + k * W * per];
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] = fmaf(f, x[k][e], acc[e]);
         }
-        *(uint32_t *)(op + d * 2) = pack2<BF>(acc[0] * inv, acc[1] * inv);
+#pragma unroll 4
+    for (int s = s0 + FIRST * W * per; s < ns; s += W * per) {
+        const f32x4 y = *(const f32x4 *)(p + (int64_t)s * a.hd);
+        const float f = s_f[w][s];
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = fmaf(f, y[e], acc[e]);
+    }
+    if constexpr (W > 1) {
+        s_o[threadIdx.x] = acc;
+        __syncthreads();
+        if (w) return;
+        acc = f32x4{};
+        if (g == 0)
+            for (int i = 0; i < W; i++)
+                for (int k = 0; k < per; k++) acc += s_o[i * 64 + k * lpr + d];
+    } else {
+        f32x4 sum = acc;
+        for (int k = 1; k < per; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] += __shfl(acc[e], lane + k * lpr);
+        acc = sum;
+    }
+    if (g == 0) {
+        uint8_t *op = a.out + (int64_t)row * a.o_row + head * a.o_head;
+        *(u32x2 *)(op + d * 8) = u32x2{pack2<BF>(acc[0], acc[1]), pack2<BF>(acc[2], acc[3])};
     }
 }
 
@@ -766,8 +901,8 @@ template <int SRC, bool BF>  // SRC: bytes of a source value
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= a.b.n_rows) return;
-    const int si = wave_find(a.b.starts, a.b.n_seq, row, [&](int s, int) { return iclamp(s, 0, a.b.n_rows); });
-    const SeqView sv = view_of(a.b, a.kv, si);
+    int si;
+    const SeqView sv = find_seq(a.b, a.kv, row, si, [&](int s, int) { return iclamp(s, 0, a.b.n_rows); });
     if (row < sv.row0 || row >= sv.row0 + sv.n_new) return;
     const int pos = sv.len - sv.n_new + row - sv.row0;
     int page;
@@ -803,7 +938,7 @@ void launch_hd(const ServeAttnArgs &a, hipStream_t st) {
             else attn_few_kernel<HD, BF, false, 2><<<grid, 256, 0, st>>>(a);
         }
     } else {
-        const dim3 grid(a.n_blocks * a.n_kv, a.S);
+        const int grid = a.n_blocks * a.n_kv * a.S;
         if (cap) attn_tile_kernel<HD, BF, true><<<grid, 256, 0, st>>>(a);
         else attn_tile_kernel<HD, BF, false><<<grid, 256, 0, st>>>(a);
     }
@@ -822,6 +957,9 @@ void launch_ty(const ServeAttnArgs &a, hipStream_t st) {
 
 int tile_kt(int hd) { return hd <= 128 ? TILE_KT<128> : TILE_KT<256>; }
 
+// (row, head) pairs up to which the splits are added up by four waves each
+constexpr int COMBINE_FEW = 2048;
+
 }  // namespace
 
 bool serve_attn_head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
@@ -836,7 +974,16 @@ SplitPlan serve_attn_splits(const ServeAttnArgs &a) {
     int64_t span = a.b.max_len;
     if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? 32 : TILE_M / a.G + 1) + KT);
     const int tiles = (int)((span + KT - 1) / KT);
-    return few ? split_plan(blocks * a.n_kv, tiles, 1024, 1, SERVE_MAX_SPLIT) : split_plan(blocks * a.n_kv, tiles, 512, 4, SERVE_MAX_SPLIT);
+    // Few rows: 4096 workgroups where there is so much, since sequences differ in length, and at
+    // least 256 positions each (48 tokens over up to 4000 positions, 8 KV heads: 85.9 us at 1024
+    // workgroups, 75.0 at 2048, 73.2 at 4096, 74.3 at 8192); a cache of under 512 positions is
+    // not split, a second launch being longer than its loads.
+    if (few) return split_plan(blocks * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
+    // Tiles: 2 us each with every slot taken (64 positions of 128 values), partials at 4.5 TB/s.
+    // Chunks in a batch of 13 (488 workgroups): 208 us in one, 202 to 248 in 2 to 5 splits;
+    // window prompts with 256-wide heads (123) 31.5 in one, 47.7 in 4; one long prompt is split.
+    const double part_us = (double)a.b.n_rows * a.n_head * a.hd * 8 / 4.5e6;
+    return tile_plan(blocks * a.n_kv, a.hd <= 128 ? 512 : 256, tiles, 2.0 * KT * a.hd / (64 * 128), part_us, SERVE_MAX_SPLIT);
 }
 
 size_t serve_attn_ws(const ServeAttnArgs &a) {
@@ -856,9 +1003,15 @@ void launch_serve_attn(ServeAttnArgs a, void *ws, hipStream_t st) {
     if (bf) launch_ty<true>(a, st);
     else launch_ty<false>(a, st);
     if (p.S > 1) {
-        const int M = few ? 32 : TILE_M, KT = few ? FEW_STEP : tile_kt(a.hd), grid = (int)(((int64_t)a.b.n_rows * a.n_head + 3) / 4);
-        if (bf) serve_combine_kernel<true><<<grid, 256, 0, st>>>(a, M, KT);
-        else serve_combine_kernel<false><<<grid, 256, 0, st>>>(a, M, KT);
+        const int M = few ? 32 : TILE_M, KT = few ? FEW_STEP : tile_kt(a.hd);
+        const int64_t n = (int64_t)a.b.n_rows * a.n_head;
+        if (n <= COMBINE_FEW) {
+            if (bf) serve_combine_kernel<true, 4><<<n, 256, 0, st>>>(a, M, KT);
+            else serve_combine_kernel<false, 4><<<n, 256, 0, st>>>(a, M, KT);
+        } else {
+            if (bf) serve_combine_kernel<true, 1><<<(n + 3) / 4, 256, 0, st>>>(a, M, KT);
+            else serve_combine_kernel<false, 1><<<(n + 3) / 4, 256, 0, st>>>(a, M, KT);
+        }
     }
 }
 

@@ -36,7 +36,7 @@ struct ServeAttnArgs {
     int C = 0, S = 1;                      // split_plan
     int n_blocks = 0;                      // blocks of query rows (tile kernel)
 };
-constexpr int SERVE_MAX_SPLIT = 64;
+constexpr int SERVE_MAX_SPLIT = 128;
 // whether the few-rows kernel takes the launch (else the tile kernel), and its splits
 bool serve_attn_few(const ServeAttnArgs &a);
 SplitPlan serve_attn_splits(const ServeAttnArgs &a);

@@ -79,4 +79,23 @@ inline SplitPlan split_plan(int64_t wgs, int tiles, int want, int least, int mos
     return p;
 }
 
+// The same for blocks whose time is arithmetic: the number of splits with the least time by
+// this estimate, in µs.  wgs workgroups without splits, slots of them at a time; tiles of the
+// longest block, tile_us each; a second launch and the partials' way to memory and back
+// (part_us per split) where there is more than one.
+inline SplitPlan tile_plan(int64_t wgs, int slots, int tiles, double tile_us, double part_us, int most) {
+    SplitPlan best{tiles > 0 ? tiles : 1, 1};
+    double least = 0;
+    for (int s = 1; s <= most && s <= tiles; s++) {
+        const int C = (tiles + s - 1) / s;
+        if (s > 1 && (tiles + C - 1) / C != s) continue;
+        const double full = (double)wgs * s / slots, us = (full > 1 ? full : 1) * C * tile_us + (s > 1 ? 6 + s * part_us : 0);
+        if (s == 1 || us < least) {
+            least = us;
+            best = SplitPlan{C, s};
+        }
+    }
+    return best;
+}
+
 }  // namespace rie
