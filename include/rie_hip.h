@@ -90,6 +90,16 @@ size_t rie_hip_weight_bytes(const rie_hip_backend *b);
 /* forward(tokens, pos) then argmax of the last logits row; returns 0 and *next. */
 int32_t rie_hip_forward_argmax(rie_hip_backend *b, const uint32_t *tokens, size_t n, size_t pos, uint32_t *next, char *err,
                                size_t err_len);
+/* forward(tokens, pos), then of every token's logits on the device (no logits readback):
+ * logprob[i] = ln p(targets[i]) (NaN for a target that is no token), the entropy in nats,
+ * and the n_top (0..64) most likely tokens in order, the lowest id first among equals, with
+ * their log probabilities ([n][n_top]); rie_hip_k_token_logprobs has the rules.  For scoring
+ * (Engine::perplexity, engine.rs:567-602) and a server's logprobs.  targets with logprob,
+ * entropy, and (n_top = 0) top_ids with top_logprobs may be NULL.  Errors: forward's, and
+ * RUNTIME for an n_top or a combination of NULLs outside these. */
+int32_t rie_hip_forward_logprobs(rie_hip_backend *b, const uint32_t *tokens, size_t n, size_t pos, const uint32_t *targets,
+                                 size_t n_top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprobs, char *err,
+                                 size_t err_len);
 /* n_gen greedy steps continuing from the token chosen by the previous
  * forward_argmax/generate call, at positions pos, pos+1, ...; out[i] receives the
  * token fed at step i. */

@@ -77,6 +77,7 @@ def lib():
         "rie_hip_forward": (I, [P, P, S, S, I, P, S, CP, S]),
         "rie_hip_hidden": (P, [P, C.POINTER(S)]),
         "rie_hip_forward_argmax": (I, [P, P, S, S, C.POINTER(C.c_uint32), CP, S]),
+        "rie_hip_forward_logprobs": (I, [P, P, S, S, P, S, P, P, P, P, CP, S]),
         "rie_hip_generate_greedy": (I, [P, S, S, P, CP, S]),
         "rie_hip_bench": (I, [P, S, S, C.POINTER(D), C.POINTER(D), CP, S]),
         "rie_hip_synth_tiny": (I, [CP, I, C.POINTER(SynthSpec)]),

@@ -121,6 +121,25 @@ class HipBackend:
         _check(rc, err)
         return nxt.value
 
+    def forward_logprobs(self, tokens, pos: int, targets=None, n_top: int = 0):
+        """forward(tokens, pos), and of every token's logits, on the device: (log probabilities of
+        ``targets`` or None, entropies in nats, ids [n, n_top] and log probabilities [n, n_top] of
+        the most likely tokens)"""
+        toks = _u32(tokens)
+        n = toks.size
+        want = None if targets is None else _u32(targets)
+        if want is not None and want.size != n:
+            raise RieError(-5, f"{want.size} targets for {n} tokens")
+        if not 0 <= n_top <= 64:
+            raise RieError(-5, "n_top has to lie in 0..64")
+        lp = None if want is None else np.empty(n, np.float32)
+        h = np.empty(n, np.float32)
+        ids, tops = np.empty((n, n_top), np.uint32), np.empty((n, n_top), np.float32)
+        at = lambda a: None if a is None or not a.size else a.ctypes.data  # noqa: E731
+        err = C.create_string_buffer(1024)
+        _check(_lib.lib().rie_hip_forward_logprobs(self._h, at(toks), n, pos, at(want), n_top, at(lp), at(h), at(ids), at(tops), err, 1024), err)
+        return lp, h, ids, tops
+
     def generate_greedy(self, pos: int, n_gen: int) -> np.ndarray:
         out = np.zeros(max(n_gen, 1), np.uint32)
         err = C.create_string_buffer(1024)

@@ -6,6 +6,7 @@
 // once in a HIP graph whose only per-step inputs live in device memory
 // ({pos} and the token id), so greedy decoding never returns to the host.
 #include "backend.hpp"
+#include "../serve.hpp"
 
 #include "../kernels.hpp"
 
@@ -853,16 +854,15 @@ bool HipBackend::moe_grouped_ok(const DevLayer &L) const {
     return L.gate.ty == L.up.ty && gemm_supported(gt, E) && gemm_supported(L.down.ty, ff) && d_moe_off_ != nullptr;
 }
 
-void HipBackend::forward(const uint32_t *tokens, size_t n, size_t pos, bool all_logits, float *logits, size_t logits_len) {
-    const ModelConfig &c = m_.cfg;
-    hidden_rows_ = 0;
+void HipBackend::check_batch(const uint32_t *tokens, size_t n, size_t pos) const {
     if (n == 0) throw rt_err("empty batch");
     if (n > max_batch_) throw rt_err("batch of " + std::to_string(n) + " tokens exceeds max batch " + std::to_string(max_batch_));
     if (pos + n > n_ctx_) throw rt_err("context window full (" + std::to_string(n_ctx_) + " tokens)");
     for (size_t t = 0; t < n; t++)
         if (tokens[t] >= m_.token_embd.rows) throw rt_err("token id " + std::to_string(tokens[t]) + " out of range");
-    const size_t m = all_logits ? n : 1;
-    if (logits_len < m * c.n_vocab) throw rt_err("logits buffer too small");
+}
+
+void HipBackend::eval(const uint32_t *tokens, size_t n, size_t pos, bool all_logits) {
     RIE_HIP_CHECK(hipSetDevice(device_));
     launch_set_tokens(d_tokens_, tokens, n, d_pos_, (int)pos, st_);
     if (n == 1 && use_graph_ && !capture_) {
@@ -870,6 +870,15 @@ void HipBackend::forward(const uint32_t *tokens, size_t n, size_t pos, bool all_
     } else {
         run_layers((int)n, pos, nullptr, all_logits, splits_for(n, pos));
     }
+}
+
+void HipBackend::forward(const uint32_t *tokens, size_t n, size_t pos, bool all_logits, float *logits, size_t logits_len) {
+    const ModelConfig &c = m_.cfg;
+    hidden_rows_ = 0;
+    check_batch(tokens, n, pos);
+    const size_t m = all_logits ? n : 1;
+    if (logits_len < m * c.n_vocab) throw rt_err("logits buffer too small");
+    eval(tokens, n, pos, all_logits);
     if (m * c.n_vocab <= h_out_cap_) {
         launch_copy_out(d_logits_, h_out_, m * c.n_vocab, d_out_cnt_, h_flag_, ++out_seq_, st_);
         check_launch("logits");
@@ -997,18 +1006,8 @@ const float *HipBackend::hidden(size_t *rows) {
 uint32_t HipBackend::forward_argmax(const uint32_t *tokens, size_t n, size_t pos) {
     const ModelConfig &c = m_.cfg;
     hidden_rows_ = 0;
-    if (n == 0) throw rt_err("empty batch");
-    if (n > max_batch_) throw rt_err("batch of " + std::to_string(n) + " tokens exceeds max batch " + std::to_string(max_batch_));
-    if (pos + n > n_ctx_) throw rt_err("context window full (" + std::to_string(n_ctx_) + " tokens)");
-    for (size_t t = 0; t < n; t++)
-        if (tokens[t] >= m_.token_embd.rows) throw rt_err("token id " + std::to_string(tokens[t]) + " out of range");
-    RIE_HIP_CHECK(hipSetDevice(device_));
-    launch_set_tokens(d_tokens_, tokens, n, d_pos_, (int)pos, st_);
-    if (n == 1 && use_graph_ && !capture_) {
-        decode_step_graph(pos);
-    } else {
-        run_layers((int)n, pos, nullptr, false, splits_for(n, pos));
-    }
+    check_batch(tokens, n, pos);
+    eval(tokens, n, pos, false);
     launch_argmax(d_logits_, (int)c.n_vocab, d_amax_idx_, d_amax_val_, n_amax_part_, d_tokens_, st_, d_amax_cnt_);
     check_launch("argmax");
     uint32_t tok = 0;
@@ -1016,6 +1015,55 @@ uint32_t HipBackend::forward_argmax(const uint32_t *tokens, size_t n, size_t pos
     RIE_HIP_CHECK(hipStreamSynchronize(st_));
     hidden_rows_ = 1;
     return tok;
+}
+
+void HipBackend::forward_logprobs(const uint32_t *tokens, size_t n, size_t pos, const uint32_t *targets, size_t n_top, float *logprob,
+                                  float *entropy, uint32_t *top_ids, float *top_logprobs) {
+    const ModelConfig &c = m_.cfg;
+    hidden_rows_ = 0;
+    if (n && !tokens) throw rt_err("tokens is NULL");
+    check_batch(tokens, n, pos);
+    if (n_top > LOGPROB_MAX_TOP || n_top > c.n_vocab) throw rt_err("n_top has to lie in 0..64 and not pass the vocabulary");
+    if (!targets != !logprob) throw rt_err("targets and logprob have to be given together");
+    if (n_top && (!top_ids || !top_logprobs)) throw rt_err("top_ids or top_logprobs is NULL");
+    if (c.n_vocab > (size_t)LOGPROB_MAX_V) throw rt_err("vocabulary of " + std::to_string(c.n_vocab) + " tokens, 2^21 at most");
+    RIE_HIP_CHECK(hipSetDevice(device_));
+    if (!d_lp_ws_) {
+        d_lp_in_ = dalloc<uint32_t>(allocs_, max_batch_ * (3 + 2 * LOGPROB_MAX_TOP));
+        d_lp_ws_ = dalloc<uint8_t>(allocs_, logprobs_ws((int)max_batch_, (int)c.n_vocab));
+    }
+    eval(tokens, n, pos, true);
+    // results one behind the other, so that one copy returns them
+    uint32_t *res = d_lp_in_ + max_batch_;
+    LogprobArgs a;
+    a.x = d_logits_;
+    a.ty = T_F32;
+    a.n = (int)n;
+    a.V = (int)c.n_vocab;
+    a.ld = (int64_t)c.n_vocab;
+    a.entropy = (float *)res;
+    a.n_top = (int)n_top;
+    a.top_ids = (int *)res + n;
+    a.top_logprobs = (float *)res + n * (1 + n_top);
+    size_t got = n * (1 + 2 * n_top);
+    if (targets) {
+        launch_set_tokens(d_lp_in_, targets, n, nullptr, 0, st_);
+        a.targets = (const int *)d_lp_in_;
+        a.logprob = (float *)res + got;
+        got += n;
+    }
+    launch_logprobs(a, d_lp_ws_, st_);
+    check_launch("logprobs");
+    std::vector<uint32_t> host(got);
+    RIE_HIP_CHECK(hipMemcpyAsync(host.data(), res, got * 4, hipMemcpyDeviceToHost, st_));
+    RIE_HIP_CHECK(hipStreamSynchronize(st_));
+    if (entropy) std::memcpy(entropy, host.data(), n * 4);
+    if (n_top) {
+        std::memcpy(top_ids, host.data() + n, n * n_top * 4);
+        std::memcpy(top_logprobs, host.data() + n * (1 + n_top), n * n_top * 4);
+    }
+    if (targets) std::memcpy(logprob, host.data() + n * (1 + 2 * n_top), n * 4);
+    hidden_rows_ = n;
 }
 
 // greedy steps without host round trips: each step's argmax is written to

@@ -43,6 +43,10 @@ class HipBackend {
 
     // Engine-side greedy decoding on the device (sampler.rs::argmax, first max).
     uint32_t forward_argmax(const uint32_t *tokens, size_t n, size_t pos);
+    // forward of all rows, and their log probabilities on the device (launch_logprobs): of
+    // targets, the entropies and the n_top most likely tokens; any output may be nullptr
+    void forward_logprobs(const uint32_t *tokens, size_t n, size_t pos, const uint32_t *targets, size_t n_top, float *logprob,
+                          float *entropy, uint32_t *top_ids, float *top_logprobs);
     // n_gen greedy steps: feeds the last argmax token at pos, pos+1, ...; writes the
     // fed tokens to out (out[0] = the token chosen by the previous forward).
     void generate_greedy(size_t pos, size_t n_gen, uint32_t *out);
@@ -98,6 +102,8 @@ class HipBackend {
     void expert_ffn(const DevWeight &g, const DevWeight &u, const DevWeight &dn, const float *x, int m, float *y);
     void head(int first, int m);
     void check_launch(const char *what);
+    void check_batch(const uint32_t *tokens, size_t n, size_t pos) const;  // forward's errors
+    void eval(const uint32_t *tokens, size_t n, size_t pos, bool all_logits);  // logits to d_logits_
     void decode_step_graph(size_t pos);
     void greedy_step_graph(size_t pos);
     // context ranges per (token, kv head) in attention; the same for every batch size so
@@ -135,6 +141,8 @@ class HipBackend {
     uint32_t out_seq_ = 0;
     void wait_out();
     int *d_amax_idx_ = nullptr, *d_amax_cnt_ = nullptr;
+    void *d_lp_ws_ = nullptr;      // log probabilities: workspace for max_batch rows, made by the first call
+    uint32_t *d_lp_in_ = nullptr;  // their targets, behind them the results
     int *d_attn_cnt_ = nullptr;  // per-KV-head arrival counters of the fused single-token attention
     int *d_out_cnt_ = nullptr;   // arrival counter of the logits' copy to the host
     int *d_route_cnt_ = nullptr;  // arrival counter of the router GEMV that routes one token

@@ -108,6 +108,12 @@ int32_t rie_hip_forward_argmax(rie_hip_backend *b, const uint32_t *tokens, size_
     });
 }
 
+int32_t rie_hip_forward_logprobs(rie_hip_backend *b, const uint32_t *tokens, size_t n, size_t pos, const uint32_t *targets,
+                                 size_t n_top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprobs, char *err,
+                                 size_t err_len) {
+    return guarded(err, err_len, [&] { b->b->forward_logprobs(tokens, n, pos, targets, n_top, logprob, entropy, top_ids, top_logprobs); });
+}
+
 int32_t rie_hip_generate_greedy(rie_hip_backend *b, size_t pos, size_t n_gen, uint32_t *out, char *err, size_t err_len) {
     return guarded(err, err_len, [&] { b->b->generate_greedy(pos, n_gen, out); });
 }

@@ -1,7 +1,7 @@
 """Engine-level loops over a Backend, mirroring crates/rie-core/src/engine.rs:
 prefix-reusing ``eval_tokens`` (250-272), ``shift_context`` (363-381),
 ``eval_next`` (384-392), the greedy path of ``generate`` (420-530), ``bench``
-(540-564) and greedy argmax (sampler.rs:199-209)."""
+(540-564), ``perplexity`` (567-602) and greedy argmax (sampler.rs:199-209)."""
 from __future__ import annotations
 
 import time
@@ -97,6 +97,36 @@ class Engine:
             raise RieError(-5, "context window full")
         self.backend.forward([token], pos, False, self._logits)
         self.cached.append(int(token))
+
+    def score(self, tokens) -> np.ndarray:
+        """ln p of every token but the first, given the ones before it, from an empty cache.  Where the backend forms log
+        probabilities on its device no logits are read back."""
+        tokens = [int(t) for t in tokens]
+        if len(tokens) > self.backend.n_ctx():
+            raise RieError(-5, f"text of {len(tokens)} tokens exceeds context window of {self.backend.n_ctx()}")
+        self.reset()
+        out, nb, n = [], self.backend.max_batch(), len(tokens) - 1
+        for pos in range(0, n, nb):
+            end = min(pos + nb, n)
+            if hasattr(self.backend, "forward_logprobs"):
+                out.append(self.backend.forward_logprobs(tokens[pos:end], pos, tokens[pos + 1:end + 1])[0].astype(np.float64))
+            else:
+                x = np.asarray(self.backend.forward(tokens[pos:end], pos, True), np.float64).reshape(end - pos, -1)
+                m = x.max(1, keepdims=True)
+                lse = m[:, 0] + np.log(np.exp(x - m).sum(1))
+                out.append(x[np.arange(end - pos), tokens[pos + 1:end + 1]] - lse)
+            self.cached.extend(tokens[pos:end])
+        return np.concatenate(out) if out else np.zeros(0)
+
+    def perplexity(self, tokens) -> float:
+        """exp of the mean of −ln p over the tokens that have one before them (Engine::perplexity, engine.rs:567-602): the
+        text is cut into windows of n_ctx tokens, each scored from an empty cache."""
+        tokens, n = [int(t) for t in tokens], self.backend.n_ctx()
+        lp = [self.score(tokens[i:i + n]) for i in range(0, len(tokens), n)]
+        lp = np.concatenate(lp) if lp else np.zeros(0)
+        if not lp.size:
+            raise RieError(-5, "perplexity needs at least two tokens")
+        return float(np.exp(-lp.mean()))
 
     def bench(self, n_prompt: int, n_gen: int):
         """Engine::bench with host-side argmax over read-back logits."""
