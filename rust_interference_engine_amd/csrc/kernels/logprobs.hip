@@ -109,7 +109,18 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
     if (row >= a.n) return;
     const void *x = (const uint8_t *)a.x + row * a.ld * (TY == T_F32 ? 4 : 2);
     const int off = misplaced<TY>(x), g0 = part * per, g1 = min(g0 + per, n_groups);
-    float M = -FLT_MAX, s = 0, t = 0, cnt = 0;  // M is the wave's; s, t and cnt are the lane's
+    // M is the wave's maximum so far; s, t and cnt are the lane's.  fs and ft are the same sums of
+    // the groups that hold no element equal to M, in log2 units against the reference −c, where
+    // c = −M · log2 e rounded: one fma forms an exponent, and the rounding of c, r = M · log2 e + c
+    // exactly, is taken out of the sums when M moves or at the end (they hold 2^r times theirs).
+    float M = -FLT_MAX, s = 0, t = 0, cnt = 0, fs = 0, ft = 0, c = 0;
+    bool plain = true;  // no fast form for this M: its product leaves the range of f32
+    auto settle = [&] {
+        const float r = plain ? 0.0f : fmaf(M, LOG2E_F, c), f = exp2_hw(-r);
+        s = fmaf(fs, f, s);
+        t = fmaf(LN2_F * f, ft - r * fs, t);
+        fs = ft = 0;
+    };
     float v[R], nx[R];
     load_group<TY>(x, g0 * GROUP - off, a.V, lane, v);
     for (int g = g0; g < g1; g++) {
@@ -121,14 +132,32 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
         mx = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(xmax_f<64>(mx))));
         mx = mx == mx ? mx : -INFINITY;  // nothing but NaN
         if (lane == 0) gmax[(int64_t)row * n_groups + g] = mx;
-        if (mx >= M) {
-            if (mx > M) {
-                const float d = fmaxf(M - mx, D_MIN), f = exp2_hw(d * LOG2E_F);
-                t = f * (t + (s + cnt) * d);
-                s = f * (s + cnt);
-                cnt = 0;
-                M = mx;
+        bool slow = mx >= M || plain;
+        if (mx > M) {
+            settle();
+            const float d = fmaxf(M - mx, D_MIN), f = exp2_hw(d * LOG2E_F);
+            t = f * (t + (s + cnt) * d);
+            s = f * (s + cnt);
+            cnt = 0;
+            M = mx;
+            plain = !(fabsf(M) < 1e30f);
+            c = plain ? 0.0f : -(M * LOG2E_F);
+        }
+        if (!slow) {
+            float gs = 0, gt = 0;
+#pragma unroll
+            for (int j = 0; j < R; j++) {
+                const float d = fmaf(v[j], LOG2E_F, c), e = exp2_hw(d);
+                gs += e;
+                gt = fmaf(e, d, gt);
             }
+            slow = __any(gt != gt);  // a −inf (0 · −inf) or a NaN: the other form
+            if (!slow) {
+                fs += gs;
+                ft += gt;
+            }
+        }
+        if (slow) {
 #pragma unroll
             for (int j = 0; j < R; j++) {
                 const bool eq = v[j] == M;
@@ -137,17 +166,11 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
                 s += e;
                 t = fmaf(e, eq ? 0.0f : fmaxf(d, D_MIN), t);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < R; j++) {
-                const float d = v[j] - M, e = exp2_hw(d * LOG2E_F);
-                s += e;
-                t = fmaf(e, fmaxf(d, D_MIN), t);
-            }
         }
 #pragma unroll
         for (int j = 0; j < R; j++) v[j] = nx[j];
     }
+    settle();
     s = xsum_f<64>(s);
     t = xsum_f<64>(t);
     cnt = xsum_f<64>(cnt);
@@ -170,13 +193,61 @@ __global__ __launch_bounds__(256) void logprob_row_kernel(LogprobArgs a, int n_g
     const int target = a.targets ? a.targets[row] : -1;
     const float xt = target >= 0 && target < a.V ? logit<TY>(x, target) : 0.0f;
 
+    // The k groups with the largest maxima: the first wave takes them out one by one, the lowest
+    // group among equals, a lane holding every 64th group's maximum in registers (in LDS beyond
+    // 512 groups).  The other waves join the runs meanwhile.
+    const int k = a.n_top, kg = min(k, n_groups);
+    if (w == 0 && k) {
+        constexpr int NREG = 8;
+        const bool many = n_groups > 64 * NREG;
+        const float *gm = gmax + (int64_t)row * n_groups;
+        float own[NREG], best = -INFINITY;
+        int at = INT32_MAX;
+#pragma unroll
+        for (int i = 0; i < NREG; i++) own[i] = lane + 64 * i < n_groups ? gm[lane + 64 * i] : NAN;
+        if (many)
+            for (int i = lane; i < n_groups; i += 64) s_gmax[i] = gm[i];
+        auto look = [&] {  // NaN (taken, or no group) compares with nothing
+            best = -INFINITY;
+            at = INT32_MAX;
+            if (!many) {
+#pragma unroll
+                for (int i = 0; i < NREG; i++) {
+                    const bool better = own[i] > best || (at == INT32_MAX && own[i] == best);
+                    best = better ? own[i] : best;
+                    at = better ? lane + 64 * i : at;
+                }
+            } else {
+                for (int i = lane; i < n_groups; i += 64) {
+                    const float v = s_gmax[i];
+                    if (v > best || (at == INT32_MAX && v == best)) {
+                        best = v;
+                        at = i;
+                    }
+                }
+            }
+        };
+        look();
+        float thr = -INFINITY;
+        for (int r = 0; r < kg; r++) {
+            thr = xmax_f<64>(best);
+            const int first = xreduce<64>(best == thr ? at : INT32_MAX, [](int x, int y) { return x < y ? x : y; });
+            if (lane == 0) s_group[r] = first;
+            if (at == first) {
+                if (many) s_gmax[at] = NAN;
+#pragma unroll
+                for (int i = 0; i < NREG; i++) own[i] = at == lane + 64 * i ? NAN : own[i];
+                look();
+            }
+        }
+        if (lane == 0) s_thr = n_groups < k ? -INFINITY : thr;
+    }
     Part p{-FLT_MAX, 0, 0, 0};
-    for (int i = tid; i < n_parts; i += 256) p = join(p, parts[(int64_t)row * n_parts + i]);
+    const int first = k ? 64 : 0;  // thread that joins the first run
+    for (int i = tid - first; i >= 0 && i < n_parts; i += 256 - first) p = join(p, parts[(int64_t)row * n_parts + i]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) p = join(p, Part{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.c, o), __shfl_xor(p.t, o)});
     if (lane == 0) s_part[w] = p;
-    if (a.n_top)
-        for (int i = tid; i < n_groups; i += 256) s_gmax[i] = gmax[(int64_t)row * n_groups + i];
     if (tid == 0) s_n = 0;
     __syncthreads();
     p = join(join(s_part[0], s_part[1]), join(s_part[2], s_part[3]));
@@ -186,58 +257,30 @@ __global__ __launch_bounds__(256) void logprob_row_kernel(LogprobArgs a, int n_g
         if (a.entropy) a.entropy[row] = log_s - p.t / (p.c + p.s);
         if (a.logprob) a.logprob[row] = target >= 0 && target < a.V ? xt - p.m - log_s : NAN;
     }
-    const int k = a.n_top;
     if (!k) return;
 
-    // The k groups with the largest maxima: the first wave takes them out one by one, a lane
-    // holding the maxima of every 64th group in LDS and the best of them (the lowest group among
-    // equals) in registers.
-    const int kg = min(k, n_groups);
-    if (w == 0) {
-        float best = -INFINITY;
-        int at = INT32_MAX;
-        auto look = [&] {
-            best = -INFINITY;
-            at = INT32_MAX;
-#pragma unroll 4
-            for (int i = lane; i < n_groups; i += 64) {
-                const float v = s_gmax[i];
-                if (v > best || (at == INT32_MAX && v == best)) {
-                    best = v;
-                    at = i;
-                }
-            }
-        };
-        look();
-        float thr = -INFINITY;
-        for (int r = 0; r < kg; r++) {
-            // at < INT32_MAX with the largest best: −inf is a value like others here
-            const float top = xmax_f<64>(at == INT32_MAX ? -INFINITY : best);
-            const int first = xreduce<64>(best == top ? at : INT32_MAX, [](int x, int y) { return x < y ? x : y; });
-            if (lane == 0) s_group[r] = first;
-            thr = top;
-            if (at == first) {
-                s_gmax[at] = NAN;  // compares with nothing
-                look();
-            }
-        }
-        if (lane == 0) s_thr = n_groups < k ? -INFINITY : thr;
-    }
-    __syncthreads();
     // their logits that may be among the first k
     const float thr = s_thr;
+    const bool all = thr == -INFINITY;
     const int off = misplaced<TY>(x);
-    for (int i = w; i < kg; i += 4) {
-        const int e0 = s_group[i] * GROUP - off;
-        float v[R];
-        load_group<TY>(x, e0, a.V, lane, v);
+    constexpr int AT_ONCE = 3;  // groups that a wave reads at once
+    for (int i0 = w; i0 < kg; i0 += 4 * AT_ONCE) {
+        float v[AT_ONCE][R];
 #pragma unroll
-        for (int j = 0; j < R; j++) {
-            const int e = e0 + place<TY>(lane, j);
-            if (e >= 0 && e < a.V && (v[j] >= thr || (v[j] != v[j] && thr == -INFINITY))) {
+        for (int u = 0; u < AT_ONCE; u++)
+            if (i0 + 4 * u < kg) load_group<TY>(x, s_group[i0 + 4 * u] * GROUP - off, a.V, lane, v[u]);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            if (i0 + 4 * u >= kg) break;
+            const int e0 = s_group[i0 + 4 * u] * GROUP - off;
+#pragma unroll
+            for (int j = 0; j < R; j++) {
+                if (!(v[u][j] >= thr) && !(all && v[u][j] != v[u][j])) continue;
+                const int e = e0 + place<TY>(lane, j);
+                if (all && (e < 0 || e >= a.V)) continue;  // the −inf behind the row's ends
                 const int c = atomicAdd(&s_n, 1);
                 if (c < CAND) {
-                    s_val[c] = v[j] != v[j] ? -INFINITY : v[j];
+                    s_val[c] = v[u][j] == v[u][j] ? v[u][j] : -INFINITY;
                     s_idx[c] = e;
                 }
             }
@@ -318,7 +361,7 @@ void launch_logprobs(const LogprobArgs &a, void *ws, hipStream_t st) {
     Part *parts = (Part *)ws;
     float *gmax = (float *)(parts + (size_t)a.n * np);
     const int grid = (int)(((int64_t)a.n * np + 3) / 4);
-    const size_t lds = a.n_top ? ng * sizeof(float) : 0;
+    const size_t lds = a.n_top && ng > 512 ? ng * sizeof(float) : 0;
     if (a.ty == T_F32) {
         logprob_part_kernel<T_F32><<<grid, 256, 0, st>>>(a, ng, per, np, gmax, parts);
         logprob_row_kernel<T_F32><<<a.n, 256, lds, st>>>(a, ng, np, gmax, parts);

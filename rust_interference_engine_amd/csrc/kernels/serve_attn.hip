@@ -95,11 +95,15 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
     return w;
 }
 
+// Addresses in LDS as numbers: sums with constants become the instructions' offsets, where
+// generic pointers took a register for every one (70 of them in the tile kernel).
+__device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)p; }
+__device__ __forceinline__ u32x4 lds_16(uint32_t at) { return *(__attribute__((address_space(3))) const u32x4 *)(uintptr_t)at; }
 // 4 values of one column: lane l of a group of 16 lanes names the 8 bytes of row l / 4 that
 // hold columns 4·(l % 4) …, and gets rows 0..3 of column l
-__device__ __forceinline__ u32x2 read_tr(const uint8_t *p) {
+__device__ __forceinline__ u32x2 read_tr(uint32_t at) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)(uint32_t)(uintptr_t)p));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)at));
 }
 
 // Probabilities are 2^(s − m + P_SHIFT)
@@ -168,7 +172,7 @@ __device__ __forceinline__ float cap_score(float s, float in, float out) {
 // no result register, and the callers wait (wait_vmem) before the barrier behind which the
 // copy is read.  Nothing else here uses m0.  Loads return in order, so waits that count without these wait longer at most.
 __device__ __forceinline__ void copy_lds(const uint8_t *base, int off, const uint8_t *dst) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(dst));
     const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32)) << 32 |
                           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(from) : "memory");
@@ -307,10 +311,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
 
     f32x16 s[2];
     u32x4 pf[2][2];
-    auto scores = [&](const uint8_t *kt, int kb, f32x16 &d) __attribute__((always_inline)) {
+    auto scores = [&](uint32_t kt, int kb, f32x16 &d) __attribute__((always_inline)) {
         d = f32x16{};
 #pragma unroll
-        for (int i = 0; i < KS; i++) d = mfma32<BF>(*(const u32x4 *)(kt + k_at + Lds::key(kb * 32, 2 * i)), qf[i], d);
+        for (int i = 0; i < KS; i++) d = mfma32<BF>(lds_16(kt + k_at + Lds::key(kb * 32, 2 * i)), qf[i], d);
     };
     auto max16 = [&](const f32x16 &x) __attribute__((always_inline)) {
         float v = fmaxf(fmaxf(x[0], x[1]), x[2]);
@@ -318,19 +322,19 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         for (int e = 3; e < 15; e += 2) v = fmaxf(fmaxf(v, x[e]), x[e + 1]);
         return fmaxf(v, x[15]);
     };
-    auto outputs = [&](const uint8_t *vt, int kb, const u32x4 (&p)[2]) __attribute__((always_inline)) {
+    auto outputs = [&](uint32_t vt, int kb, const u32x4 (&p)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int st = 0; st < 2; st++)
 #pragma unroll
             for (int d = 0; d < DB; d++) {
-                const uint8_t *vp = vt + v_at + Lds::value(kb * 32 + st * 16, 4 * d);
+                const uint32_t vp = vt + v_at + Lds::value(kb * 32 + st * 16, 4 * d);
                 const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
                 o[d] = mfma32<BF>(u32x4{v0[0], v0[1], v1[0], v1[1]}, p[st], o[d]);
             }
     };
     // group (t, kb): probabilities of its scores x → p; outputs of the group before from values
     // (vt, vkb) and probabilities po; scores of the group behind from keys (kt, nkb) → y
-    auto group = [&](int key0, int bad2, f32x16 &x, u32x4 (&p)[2], const u32x4 (&po)[2], f32x16 &y, const uint8_t *vt, int vkb, const uint8_t *kt, int nkb) __attribute__((always_inline)) {
+    auto group = [&](int key0, int bad2, f32x16 &x, u32x4 (&p)[2], const u32x4 (&po)[2], f32x16 &y, uint32_t vt, int vkb, uint32_t kt, int nkb) __attribute__((always_inline)) {
         // positions of the lane's scores: key0 + 4 h + (8 (e / 4) + e % 4)
         float mx = ym;
         const bool late = key0 + 31 > all_hi, early = key0 <= all_lo;
@@ -374,10 +378,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         const float ref = P_SHIFT<BF> - m;
         u32x4 fr[NM];
         auto read = [&](int u) __attribute__((always_inline)) {
+            if (u >= NM) return;
             if (u < KS) {
-                fr[u] = *(const u32x4 *)(kt + k_at + Lds::key(nkb * 32, 2 * u));
-            } else if (u < NM) {
-                const uint8_t *vp = vt + v_at + Lds::value(vkb * 32 + (u - KS) / DB * 16, (u - KS) % DB * 4);
+                fr[u] = lds_16(kt + k_at + Lds::key(nkb * 32, 2 * u));
+            } else {
+                const uint32_t vp = vt + v_at + Lds::value(vkb * 32 + (u - KS) / DB * 16, (u - KS) % DB * 4);
                 const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
                 fr[u] = u32x4{v0[0], v0[1], v1[0], v1[1]};
             }
@@ -461,6 +466,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
                 for (int e = 0; e < 16; e++) {  // dim 32 d + 8 (e / 4) + 4 h + e % 4
                     const float v = value16<BF>(*(const uint16_t *)(vp + Lds::value(0, 4 * d + e / 4) + e % 4 * 2));
                     o[d][e] += (see & !(fabsf(v) <= FLT_MAX)) ? v : 0.0f;
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few values in registers at a time
                 }
         }
         lds_barrier();
@@ -488,12 +494,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         wait_vmem();
         lds_barrier();
         if (wave_live) {
-            scores(s_k0, 0, s[0]);
+            scores(lds_at(s_k0), 0, s[0]);
             ym = max16(s[0]);
         }
         auto tile = [&](int t, uint8_t *k_t, uint8_t *k_n, uint8_t *v_t, uint8_t *v_n, f32x16 &x0, f32x16 &x1, u32x4 (&p0)[2], u32x4 (&p1)[2]) __attribute__((always_inline)) {
             if constexpr (KB == 2)
-                if (wave_live) group(t * KT, cur.bad & 3, x0, p0, p1, x1, v_n, 1, k_t, 1);
+                if (wave_live) group(t * KT, cur.bad & 3, x0, p0, p1, x1, lds_at(v_n), 1, lds_at(k_t), 1);
             wait_vmem();
             lds_barrier();
             Tile third{};
@@ -505,11 +511,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
             if constexpr (KB == 2) {
                 if (t + 1 < t_end) copy(V_{}, vbase + nxt.v, nxt.rows, v_n);
                 apart(t, cur.bad, v_t);
-                if (wave_live) group(t * KT + 32, cur.bad >> 2, x1, p1, p0, x0, v_t, 0, k_n, 0);
+                if (wave_live) group(t * KT + 32, cur.bad >> 2, x1, p1, p0, x0, lds_at(v_t), 0, lds_at(k_n), 0);
             } else {
                 copy(V_{}, vbase + cur.v, cur.rows, v_t);
                 if (t > t_begin) apart(t - 1, bad_before, v_n);
-                if (wave_live) group(t * KT, cur.bad, x0, p0, p1, x1, v_n, 0, k_n, 0);
+                if (wave_live) group(t * KT, cur.bad, x0, p0, p1, x1, lds_at(v_n), 0, lds_at(k_n), 0);
                 bad_before = cur.bad;
             }
             cur = nxt;
@@ -531,8 +537,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
             apart(t_end - 1, bad_before, odd ? s_v0 : s_v1);
         }
         if (wave_live) {
-            if (odd) outputs(s_v0, KB - 1, pf[KB == 2 ? 1 : 0]);
-            else outputs(s_v1, KB - 1, pf[1]);
+            if (odd) outputs(lds_at(s_v0), KB - 1, pf[KB == 2 ? 1 : 0]);
+            else outputs(lds_at(s_v1), KB - 1, pf[1]);
         }
     }
 
@@ -540,9 +546,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     pair_f<32>(l, l0, l1);
     l = l0 + l1;
     if (!live) return;
+    // arguments that only the end needs are read here again: kept from the start they would be
+    // spilled, and read back in the loop
+    auto *late = (const __attribute__((address_space(4))) ServeAttnArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(late));
     if (ns == 1) {
         const float inv = l > 0 || l != l ? 1.0f / l : 0.0f;
-        uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + h * 8;
+        uint8_t *op = late->out + (int64_t)(sv.row0 + tok) * late->o_row + head * late->o_head + h * 8;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -551,13 +561,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
                 *(u32x2 *)(op + d * 64 + e * 16) = v;
             }
     } else {
-        const int64_t at = ((int64_t)(sv.row0 + tok) * a.n_head + head) * a.S + sp;
-        float *pp = a.part + at * HD + 4 * h;
+        const int64_t at = ((int64_t)(sv.row0 + tok) * late->n_head + head) * late->S + sp;
+        float *pp = late->part + at * HD + 4 * h;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int e = 0; e < 4; e++) *(f32x4 *)(pp + d * 32 + e * 8) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
-        if (h == 0) *(f32x2 *)(a.ml + at * 2) = f32x2{m, l};
+        if (h == 0) *(f32x2 *)(late->ml + at * 2) = f32x2{m, l};
     }
 }
 
@@ -761,7 +771,7 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
         }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
-            const uint8_t *vp = vt + v_at + Lds::value(0, 2 * d);
+            const uint32_t vp = lds_at(vt) + v_at + Lds::value(0, 2 * d);
             const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(16, 0));
             const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
