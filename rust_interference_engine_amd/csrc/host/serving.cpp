@@ -63,11 +63,11 @@ void check_rows(const void *p, int64_t row, int64_t head, int es, const char *wh
     if (row < 0 || row > most || head < 0 || head > most) throw bad(std::string(what) + ": strides have to lie in 0.." + std::to_string(most));
 }
 
-constexpr int MOST = 1 << 30;  // rows, positions
+constexpr int MOST = 1 << 30;  // positions
 
 rie::BatchView batch(const rie_hip_seqs *s, bool lens) {
     if (!s) throw bad("seqs is NULL");
-    if (s->n_seq < 1 || s->n_rows < 1 || s->n_seq > MOST || s->n_rows > MOST) throw bad("n_seq and n_rows have to lie in 1..2^30");
+    if (s->n_seq < 1 || s->n_rows < 1 || s->n_seq >= 1 << 24 || s->n_rows >= 1 << 26) throw bad("n_seq has to lie in 1..2^24-1, n_rows in 1..2^26-1");
     if (s->max_new < 1 || s->max_len < 1 || s->max_new > MOST || s->max_len > MOST) throw bad("max_new and max_len have to lie in 1..2^30");
     rie::BatchView b;
     b.starts = s->starts;
@@ -133,10 +133,9 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
     a.softcap = at->softcap;
     if (!kv.table) a.b.max_len = std::min(a.b.max_len, a.b.max_new);
     else a.b.max_len = std::min(a.b.max_len, kv.cap);
-    // workgroup and (row, head) numbers are 32-bit
-    if ((int64_t)a.b.n_rows * a.n_head > MOST || (int64_t)a.b.n_seq * n_kv > MOST ||
-        rie::block_count(a.b.n_rows, a.b.n_seq, a.G, 128) * n_kv > MOST)
-        throw bad("n_rows*n_head and n_seq*n_kv have to stay under 2^30");
+    // a launch has under 2^32 threads: 256 to a workgroup, 4 (row, head) pairs to one where the splits are added up
+    if ((int64_t)a.b.n_rows * a.n_head >= 1 << 26 || ((int64_t)a.b.n_seq + (int64_t)a.b.n_rows * a.G / 128) * n_kv >= 1 << 24)
+        throw bad("n_rows*n_head has to stay under 2^26, n_seq*n_kv under 2^24");
     return a;
 }
 
@@ -256,6 +255,7 @@ int32_t rie_hip_k_token_logprobs(int32_t ty, const void *logits, int32_t n, int3
     return guarded(err, err_len, [&] {
         if (ty != rie::T_F32 && !is16(ty)) throw Error{rie::E_UNSUPPORTED, "logits have to be f32, f16 or bf16"};
         if (n < 1 || n > 1 << 22 || n_vocab < 1 || n_vocab > rie::LOGPROB_MAX_V) throw bad("n has to lie in 1..2^22, n_vocab in 1..2^21");
+        if ((int64_t)n * n_vocab > (int64_t)1 << 40) throw bad("n*n_vocab has to stay under 2^40");  // 2^32 threads
         const int es = ty == rie::T_F32 ? 4 : 2;
         if ((uintptr_t)logits % es) throw bad("logits have to be aligned to their type");
         if (row_stride < 0 || row_stride > (int64_t)1 << 40) throw bad("row_stride has to lie in 0..2^40");

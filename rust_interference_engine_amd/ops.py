@@ -7,7 +7,8 @@ them, holds them and takes its workspace, and is then called as often as wanted:
 only queues the kernels, on ``stream`` (a ``torch.cuda.Stream``) or else on torch's
 current stream of the tensors' device, and reads the tensors as they are by then, so it
 can be captured into a graph.  An object's calls share its workspace: two that may run at
-the same time need an object each.
+the same time need an object each.  Keep the object until its calls have finished (one
+that a graph has captured: as long as the graph is replayed).  There are no gradients.
 
     kv = ops.PagedKv(k_pages, v_pages, table)
     seqs = ops.Seqs(starts, lens, max_new=1, max_len=4096)
@@ -47,6 +48,7 @@ def _type(t: torch.Tensor, what: str) -> int:
 def _device(*tensors) -> torch.device:
     d = tensors[0].device
     for t in tensors:
+        _need(not t.requires_grad, "these operators have no gradients: detach the tensors")
         _need(t.device == d and d.type == "cuda", f"tensors have to be on one GPU: got {t.device} and {d}")
     return d
 

@@ -377,6 +377,97 @@ def test_two_calls_at_once_on_two_streams(ops):
         assert torch.equal(out.cpu(), want)
 
 
+@pytest.mark.parametrize("H,KV,new", [(40, 1, 1), (71, 1, 3), (33, 1, 1), (256, 2, 2), (32, 1, 1), (17, 1, 1)])
+def test_many_query_heads_on_one_kv_head(ops, H, KV, new):
+    b = S.Batch([(new, 150), (new, new), (1, 700)], H, KV, 64, dtype=BF16, seed=21)
+    check(b, paged(ops, b))
+
+
+def test_the_first_sequence_may_start_behind_other_rows(ops):
+    b = S.Batch([(5, 70), (40, 300), (1, 9)], 8, 2, 64, seed=22)
+    shift = 37
+    b.q = torch.cat([torch.full((shift, 8, 64), math.nan, dtype=F16), b.q])
+    b.starts += shift
+    b.rows += shift
+    for kw in (dict(), dict(max_len=20000)):  # without and with splits
+        out = paged(ops, b, **kw)
+        assert bool((out[:shift] == 7).all())
+        check(b, out)
+    g = torch.Generator().manual_seed(23)
+    new = torch.randn(b.rows, 2, 64, generator=g).half()
+    k, v, dev = b.k_pages.to(GPU), b.v_pages.to(GPU), new.to(GPU)
+    ops.PagedAppend(ops.PagedKv(b.paged(k), b.paged(v), b.table.to(GPU)), ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=40, max_len=300), dev, dev)()
+    b.k_pages = k.cpu()
+    assert torch.equal(b.cached(b.k_pages, 1)[-40:], new[shift + 5:shift + 45]) and torch.equal(b.cached(b.k_pages, 2)[-1:], new[-1:])
+
+
+@pytest.mark.parametrize("new", [1, 3, 60])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_pages_below_the_window_may_be_gone(ops, new, hd):
+    b = S.Batch([(new, 400), (1, 333)], 4, 1, hd, dtype=BF16, seed=24)
+    whole = paged(ops, b, 100)
+    check(b, whole, 100)
+    for i, (n, L) in enumerate(b.lens):
+        gone = (L - n - 99) // 16  # pages that no token's window reaches
+        b.table[i, :gone] = torch.tensor([-1, 2 ** 31 - 1, b.n_pages])[torch.arange(gone) % 3].int()
+        page = int(b.table[i, gone])
+        b.v_pages[page, :, :(L - n - 99) % 16] = math.nan  # and the slots of the last page that it only ends in
+        b.k_pages[page, :, :(L - n - 99) % 16] = math.inf
+    assert torch.equal(paged(ops, b, 100), whole)
+
+
+@pytest.mark.parametrize("new", [2, 50])
+def test_a_query_that_is_nan_or_infinite_spoils_its_own_row_only(ops, new):
+    b = S.Batch([(new, 130), (1, 50)], 8, 2, 64, seed=25)
+    clean = paged(ops, b)
+    b.q[1, 3, 7], b.q[new, 0, 0] = math.nan, math.inf
+    out = paged(ops, b)
+    assert bool(out[1, 3].isnan().all()) and bool((~torch.isfinite(out[new, 0])).all())
+    out[1, 3], out[new, 0] = clean[1, 3], clean[new, 0]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+def test_packed_prompts_keep_infinite_and_nan_values_to_the_tokens_behind_them(ops, hd):
+    lens, H, KV = [70, 40, 90], 4, 2
+    g = torch.Generator().manual_seed(26)
+    q, k, v = (torch.randn(200, x, hd, generator=g).to(BF16) for x in (H, KV, KV))
+    starts = torch.tensor([0] + lens).cumsum(0).int().to(GPU)
+
+    def run():
+        out = torch.empty(200, H, hd, dtype=BF16, device=GPU)
+        ops.PackedAttention(ops.Seqs(starts, max_new=90, max_len=90), q.to(GPU), k.to(GPU), v.to(GPU), out)()
+        return out.cpu()
+
+    clean = run()
+    v[70 + 17, 1, 2], v[69, 0, 0], v[110, 0, hd - 1] = math.inf, math.nan, -math.inf
+    out = run()
+    hit = torch.zeros(200, H, hd, dtype=torch.bool)
+    hit[70 + 17:110, 2:, 2] = True   # of sequence 1, behind its token 17, heads of KV head 1
+    hit[69, :2, 0] = True            # the last token of sequence 0
+    hit[110:, :2, hd - 1] = True     # all of sequence 2
+    assert bool((~torch.isfinite(out[hit])).all()) and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logprobs_where_every_group_counts(ops, dtype):
+    """vocabularies past the registers' groups, equal maxima in many groups, masked heads and tails"""
+    g = torch.Generator().manual_seed(27)
+    V = 700001
+    x = torch.randn(3, V, generator=g).to(dtype)
+    x[0, ::4096] = 9.0           # 171 groups with the same maximum
+    x[1, :500000] = -math.inf
+    x[2, 3:] = -math.inf
+    t = torch.tensor([4096, 600000, 2], dtype=torch.int32)
+    lp, h, ids, tops = run_logprobs(ops, x.to(GPU), t, 64)
+    wl, wh, wi, wt = S.logprobs(x, t, 64)
+    assert torch.equal(ids.long(), wi)
+    tol = 2.0 ** -18 * (1 + math.log(V)) ** 2
+    for a, b in ((lp, wl), (h, wh), (tops, wt)):
+        fine = torch.isfinite(b)
+        assert torch.equal(a[~fine], b[~fine]) and bool(((a - b).abs()[fine] <= tol).all())
+
+
 def test_refused_on_the_gpu(ops):
     from rust_interference_engine_amd import RieError, _lib
     import ctypes as C

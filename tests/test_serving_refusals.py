@@ -47,7 +47,8 @@ def paged(pg=None, sq=None, at=None, ws=P, n=1 << 40):
     (dict(pg=pages(slot_stride=68)), -5, "16-byte aligned"), (dict(pg=pages(slot_stride=-64)), -5, "strides"), (dict(pg=pages(slot_stride=1 << 40)), -5, "strides"),
     (dict(pg=pages(page_stride=-8)), -5, "page_stride"), (dict(pg=pages(page_stride=12)), -5, "page_stride"), (dict(pg=pages(table=0)), -5, "table is NULL"),
     (dict(sq=seqs(n_seq=0)), -5, "n_seq"), (dict(sq=seqs(n_rows=0)), -5, "n_rows"), (dict(sq=seqs(max_new=0)), -5, "max_new"), (dict(sq=seqs(max_len=-1)), -5, "max_len"),
-    (dict(sq=seqs(n_rows=1 << 30)), -5, "2^30"),
+    (dict(sq=seqs(n_rows=1 << 30)), -5, "2^26"), (dict(sq=seqs(n_rows=1 << 25)), -5, "2^26"), (dict(sq=seqs(n_seq=1 << 24)), -5, "2^24"),
+    (dict(sq=seqs(n_seq=(1 << 23) + 1)), -5, "2^24"),
     (dict(at=attn(n_head=3)), -5, "n_head"), (dict(at=attn(n_head=0)), -5, "n_head"), (dict(at=attn(scale=0.0)), -5, "scale"), (dict(at=attn(scale=-1.0)), -5, "scale"),
     (dict(at=attn(scale=float("nan"))), -5, "scale"), (dict(at=attn(scale=float("inf"))), -5, "scale"), (dict(at=attn(softcap=-1.0)), -5, "softcap"),
     (dict(at=attn(softcap=float("nan"))), -5, "softcap"), (dict(at=attn(window=-1)), -5, "window"), (dict(at=attn(q=P + 2)), -5, "16-byte aligned"),
@@ -106,7 +107,7 @@ def test_paged_append(ty, k, row, head, code, text):
 
 @pytest.mark.parametrize("kw,code,text", [
     (dict(ty=2), -3, "logits have to be"), (dict(n=0), -5, "n has to"), (dict(V=0), -5, "n_vocab"), (dict(V=(1 << 21) + 1), -5, "n_vocab"), (dict(x=P + 2), -5, "aligned"),
-    (dict(ld=-1), -5, "row_stride"), (dict(top=65), -5, "n_top"), (dict(top=-1), -5, "n_top"), (dict(V=10, top=11), -5, "n_top"), (dict(lp=None), -5, "together"),
+    (dict(ld=-1), -5, "row_stride"), (dict(n=1 << 22, V=1 << 20, ld=0), -5, "2^40"), (dict(top=65), -5, "n_top"), (dict(top=-1), -5, "n_top"), (dict(V=10, top=11), -5, "n_top"), (dict(lp=None), -5, "together"),
     (dict(targets=None), -5, "together"), (dict(top=2, ids=None), -5, "top_ids"), (dict(top=2, tops=None), -5, "top_ids"), (dict(bytes=10), -5, "needed"), (dict(ws=P + 8), -5, "ws has"),
 ])
 def test_token_logprobs(kw, code, text):
@@ -136,6 +137,7 @@ def test_the_python_layers_own_checks():
         (lambda: ops.TokenLogprobs(z(5, 4), entropy=z(4)), "entropy has to be"),
         (lambda: ops.TokenLogprobs(z(4, 5).t()), "consecutive"),
         (lambda: ops.TokenLogprobs(z(5, 4)), "on one GPU"),
+        (lambda: ops.TokenLogprobs(z(5, 4, requires_grad=True)), "no gradients"),
     ]:
         with pytest.raises(RieError, match=text):
             make()
