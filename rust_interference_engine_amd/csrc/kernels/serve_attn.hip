@@ -158,6 +158,26 @@ __device__ __forceinline__ bool page_of(const KvView &kv, const int *trow, int g
 
 template <int HD>
 constexpr int HDP = HD <= 64 ? 64 : HD <= 128 ? 128 : HD;  // values between rows of a tile in LDS
+// An output that came out as NaN, of a row whose probabilities' sum is a number: an infinite value
+// has met a probability that was rounded to zero, or a rounding's remainder of either sign.  The
+// true one is the sum of the infinite and NaN values at positions [j0, j1), which its token sees
+// (NaN itself where there are none).
+template <bool BF>
+__device__ __forceinline__ float nonfinite_sum(const KvView &kv, const int *trow, int row0, const uint8_t *v, int j0, int j1) {
+    float sum = 0;
+    for (int j = j0; j < j1; j++) {
+        int64_t at = (int64_t)(row0 + j) * kv.v_row;
+        if (trow) {
+            int page;
+            if (!page_of(kv, trow, j, page)) continue;
+            at = page * kv.page + (j & ((1 << kv.page_shift) - 1)) * kv.v_row;
+        }
+        const float x = value16<BF>(*(const uint16_t *)(v + at));
+        if (!(fabsf(x) <= FLT_MAX)) sum += x;
+    }
+    return sum == 0 ? NAN : sum;
+}
+
 // score → exponent in log2 units, where the softcap makes it one already
 template <bool CAP>
 __device__ __forceinline__ float cap_score(float s, float in, float out) {
@@ -550,9 +570,16 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     // spilled, and read back in the loop
     auto *late = (const __attribute__((address_space(4))) ServeAttnArgs *)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(late));
+    bool nan = false;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) nan |= o[d][e] != o[d][e];
+    const float inv = ns > 1 ? 1.0f : l > 0 || l != l ? 1.0f / l : 0.0f;
+    uint8_t *op = late->out + (int64_t)(sv.row0 + tok) * late->o_row + head * late->o_head + h * 8;
+    const int64_t at = ((int64_t)(sv.row0 + tok) * late->n_head + head) * late->S + sp;
+    float *pp = late->part + at * HD + 4 * h;
     if (ns == 1) {
-        const float inv = l > 0 || l != l ? 1.0f / l : 0.0f;
-        uint8_t *op = late->out + (int64_t)(sv.row0 + tok) * late->o_row + head * late->o_head + h * 8;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -561,13 +588,22 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
                 *(u32x2 *)(op + d * 64 + e * 16) = v;
             }
     } else {
-        const int64_t at = ((int64_t)(sv.row0 + tok) * late->n_head + head) * late->S + sp;
-        float *pp = late->part + at * HD + 4 * h;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int e = 0; e < 4; e++) *(f32x4 *)(pp + d * 32 + e * 8) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
         if (h == 0) *(f32x2 *)(late->ml + at * 2) = f32x2{m, l};
+    }
+    if (nan && l == l) {  // rare
+        const int j0 = imax(imax(lo_q + 1, 0), t_begin * KT), j1 = imin(p_q + 1, t_end * KT);
+        for (int i = 0; i < HD / 2; i++) {  // the lane's dims: 8 (i / 4) + 4 h + i % 4
+            const int dim = i / 4 * 8 + i % 4;
+            uint16_t *x = (uint16_t *)op + dim;
+            if (ns == 1 ? value16<BF>(*x) == value16<BF>(*x) : pp[dim] == pp[dim]) continue;
+            const float v = nonfinite_sum<BF>(a.kv, trow, sv.row0, vbase + (dim + 4 * h) * 2, j0, j1);
+            if (ns == 1) *x = (uint16_t)pack2<BF>(v, v);
+            else pp[dim] = v;
+        }
     }
 }
 
@@ -815,6 +851,12 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] = fmaf(f, x[e], acc[e]);
         }
+        for (int e = 0; e < 4; e++)
+            if (acc[e] != acc[e] && L == L) {  // rare
+                const int p = pos0 + tok, j0 = imax(a.window > 0 ? imax(p + 1 - a.window, 0) : 0, (t0 + sp * a.C) * FEW_STEP);
+                const int j1 = imin(p + 1, (sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * FEW_STEP);
+                acc[e] = nonfinite_sum<BF>(a.kv, trow, 0, vbase + (d4 * 4 + e) * 2, j0, j1);
+            }
         if (ns == 1) {
             const float inv = L > 0 || L != L ? 1.0f / L : 0.0f;
             uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d4 * 8;
