@@ -7,17 +7,20 @@
 // p_t of its sequence.  A token that sees nothing gets zeros.  q, k, v and o are all f16
 // or all bf16; scores, the softmax's maximum and sum, and the outputs are f32 sums.
 //
-// Rounding.  A probability enters the second product in the tensors' own type, rounded to
-// nearest; the sum that the output is divided by adds the same rounded values, so that a
-// row's weights add up to one.  The error this brings is about that of rounding the output
-// once more (2^-9 of a bf16 value, 2^-12 of an f16 one, both root mean square).  The
-// maximum that is subtracted is only moved when a score passes it by 2^8, so a probability
-// lies in 0..2^8; f16 ones are multiplied by 2^6, since small ones would be subnormal.
+// Rounding.  In the tile kernel a probability enters the second product in the tensors' own
+// type, rounded to nearest; the sum that the output is divided by adds the same rounded values,
+// so that a row's weights add up to one.  The error this brings is about that of rounding the
+// output once more (2-norm against float64, bf16: 2.1e-3, the output's own rounding 1.6e-3).
+// The few-rows kernel takes what that rounding leaves as a second product, its matrix units
+// being idle (1.6e-3 and 1.6e-3).  The maximum that is subtracted is only moved when a score
+// passes it by 2^8, so a probability lies in 0..2^8; f16 ones are multiplied by 2^6, since
+// small ones would be subnormal.
 //
 // Values that are infinite or NaN reach the tokens that see them and no others: a tile that
-// some token sees in part is searched for them as it is staged, and if there are any, they
-// are added to the outputs one by one and replaced by zeros in the matrix product, where
-// they would meet probabilities of zero.
+// some token sees in part is searched for them, and if there are any, they are added to the
+// outputs one by one and replaced by zeros in the matrix product, where they would meet
+// probabilities of zero.  Outputs that are NaN all the same are formed from the infinite and NaN
+// values alone at the end (nonfinite_sum).
 //
 // Two kernels.  attn_tile_kernel takes 128 query rows (token · group + head of the group,
 // so the heads of a group share their keys) per workgroup and goes through the positions in
@@ -38,13 +41,11 @@ namespace rie {
 
 namespace {
 
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -96,7 +97,10 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
 }
 
 // Addresses in LDS as numbers: sums with constants become the instructions' offsets, where
-// generic pointers took a register for every one (70 of them in the tile kernel).
+// generic pointers take a register for every one, 50 to 70 of them in the tile kernel, which
+// then holds all 256 (and one more is a spill whose reload waits for the copies: 219 to 272 us
+// for chunks in a batch of 13; 202 without a spill, 216 here with 209 registers; four prompts
+// of 64-wide heads, 3 waves on a SIMD instead of 2: 187, with pointers 201).
 __device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)p; }
 __device__ __forceinline__ u32x4 lds_16(uint32_t at) { return *(__attribute__((address_space(3))) const u32x4 *)(uintptr_t)at; }
 // 4 values of one column: lane l of a group of 16 lanes names the 8 bytes of row l / 4 that
@@ -105,7 +109,6 @@ __device__ __forceinline__ u32x2 read_tr(uint32_t at) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)at));
 }
-
 // Probabilities are 2^(s − m + P_SHIFT)
 template <bool BF>
 constexpr float P_SHIFT = BF ? 0.0f : 6.0f;
@@ -228,12 +231,20 @@ constexpr int TILE_KT = HD <= 128 ? 64 : 32;  // positions of a tile
 // each, one barrier per tile: at tile t's barrier the loads of K(t + 1) and V(t + KB − 2) are
 // complete, K(t) and V(t + KB − 3) have been read, and K(t + 2) and V(t + KB − 1) are
 // requested into their places.
+//
+// Four packed prompts of up to 5000 tokens, 32 heads on 8 of 128, bf16: 428 us, 890 TFLOP/s
+// (381 GFLOP), three quarters of what a library product of 8192 reaches on the card; 486 us
+// with tiles staged through registers and the steps one behind the other.  Counters: matrix
+// units busy 39 % of the cycles, vector units about as much, LDS 21 %, a quarter of the waves'
+// time in waits.  Four buffers of 32 positions instead of two of 64 (loads three tiles ahead, a
+// barrier every 32 positions): 429 us, and 248 for 208 us on chunks over pages; products in
+// turns instead of scores first: 430; the next products' operands read 5 ahead: 427.
 template <int HD, bool BF, bool CAP>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(ServeAttnArgs a) {
     constexpr int KT = TILE_KT<HD>, KB = KT / 32, RW = KT / 4, KS = HD / 16, DB = HD / 32;
     using Lds = TileLds<HD>;
     constexpr int RPI = Lds::RPI, NLD = RW / RPI, KBYTES = KT / RPI * Lds::K_BLOCK, VBYTES = KT / RPI * Lds::V_BLOCK;
-    constexpr int NG = KT / 16;                                     // groups of 16 positions, which lie in one page
+    constexpr int NG = KT / 16;  // groups of 16 positions, which lie in one page
     __shared__ __align__(16) uint8_t s_k0[KBYTES], s_k1[KBYTES], s_v0[VBYTES], s_v1[VBYTES];
     __shared__ __align__(16) int s_nf[4];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -390,7 +401,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
             m = mn;
             l *= al;
         }
-        // Eight rounds of matrix products, first the scores', then the outputs', operands read two
+        // Eight rounds of matrix products, first the scores', then the outputs', operands read three
         // products ahead, with a share of the probabilities after each; the next group's maximum
         // at the end, so that its own round begins with it.  The fences keep the order.
         constexpr int NV = 2 * DB, NM = KS + NV;
@@ -614,6 +625,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
 // is free, and the other waves of the CU (16 at head size 128) keep the memory busy meanwhile.
 // The matrix units being idle, a probability is two values of the tensors' type (value and
 // remainder), and the outputs are as exact as their own rounding.
+//
+// Bound: HBM.  One token over 100003 positions (4 KV heads of 128, bf16, 205 MB): 40 us, 5.1
+// TB/s, what a copy reaches, and 5.7 for the join of 112 splits; of 48 sequences (8 KV heads,
+// f16, up to 4000 positions, 298 MB): 67 us, 4.4 TB/s, and 6.8, the sequences' different lengths
+// being the difference.  Values through registers, 8 waves on a CU: 74 us.
 constexpr int FEW_KT = 32, FEW_STEP = 4 * FEW_KT;
 template <int HD, int NB>
 constexpr int FEW_WAVES = NB == 1 ? (HD <= 128 ? 4 : 2) : (HD <= 64 ? 3 : HD <= 128 ? 2 : 1);  // of a SIMD, as registers allow
@@ -949,6 +965,8 @@ __global__ __launch_bounds__(256) void serve_combine_kernel(ServeAttnArgs a, int
 }
 
 // New rows into their pages: a wave per token row, 8 values of K or V per lane and step.
+// Bound: HBM, 2854 rows of 2 x 8 heads of 128, f32 to bf16 (35 MB) 7.1 us, 4.9 TB/s; a step of
+// 61 rows 3 us, which is a launch.
 template <int SRC, bool BF>  // SRC: bytes of a source value
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
