@@ -959,6 +959,16 @@ __global__ __launch_bounds__(256) void serve_combine_kernel(ServeAttnArgs a, int
         acc = sum;
     }
     if (g == 0) {
+        if (L == L)  // rare: a split's infinity has met a weight of zero
+            for (int e = 0; e < 4; e++)
+                if (acc[e] != acc[e]) {
+                    float sum = 0;
+                    for (int s = 0; s < ns; s++) {
+                        const float y = p[(int64_t)s * a.hd + e];
+                        if (!(fabsf(y) <= FLT_MAX)) sum += y;
+                    }
+                    acc[e] = sum;
+                }
         uint8_t *op = a.out + (int64_t)row * a.o_row + head * a.o_head;
         *(u32x2 *)(op + d * 8) = u32x2{pack2<BF>(acc[0], acc[1]), pack2<BF>(acc[2], acc[3])};
     }

@@ -133,6 +133,24 @@ def test_an_infinite_value_among_many_makes_that_infinity(ops, dtype, lens):
         assert bool(torch.isfinite(out[rest]).all())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens", [[(1, 3000)], [(3, 3000)], [(70, 3000), (1, 2000)], [(1, 3000)] + [(1, 20)] * 299])
+def test_an_infinite_value_of_a_split_that_weighs_nothing(ops, dtype, lens):
+    """the first half of the positions scores hundreds below the second for one row: e^-471 or so of their sum"""
+    b = S.Batch(lens, 8, 2, 128, page=64, dtype=dtype, seed=41)
+    t = b.table[0, :47].long()
+    b.k_pages[t[:24], 1] = -40 * b.q[0, 4].sign()
+    b.v_pages[t[2], 1, 9, 65] = math.inf
+    b.v_pages[t[20], 1, 9, 66] = -math.inf
+    for kw in (dict(), dict(max_len=60000)):
+        out = paged(ops, b, **kw)
+        n = lens[0][0]
+        assert bool((out[:n, 4:, 65] == math.inf).all()) and bool((out[:n, 4:, 66] == -math.inf).all())
+        rest = torch.ones(out.shape, dtype=torch.bool)
+        rest[:n, 4:, 65:67] = False
+        assert bool(torch.isfinite(out[rest]).all())
+
+
 def test_slots_behind_the_last_position_may_hold_anything(ops):
     b = S.Batch([(1, 37), (20, 50), (2, 33)], 4, 2, 64, seed=7)
     clean = paged(ops, b)
