@@ -225,7 +225,9 @@ int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, v
  *
  * Types are ggml ids: 0 f32, 1 f16, 30 bf16.  Strides count elements.  Pointers and
  * strides of q, k, v, the pages and the outputs have to keep every row (of head_dim
- * consecutive values) 16-byte aligned.  head_dim: 32, 64, 96, 128 or 256.
+ * consecutive values) 16-byte aligned; strides of rows, slots and heads go up to 2^26
+ * bytes.  head_dim: 32, 64, 96, 128 or 256.  What a call writes may share no memory with
+ * what it reads, and its rows none with one another.
  *
  * stream: a hipStream_t of any device (NULL: the current device's null stream); the call
  * queues its kernels there and returns.  Pointers of host memory, or of another device
@@ -240,7 +242,8 @@ int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, v
  * bring no token; a token before position 0 (more new tokens than positions) is not
  * written to the cache and attends to nothing.  max_new and max_len bound the new tokens
  * and the positions of any one sequence: they choose kernels and splits, and of a
- * sequence that exceeds max_new only some rows may be computed. */
+ * sequence that exceeds max_new only some rows may be computed, the others of its rows
+ * holding anything. */
 typedef struct rie_hip_seqs {
     int32_t n_seq, n_rows, max_new, max_len;
     const int32_t *starts; /* [n_seq + 1] */
@@ -251,7 +254,9 @@ typedef struct rie_hip_seqs {
  * table[i*table_stride + p/page_size], slot p%page_size, and head h's values start at
  * page*page_stride + slot*slot_stride + h*head_stride of k and of v.  page_size: a power
  * of two, 16 to 4096.  Positions at and past table_cols*page_size do not exist, and
- * those of a page id outside 0..n_pages-1 are neither written nor seen. */
+ * those of a page id outside 0..n_pages-1 are neither written nor seen.  Sequences may
+ * share pages (a common prefix); where two new tokens come to the same slot, it holds
+ * values of either. */
 typedef struct rie_hip_pages {
     int32_t ty, head_dim, n_kv, n_pages, page_size, table_cols;
     void *k, *v;
@@ -280,7 +285,9 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
 /* Causal attention of every sequence's new tokens over its pages, which already hold them:
  * chunks of prompts and single tokens in one batch.  A token that sees nothing gets zeros.
  * An infinite or NaN key or value reaches only the tokens that see it (an infinite value as
- * that infinity). */
+ * that infinity).  Outputs are f32 sums of up to 2^8 times the values before they are
+ * divided, so bf16 values may not be so large that their sum over the positions, times
+ * 2^8, passes 3e38. */
 size_t rie_hip_k_paged_attention_ws(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn);
 int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn, void *ws,
                                   size_t ws_bytes, void *stream, char *err, size_t err_len);

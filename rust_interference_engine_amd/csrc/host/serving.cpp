@@ -63,6 +63,11 @@ void check_rows(const void *p, int64_t row, int64_t head, int es, const char *wh
     if (row < 0 || row > most || head < 0 || head > most) throw bad(std::string(what) + ": strides have to lie in 0.." + std::to_string(most));
 }
 
+// Rows that are written: no two of them share a value by a stride that is too small
+void check_apart(int64_t n, int64_t stride, int hd, const char *what) {
+    if (n > 1 && stride < hd) throw bad(std::string(what) + ": strides below head_dim would make rows overlap");
+}
+
 constexpr int MOST = 1 << 30;  // positions
 
 rie::BatchView batch(const rie_hip_seqs *s, bool lens) {
@@ -142,6 +147,8 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
 void run_attention(const rie::ServeAttnArgs &a, const rie_hip_attn *at, void *ws, size_t ws_bytes, void *stream) {
     check_rows(at->q, at->q_row_stride, at->q_head_stride, 2, "q");
     check_rows(at->out, at->out_row_stride, at->out_head_stride, 2, "out");
+    check_apart(a.b.n_rows, at->out_row_stride, a.hd, "out");
+    check_apart(a.n_head, at->out_head_stride, a.hd, "out");
     const size_t need = rie::serve_attn_ws(a);
     if (ws_bytes < need) throw bad("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
     if ((uintptr_t)ws % 16) throw bad("ws has to be 16-byte aligned");
@@ -188,6 +195,9 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
         const int es = src_ty == rie::T_F32 ? 4 : 2;
         check_rows(k, row_stride, head_stride, es, "k");
         check_rows(v, row_stride, head_stride, es, "v");
+        check_apart(pages->page_size, pages->slot_stride, pages->head_dim, "pages");
+        check_apart(pages->n_kv, pages->head_stride, pages->head_dim, "pages");
+        check_apart(pages->n_pages, pages->page_stride, pages->head_dim, "pages");
         a.k = (const uint8_t *)k;
         a.v = (const uint8_t *)v;
         a.k_row = a.v_row = row_stride * es;

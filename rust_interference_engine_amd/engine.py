@@ -104,6 +104,9 @@ class Engine:
         tokens = [int(t) for t in tokens]
         if len(tokens) > self.backend.n_ctx():
             raise RieError(-5, f"text of {len(tokens)} tokens exceeds context window of {self.backend.n_ctx()}")
+        wrong = [t for t in tokens if not 0 <= t < self.backend.n_vocab]
+        if wrong:
+            raise RieError(-5, f"token id {wrong[0]} out of range")
         self.reset()
         out, nb, n = [], self.backend.max_batch(), len(tokens) - 1
         for pos in range(0, n, nb):

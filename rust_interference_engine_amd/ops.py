@@ -45,6 +45,15 @@ def _type(t: torch.Tensor, what: str) -> int:
     return _TYPES[t.dtype]
 
 
+def _int(x, what: str, least: int, most: int) -> int:
+    _need(int(x) == x and least <= x <= most, f"{what} has to lie in {least}..{most}, got {x}")
+    return int(x)
+
+
+def _written(t: torch.Tensor, what: str) -> None:
+    _need(all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride())), f"{what} is expanded: its rows would be written over one another")
+
+
 def _device(*tensors) -> torch.device:
     d = tensors[0].device
     for t in tensors:
@@ -105,9 +114,11 @@ class Seqs:
             _ints(lens, "lens", 1)
             _need(lens.numel() == starts.numel() - 1, f"{lens.numel()} lens for {starts.numel() - 1} sequences")
             _device(starts, lens)
-        self.starts, self.lens, self.max_new, self.max_len = starts, lens, int(max_new), int(max_len)
+        self.starts, self.lens = starts, lens
+        self.max_new, self.max_len = _int(max_new, "max_new", 1, 1 << 30), _int(max_len, "max_len", 1, 1 << 30)
 
     def _struct(self, n_rows: int) -> _lib.Seqs:
+        _int(n_rows, "rows", 1, (1 << 26) - 1)
         return _lib.Seqs(self.starts.numel() - 1, n_rows, self.max_new, self.max_len, self.starts.data_ptr(),
                          self.lens.data_ptr() if self.lens is not None else None)
 
@@ -146,6 +157,7 @@ class PagedAppend(_Op):
         _need(k.shape == v.shape and k.dtype == v.dtype and k.stride() == v.stride(), "k and v have to have one shape, type and strides")
         _need(k.shape[1] == kv.k.shape[2], f"k has {k.shape[1]} heads, the pages {kv.k.shape[2]}")
         _check_seqs(seqs, kv.table)
+        _written(kv.k, "pages")
         dev = _device(kv.k, k, v, seqs.starts, seqs.lens)
         sq = seqs._struct(k.shape[0])
         self._ready(_lib.lib().rie_hip_k_paged_append, [C.byref(kv._struct), C.byref(sq), _type(k, "k"), k.data_ptr(), v.data_ptr(),
@@ -156,7 +168,8 @@ def _attn(q: torch.Tensor, out: torch.Tensor, n_kv: int, ty: torch.dtype, hd: in
     _rows(q, "q", hd), _rows(out, "out", hd)
     _need(q.shape == out.shape and q.dtype == out.dtype == ty, "q and out have to have one shape, and the keys' type")
     _need(q.shape[1] % n_kv == 0, f"{q.shape[1]} query heads on {n_kv} KV heads")
-    return _lib.Attn(q.shape[1], window, 1 / math.sqrt(hd) if scale is None else scale, softcap, q.data_ptr(), q.stride(0), q.stride(1),
+    _written(out, "out")
+    return _lib.Attn(q.shape[1], _int(window, "window", 0, 2**31 - 1), 1 / math.sqrt(hd) if scale is None else scale, softcap, q.data_ptr(), q.stride(0), q.stride(1),
                      out.data_ptr(), out.stride(0), out.stride(1))
 
 
@@ -202,7 +215,7 @@ class TokenLogprobs(_Op):
                  entropy: torch.Tensor | None = None, top_ids: torch.Tensor | None = None, top_logprobs: torch.Tensor | None = None):
         _need(logits.dim() == 2 and logits.numel() > 0, f"logits have to be [rows, vocabulary], got {tuple(logits.shape)}")
         _need(logits.shape[1] == 1 or logits.stride(1) == 1, "a row's logits have to be consecutive")
-        n, n_vocab = logits.shape
+        n, n_vocab = _int(logits.shape[0], "rows", 1, 1 << 22), _int(logits.shape[1], "vocabulary", 1, 1 << 21)
         _need((targets is None) == (logprob is None), "targets and logprob have to be given together")
         _need((top_ids is None) == (top_logprobs is None), "top_ids and top_logprobs have to be given together")
         top = 0
@@ -212,8 +225,8 @@ class TokenLogprobs(_Op):
         for t, what, dtype in ((targets, "targets", torch.int32), (logprob, "logprob", torch.float32), (entropy, "entropy", torch.float32),
                                (top_ids, "top_ids", torch.int32), (top_logprobs, "top_logprobs", torch.float32)):
             if t is not None:
-                _need(t.dtype == dtype and t.shape[0] == n and t.is_contiguous(), f"{what} has to be contiguous {dtype} for {n} rows")
                 _need(t.dim() == (2 if what.startswith("top") else 1), f"{what} has {t.dim()} dimensions")
+                _need(t.dtype == dtype and t.shape[0] == n and t.is_contiguous(), f"{what} has to be contiguous {dtype} for {n} rows")
         given = [t for t in (targets, logprob, entropy, top_ids, top_logprobs) if t is not None]
         dev = _device(logits, *given)
         ptr = [None if t is None or not t.numel() else t.data_ptr() for t in (targets, logprob, entropy, top_ids, top_logprobs)]

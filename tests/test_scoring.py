@@ -45,6 +45,16 @@ def test_score_and_perplexity_over_the_oracle(oracle):
         e.perplexity([1])
 
 
+@pytest.mark.parametrize("bad", [-1, 1 << 30, 1 << 40])
+def test_score_refuses_a_last_token_that_is_none(oracle, bad):
+    e = R.Engine(oracle.Backend(oracle.Model(synth.build(synth.tiny("llama", F16))), 32, 8, n_threads=2))
+    e.eval_tokens(TOKS[:3])
+    for call in (e.score, e.perplexity):
+        with pytest.raises(R.RieError, match="out of range"):
+            call(TOKS[:4] + [bad])
+    assert e.cached == TOKS[:3]  # refused before anything was evaluated
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("arch", ["llama", "qwen3", "gemma2", "qwen3moe"])
 def test_forward_logprobs_are_those_of_the_logits(arch):

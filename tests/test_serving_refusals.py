@@ -141,3 +141,42 @@ def test_the_python_layers_own_checks():
     ]:
         with pytest.raises(RieError, match=text):
             make()
+
+
+@pytest.mark.parametrize("at,text", [
+    (dict(out_row_stride=0), "out: strides below"), (dict(out_row_stride=32), "out: strides below"), (dict(out_head_stride=0), "out: strides below"),
+])
+def test_outputs_whose_rows_overlap(at, text):
+    rc, m = paged(at=attn(**at))
+    assert rc == -5 and text in m, (rc, m)
+
+
+@pytest.mark.parametrize("pg", [dict(slot_stride=0), dict(head_stride=32), dict(page_stride=0)])
+def test_pages_whose_rows_overlap_are_read_and_not_written(pg):
+    L = _lib.lib()
+    rc, m = said(lambda e: L.rie_hip_k_paged_append(C.byref(pages(**pg)), C.byref(seqs()), 1, P, P, 128, 64, None, e, 256))
+    assert rc == -5 and "pages: strides below" in m, (rc, m)
+    sq = seqs(max_len=100000, max_new=1)
+    assert L.rie_hip_k_paged_attention_ws(C.byref(pages(table_cols=10000, **pg)), C.byref(sq), C.byref(attn())) > 0
+
+
+def test_the_python_layers_numbers_and_dimensions():
+    torch = pytest.importorskip("torch")
+    from rust_interference_engine_amd import RieError, ops
+
+    z, i32 = torch.zeros, torch.int32
+    st = z(3, dtype=i32)
+    sq = ops.Seqs(st, max_new=4, max_len=4)
+    q = z(4, 2, 64, dtype=torch.float16)
+    for make, text in [
+        (lambda: ops.Seqs(st, max_new=(1 << 32) + 1, max_len=1), "max_new has to lie"),
+        (lambda: ops.Seqs(st, max_new=1, max_len=(1 << 32) + 1), "max_len has to lie"),
+        (lambda: ops.Seqs(st, max_new=0, max_len=1), "max_new has to lie"),
+        (lambda: ops.Seqs(st, max_new=1.5, max_len=2), "max_new has to lie"),
+        (lambda: ops.PackedAttention(sq, q, q, q, z(4, 2, 64, dtype=torch.float16), window=(1 << 32) + 1), "window has to lie"),
+        (lambda: ops.PackedAttention(sq, q, q, q, q[:1].expand(4, 2, 64)), "out is expanded"),
+        (lambda: ops.TokenLogprobs(z(5, 4), entropy=z(())), "entropy has 0"),
+        (lambda: ops.TokenLogprobs(z(1, (1 << 21) + 1)), "vocabulary has to lie"),
+    ]:
+        with pytest.raises(RieError, match=text):
+            make()
