@@ -34,6 +34,7 @@ namespace rie {
 namespace {
 
 constexpr int R = 16, GROUP = 64 * R;  // logits of a lane and of a group
+constexpr float FAST_M = 1 << 20;      // size of a maximum below which an exponent is one fma
 constexpr float D_MIN = -200;          // e^-200 is 0 in f32: the weighted sum's factor is cut there, so that 0 · -inf is not NaN
 
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
@@ -117,8 +118,10 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
     // the groups that hold no element equal to M, in log2 units against the reference −c, where
     // c = −M · log2 e rounded: one fma forms an exponent, and the rounding of c, r = M · log2 e + c
     // exactly, is taken out of the sums when M moves or at the end (they hold 2^r times theirs).
+    // r is at most half a step of c, 2^-4 for |M| < 2^20; from 3e9 on it could pass 128, and 2^-r
+    // be infinite.  Larger M (a run of masked logits, say) take the form with a subtraction.
     float M = -FLT_MAX, s = 0, t = 0, cnt = 0, fs = 0, ft = 0, c = 0;
-    bool plain = true;  // no fast form for this M: its product leaves the range of f32
+    bool plain = true;  // no fast form for this M
     auto settle = [&] {
         const float r = plain ? 0.0f : fmaf(M, LOG2E_F, c), f = exp2_hw(-r);
         s = fmaf(fs, f, s);
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a, int n_
             s = f * (s + cnt);
             cnt = 0;
             M = mx;
-            plain = !(fabsf(M) < 1e30f);
+            plain = !(fabsf(M) < FAST_M);
             c = plain ? 0.0f : -(M * LOG2E_F);
         }
         if (!slow) {

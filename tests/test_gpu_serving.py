@@ -349,6 +349,41 @@ def test_logprobs_of_odd_rows(ops, dtype):
             assert torch.equal(a[~fine & ~b.isnan()], b[~fine & ~b.isnan()]), r
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [6, 2001])  # 2001 rows: runs of more than one group
+@pytest.mark.parametrize("mag", [6e4, 1e6, 1.1e6, 3e7, 1e9, 5e9, 1e10, 1e12, 1e15, 1e20, 1e25, 1e29, 3e30, 3e38])
+def test_logprobs_of_large_finite_logits(ops, mag, n, dtype):
+    """masks and logits of any finite size: whole runs of them, single ones, and rows of nothing else"""
+    if mag > torch.finfo(dtype).max:
+        mag = 6e4
+    V = 20016
+    g = torch.Generator().manual_seed(31)
+    x = torch.randn(6, V, generator=g) * 3
+    x[0, 3000:9000] = -mag            # runs of groups that hold nothing else
+    x[1, 777] = -mag                  # one masked
+    x[2, 12345] = mag                 # one that takes all
+    x[3] = x[3] + mag                 # all large, as far apart as their steps let them
+    x[4] = x[4] - mag
+    x[5, :] = -mag
+    x[5, 4000] = 1.5                  # all masked but one
+    x = x.to(dtype)
+    x[3:5] = x[3:5].clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max)
+    t = torch.tensor([5, 777, 12345, 9, 10, 4000], dtype=torch.int32)
+    rep = -(-n // 6)
+    lp, h, ids, tops = run_logprobs(ops, x.repeat(rep, 1)[:n].to(GPU), t.repeat(rep)[:n], 4)
+    for a in (lp, h, ids, tops):
+        assert torch.equal(a, torch.cat([a[:6]] * rep)[:n])
+    wl, wh, wi, wt = S.logprobs(x, t, 4)
+    assert torch.equal(ids[:6].long(), wi)
+    for r in range(6):
+        row = x[r].double()
+        near = row[row > row.max() - 200]  # the others' probabilities are zeros in f32
+        tol = logprob_tol(near, V)
+        for a, b, tl in ((lp[r:r + 1], wl[r:r + 1], tol), (h[r:r + 1], wh[r:r + 1], tol * (1 + 2 * math.log(V))), (tops[r], wt[r], tol)):
+            # two differences of numbers of the size of b, each rounded once: 2 * 2^-24 |b|
+            assert bool(((a - b).abs() <= tl + b.abs() * 2.0 ** -23).all()), (r, a, b)
+
+
 def test_logprobs_of_a_nearly_certain_token(ops):
     x = torch.zeros(1, 4000)
     x[0, 1234] = 30.0
