@@ -253,8 +253,9 @@ typedef struct rie_hip_seqs {
 /* A layer's keys and values in pages: position p of sequence i lies in page
  * table[i*table_stride + p/page_size], slot p%page_size, and head h's values start at
  * page*page_stride + slot*slot_stride + h*head_stride of k and of v.  page_size: a power
- * of two, 16 to 4096.  Positions at and past table_cols*page_size do not exist, and
- * those of a page id outside 0..n_pages-1 are neither written nor seen.  Sequences may
+ * of two, 16 to 4096.  Positions at and past table_cols*page_size, and those of a page id
+ * outside 0..n_pages-1, are neither written nor seen (of a sequence whose length passes
+ * its table, a token keeps its position and sees what the table holds).  Sequences may
  * share pages (a common prefix); where two new tokens come to the same slot, it holds
  * values of either. */
 typedef struct rie_hip_pages {

@@ -115,7 +115,8 @@ constexpr float P_SHIFT = BF ? 0.0f : 6.0f;
 constexpr float M_SLACK = 8.0f;  // how far a score may pass the maximum that is subtracted
 
 __device__ __forceinline__ SeqView uniform(const SeqView &v) {
-    return SeqView{__builtin_amdgcn_readfirstlane(v.row0), __builtin_amdgcn_readfirstlane(v.n_new), __builtin_amdgcn_readfirstlane(v.len)};
+    return SeqView{__builtin_amdgcn_readfirstlane(v.row0), __builtin_amdgcn_readfirstlane(v.n_new), __builtin_amdgcn_readfirstlane(v.len),
+                   __builtin_amdgcn_readfirstlane(v.over)};
 }
 // x, the same for the whole wave, where the compiler cannot see it (behind divisions, say):
 // kept in a scalar register, with branches on it that are no masks
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const int lb = (n_rows + TILE_M - 1) / TILE_M - 1 - (blk - block_base(sv.row0, si, G, TILE_M));  // a sequence's longest rows first
     if (lb < 0 || lb >= (n_rows + TILE_M - 1) / TILE_M) return;
     const int r0 = same(lb * TILE_M), r1 = same(imin(r0 + TILE_M, n_rows) - 1), tok0 = same(r0 / G), tok1 = same(r1 / G);
-    const int pos0 = sv.len - sv.n_new;  // position of token 0
+    const int pos0 = sv.pos0();  // position of token 0
     const KeyRange kr = key_range(sv, tok0, tok1, a.window);
     const int hi = same(kr.hi), nt = same(tile_count(kr, KT)), ns = same(split_count(nt, a.C, a.S));
     if (sp >= ns) return;
@@ -266,12 +267,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const int row = r0 + w * 32 + (lane & 31);
     const bool live = row < n_rows;
     const int tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
-    const int p_q = live ? pos0 + tok : -1;
-    const int lo_q = a.window > 0 ? p_q - a.window : -1;  // sees j in (lo_q, p_q]
+    const int p_q = live ? imin(pos0 + tok, sv.len - 1) : -1;
+    const int lo_q = a.window > 0 ? pos0 + tok - a.window : -1;  // sees j in (lo_q, p_q]
     const bool wave_live = r0 + w * 32 <= r1;
     const int w_t0 = same(imin(r0 + w * 32, r1) / G), w_t1 = same(imin(r0 + w * 32 + 31, r1) / G);
-    const int all_hi = pos0 + w_t0, all_lo = a.window > 0 ? pos0 + w_t1 - a.window : -1;  // every row of the wave sees (all_lo, all_hi]
-    const int wg_hi = pos0 + tok0, wg_lo = a.window > 0 ? pos0 + tok1 - a.window : -1;    // and of the workgroup
+    const int all_hi = imin(pos0 + w_t0, sv.len - 1), all_lo = a.window > 0 ? pos0 + w_t1 - a.window : -1;  // every row of the wave sees (all_lo, all_hi]
+    const int wg_hi = imin(pos0 + tok0, sv.len - 1), wg_lo = a.window > 0 ? pos0 + tok1 - a.window : -1;    // and of the workgroup
     u32x4 qf[KS];
     {
         const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + h * 16;
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
     const SeqView sv = view_of(a.b, a.kv, si);
     const int n_rows = imin(sv.n_new * G, 16 * NB);
     if (n_rows == 0) return;
-    const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.len - sv.n_new;
+    const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.pos0();
     const KeyRange kr = key_range(sv, 0, n_tok - 1, a.window);
     const int hi = same(kr.hi), t0 = same(first_tile(kr, FEW_STEP)), nt = same(tile_count(kr, FEW_STEP)), ns = same(split_count(nt, a.C, a.S)), sp = blockIdx.y;
     if (sp >= ns) return;
@@ -665,13 +666,13 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
     for (int b = 0; b < NB; b++) {
         const int row = b * 16 + col, tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
         const bool live = row < n_rows;
-        p_q[b] = live ? pos0 + tok : -1;
-        lo_q[b] = a.window > 0 ? p_q[b] - a.window : -1;
+        p_q[b] = live ? imin(pos0 + tok, sv.len - 1) : -1;
+        lo_q[b] = a.window > 0 ? pos0 + tok - a.window : -1;
         const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + g * 16;
 #pragma unroll
         for (int i = 0; i < KS; i++) qf[b][i] = live ? *(const u32x4 *)(qp + i * 64) : u32x4{0, 0, 0, 0};
     }
-    const int all_hi = pos0, all_lo = a.window > 0 ? pos0 + n_tok - 1 - a.window : -1;
+    const int all_hi = imin(pos0, sv.len - 1), all_lo = a.window > 0 ? pos0 + n_tok - 1 - a.window : -1;
 
     const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
     const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
@@ -870,7 +871,7 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
         for (int e = 0; e < 4; e++)
             if (acc[e] != acc[e] && L == L) {  // rare
                 const int p = pos0 + tok, j0 = imax(a.window > 0 ? imax(p + 1 - a.window, 0) : 0, (t0 + sp * a.C) * FEW_STEP);
-                const int j1 = imin(p + 1, (sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * FEW_STEP);
+                const int j1 = imin(imin(p + 1, sv.len), (sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * FEW_STEP);
                 acc[e] = nonfinite_sum<BF>(a.kv, trow, 0, vbase + (d4 * 4 + e) * 2, j0, j1);
             }
         if (ns == 1) {
@@ -984,9 +985,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     int si;
     const SeqView sv = find_seq(a.b, a.kv, row, si, [&](int s, int) { return iclamp(s, 0, a.b.n_rows); });
     if (row < sv.row0 || row >= sv.row0 + sv.n_new) return;
-    const int pos = sv.len - sv.n_new + row - sv.row0;
+    const int pos = sv.pos0() + row - sv.row0;
     int page;
-    if (pos < 0 || !page_of(a.kv, a.kv.table + (int64_t)si * a.kv.table_stride, pos, page)) return;
+    if (pos < 0 || pos >= sv.len || !page_of(a.kv, a.kv.table + (int64_t)si * a.kv.table_stride, pos, page)) return;
     const int64_t slot = pos & ((1 << a.kv.page_shift) - 1);
     const int per = a.hd / 8, n = a.n_kv * per;
     for (int i = lane; i < 2 * n; i += 64) {

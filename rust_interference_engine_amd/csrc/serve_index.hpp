@@ -21,10 +21,12 @@ RIE_HD int imin(int a, int b) { return a < b ? a : b; }
 RIE_HD int imax(int a, int b) { return a > b ? a : b; }
 
 // One sequence of a batch: rows [row0, row0 + n_new) hold its new tokens, the last of
-// its len positions.  Token t is at position len − n_new + t (negative: before the
-// sequence's first position, a token that sees nothing).
+// its len + over positions, of which the first len can be addressed.  Token t is at position
+// pos0() + t (negative: before the sequence's first position, a token that sees nothing;
+// len or more: a token that is written nowhere and sees the addressable ones before it).
 struct SeqView {
-    int row0, n_new, len;
+    int row0, n_new, len, over = 0;
+    RIE_HD int pos0() const { return len + over - n_new; }
 };
 // starts[i], starts[i + 1] and lens[i] as the device memory has them; n_rows rows exist,
 // cap positions can be addressed
@@ -33,6 +35,7 @@ RIE_HD SeqView seq_view(int start, int end, int len, int n_rows, int cap) {
     s.row0 = iclamp(start, 0, n_rows);
     s.n_new = iclamp(end, s.row0, n_rows) - s.row0;
     s.len = iclamp(len, 0, cap);
+    s.over = len > cap ? len - cap : 0;
     return s;
 }
 
@@ -49,8 +52,8 @@ struct KeyRange {
 };
 RIE_HD KeyRange key_range(const SeqView &s, int t0, int t1, int window) {
     KeyRange r;
-    const int p0 = s.len - s.n_new + t0, p1 = s.len - s.n_new + t1;
-    r.hi = imax(p1 + 1, 0);
+    const int p0 = s.pos0() + t0, p1 = s.pos0() + t1;
+    r.hi = iclamp(p1 + 1, 0, s.len);
     r.lo = window > 0 ? imax(imax(p0, 0) + 1 - window, 0) : 0;
     if (r.lo > r.hi) r.lo = r.hi;
     return r;

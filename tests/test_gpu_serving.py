@@ -176,6 +176,65 @@ def test_positions_of_pages_that_are_none_are_not_seen(ops, new):
         b.table.copy_(good)
 
 
+def past_the_table(lens, cap, *args, **kw):
+    """a batch whose tables address `cap` positions each, with lengths that may pass them"""
+    b = S.Batch([(n, cap) for n, _ in lens], *args, **kw)
+    b.L = torch.tensor([x for _, x in lens], dtype=torch.int32)
+    return b
+
+
+# (1, 90) and (6, 100) begin past the table; 2^31 - 1 lies behind any window
+PAST = [(1, 49), (3, 50), (1, 48), (1, 90), (6, 50), (6, 100), (2, 2 ** 31 - 1)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,KV,hd", [(2, 1, 32), (4, 1, 64), (4, 2, 96), (8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("window", [0, 1, 5, 40])
+@pytest.mark.parametrize("more", [[], [(70, 52), (30, 49), (20, 90)]])  # with the chunks, the tile kernel
+def test_tokens_past_the_table_see_what_it_addresses(ops, more, window, H, KV, hd, dtype):
+    lens = PAST + more
+    b = past_the_table(lens, 48, H, KV, hd, dtype=dtype, seed=32, extra_rows=1)
+    for kw in (dict(), dict(max_len=2 ** 30)):
+        got = paged(ops, b, window, **kw)
+        for i, (n, L) in enumerate(lens):
+            r = int(b.starts[i])
+            o, a, size = S.attend(b.q[r:r + n], b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, 1 / math.sqrt(hd), window)
+            tol = S.tolerance(o, a, size, 48, hd, dtype)
+            assert bool(((got[r:r + n].double() - o).abs() <= tol).all()), (i, n, L)
+        assert bool((got[-1] == 7).all())
+
+
+@pytest.mark.parametrize("new", [3, 40])
+def test_long_tables_that_end_before_the_sequence(ops, new):
+    lens = [(new, 3010), (1, 3001), (1, 2900)]
+    b = past_the_table(lens, 2944, 8, 2, 64, dtype=BF16, seed=33)
+    for window in (0, 700):
+        for kw in (dict(), dict(max_len=60000)):
+            got = paged(ops, b, window, **kw)
+            for i, (n, L) in enumerate(lens):
+                r = int(b.starts[i])
+                o, a, size = S.attend(b.q[r:r + n], b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, 1 / 8, window)
+                assert bool(((got[r:r + n].double() - o).abs() <= S.tolerance(o, a, size, 2944, 64, BF16)).all()), (i, n, L)
+
+
+def test_append_drops_the_tokens_past_the_table(ops):
+    lens = [(1, 33), (10, 37), (1, 32), (8, 40), (5, 2 ** 31 - 1), (40, 36), (1, -4)]
+    b = past_the_table(lens, 32, 2, 2, 64, seed=34)
+    g = torch.Generator().manual_seed(35)
+    new = torch.randn(b.rows, 4, 64, generator=g).half()
+    dev, k, v = new.to(GPU), b.k_pages.to(GPU), b.v_pages.to(GPU)
+    kv = ops.PagedKv(b.paged(k), b.paged(v), b.table.to(GPU))
+    ops.PagedAppend(kv, ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=40, max_len=64), dev[:, :2], dev[:, 2:])()
+    want_k, want_v = b.paged(b.k_pages).clone(), b.paged(b.v_pages).clone()
+    for i, (n, L) in enumerate(lens):
+        for t in range(n):
+            p = L - n + t
+            if 0 <= p < 32:
+                at = (int(b.table[i, p // 16]), p % 16)
+                want_k[at], want_v[at] = new[int(b.starts[i]) + t, :2], new[int(b.starts[i]) + t, 2:]
+    assert torch.equal(b.paged(k.cpu()), want_k) and torch.equal(b.paged(v.cpu()), want_v)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("H,KV,hd", [(4, 2, 32), (15, 5, 64), (4, 4, 96), (8, 2, 128), (8, 1, 128), (4, 1, 256)])
 @pytest.mark.parametrize("window,softcap", [(0, 0.0), (50, 0.0), (0, 4.0)])
