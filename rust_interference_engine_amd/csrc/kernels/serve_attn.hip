@@ -20,7 +20,7 @@
 // some token sees in part is searched for them, and if there are any, they are added to the
 // outputs one by one and replaced by zeros in the matrix product, where they would meet
 // probabilities of zero.  Outputs that are NaN all the same are formed from the infinite and NaN
-// values alone at the end (nonfinite_sum).
+// values alone at the end (NonFinite).
 //
 // Two kernels.  attn_tile_kernel takes 128 query rows (token · group + head of the group,
 // so the heads of a group share their keys) per workgroup and goes through the positions in
@@ -162,25 +162,97 @@ __device__ __forceinline__ bool page_of(const KvView &kv, const int *trow, int g
 
 template <int HD>
 constexpr int HDP = HD <= 64 ? 64 : HD <= 128 ? 128 : HD;  // values between rows of a tile in LDS
-// An output that came out as NaN, of a row whose probabilities' sum is a number: an infinite value
-// has met a probability that was rounded to zero, or a rounding's remainder of either sign.  The
-// true one is the sum of the infinite and NaN values at positions [j0, j1), which its token sees
-// (NaN itself where there are none).
-template <bool BF>
-__device__ __forceinline__ float nonfinite_sum(const KvView &kv, const int *trow, int row0, const uint8_t *v, int j0, int j1) {
-    float sum = 0;
-    for (int j = j0; j < j1; j++) {
-        int64_t at = (int64_t)(row0 + j) * kv.v_row;
-        if (trow) {
-            int page;
-            if (!page_of(kv, trow, j, page)) continue;
-            at = page * kv.page + (j & ((1 << kv.page_shift) - 1)) * kv.v_row;
-        }
-        const float x = value16<BF>(*(const uint16_t *)(v + at));
-        if (!(fabsf(x) <= FLT_MAX)) sum += x;
-    }
-    return sum == 0 ? NAN : sum;
+// Outputs that came out as NaN, of rows whose probabilities' sum is a number: an infinite value
+// has met a probability that was rounded to zero, or a rounding's remainder of either sign, or
+// there is a NaN.  The true one is the sum of the infinite and NaN values at the positions that
+// its token sees (NaN itself where there are none).  A wave searches them once for all of its
+// rows: the positions that every row sees 16 bytes to a lane, into sums that the rows share; of
+// those at either end that only some see, 31 at most (a wave's rows are of 32 tokens at most),
+// which ones hold such a value.  A prompt of 3000 tokens, 32 heads on 8 of 128: 107 us, with a
+// NaN row at its start 412, with nothing but NaN 589; 4 tokens over 40000 positions 40, 129, 152.
+// The kernels' arguments are read here again (late_args): kept for this from the start they would
+// be spilled, and read back in the loops.
+typedef const __attribute__((address_space(4))) ServeAttnArgs *LateArgs;
+__device__ __forceinline__ LateArgs late_args() {
+    auto *a = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return a;
 }
+template <int HD, bool BF>
+struct NonFinite {
+    float sum[8];   // over positions [s0, s1), of the 8 dims of chunk (lane % CPR)
+    uint64_t some;  // bit b: position(b) holds an infinite or NaN value
+    int u0, s0, s1;
+
+    __device__ __forceinline__ int position(int b) const { return b < s0 - u0 ? u0 + b : s1 + b - (s0 - u0); }
+    // sequence si's values of KV head kvh at position j, or nullptr; row0: its first row, in packed prompts
+    static __device__ __forceinline__ const uint8_t *row(LateArgs a, int si, int row0, int kvh, int j) {
+        const uint8_t *v = a->kv.v + kvh * a->kv.v_head;
+        if (!a->kv.table) return v + (int64_t)(row0 + j) * a->kv.v_row;
+        const int page = a->kv.table[(int64_t)si * a->kv.table_stride + (j >> a->kv.page_shift)];
+        if ((unsigned)page >= (unsigned)a->kv.n_pages) return nullptr;
+        return v + page * a->kv.page + (j & ((1 << a->kv.page_shift) - 1)) * a->kv.v_row;
+    }
+    static __device__ __forceinline__ float kept(uint32_t bits) {
+        const float x = value16<BF>(bits);
+        return fabsf(x) <= FLT_MAX ? 0.0f : x;
+    }
+    // Some row sees [from, to), all rows [all_from, all_to); the positions of the launch's split are
+    // [lo, hi).  The same for the wave, and all of its lanes call this.
+    __device__ __forceinline__ void search(LateArgs a, int si, int row0, int kvh, int from, int to, int all_from, int all_to, int lo, int hi) {
+        constexpr int CPR = HDP<HD> / 8, RPI = 64 / CPR, AT_ONCE = 4;
+        const int lane = threadIdx.x & 63, c = imin(lane % CPR, HD / 8 - 1) * 16, r = lane / CPR;
+        u0 = imax(from, lo);
+        const int u1 = imax(imin(to, hi), u0);
+        s0 = iclamp(all_from, u0, u1);
+        s1 = iclamp(all_to, s0, u1);
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum[e] = 0;
+        for (int j0 = s0; j0 < s1; j0 += AT_ONCE * RPI) {
+            u32x4 x[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++) {
+                const int j = j0 + i * RPI + r;
+                const uint8_t *p = j < s1 ? row(a, si, row0, kvh, j) : nullptr;
+                x[i] = p ? *(const u32x4 *)(p + c) : u32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++)
+                if (nonfinite8<BF>(x[i]))
+#pragma unroll
+                    for (int e = 0; e < 8; e++) sum[e] += kept(x[i][e / 2] >> (e & 1) * 16 & 0xFFFF);
+        }
+#pragma unroll
+        for (int o = CPR; o < 64; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum[e] += __shfl_xor(sum[e], o);
+        const int j = position(lane);
+        const uint8_t *p = j < (lane < s0 - u0 ? s0 : u1) ? row(a, si, row0, kvh, j) : nullptr;
+        bool any = false;
+        if (p)
+            for (int i = 0; i < HD / 8; i++) any = any || nonfinite8<BF>(*(const u32x4 *)(p + i * 16));
+        some = __ballot(any);
+    }
+    // of dims 8 c + 4 half …, for a row that sees positions (lo, hi]; all lanes call this
+    __device__ __forceinline__ f32x4 of(LateArgs a, int si, int row0, int kvh, int c, int half, int lo, int hi) const {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float s_lo = __shfl(sum[e], c), s_hi = __shfl(sum[4 + e], c);
+            x[e] = half ? s_hi : s_lo;
+        }
+        for (uint64_t m = some; m; m &= m - 1) {
+            const int j = position(__builtin_ctzll(m));
+            if (j <= lo || j > hi) continue;
+            const u32x2 y = *(const u32x2 *)(row(a, si, row0, kvh, j) + c * 16 + half * 8);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] += kept(y[e / 2] >> (e & 1) * 16 & 0xFFFF);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = x[e] == 0 ? NAN : x[e];
+        return x;
+    }
+};
 
 // score → exponent in log2 units, where the softcap makes it one already
 template <bool CAP>
@@ -577,11 +649,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     float l0, l1;
     pair_f<32>(l, l0, l1);
     l = l0 + l1;
-    if (!live) return;
-    // arguments that only the end needs are read here again: kept from the start they would be
-    // spilled, and read back in the loop
-    auto *late = (const __attribute__((address_space(4))) ServeAttnArgs *)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(late));
+    const LateArgs late = late_args();  // also what the stores need
     bool nan = false;
 #pragma unroll
     for (int d = 0; d < DB; d++)
@@ -591,7 +659,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     uint8_t *op = late->out + (int64_t)(sv.row0 + tok) * late->o_row + head * late->o_head + h * 8;
     const int64_t at = ((int64_t)(sv.row0 + tok) * late->n_head + head) * late->S + sp;
     float *pp = late->part + at * HD + 4 * h;
-    if (ns == 1) {
+    if (!live) {
+        // nothing to store; the search below is the whole wave's
+    } else if (ns == 1) {
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -606,15 +676,21 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
             for (int e = 0; e < 4; e++) *(f32x4 *)(pp + d * 32 + e * 8) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
         if (h == 0) *(f32x2 *)(late->ml + at * 2) = f32x2{m, l};
     }
-    if (nan && l == l) {  // rare
-        const int j0 = imax(imax(lo_q + 1, 0), t_begin * KT), j1 = imin(p_q + 1, t_end * KT);
-        for (int i = 0; i < HD / 2; i++) {  // the lane's dims: 8 (i / 4) + 4 h + i % 4
-            const int dim = i / 4 * 8 + i % 4;
-            uint16_t *x = (uint16_t *)op + dim;
-            if (ns == 1 ? value16<BF>(*x) == value16<BF>(*x) : pp[dim] == pp[dim]) continue;
-            const float v = nonfinite_sum<BF>(a.kv, trow, sv.row0, vbase + (dim + 4 * h) * 2, j0, j1);
-            if (ns == 1) *x = (uint16_t)pack2<BF>(v, v);
-            else pp[dim] = v;
+    const bool again = live && nan && l == l;
+    if (!__any(again)) return;
+    NonFinite<HD, BF> nf;
+    nf.search(late, si, sv.row0, kvh, late->window > 0 ? imax(pos0 + w_t0 - late->window + 1, 0) : 0, imin(pos0 + w_t1, sv.len - 1) + 1, all_lo + 1, all_hi + 1,
+              t_begin * KT, t_end * KT);
+    for (int k = 0; k < HD / 8; k++) {  // the lane's dims: 8 k + 4 h …
+        const f32x4 x = nf.of(late, si, sv.row0, kvh, k, h, lo_q, p_q);
+        if (!again) continue;
+        for (int e = 0; e < 4; e++) {
+            if (ns == 1) {
+                uint16_t *y = (uint16_t *)(op + k * 16) + e;
+                if (value16<BF>(*y) != value16<BF>(*y)) *y = (uint16_t)pack2<BF>(x[e], x[e]);
+            } else if (pp[k * 8 + e] != pp[k * 8 + e]) {
+                pp[k * 8 + e] = x[e];
+            }
         }
     }
 }
@@ -853,8 +929,12 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n_rows * (HD / 4); i += 256) {
-        const int r = i / (HD / 4), d4 = i % (HD / 4), tok = r / G, head = kvh * G + r - tok * G;
+    const LateArgs late = late_args();
+    NonFinite<HD, BF> nf;
+    bool searched = false;
+    for (int i0 = w * 64; i0 < n_rows * (HD / 4); i0 += 256) {
+        const bool live = i0 + lane < n_rows * (HD / 4);
+        const int i = live ? i0 + lane : i0, r = i / (HD / 4), d4 = i % (HD / 4), tok = r / G, head = kvh * G + r - tok * G;
         float mm = s_ml[0][r][0];
 #pragma unroll
         for (int k = 1; k < 4; k++) mm = fmaxf(mm, s_ml[k][r][0]);
@@ -868,20 +948,24 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] = fmaf(f, x[e], acc[e]);
         }
-        for (int e = 0; e < 4; e++)
-            if (acc[e] != acc[e] && L == L) {  // rare
-                const int p = pos0 + tok, j0 = imax(a.window > 0 ? imax(p + 1 - a.window, 0) : 0, (t0 + sp * a.C) * FEW_STEP);
-                const int j1 = imin(imin(p + 1, sv.len), (sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * FEW_STEP);
-                acc[e] = nonfinite_sum<BF>(a.kv, trow, 0, vbase + (d4 * 4 + e) * 2, j0, j1);
-            }
+        if (__any(L == L && (acc[0] != acc[0] || acc[1] != acc[1] || acc[2] != acc[2] || acc[3] != acc[3]))) {  // rare
+            if (!searched)
+                nf.search(late, si, 0, kvh, late->window > 0 ? imax(pos0 - late->window + 1, 0) : 0, imin(pos0 + n_tok - 1, sv.len - 1) + 1, all_lo + 1, all_hi + 1,
+                          (t0 + sp * late->C) * FEW_STEP, (sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * late->C) * FEW_STEP);
+            searched = true;
+            const f32x4 x = nf.of(late, si, 0, kvh, d4 / 2, d4 & 1, late->window > 0 ? pos0 + tok - late->window : -1, imin(pos0 + tok, sv.len - 1));
+            for (int e = 0; e < 4; e++)
+                if (L == L && acc[e] != acc[e]) acc[e] = x[e];
+        }
+        if (!live) break;
         if (ns == 1) {
             const float inv = L > 0 || L != L ? 1.0f / L : 0.0f;
-            uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d4 * 8;
+            uint8_t *op = late->out + (int64_t)(sv.row0 + tok) * late->o_row + head * late->o_head + d4 * 8;
             *(u32x2 *)op = u32x2{pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
         } else {
-            const int64_t at = ((int64_t)(sv.row0 + tok) * a.n_head + head) * a.S + sp;
-            *(f32x4 *)(a.part + at * HD + d4 * 4) = acc;
-            if (d4 == 0) *(f32x2 *)(a.ml + at * 2) = f32x2{mm, L};
+            const int64_t at = ((int64_t)(sv.row0 + tok) * late->n_head + head) * late->S + sp;
+            *(f32x4 *)(late->part + at * HD + d4 * 4) = acc;
+            if (d4 == 0) *(f32x2 *)(late->ml + at * 2) = f32x2{mm, L};
         }
     }
 }

@@ -151,6 +151,112 @@ def test_an_infinite_value_of_a_split_that_weighs_nothing(ops, dtype, lens):
         assert bool(torch.isfinite(out[rest]).all())
 
 
+def spoil(v, share, seed):
+    """a copy of values v with that share of them infinite or NaN"""
+    g = torch.Generator().manual_seed(seed)
+    v = v.clone()
+    at = torch.rand(v.shape, generator=g) < share
+    v[at] = torch.tensor([math.inf, -math.inf, math.nan])[torch.randint(0, 3, (int(at.sum()),), generator=g)].to(v.dtype)
+    return v
+
+
+def spoilt(v, pos0, n, window, H):
+    """[n, H, hd]: the sum of the infinite and NaN values that each of n tokens sees, 0 without one"""
+    L, KV, hd = v.shape
+    seen = []
+    for bad in (v.isnan(), v == math.inf, v == -math.inf):
+        c = torch.cat([torch.zeros(1, KV, hd), bad.float().cumsum(0)])
+        p = pos0 + torch.arange(n)
+        hi = (p + 1).clamp(0, L)
+        lo = (p + 1 - window).clamp(0, L) if window else torch.zeros_like(p)
+        seen.append((c[hi] - c[torch.minimum(lo, hi)]) > 0)
+    nan, up, down = seen
+    x = torch.where(nan | (up & down), math.nan, torch.where(up, math.inf, torch.where(down, -math.inf, 0.0)))
+    return x.repeat_interleave(H // KV, 1)
+
+
+def check_spoilt(got, q, k, v, pos0, window, dtype, hd):
+    n, H = q.shape[:2]
+    want = spoilt(v, pos0, n, window, H)
+    o, a, size = S.attend(q, k, torch.where(torch.isfinite(v.float()), v, torch.zeros((), dtype=dtype)), pos0, 1 / math.sqrt(hd), window)
+    fine = want == 0
+    assert torch.equal(got.float()[~fine].nan_to_num(1.0, 2.0, 3.0), want[~fine].float().nan_to_num(1.0, 2.0, 3.0))
+    tol = S.tolerance(o, a, size, k.shape[0], hd, dtype)
+    assert bool(((got.double() - o).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("share", [1e-4, 2e-3, 0.3])
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 32), (4, 1, 64), (6, 6, 96), (8, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("window", [0, 3, 40, 300])
+@pytest.mark.parametrize("lens", [[(1, 700), (5, 90), (3, 900), (1, 1)], [(1, 700), (130, 900), (77, 77)]])  # few rows; tiles
+def test_infinite_and_nan_values_anywhere(ops, lens, window, H, KV, hd, share, dtype):
+    b = S.Batch(lens, H, KV, hd, page=32, dtype=dtype, seed=36)
+    b.v_pages = spoil(b.v_pages, share, 37)
+    for kw in (dict(), dict(max_len=60000)):  # whole, and in splits
+        got = paged(ops, b, window, **kw)
+        for i, (n, L) in enumerate(lens):
+            r = int(b.starts[i])
+            check_spoilt(got[r:r + n], b.q[r:r + n], b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, window, dtype, hd)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 32), (4, 1, 64), (6, 6, 96), (8, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_infinite_and_nan_values_anywhere_in_packed_prompts(ops, window, H, KV, hd, dtype):
+    lens = [300, 1, 64, 130]
+    n = sum(lens)
+    g = torch.Generator().manual_seed(38)
+    q, k, v = (torch.randn(n, x, hd, generator=g).to(dtype) for x in (H, KV, KV))
+    v = spoil(v, 2e-3, 39)
+    starts = torch.tensor([0] + lens).cumsum(0).int()
+    out = torch.empty(n, H, hd, dtype=dtype, device=GPU)
+    ops.PackedAttention(ops.Seqs(starts.to(GPU), max_new=300, max_len=300), q.to(GPU), k.to(GPU), v.to(GPU), out, window=window)()
+    for i, L in enumerate(lens):
+        r = slice(int(starts[i]), int(starts[i]) + L)
+        check_spoilt(out.cpu()[r], q[r], k[r], v[r], 0, window, dtype, hd)
+
+
+@pytest.mark.parametrize("what", ["first row NaN", "last row NaN", "all NaN", "all infinite"])
+@pytest.mark.parametrize("case", ["packed", "chunk", "tokens"])
+def test_values_that_are_nan_do_not_stall_a_call(ops, case, what):
+    """the positions are searched once for all of a wave's rows: a call takes a few times its time, where a search for every
+    output took hundreds"""
+    H, KV, hd = 32, 8, 128
+    g = torch.Generator(device=GPU).manual_seed(40)
+    new, L = {"packed": (3000, 3000), "chunk": (500, 8000), "tokens": (4, 40000)}[case]
+    q = torch.randn(new, H, hd, device=GPU, generator=g).to(BF16)
+    k, v = (torch.randn(L // 64 + 1, 64, KV, hd, device=GPU, generator=g).to(BF16) for _ in range(2))
+    out = torch.empty_like(q)
+    starts, lens = torch.tensor([0, new], dtype=torch.int32, device=GPU), torch.tensor([L], dtype=torch.int32, device=GPU)
+    seqs = ops.Seqs(starts, lens, max_new=new, max_len=L)
+    if case == "packed":
+        call = ops.PackedAttention(seqs, q, k.flatten(0, 1)[:L], v.flatten(0, 1)[:L], out)
+    else:
+        call = ops.PagedAttention(ops.PagedKv(k, v, torch.arange(L // 64 + 1, dtype=torch.int32, device=GPU)[None]), seqs, q, out)
+
+    def time():
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(8)]
+        for x in e:
+            x.record()
+            call()
+        torch.cuda.synchronize()
+        return min(a.elapsed_time(b) for a, b in zip(e[1:], e[2:]))
+
+    clean = time()
+    assert bool(torch.isfinite(out).all())
+    rows = v.flatten(0, 1)[:L]
+    if what == "all infinite":
+        rows[:] = math.inf
+    else:
+        rows[{"first row NaN": slice(0, 1), "last row NaN": slice(L - 1, L), "all NaN": slice(0, L)}[what]] = math.nan
+    spoilt_ms = time()
+    print(f"{case}, {what}: {clean * 1e3:.0f} us, {spoilt_ms * 1e3:.0f} us")
+    sees = torch.arange(new, device=GPU) == new - 1 if what == "last row NaN" else torch.ones(new, dtype=torch.bool, device=GPU)
+    assert bool((out[sees] == math.inf).all() if what == "all infinite" else out[sees].isnan().all()) and bool(torch.isfinite(out[~sees]).all())
+    assert spoilt_ms < 20 * clean + 1, (clean, spoilt_ms)
+
+
 def test_slots_behind_the_last_position_may_hold_anything(ops):
     b = S.Batch([(1, 37), (20, 50), (2, 33)], 4, 2, 64, seed=7)
     clean = paged(ops, b)
