@@ -227,7 +227,8 @@ int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, v
  * strides of q, k, v, the pages and the outputs have to keep every row (of head_dim
  * consecutive values) 16-byte aligned; strides of rows, slots and heads go up to 2^26
  * bytes.  head_dim: 32, 64, 96, 128 or 256.  What a call writes may share no memory with
- * what it reads, and its rows none with one another.
+ * what it reads, and its rows none with one another: of the strides of what is written,
+ * every one has to cover what the smaller ones span (refused otherwise).
  *
  * stream: a hipStream_t of any device (NULL: the current device's null stream); the call
  * queues its kernels there and returns.  Pointers of host memory, or of another device

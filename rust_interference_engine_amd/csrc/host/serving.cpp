@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <vector>
 
 using rie::Error;
 using rie::guarded;
@@ -63,9 +64,19 @@ void check_rows(const void *p, int64_t row, int64_t head, int es, const char *wh
     if (row < 0 || row > most || head < 0 || head > most) throw bad(std::string(what) + ": strides have to lie in 0.." + std::to_string(most));
 }
 
-// Rows that are written: no two of them share a value by a stride that is too small
-void check_apart(int64_t n, int64_t stride, int hd, const char *what) {
-    if (n > 1 && stride < hd) throw bad(std::string(what) + ": strides below head_dim would make rows overlap");
+// Rows that are written, n of each dimension a stride apart: no two of them share a value.  Every
+// stride has to cover what the smaller ones span.
+struct Dim {
+    int64_t n, stride;
+};
+void check_apart(std::vector<Dim> dims, int hd, const char *what) {
+    std::sort(dims.begin(), dims.end(), [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+    __int128 span = hd;  // strides of up to 2^40 by counts of up to 2^31
+    for (const Dim &d : dims) {
+        if (d.n <= 1) continue;
+        if (d.stride < span) throw bad(std::string(what) + ": strides below head_dim, or below what the smaller ones span, would make rows overlap");
+        span += (__int128)(d.n - 1) * d.stride;
+    }
 }
 
 constexpr int MOST = 1 << 30;  // positions
@@ -147,8 +158,7 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
 void run_attention(const rie::ServeAttnArgs &a, const rie_hip_attn *at, void *ws, size_t ws_bytes, void *stream) {
     check_rows(at->q, at->q_row_stride, at->q_head_stride, 2, "q");
     check_rows(at->out, at->out_row_stride, at->out_head_stride, 2, "out");
-    check_apart(a.b.n_rows, at->out_row_stride, a.hd, "out");
-    check_apart(a.n_head, at->out_head_stride, a.hd, "out");
+    check_apart({{a.b.n_rows, at->out_row_stride}, {a.n_head, at->out_head_stride}}, a.hd, "out");
     const size_t need = rie::serve_attn_ws(a);
     if (ws_bytes < need) throw bad("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
     if ((uintptr_t)ws % 16) throw bad("ws has to be 16-byte aligned");
@@ -195,9 +205,10 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
         const int es = src_ty == rie::T_F32 ? 4 : 2;
         check_rows(k, row_stride, head_stride, es, "k");
         check_rows(v, row_stride, head_stride, es, "v");
-        check_apart(pages->page_size, pages->slot_stride, pages->head_dim, "pages");
-        check_apart(pages->n_kv, pages->head_stride, pages->head_dim, "pages");
-        check_apart(pages->n_pages, pages->page_stride, pages->head_dim, "pages");
+        // keys and values too, which may lie between one another
+        const int64_t apart = (const uint16_t *)pages->v - (const uint16_t *)pages->k;
+        check_apart({{pages->page_size, pages->slot_stride}, {pages->n_kv, pages->head_stride}, {pages->n_pages, pages->page_stride},
+                     {2, apart < 0 ? -apart : apart}}, pages->head_dim, "pages");
         a.k = (const uint8_t *)k;
         a.v = (const uint8_t *)v;
         a.k_row = a.v_row = row_stride * es;

@@ -51,7 +51,10 @@ def _int(x, what: str, least: int, most: int) -> int:
 
 
 def _written(t: torch.Tensor, what: str) -> None:
-    _need(all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride())), f"{what} is expanded: its rows would be written over one another")
+    span = 1  # of the dimensions with smaller strides
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        _need(st >= span, f"{what} is expanded or overlaps itself: its rows would be written over one another")
+        span += (n - 1) * st
 
 
 def _device(*tensors) -> torch.device:

@@ -180,3 +180,55 @@ def test_the_python_layers_numbers_and_dimensions():
     ]:
         with pytest.raises(RieError, match=text):
             make()
+
+
+@pytest.mark.parametrize("at", [
+    dict(out_row_stride=64),                                     # row r, head h + 1 is row r + 1, head h
+    dict(out_row_stride=192),                                    # the last head is the next row's first
+    dict(out_row_stride=64, out_head_stride=64 * 7),             # heads apart, by one row too little
+])
+def test_outputs_whose_rows_overlap_by_two_strides(at):
+    rc, m = paged(at=attn(**at))
+    assert rc == -5 and "out: strides below" in m, (rc, m)
+
+
+def append_refusal(pg):
+    L = _lib.lib()
+    return said(lambda e: L.rie_hip_k_paged_append(C.byref(pg), C.byref(seqs()), 1, P, P, 128, 64, None, e, 256))
+
+
+@pytest.mark.parametrize("pg", [
+    dict(slot_stride=64, head_stride=64, page_stride=64), dict(page_stride=64), dict(page_stride=1984), dict(head_stride=960), dict(slot_stride=128, head_stride=64, page_stride=1984),
+    dict(v=P), dict(v=P + 64), dict(v=P + 9 * 2048 * 2 - 16), dict(k=P + 2048, v=P),
+])
+def test_pages_whose_rows_overlap_by_two_strides(pg):
+    rc, m = append_refusal(pages(**{"v": P + (1 << 20), **pg}))
+    assert rc == -5 and "pages: strides below" in m, (rc, m)
+
+
+@pytest.mark.parametrize("pg", [
+    dict(), dict(v=P - 9 * 2048 * 2), dict(slot_stride=128, head_stride=64), dict(page_stride=4096, v=P + 2048 * 2),  # keys and values by the page
+    dict(slot_stride=128, head_stride=2048, page_stride=4096, v=P + 128),                                             # by the slot
+    dict(page_stride=1 << 40, n_pages=2 ** 31 - 1, v=P + (1 << 20)),
+])
+def test_pages_whose_rows_lie_apart_get_past_the_strides(pg):
+    if "page_stride" in pg and pg["page_stride"] == 1 << 40:  # a span of 2^71 values
+        rc, m = append_refusal(pages(**pg))
+    else:
+        rc, m = append_refusal(pages(**{"v": P + (1 << 20), **pg}))
+    assert rc == -5 and "overlap" not in m, (rc, m)  # made-up pointers, or no GPU at all
+
+
+def test_the_python_layers_written_tensors():
+    torch = pytest.importorskip("torch")
+    from rust_interference_engine_amd import RieError, ops
+
+    z = torch.zeros(100000, dtype=torch.float16)
+    q = z[:4 * 2 * 64].view(4, 2, 64)
+    sq = ops.Seqs(torch.zeros(3, dtype=torch.int32), max_new=4, max_len=4)
+    for stride in ((64, 64, 1), (96, 64, 1), (0, 64, 1), (64, 192, 1)):
+        with pytest.raises(RieError, match="out is expanded or overlaps"):
+            ops.PackedAttention(sq, q, q, q, z.as_strided((4, 2, 64), stride))
+    for stride in ((128, 64, 1), (64, 256, 1), (200, 72, 1)):
+        with pytest.raises(RieError, match="on one GPU"):  # past the strides
+            ops.PackedAttention(sq, q, q, q, z.as_strided((4, 2, 64), stride))
