@@ -144,7 +144,7 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
     a.G = at->n_head / n_kv;
     a.hd = hd;
     a.ty = ty;
-    a.window = std::min(at->window, MOST);
+    a.window = at->window;
     a.scale = at->scale;
     a.softcap = at->softcap;
     if (!kv.table) a.b.max_len = std::min(a.b.max_len, a.b.max_new);

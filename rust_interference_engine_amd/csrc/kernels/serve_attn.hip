@@ -340,11 +340,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const bool live = row < n_rows;
     const int tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
     const int p_q = live ? imin(pos0 + tok, sv.len - 1) : -1;
-    const int lo_q = a.window > 0 ? pos0 + tok - a.window : -1;  // sees j in (lo_q, p_q]
+    const int lo_q = before_window(pos0 + tok, a.window);  // sees j in (lo_q, p_q]
     const bool wave_live = r0 + w * 32 <= r1;
     const int w_t0 = same(imin(r0 + w * 32, r1) / G), w_t1 = same(imin(r0 + w * 32 + 31, r1) / G);
-    const int all_hi = imin(pos0 + w_t0, sv.len - 1), all_lo = a.window > 0 ? pos0 + w_t1 - a.window : -1;  // every row of the wave sees (all_lo, all_hi]
-    const int wg_hi = imin(pos0 + tok0, sv.len - 1), wg_lo = a.window > 0 ? pos0 + tok1 - a.window : -1;    // and of the workgroup
+    const int all_hi = imin(pos0 + w_t0, sv.len - 1), all_lo = before_window(pos0 + w_t1, a.window);  // every row of the wave sees (all_lo, all_hi]
+    const int wg_hi = imin(pos0 + tok0, sv.len - 1), wg_lo = before_window(pos0 + tok1, a.window);    // and of the workgroup
     u32x4 qf[KS];
     {
         const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + h * 16;
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     const bool again = live && nan && l == l;
     if (!__any(again)) return;
     NonFinite<HD, BF> nf;
-    nf.search(late, si, sv.row0, kvh, late->window > 0 ? imax(pos0 + w_t0 - late->window + 1, 0) : 0, imin(pos0 + w_t1, sv.len - 1) + 1, all_lo + 1, all_hi + 1,
+    nf.search(late, si, sv.row0, kvh, imax(before_window(pos0 + w_t0, late->window) + 1, 0), imin(pos0 + w_t1, sv.len - 1) + 1, all_lo + 1, all_hi + 1,
               t_begin * KT, t_end * KT);
     for (int k = 0; k < HD / 8; k++) {  // the lane's dims: 8 k + 4 h …
         const f32x4 x = nf.of(late, si, sv.row0, kvh, k, h, lo_q, p_q);
@@ -743,12 +743,12 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
         const int row = b * 16 + col, tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
         const bool live = row < n_rows;
         p_q[b] = live ? imin(pos0 + tok, sv.len - 1) : -1;
-        lo_q[b] = a.window > 0 ? pos0 + tok - a.window : -1;
+        lo_q[b] = before_window(pos0 + tok, a.window);
         const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + g * 16;
 #pragma unroll
         for (int i = 0; i < KS; i++) qf[b][i] = live ? *(const u32x4 *)(qp + i * 64) : u32x4{0, 0, 0, 0};
     }
-    const int all_hi = imin(pos0, sv.len - 1), all_lo = a.window > 0 ? pos0 + n_tok - 1 - a.window : -1;
+    const int all_hi = imin(pos0, sv.len - 1), all_lo = before_window(pos0 + n_tok - 1, a.window);
 
     const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
     const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
@@ -950,10 +950,10 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
         }
         if (__any(L == L && (acc[0] != acc[0] || acc[1] != acc[1] || acc[2] != acc[2] || acc[3] != acc[3]))) {  // rare
             if (!searched)
-                nf.search(late, si, 0, kvh, late->window > 0 ? imax(pos0 - late->window + 1, 0) : 0, imin(pos0 + n_tok - 1, sv.len - 1) + 1, all_lo + 1, all_hi + 1,
+                nf.search(late, si, 0, kvh, imax(before_window(pos0, late->window) + 1, 0), imin(pos0 + n_tok - 1, sv.len - 1) + 1, all_lo + 1, all_hi + 1,
                           (t0 + sp * late->C) * FEW_STEP, (sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * late->C) * FEW_STEP);
             searched = true;
-            const f32x4 x = nf.of(late, si, 0, kvh, d4 / 2, d4 & 1, late->window > 0 ? pos0 + tok - late->window : -1, imin(pos0 + tok, sv.len - 1));
+            const f32x4 x = nf.of(late, si, 0, kvh, d4 / 2, d4 & 1, before_window(pos0 + tok, late->window), imin(pos0 + tok, sv.len - 1));
             for (int e = 0; e < 4; e++)
                 if (L == L && acc[e] != acc[e]) acc[e] = x[e];
         }

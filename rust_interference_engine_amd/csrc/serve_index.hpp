@@ -46,6 +46,9 @@ RIE_HD SeqView seq_view(int start, int end, int len, int n_rows, int cap) {
 RIE_HD int block_base(int start, int i, int G, int M) { return (int)((int64_t)start * G / M) + i; }
 inline int64_t block_count(int n_rows, int n_seq, int G, int M) { return (int64_t)n_rows * G / M + n_seq; }
 
+// the last position before the window of a token at position p (window 0: none), for any p and
+// any window of 31 bits
+RIE_HD int before_window(int p, int window) { return window > 0 ? imax(p, -1) - window : -1; }
 // Positions [lo, hi) that at least one of tokens t0..t1 of s sees (window 0: all up to its own)
 struct KeyRange {
     int lo, hi;
@@ -54,7 +57,7 @@ RIE_HD KeyRange key_range(const SeqView &s, int t0, int t1, int window) {
     KeyRange r;
     const int p0 = s.pos0() + t0, p1 = s.pos0() + t1;
     r.hi = iclamp(p1 + 1, 0, s.len);
-    r.lo = window > 0 ? imax(imax(p0, 0) + 1 - window, 0) : 0;
+    r.lo = imax(before_window(p0, window) + 1, 0);
     if (r.lo > r.hi) r.lo = r.hi;
     return r;
 }

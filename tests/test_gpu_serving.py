@@ -310,6 +310,18 @@ def test_tokens_past_the_table_see_what_it_addresses(ops, more, window, H, KV, h
         assert bool((got[-1] == 7).all())
 
 
+@pytest.mark.parametrize("new", [2, 60])
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 30 + 20, 2 ** 31 - 1])
+def test_windows_as_long_as_they_may_be(ops, window, new):
+    lens = [(new, 2 ** 30 + 40), (1, 2 ** 31 - 1), (1, 48), (new, 30), (1, 2 ** 30 + 20)]
+    b = past_the_table(lens, 48, 8, 2, 64, seed=42)
+    got = paged(ops, b, window)
+    for i, (n, L) in enumerate(lens):
+        r = int(b.starts[i])
+        o, a, size = S.attend(b.q[r:r + n], b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, 1 / 8, window)
+        assert bool(((got[r:r + n].double() - o).abs() <= S.tolerance(o, a, size, 48, 64, F16)).all()), (i, n, L)
+
+
 @pytest.mark.parametrize("new", [3, 40])
 def test_long_tables_that_end_before_the_sequence(ops, new):
     lens = [(new, 3010), (1, 3001), (1, 2900)]

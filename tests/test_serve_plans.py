@@ -47,7 +47,7 @@ def test_key_ranges_end_with_the_table(lib):
         n, length = r.randint(1, 50), r.choice([r.randint(0, 200), r.randint(cap, cap + 60), 2 ** 31 - 1])
         t0 = r.randrange(n)
         t1 = r.randrange(t0, n)
-        window = r.choice([0, 1, 2, 30, 500, 2 ** 30])
+        window = r.choice([0, 1, 2, 30, 500, 2 ** 30, 2 ** 31 - 1])
         KT = r.choice([32, 64, 128])
         seen = set()
         for t in range(t0, t1 + 1):
