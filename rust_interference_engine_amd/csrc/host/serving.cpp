@@ -56,8 +56,8 @@ class OnDevice {
 
 bool is16(int ty) { return ty == rie::T_F16 || ty == rie::T_BF16; }
 
-// Rows of `values` of es bytes each start at p + any multiples of the strides: all 16-byte
-// aligned, and offsets within 2^27 bytes of a row step, so that 16 rows stay within 32 bits
+// Rows of values of es bytes each start at p + any multiples of the strides: all 16-byte
+// aligned, and strides of 2^26 bytes at most, so that 16 rows stay within 31 bits
 void check_rows(const void *p, int64_t row, int64_t head, int es, const char *what) {
     const int64_t a = 16 / es, most = ((int64_t)1 << 26) / es;
     if ((uintptr_t)p % 16 || row % a || head % a) throw bad(std::string(what) + ": rows have to be 16-byte aligned");
@@ -80,10 +80,11 @@ void check_apart(std::vector<Dim> dims, int hd, const char *what) {
 }
 
 constexpr int MOST = 1 << 30;  // positions
+constexpr int MOST_ROWS = (1 << 26) - 4;  // 4 to a workgroup of 256: a launch has under 2^32 threads
 
 rie::BatchView batch(const rie_hip_seqs *s, bool lens) {
     if (!s) throw bad("seqs is NULL");
-    if (s->n_seq < 1 || s->n_rows < 1 || s->n_seq >= 1 << 24 || s->n_rows >= 1 << 26) throw bad("n_seq has to lie in 1..2^24-1, n_rows in 1..2^26-1");
+    if (s->n_seq < 1 || s->n_rows < 1 || s->n_seq >= 1 << 24 || s->n_rows > MOST_ROWS) throw bad("n_seq has to lie in 1..2^24-1, n_rows in 1..2^26-4");
     if (s->max_new < 1 || s->max_len < 1 || s->max_new > MOST || s->max_len > MOST) throw bad("max_new and max_len have to lie in 1..2^30");
     rie::BatchView b;
     b.starts = s->starts;
@@ -150,8 +151,8 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
     if (!kv.table) a.b.max_len = std::min(a.b.max_len, a.b.max_new);
     else a.b.max_len = std::min(a.b.max_len, kv.cap);
     // a launch has under 2^32 threads: 256 to a workgroup, 4 (row, head) pairs to one where the splits are added up
-    if ((int64_t)a.b.n_rows * a.n_head >= 1 << 26 || ((int64_t)a.b.n_seq + (int64_t)a.b.n_rows * a.G / 128) * n_kv >= 1 << 24)
-        throw bad("n_rows*n_head has to stay under 2^26, n_seq*n_kv under 2^24");
+    if ((int64_t)a.b.n_rows * a.n_head > MOST_ROWS || ((int64_t)a.b.n_seq + (int64_t)a.b.n_rows * a.G / 128) * n_kv >= 1 << 24)
+        throw bad("n_rows*n_head has to lie in 1..2^26-4, n_seq*n_kv under 2^24");
     return a;
 }
 

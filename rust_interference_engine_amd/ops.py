@@ -121,7 +121,7 @@ class Seqs:
         self.max_new, self.max_len = _int(max_new, "max_new", 1, 1 << 30), _int(max_len, "max_len", 1, 1 << 30)
 
     def _struct(self, n_rows: int) -> _lib.Seqs:
-        _int(n_rows, "rows", 1, (1 << 26) - 1)
+        _int(n_rows, "rows", 1, (1 << 26) - 4)
         return _lib.Seqs(self.starts.numel() - 1, n_rows, self.max_new, self.max_len, self.starts.data_ptr(),
                          self.lens.data_ptr() if self.lens is not None else None)
 

@@ -232,3 +232,24 @@ def test_the_python_layers_written_tensors():
     for stride in ((128, 64, 1), (64, 256, 1), (200, 72, 1)):
         with pytest.raises(RieError, match="on one GPU"):  # past the strides
             ops.PackedAttention(sq, q, q, q, z.as_strided((4, 2, 64), stride))
+
+
+@pytest.mark.parametrize("n,refused", [((1 << 26) - 4, False), ((1 << 26) - 3, True), ((1 << 26) - 1, True)])
+def test_rows_that_a_launch_has_threads_for(n, refused):
+    L = _lib.lib()
+    pg = pages(v=P + (1 << 20))
+    rc, m = said(lambda e: L.rie_hip_k_paged_append(C.byref(pg), C.byref(seqs(n_rows=n)), 1, P, P, 128, 64, None, e, 256))
+    assert rc == -5 and ("1..2^26-4" in m) == refused, (rc, m)
+    rc, m = paged(pages(n_kv=1), seqs(n_rows=n), attn(n_head=1))
+    assert rc == -5 and ("1..2^26-4" in m) == refused, (rc, m)
+    rc, m = paged(pages(n_kv=1), seqs(n_rows=n // 2), attn(n_head=2))  # pairs of rows and heads
+    assert rc == -5 and ("1..2^26-4" in m) == (n // 2 * 2 > (1 << 26) - 4), (rc, m)
+    torch = pytest.importorskip("torch")
+    from rust_interference_engine_amd import RieError, ops
+
+    sq = ops.Seqs(torch.zeros(3, dtype=torch.int32), max_new=4, max_len=4)
+    if refused:
+        with pytest.raises(RieError, match="rows has to lie"):
+            sq._struct(n)
+    else:
+        assert sq._struct(n).n_rows == n
