@@ -229,6 +229,7 @@ int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, v
  * bytes.  head_dim: 32, 64, 96, 128 or 256.  What a call writes may share no memory with
  * what it reads, and its rows none with one another: of the strides of what is written,
  * every one has to cover what the smaller ones span (refused otherwise).
+ * The stride of a dimension with one entry (one row, head or page) is not looked at.
  *
  * stream: a hipStream_t of any device (NULL: the current device's null stream); the call
  * queues its kernels there and returns.  Pointers of host memory, or of another device

@@ -8,7 +8,6 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
-#include <vector>
 
 using rie::Error;
 using rie::guarded;
@@ -56,6 +55,9 @@ class OnDevice {
 
 bool is16(int ty) { return ty == rie::T_F16 || ty == rie::T_BF16; }
 
+// A dimension of one entry is at 0, whatever its stride says (that of a tensor's is arbitrary)
+int64_t used(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
+
 // Rows of values of es bytes each start at p + any multiples of the strides: all 16-byte
 // aligned, and strides of 2^26 bytes at most, so that 16 rows stay within 31 bits
 void check_rows(const void *p, int64_t row, int64_t head, int es, const char *what) {
@@ -69,8 +71,9 @@ void check_rows(const void *p, int64_t row, int64_t head, int es, const char *wh
 struct Dim {
     int64_t n, stride;
 };
-void check_apart(std::vector<Dim> dims, int hd, const char *what) {
-    std::sort(dims.begin(), dims.end(), [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+template <size_t N>
+void check_apart(Dim (&&dims)[N], int hd, const char *what) {
+    std::sort(dims, dims + N, [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
     __int128 span = hd;  // strides of up to 2^40 by counts of up to 2^31
     for (const Dim &d : dims) {
         if (d.n <= 1) continue;
@@ -108,15 +111,16 @@ rie::KvView pages_view(const rie_hip_pages *p) {
     if (p->page_size < 16 || p->page_size > 4096 || (p->page_size & (p->page_size - 1)))
         throw Error{rie::E_UNSUPPORTED, "page_size has to be a power of two in 16..4096"};
     if (p->n_pages < 1 || p->table_cols < 1 || p->table_stride < 0) throw bad("n_pages and table_cols have to be positive");
-    check_rows(p->k, p->slot_stride, p->head_stride, 2, "pages");
-    check_rows(p->v, p->slot_stride, p->head_stride, 2, "pages");
-    if (p->page_stride < 0 || p->page_stride % 8 || p->page_stride > ((int64_t)1 << 40)) throw bad("pages: page_stride has to be a multiple of 8 in 0..2^40");
+    const int64_t head = used(p->n_kv, p->head_stride), page = used(p->n_pages, p->page_stride);
+    check_rows(p->k, p->slot_stride, head, 2, "pages");
+    check_rows(p->v, p->slot_stride, head, 2, "pages");
+    if (page < 0 || page % 8 || page > ((int64_t)1 << 40)) throw bad("pages: page_stride has to be a multiple of 8 in 0..2^40");
     rie::KvView v;
     v.k = (const uint8_t *)p->k;
     v.v = (const uint8_t *)p->v;
     v.k_row = v.v_row = p->slot_stride * 2;
-    v.k_head = v.v_head = p->head_stride * 2;
-    v.page = p->page_stride * 2;
+    v.k_head = v.v_head = head * 2;
+    v.page = page * 2;
     v.table = p->table;
     v.table_stride = p->table_stride;
     v.page_shift = __builtin_ctz((unsigned)p->page_size);
@@ -136,10 +140,10 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
     if (at->window < 0) throw bad("window has to be 0 (none) or positive");
     a.q = (const uint8_t *)at->q;
     a.out = (uint8_t *)at->out;
-    a.q_row = at->q_row_stride * 2;
-    a.q_head = at->q_head_stride * 2;
-    a.o_row = at->out_row_stride * 2;
-    a.o_head = at->out_head_stride * 2;
+    a.q_row = used(a.b.n_rows, at->q_row_stride) * 2;
+    a.q_head = used(at->n_head, at->q_head_stride) * 2;
+    a.o_row = used(a.b.n_rows, at->out_row_stride) * 2;
+    a.o_head = used(at->n_head, at->out_head_stride) * 2;
     a.n_head = at->n_head;
     a.n_kv = n_kv;
     a.G = at->n_head / n_kv;
@@ -156,10 +160,10 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
     return a;
 }
 
-void run_attention(const rie::ServeAttnArgs &a, const rie_hip_attn *at, void *ws, size_t ws_bytes, void *stream) {
-    check_rows(at->q, at->q_row_stride, at->q_head_stride, 2, "q");
-    check_rows(at->out, at->out_row_stride, at->out_head_stride, 2, "out");
-    check_apart({{a.b.n_rows, at->out_row_stride}, {a.n_head, at->out_head_stride}}, a.hd, "out");
+void run_attention(const rie::ServeAttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
+    check_rows(a.q, a.q_row / 2, a.q_head / 2, 2, "q");
+    check_rows(a.out, a.o_row / 2, a.o_head / 2, 2, "out");
+    check_apart({{a.b.n_rows, a.o_row / 2}, {a.n_head, a.o_head / 2}}, a.hd, "out");
     const size_t need = rie::serve_attn_ws(a);
     if (ws_bytes < need) throw bad("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
     if ((uintptr_t)ws % 16) throw bad("ws has to be 16-byte aligned");
@@ -178,8 +182,12 @@ void run_attention(const rie::ServeAttnArgs &a, const rie_hip_attn *at, void *ws
     RIE_HIP_CHECK(hipGetLastError());
 }
 
-rie::KvView packed_view(int ty, int hd, int n_kv, const void *k, const void *v, int64_t kr, int64_t kh, int64_t vr, int64_t vh) {
+rie::KvView packed_view(int ty, int hd, int n_kv, int n_rows, const void *k, const void *v, int64_t kr, int64_t kh, int64_t vr, int64_t vh) {
     check_heads(ty, hd, n_kv);
+    kr = used(n_rows, kr);
+    vr = used(n_rows, vr);
+    kh = used(n_kv, kh);
+    vh = used(n_kv, vh);
     check_rows(k, kr, kh, 2, "k");
     check_rows(v, vr, vh, 2, "v");
     rie::KvView x;
@@ -204,16 +212,17 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
         a.b = batch(seqs, true);
         if (src_ty != rie::T_F32 && src_ty != pages->ty) throw Error{rie::E_UNSUPPORTED, "new rows have to be f32 or of the pages' type"};
         const int es = src_ty == rie::T_F32 ? 4 : 2;
-        check_rows(k, row_stride, head_stride, es, "k");
-        check_rows(v, row_stride, head_stride, es, "v");
+        const int64_t row = used(a.b.n_rows, row_stride), head = used(pages->n_kv, head_stride);
+        check_rows(k, row, head, es, "k");
+        check_rows(v, row, head, es, "v");
         // keys and values too, which may lie between one another
         const int64_t apart = (const uint16_t *)pages->v - (const uint16_t *)pages->k;
         check_apart({{pages->page_size, pages->slot_stride}, {pages->n_kv, pages->head_stride}, {pages->n_pages, pages->page_stride},
                      {2, apart < 0 ? -apart : apart}}, pages->head_dim, "pages");
         a.k = (const uint8_t *)k;
         a.v = (const uint8_t *)v;
-        a.k_row = a.v_row = row_stride * es;
-        a.k_head = a.v_head = head_stride * es;
+        a.k_row = a.v_row = row * es;
+        a.k_head = a.v_head = head * es;
         a.n_kv = pages->n_kv;
         a.hd = pages->head_dim;
         a.ty = pages->ty;
@@ -245,7 +254,7 @@ int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs
     return guarded(err, err_len, [&] {
         const rie::KvView kv = pages_view(pages);
         if (!kv.table) throw bad("table is NULL");
-        run_attention(attention(seqs, attn, pages->ty, pages->head_dim, pages->n_kv, kv), attn, ws, ws_bytes, stream);
+        run_attention(attention(seqs, attn, pages->ty, pages->head_dim, pages->n_kv, kv), ws, ws_bytes, stream);
     });
 }
 
@@ -262,8 +271,9 @@ int32_t rie_hip_k_packed_attention(const rie_hip_seqs *seqs, int32_t ty, int32_t
                                    int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
                                    const rie_hip_attn *attn, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len) {
     return guarded(err, err_len, [&] {
-        const rie::KvView kv = packed_view(ty, head_dim, n_kv, k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride);
-        run_attention(attention(seqs, attn, ty, head_dim, n_kv, kv), attn, ws, ws_bytes, stream);
+        if (!seqs) throw bad("seqs is NULL");
+        const rie::KvView kv = packed_view(ty, head_dim, n_kv, seqs->n_rows, k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride);
+        run_attention(attention(seqs, attn, ty, head_dim, n_kv, kv), ws, ws_bytes, stream);
     });
 }
 

@@ -57,6 +57,11 @@ def _written(t: torch.Tensor, what: str) -> None:
         span += (n - 1) * st
 
 
+def _strides(t: torch.Tensor) -> tuple:
+    """strides that count: a dimension of one entry has none"""
+    return tuple(st if n > 1 else 0 for n, st in zip(t.shape, t.stride()))
+
+
 def _device(*tensors) -> torch.device:
     d = tensors[0].device
     for t in tensors:
@@ -133,8 +138,8 @@ class PagedKv:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
         _need(k.dim() == 4 and k.numel() > 0, f"pages have to be [pages, page size, KV heads, head size], got {tuple(k.shape)}")
-        _need(k.shape == v.shape and k.dtype == v.dtype and k.stride() == v.stride(), "k and v have to have one shape, type and strides")
-        _need(k.stride(3) == 1, "pages: a row's values have to be consecutive")
+        _need(k.shape == v.shape and k.dtype == v.dtype and _strides(k) == _strides(v), "k and v have to have one shape, type and strides")
+        _need(k.shape[3] == 1 or k.stride(3) == 1, "pages: a row's values have to be consecutive")
         _ints(table, "table", 2)
         _need(table.numel() > 0, "table is empty")
         self.device = _device(k, v, table)
@@ -157,7 +162,7 @@ class PagedAppend(_Op):
     def __init__(self, kv: PagedKv, seqs: Seqs, k: torch.Tensor, v: torch.Tensor):
         hd = kv.k.shape[3]
         _rows(k, "k", hd), _rows(v, "v", hd)
-        _need(k.shape == v.shape and k.dtype == v.dtype and k.stride() == v.stride(), "k and v have to have one shape, type and strides")
+        _need(k.shape == v.shape and k.dtype == v.dtype and _strides(k) == _strides(v), "k and v have to have one shape, type and strides")
         _need(k.shape[1] == kv.k.shape[2], f"k has {k.shape[1]} heads, the pages {kv.k.shape[2]}")
         _check_seqs(seqs, kv.table)
         _written(kv.k, "pages")

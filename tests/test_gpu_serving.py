@@ -699,6 +699,48 @@ def test_packed_prompts_keep_infinite_and_nan_values_to_the_tokens_behind_them(o
     assert bool((out[70 + 17:110, 2:, 2] == math.inf).all()) and bool(out[69, :2, 0].isnan().all()) and bool((out[110:, :2, hd - 1] == -math.inf).all())
 
 
+def test_strides_of_dimensions_with_one_entry_mean_nothing(ops):
+    """one KV head, one row, one page: views whose strides there are odd, far too large or different"""
+    g = torch.Generator(device=GPU).manual_seed(43)
+    i32 = dict(dtype=torch.int32, device=GPU)
+    mk = lambda *shape: torch.randn(*shape, device=GPU, generator=g).half()  # noqa: E731
+    n, hd = 30, 64
+    k, v = mk(n, hd), mk(n, hd)
+    heads = [k.as_strided((n, 1, hd), (hd, 7, 1)), v.as_strided((n, 1, hd), (hd, 1 << 40, 1))]
+    plain = [k.view(n, 1, hd), v.view(n, 1, hd)]
+    q = mk(n, 2, hd)
+    prompts = ops.Seqs(torch.tensor([0, n], **i32), max_new=n, max_len=n)
+    outs = []
+    for kk, vv in (heads, plain):
+        outs.append(torch.empty_like(q))
+        ops.PackedAttention(prompts, q, kk, vv, outs[-1])()
+    assert torch.equal(*outs)
+
+    pages = [[mk(2, 16, 1, hd), mk(2, 16, 1, hd)] for _ in range(1)] * 2
+    table = torch.tensor([[1, 0]], **i32)
+    kept = []
+    for i, (kk, vv) in enumerate((heads, plain)):
+        pk, pv = (x.clone() for x in pages[i])
+        if i == 0:
+            pk, pv = pk.as_strided(pk.shape, (16 * hd, hd, 3, 1)), pv.as_strided(pv.shape, (16 * hd, hd, 1 << 50, 1))
+        kv = ops.PagedKv(pk, pv, table)
+        seqs = ops.Seqs(torch.tensor([0, n], **i32), torch.tensor([n], **i32), max_new=n, max_len=32)
+        ops.PagedAppend(kv, seqs, kk, vv)()
+        one = ops.Seqs(torch.tensor([0, 1], **i32), torch.tensor([n], **i32), max_new=1, max_len=32)
+        q1 = mk(1, 2, hd) if i == 0 else q1
+        out = torch.empty(200, dtype=F16, device=GPU).as_strided((1, 2, hd), (13, hd, 1)) if i == 0 else torch.empty(1, 2, hd, dtype=F16, device=GPU)
+        ops.PagedAttention(kv, one, q1.as_strided((1, 2, hd), (5, hd, 1)) if i == 0 else q1, out)()
+        kept.append((pk.reshape(-1).clone(), pv.reshape(-1).clone(), out.reshape(-1).clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*kept))
+    assert torch.equal(kept[0][0].view(2, 16, hd)[1], k[:16]) and torch.equal(kept[0][1].view(2, 16, hd)[0, :14], v[16:])
+
+    page = mk(1, 16, 2, hd)  # one page
+    a = ops.PagedKv(page.as_strided(page.shape, (9, 2 * hd, hd, 1)), page.clone().as_strided(page.shape, (1 << 45, 2 * hd, hd, 1)), torch.zeros(1, 1, **i32))
+    out = torch.empty(1, 2, hd, dtype=F16, device=GPU)
+    ops.PagedAttention(a, ops.Seqs(torch.tensor([0, 1], **i32), torch.tensor([1], **i32), max_new=1, max_len=16), q[:1], out)()
+    assert torch.equal(out[0], page[0, 0])  # of one position its value
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_logprobs_where_every_group_counts(ops, dtype):
     """vocabularies past the registers' groups, equal maxima in many groups, masked heads and tails"""

@@ -253,3 +253,21 @@ def test_rows_that_a_launch_has_threads_for(n, refused):
             sq._struct(n)
     else:
         assert sq._struct(n).n_rows == n
+
+
+def test_strides_of_dimensions_with_one_entry_are_not_looked_at():
+    L = _lib.lib()
+    odd = 3
+    one = pages(n_kv=1, n_pages=1, head_stride=odd, page_stride=-odd, v=P + (1 << 20))
+    for call in (lambda e: L.rie_hip_k_paged_append(C.byref(one), C.byref(seqs(n_rows=1)), 1, P, P, odd, -odd, None, e, 256),
+                 lambda e: L.rie_hip_k_paged_attention(C.byref(one), C.byref(seqs(n_rows=1)), C.byref(attn(
+                     n_head=1, q_row_stride=odd, q_head_stride=1 << 50, out_row_stride=odd, out_head_stride=-1)), P, 1 << 40, None, e, 256),
+                 lambda e: L.rie_hip_k_packed_attention(C.byref(seqs(n_rows=1)), 1, 64, 1, P, P, odd, odd, -odd, 1 << 50, C.byref(attn(n_head=1, out_row_stride=0)), P, 1 << 40, None, e, 256)):
+        rc, m = said(call)
+        assert rc == -5 and "stride" not in m and "aligned" not in m, (rc, m)  # made-up pointers, or no GPU at all
+    torch = pytest.importorskip("torch")
+    from rust_interference_engine_amd import RieError, ops
+
+    z = torch.zeros(4096, dtype=torch.float16)
+    with pytest.raises(RieError, match="on one GPU"):  # past the strides
+        ops.PagedKv(z.as_strided((2, 16, 1, 64), (1024, 64, 5, 1)), z.as_strided((2, 16, 1, 64), (1024, 64, 64, 1)), torch.zeros(1, 1, dtype=torch.int32))
