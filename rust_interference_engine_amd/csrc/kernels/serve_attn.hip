@@ -266,12 +266,12 @@ __device__ __forceinline__ float cap_score(float s, float in, float out) {
 // and dst the same for the wave.  Written as the instruction, since the compiler waits for the
 // builtin's copies before it reads any LDS, also of the buffers that they do not write; it has
 // no result register, and the callers wait (wait_vmem) before the barrier behind which the
-// copy is read.  Nothing else here uses m0.  Loads return in order, so waits that count without these wait longer at most.
+// copy is read.  Loads return in order, so waits that count without these wait longer at most.
 __device__ __forceinline__ void copy_lds(const uint8_t *base, int off, const uint8_t *dst) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(dst));
     const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32)) << 32 |
                           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(from) : "m0", "memory");
 }
 
 constexpr int TILE_M = 128;  // query rows of a workgroup

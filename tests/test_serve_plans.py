@@ -1,4 +1,4 @@
-"""More of csrc/serve_index.hpp on the host: sequences whose length passes what their table can address."""
+"""More of csrc on the host: sequences whose length passes what their table can address (serve_index.hpp), inline assembly."""
 import ctypes
 import os
 import random
@@ -61,3 +61,19 @@ def test_key_ranges_end_with_the_table(lib):
             continue
         assert (lo, hi) == (min(seen), max(seen) + 1)
         assert first * KT <= lo and (first + tiles) * KT >= hi and (first + tiles - 1) * KT < hi
+
+
+def test_inline_assembly_names_the_registers_it_writes():
+    """m0 is the compiler's too: a block that writes it says so"""
+    found = 0
+    for folder in (CSRC, os.path.join(CSRC, "kernels")):
+        for name in sorted(os.listdir(folder)):
+            if not name.endswith((".hip", ".hpp")):
+                continue
+            with open(os.path.join(folder, name)) as f:
+                text = f.read()
+            for at in [i for i in range(len(text)) if text.startswith("s_mov_b32 m0", i)]:
+                block = text[at:text.index(";\n", at)]
+                assert '"m0"' in block.rsplit(":", 1)[1], (name, block)
+                found += 1
+    assert found
