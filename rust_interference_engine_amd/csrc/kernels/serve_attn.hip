@@ -254,12 +254,24 @@ struct NonFinite {
     }
 };
 
-// score → exponent in log2 units, where the softcap makes it one already
+// score → exponent in log2 units where there is a softcap (the same score where there is none).
+// With x = score / cap, cap · tanh(x) is score · (1 − x²/3 + 2x⁴/15 − 17x⁶/315) for |x| under 0.2
+// (the next term is 2^-24), and cap · (1 − 2 / (e^2x + 1)) beyond, whose difference keeps 2^-22 of
+// the cap: of a score that is a small part of a large cap it would keep nothing.  A scale by cap
+// beyond the range of f32 is cut there, so that a score of 0 stays 0.
+struct SoftCap {
+    float in, lin, out;
+};
+__device__ __forceinline__ SoftCap soft_cap(const ServeAttnArgs &a) {
+    return SoftCap{fminf(a.scale / a.softcap, FLT_MAX), a.scale * LOG2E_F, fminf(a.softcap * LOG2E_F, FLT_MAX)};
+}
 template <bool CAP>
-__device__ __forceinline__ float cap_score(float s, float in, float out) {
+__device__ __forceinline__ float cap_score(float s, const SoftCap &k) {
     if constexpr (!CAP) return s;
-    const float e = exp2_hw(s * in);  // e^(2 s / cap)
-    return out * (1.0f - 2.0f / (e + 1.0f));
+    const float x = s * k.in, t = x * x, e = exp2_hw(x * (2.0f * LOG2E_F));
+    const float near = s * k.lin * fmaf(fmaf(fmaf(-17.0f / 315.0f, t, 2.0f / 15.0f), t, -1.0f / 3.0f), t, 1.0f);
+    const float far = k.out * fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    return fabsf(x) < 0.2f ? near : far;
 }
 
 // 16 bytes per lane from global memory (base + off) to LDS: lane l's go to dst + 16·l, with base
@@ -409,7 +421,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
     float m = -FLT_MAX, l = 0, ym = 0;  // ym: largest score of the group whose turn is next
     // exponent of a score in log2 units is s · c
-    const float c = CAP ? 1.0f : a.scale * LOG2E_F, cap_in = CAP ? 2.0f * LOG2E_F * a.scale / a.softcap : 0.0f, cap_out = CAP ? a.softcap * LOG2E_F : 0.0f;
+    const float c = CAP ? 1.0f : a.scale * LOG2E_F;
+    const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
     // the lane's places in a tile: keys row-wise, values transposed
     const int k_at = Lds::key(lane & 31, h), v_at = Lds::value(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
 
@@ -445,7 +458,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_tile_kernel(Serve
         if (CAP || late || early || bad2) {
             if constexpr (CAP) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) x[e] = cap_score<CAP>(x[e], cap_in, cap_out);
+                for (int e = 0; e < 16; e++) x[e] = cap_score<CAP>(x[e], cap);
             }
             if (late) {
                 const int d = p_q - key0 - 4 * h;
@@ -801,7 +814,8 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
 #pragma unroll
         for (int d = 0; d < DB; d++) o[b][d] = f32x4{};
     }
-    const float c = CAP ? 1.0f : a.scale * LOG2E_F, cap_in = CAP ? 2.0f * LOG2E_F * a.scale / a.softcap : 0.0f, cap_out = CAP ? a.softcap * LOG2E_F : 0.0f;
+    const float c = CAP ? 1.0f : a.scale * LOG2E_F;
+    const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
     const int v_at = Lds::value(4 * g + (col >> 2), (lane & 3) >> 1) + (lane & 1) * 8;
 
     Pages pg{};
@@ -870,7 +884,7 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    if constexpr (CAP) s[b][kb][e] = cap_score<CAP>(s[b][kb][e], cap_in, cap_out);
+                    if constexpr (CAP) s[b][kb][e] = cap_score<CAP>(s[b][kb][e], cap);
                     if (part) {
                         const int j = key0 + kb * 16 + 4 * g + e;
                         s[b][kb][e] = (j > p_q[b]) | (j <= lo_q[b]) | (bad >> kb & 1) ? -INFINITY : s[b][kb][e];

@@ -699,6 +699,26 @@ def test_packed_prompts_keep_infinite_and_nan_values_to_the_tokens_behind_them(o
     assert bool((out[70 + 17:110, 2:, 2] == math.inf).all()) and bool(out[69, :2, 0].isnan().all()) and bool((out[110:, :2, hd - 1] == -math.inf).all())
 
 
+@pytest.mark.parametrize("softcap", [1e-38, 1e-3, 0.5, 30.0, 50.0, 1e3, 1e5, 1e7, 1e12, 1e30, 3e38])
+@pytest.mark.parametrize("lens", [[(1, 300), (3, 77)], [(1, 300), (60, 100)]])  # few rows; tiles
+def test_softcaps_of_any_size(ops, lens, softcap):
+    b = S.Batch(lens, 8, 2, 64, dtype=F16, seed=44)
+    b.q *= 4  # scores of up to 30 or so
+    scale = 1 / 8
+    got = paged(ops, b, softcap=softcap)
+    for i, (n, L) in enumerate(b.lens):
+        r = int(b.starts[i])
+        q, k = b.q[r:r + n], b.cached(b.k_pages, i)
+        o, a, size = S.attend(q, k, b.cached(b.v_pages, i), L - n, scale, 0, softcap)
+        # a capped score is off by 2^-21 of the cap where it is a fifth of it at least, and by a few steps of its own size
+        # below that: 2^-19 of the score itself in any case, next to the score's own error, which the cap only makes smaller
+        s = q.double().transpose(0, 1) @ k.double().transpose(0, 1).repeat_interleave(4, 0).transpose(1, 2) * scale
+        top = float((softcap * torch.tanh(s / softcap)).abs().max())
+        tol = S.tolerance(o, a, size, L, 64, F16) + 2 * 2.0 ** -19 * top * a
+        err = (got[r:r + n].double() - o).abs()
+        assert bool((err <= tol).all()), (i, float((err / tol).max()))
+
+
 def test_strides_of_dimensions_with_one_entry_mean_nothing(ops):
     """one KV head, one row, one page: views whose strides there are odd, far too large or different"""
     g = torch.Generator(device=GPU).manual_seed(43)
