@@ -8,7 +8,8 @@ only queues the kernels, on ``stream`` (a ``torch.cuda.Stream``) or else on torc
 current stream of the tensors' device, and reads the tensors as they are by then, so it
 can be captured into a graph.  An object's calls share its workspace: two that may run at
 the same time need an object each.  Keep the object until its calls have finished (one
-that a graph has captured: as long as the graph is replayed).  There are no gradients.
+that a graph has captured: as long as the graph is replayed); one that is made within a
+capture belongs to that graph.  There are no gradients.
 
     kv = ops.PagedKv(k_pages, v_pages, table)
     seqs = ops.Seqs(starts, lens, max_new=1, max_len=4096)
@@ -32,6 +33,11 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml type i
 def _current_stream(device: int) -> int:
     """the handle of torch's current stream: 0.1 us, where torch.cuda.current_stream takes 2"""
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _capturing(stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _need(ok, what: str) -> None:
@@ -91,6 +97,11 @@ class _Op:
         self._fn, self._device, self._keep = fn, device, keep
         self._err = C.create_string_buffer(512)
         self.workspace = torch.empty(workspace, dtype=torch.uint8, device=device) if workspace else None
+        if workspace:
+            # Its memory may still be in use by what the current stream has queued: a call on another one waits for that.
+            made_on = torch.cuda.current_stream(device)
+            self._ordered, self._captured = {made_on.cuda_stream}, _capturing(made_on)
+            self._made = made_on.record_event()
         if ws_at is not None:
             args = args[:ws_at] + [self.workspace.data_ptr() if workspace else None, workspace] + args[ws_at:]
         self._args = args
@@ -101,6 +112,8 @@ class _Op:
         else:
             _need(stream.device == self._device, f"stream of {stream.device}, tensors on {self._device}")
             handle = stream.cuda_stream
+        if self.workspace is not None and handle not in self._ordered:
+            self._order(torch.cuda.current_stream(self._device) if stream is None else stream)
         if handle == 0 and torch.cuda.current_device() != self._device.index:  # every device's null stream is 0
             with torch.cuda.device(self._device):
                 rc = self._fn(*self._args, None, self._err, 512)
@@ -108,6 +121,13 @@ class _Op:
             rc = self._fn(*self._args, handle, self._err, 512)
         if rc:
             raise RieError(rc, self._err.value.decode(errors="replace"))
+
+    def _order(self, stream) -> None:
+        # a capture waits for events of its own only (torch.cuda.graph has waited for the device before it begins)
+        if _capturing(stream) == self._captured:
+            stream.wait_event(self._made)
+            if not self._captured:
+                self._ordered.add(stream.cuda_stream)
 
 
 class Seqs:

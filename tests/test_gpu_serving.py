@@ -719,6 +719,63 @@ def test_softcaps_of_any_size(ops, lens, softcap):
         assert bool((err <= tol).all()), (i, float((err / tol).max()))
 
 
+def test_a_workspace_waits_for_what_its_memory_was_used_by(ops):
+    """made from memory that the stream it was made on still writes, and called on another one: eagerly, in a capture, and
+    made within one"""
+    b = S.Batch([(1, 3000), (1, 500)], 8, 2, 128, seed=45)
+    want = paged(ops, b)
+    kv = ops.PagedKv(b.paged(b.k_pages.to(GPU)), b.paged(b.v_pages.to(GPU)), b.table.to(GPU))
+    seqs = ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=1, max_len=3000)
+    q, out = b.q.to(GPU), torch.zeros(b.rows, 8, 128, dtype=F16, device=GPU)
+    size = ops.PagedAttention(kv, seqs, q, out).workspace.numel()
+    a = torch.randn(8192, 8192, device=GPU).half()
+    a @ a
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    junk = torch.empty(size, dtype=torch.uint8, device=GPU)
+    at = junk.data_ptr()
+    x = a
+    for _ in range(30):  # some 30 ms
+        x = x @ a
+    junk.fill_(255)
+    written = torch.cuda.current_stream().record_event()
+    del junk
+    call = ops.PagedAttention(kv, seqs, q, out)
+    same = call.workspace.data_ptr() == at
+    call(stream=side)
+    side.synchronize()
+    assert written.query() or not same
+    assert same and torch.equal(out.cpu(), want)
+    out.zero_()
+    torch.cuda.synchronize()
+    call(stream=side)  # not again
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    assert torch.equal(out.cpu(), want)
+
+    graph = torch.cuda.CUDAGraph()
+    late = ops.PagedAttention(kv, seqs, q, out)
+    with torch.cuda.graph(graph, stream=side):
+        late()
+        inner = ops.PagedAttention(kv, seqs, q, out)
+        inner()
+        other = torch.cuda.Stream()
+        other.wait_stream(side)
+        inner(stream=other)
+        side.wait_stream(other)
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.cpu(), want)
+        out.zero_()
+        late(stream=side)
+        side.synchronize()
+        assert torch.equal(out.cpu(), want)
+
+
 def test_strides_of_dimensions_with_one_entry_mean_nothing(ops):
     """one KV head, one row, one page: views whose strides there are odd, far too large or different"""
     g = torch.Generator(device=GPU).manual_seed(43)
