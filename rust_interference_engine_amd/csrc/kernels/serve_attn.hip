@@ -1109,7 +1109,7 @@ void launch_hd(const ServeAttnArgs &a, hipStream_t st) {
     const bool cap = a.softcap > 0;
     if (serve_attn_few(a)) {
         const dim3 grid(a.b.n_seq * a.n_kv, a.S);
-        if (a.b.max_new * a.G <= 16) {
+        if (few_row_blocks(true, a.b.max_new, a.G) == 1) {
             if (cap) attn_few_kernel<HD, BF, true, 1><<<grid, 256, 0, st>>>(a);
             else attn_few_kernel<HD, BF, false, 1><<<grid, 256, 0, st>>>(a);
         } else {
@@ -1143,7 +1143,7 @@ constexpr int COMBINE_FEW = 2048;
 
 bool serve_attn_head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
-bool serve_attn_few(const ServeAttnArgs &a) { return a.kv.table && (int64_t)a.b.max_new * a.G <= 32; }
+bool serve_attn_few(const ServeAttnArgs &a) { return few_row_blocks(a.kv.table, a.b.max_new, a.G) > 0; }
 
 SplitPlan serve_attn_splits(const ServeAttnArgs &a) {
     const bool few = serve_attn_few(a);
@@ -1151,7 +1151,7 @@ SplitPlan serve_attn_splits(const ServeAttnArgs &a) {
     const int64_t blocks = few ? a.b.n_seq : block_count(a.b.n_rows, a.b.n_seq, a.G, TILE_M);
     // positions that a block's rows see, at most
     int64_t span = a.b.max_len;
-    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? 32 : TILE_M / a.G + 1) + KT);
+    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? FEW_ROWS : TILE_M / a.G + 1) + KT);
     const int tiles = (int)((span + KT - 1) / KT);
     // Few rows: 4096 workgroups where there is so much, since sequences differ in length, and at
     // least 256 positions each (48 tokens over up to 4000 positions, 8 KV heads: 85.9 us at 1024
@@ -1182,7 +1182,7 @@ void launch_serve_attn(ServeAttnArgs a, void *ws, hipStream_t st) {
     if (bf) launch_ty<true>(a, st);
     else launch_ty<false>(a, st);
     if (p.S > 1) {
-        const int M = few ? 32 : TILE_M, KT = few ? FEW_STEP : tile_kt(a.hd);
+        const int M = few ? FEW_ROWS : TILE_M, KT = few ? FEW_STEP : tile_kt(a.hd);
         const int64_t n = (int64_t)a.b.n_rows * a.n_head;
         if (n <= COMBINE_FEW) {
             if (bf) serve_combine_kernel<true, 4><<<n, 256, 0, st>>>(a, M, KT);

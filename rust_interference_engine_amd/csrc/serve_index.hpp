@@ -67,6 +67,15 @@ RIE_HD int tile_count(const KeyRange &r, int KT) { return r.hi > r.lo ? (r.hi + 
 // splits of nt tiles when a split takes C of them and the last of S all that are left
 RIE_HD int split_count(int nt, int C, int S) { return imax(1, imin(S, (nt + C - 1) / C)); }
 
+// Which kernel a launch over sequences of at most max_new tokens takes, G query heads to a KV
+// head: 1 or 2, the blocks of 16 query rows of the few-rows kernel, or 0, the tile kernel.  The
+// few-rows kernel reads pages only.
+constexpr int FEW_ROWS = 32;
+inline int few_row_blocks(bool paged, int max_new, int G) {
+    const int64_t rows = (int64_t)max_new * G;
+    return !paged || rows > FEW_ROWS ? 0 : rows <= 16 ? 1 : 2;
+}
+
 // How a launch divides the positions of a block: every split takes C tiles, S at most.
 struct SplitPlan {
     int C, S;

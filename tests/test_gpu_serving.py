@@ -699,6 +699,44 @@ def test_packed_prompts_keep_infinite_and_nan_values_to_the_tokens_behind_them(o
     assert bool((out[70 + 17:110, 2:, 2] == math.inf).all()) and bool(out[69, :2, 0].isnan().all()) and bool((out[110:, :2, hd - 1] == -math.inf).all())
 
 
+# query heads of a KV head and new tokens: 16 rows (one block), 17 and up to 32 (two), 33 (tiles)
+ROWS = [(4, 4), (17, 1), (3, 6), (5, 6), (8, 4), (1, 32), (11, 3)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("G,new", ROWS)
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (40, 0.0), (0, 5.0), (7, 3.0)])
+def test_sixteen_to_thirty_three_rows_of_a_sequence(ops, G, new, hd, window, softcap, dtype):
+    b = S.Batch([(new, 700), (new, new), (1, 45), (new, 300), (new, new - 1), (0, 30)], 2 * G, 2, hd, page=32, dtype=dtype, seed=46, extra_rows=1)
+    for kw in (dict(), dict(max_len=60000)):  # whole, and in splits
+        check(b, paged(ops, b, window, softcap, **kw), window, softcap)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("G,new", ROWS)
+@pytest.mark.parametrize("window", [0, 40])
+def test_sixteen_to_thirty_three_rows_with_odd_values_and_pages(ops, G, new, hd, window, dtype):
+    lens = [(new, 700), (new, 90), (1, 45)]
+    b = S.Batch(lens, 2 * G, 2, hd, page=16, dtype=dtype, seed=47)
+    b.v_pages = spoil(b.v_pages, 2e-3, 48)
+    for kw in (dict(), dict(max_len=60000)):
+        got = paged(ops, b, window, **kw)
+        for i, (n, L) in enumerate(lens):
+            r = int(b.starts[i])
+            check_spoilt(got[r:r + n], b.q[r:r + n], b.cached(b.k_pages, i), b.cached(b.v_pages, i), L - n, window, dtype, hd)
+    # a page that is none: its 16 positions are not seen, which is as if they lay below a window of their own
+    good = b.table.clone()
+    for at in (0, 20):
+        for bad in (-1, b.n_pages):
+            b.table[0, at] = bad
+            got = paged(ops, b, 0)
+            k, v = (torch.cat([x[:16 * at], x[16 * at + 16:]]) for x in (b.paged(p)[good[0].long().clamp(0, b.n_pages - 1)].reshape(-1, 2, hd)[:700] for p in (b.k_pages, b.v_pages)))
+            check_spoilt(got[:new], b.q[:new], k, v, 684 - new, 0, dtype, hd)
+            b.table.copy_(good)
+
+
 @pytest.mark.parametrize("softcap", [1e-38, 1e-3, 0.5, 30.0, 50.0, 1e3, 1e5, 1e7, 1e12, 1e30, 3e38])
 @pytest.mark.parametrize("lens", [[(1, 300), (3, 77)], [(1, 300), (60, 100)]])  # few rows; tiles
 def test_softcaps_of_any_size(ops, lens, softcap):
