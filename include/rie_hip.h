@@ -288,9 +288,7 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
 /* Causal attention of every sequence's new tokens over its pages, which already hold them:
  * chunks of prompts and single tokens in one batch.  A token that sees nothing gets zeros.
  * An infinite or NaN key or value reaches only the tokens that see it (an infinite value as
- * that infinity).  Outputs are f32 sums of up to 2^8 times the values before they are
- * divided, so bf16 values may not be so large that their sum over the positions, times
- * 2^8, passes 3e38. */
+ * that infinity). */
 size_t rie_hip_k_paged_attention_ws(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn);
 int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn, void *ws,
                                   size_t ws_bytes, void *stream, char *err, size_t err_len);

@@ -699,6 +699,19 @@ def test_packed_prompts_keep_infinite_and_nan_values_to_the_tokens_behind_them(o
     assert bool((out[70 + 17:110, 2:, 2] == math.inf).all()) and bool(out[69, :2, 0].isnan().all()) and bool((out[110:, :2, hd - 1] == -math.inf).all())
 
 
+@pytest.mark.parametrize("sign", [False, True])
+@pytest.mark.parametrize("lens", [[(1, 3000), (3, 77)], [(1, 3000), (60, 700)]])  # few rows; tiles
+@pytest.mark.parametrize("hd", [64, 256])
+def test_values_as_large_as_the_type_holds(ops, hd, lens, sign):
+    b = S.Batch(lens, 4, 2, hd, page=64, dtype=BF16, seed=49)
+    big = torch.finfo(BF16).max
+    b.v_pages = (torch.where(b.v_pages < 0, -1.0, 1.0) * big).to(BF16) if sign else torch.full_like(b.v_pages, big)
+    for kw in (dict(), dict(max_len=60000)):
+        got = paged(ops, b, **kw)
+        check(b, got)
+        assert bool(torch.isfinite(got).all())
+
+
 # query heads of a KV head and new tokens: 16 rows (one block), 17 and up to 32 (two), 33 (tiles)
 ROWS = [(4, 4), (17, 1), (3, 6), (5, 6), (8, 4), (1, 32), (11, 3)]
 
