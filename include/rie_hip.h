@@ -288,7 +288,8 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
 /* Causal attention of every sequence's new tokens over its pages, which already hold them:
  * chunks of prompts and single tokens in one batch.  A token that sees nothing gets zeros.
  * An infinite or NaN key or value reaches only the tokens that see it (an infinite value as
- * that infinity). */
+ * that infinity).  Finite values have finite outputs (bf16: over up to 2^24 positions; bf16
+ * values under 2^-94 may count as zeros). */
 size_t rie_hip_k_paged_attention_ws(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn);
 int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn, void *ws,
                                   size_t ws_bytes, void *stream, char *err, size_t err_len);

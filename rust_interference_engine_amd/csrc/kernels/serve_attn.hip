@@ -14,7 +14,7 @@
 // The few-rows kernel takes what that rounding leaves as a second product, its matrix units
 // being idle (1.6e-3 and 1.6e-3).  The maximum that is subtracted is only moved when a score
 // passes it by 2^8, so a probability lies in 0..2^8; f16 ones are multiplied by 2^6, since
-// small ones would be subnormal, bf16 ones by 2^-40 (P_SHIFT).
+// small ones would be subnormal, bf16 ones by 2^-32 (P_SHIFT).
 //
 // Values that are infinite or NaN reach the tokens that see them and no others: a tile that
 // some token sees in part is searched for them, and if there are any, they are added to the
@@ -109,10 +109,11 @@ __device__ __forceinline__ u32x2 read_tr(uint32_t at) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)at));
 }
-// Probabilities are 2^(s − m + P_SHIFT).  bf16 ones are made so small that no sum over 2^30 positions
-// passes the largest value, which may be the largest of f32; they have its exponents.
+// Probabilities are 2^(s − m + P_SHIFT).  bf16 ones are made so small that no sum over 2^24 positions
+// passes the largest value, which may be the largest of f32; they have its exponents.  What that
+// takes at the other end: terms under 2^-126, which are values under 2^-94, may count as zeros.
 template <bool BF>
-constexpr float P_SHIFT = BF ? -40.0f : 6.0f;
+constexpr float P_SHIFT = BF ? -32.0f : 6.0f;
 constexpr float M_SLACK = 8.0f;  // how far a score may pass the maximum that is subtracted
 
 __device__ __forceinline__ SeqView uniform(const SeqView &v) {

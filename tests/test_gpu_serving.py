@@ -712,6 +712,16 @@ def test_values_as_large_as_the_type_holds(ops, hd, lens, sign):
         assert bool(torch.isfinite(got).all())
 
 
+@pytest.mark.parametrize("lens", [[(1, 3000), (3, 77)], [(1, 3000), (60, 700)]])  # few rows; tiles
+@pytest.mark.parametrize("power", [-40, -70, -80])
+def test_small_values_keep_their_digits(ops, power, lens):
+    b = S.Batch(lens, 4, 2, 64, page=64, dtype=BF16, seed=50)
+    b.v_pages = (b.v_pages.double() * 2.0 ** power).to(BF16)
+    for kw in (dict(), dict(max_len=60000)):
+        # terms under 2^-126 may be lost, 2^-94 of the values' weights of one
+        check(b, paged(ops, b, **kw))
+
+
 # query heads of a KV head and new tokens: 16 rows (one block), 17 and up to 32 (two), 33 (tiles)
 ROWS = [(4, 4), (17, 1), (3, 6), (5, 6), (8, 4), (1, 32), (11, 3)]
 
