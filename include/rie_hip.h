@@ -286,7 +286,8 @@ typedef struct rie_hip_attn {
 int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *seqs, int32_t src_ty, const void *k, const void *v,
                                int64_t row_stride, int64_t head_stride, void *stream, char *err, size_t err_len);
 /* Causal attention of every sequence's new tokens over its pages, which already hold them:
- * chunks of prompts and single tokens in one batch.  A token that sees nothing gets zeros.
+ * chunks of prompts and single tokens in one batch.  A token that sees nothing, or
+ * nothing that scores above −inf, gets zeros.
  * An infinite or NaN key or value reaches only the tokens that see it (an infinite value as
  * that infinity).  Finite values have finite outputs (bf16: over up to 2^24 positions; bf16
  * values under 2^-94 may count as zeros). */

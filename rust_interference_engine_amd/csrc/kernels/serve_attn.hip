@@ -4,7 +4,7 @@
 //   o_t = Σ_j softmax_j(s_tj) v_j,  s_tj = scale · q_t·k_j  (cap · tanh(s / cap) with a softcap)
 //
 // over the positions j ≤ p_t, and j > p_t − window with a window, of token t at position
-// p_t of its sequence.  A token that sees nothing gets zeros.  q, k, v and o are all f16
+// p_t of its sequence.  A token that sees nothing, or nothing above −inf, gets zeros.  q, k, v and o are all f16
 // or all bf16; scores, the softmax's maximum and sum, and the outputs are f32 sums.
 //
 // Rounding.  In the tile kernel a probability enters the second product in the tensors' own

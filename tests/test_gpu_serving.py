@@ -722,6 +722,34 @@ def test_small_values_keep_their_digits(ops, power, lens):
         check(b, paged(ops, b, **kw))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens", [[(1, 3000), (3, 77)], [(1, 3000), (60, 700)]])  # few rows; tiles
+def test_keys_of_minus_infinity_have_no_weight(ops, lens, dtype):
+    b = S.Batch(lens, 4, 2, 64, page=64, dtype=dtype, seed=51)
+    b.q[..., 0] = b.q[..., 0].abs() + 0.5
+    keys = b.paged(b.k_pages)
+    keep = [(0, 2990), (0, 100), (1, 10), (1, 70)]  # of sequence and position; KV head 1 has none
+    values = keys[..., 0].clone()
+    keys[..., 0] = -math.inf
+    for i, j in keep:
+        at = int(b.table[i, j // 64]), j % 64, 0
+        keys[at][0] = values[at]
+    for kw in (dict(), dict(max_len=60000)):
+        got = paged(ops, b, **kw)
+        for i, (n, L) in enumerate(lens):
+            r = int(b.starts[i])
+            mine = [j for e, j in keep if e == i]
+            k, v = b.cached(b.k_pages, i), b.cached(b.v_pages, i)
+            for t in range(n):
+                see = [j for j in mine if j <= L - n + t]
+                assert bool((got[r + t, 2:] == 0).all())  # nothing above -inf: zeros
+                if not see:
+                    assert bool((got[r + t] == 0).all())
+                    continue
+                o, a, size = S.attend(b.q[r + t:r + t + 1, :2], k[see, :1], v[see, :1], len(see) - 1, 1 / 8)
+                assert bool(((got[r + t, :2].double() - o[0]).abs() <= S.tolerance(o, a, size, L, 64, dtype)[0]).all())
+
+
 # query heads of a KV head and new tokens: 16 rows (one block), 17 and up to 32 (two), 33 (tiles)
 ROWS = [(4, 4), (17, 1), (3, 6), (5, 6), (8, 4), (1, 32), (11, 3)]
 
