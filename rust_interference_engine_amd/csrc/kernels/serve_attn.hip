@@ -773,7 +773,14 @@ __global__ __launch_bounds__(256, (FEW_WAVES<HD, NB>)) void attn_few_kernel(Serv
     // Page ids of a tile's two groups of 16 positions (lanes 0 and 1), requested a tile ahead.
     // Positions behind the last one seen are read as copies of it.
     auto first_of = [&](int t, int b) { return imin(t * KT + b * 16, (hi - 1) & ~15); };
-    auto request_pages = [&](int t) { return t < end ? trow[first_of(t, lane & 1) >> a.kv.page_shift] : 0; };
+    // The lane's number is taken anew each time: what it adds, kept, was a register too many at
+    // 128-wide heads with a softcap, whose reload waits for the copies (64 tokens over 2000
+    // positions, 8 KV heads: 122.4 us, now 117.5).
+    auto request_pages = [&](int t) {
+        int id = threadIdx.x;
+        asm volatile("" : "+v"(id));
+        return t < end ? trow[first_of(t, id & 1) >> a.kv.page_shift] : 0;
+    };
     struct Pages {
         int id[2], bad;  // bad bit b: the page of group b is none (any that exists is read, and nobody sees it)
     };
