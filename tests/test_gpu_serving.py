@@ -750,6 +750,50 @@ def test_keys_of_minus_infinity_have_no_weight(ops, lens, dtype):
                 assert bool(((got[r + t, :2].double() - o[0]).abs() <= S.tolerance(o, a, size, L, 64, dtype)[0]).all())
 
 
+@pytest.mark.parametrize("new", [2, 40])  # few rows; tiles
+def test_offsets_past_four_gigabytes(ops, new):
+    """pages, rows of queries, of outputs and of packed prompts, and logits, far apart in buffers of 5 GB and more"""
+    KV, G, hd, page = 2, 4, 64, 16
+    b = S.Batch([(new, 100), (1, 40)], KV * G, KV, hd, page=page, dtype=BF16, seed=52)
+    want = paged(ops, b)
+    far = 5 * 2 ** 30 // (page * KV * hd * 2)  # that many pages behind
+    spread = [torch.empty(far + b.n_pages, KV, page, hd, dtype=BF16, device=GPU) for _ in range(2)]
+    for x, y in zip(spread, (b.k_pages, b.v_pages)):
+        x[far:] = y.to(GPU)
+    last = spread[0][far:].clone()
+    step = 2 ** 25  # values from one row to the next: 64 MB, the largest
+    rows = b.rows
+    wide = torch.empty(rows * step, dtype=BF16, device=GPU)  # 40 new: 2.7 GB
+    q, out = wide.as_strided((rows, KV * G, hd), (step, hd, 1)), wide.as_strided((rows, KV * G, hd), (step, hd, 1), 4096)
+    q[:] = b.q.to(GPU)
+    kv = ops.PagedKv(*(x.transpose(1, 2) for x in spread), (b.table.long().clamp(max=b.n_pages - 1) + far).int().to(GPU))
+    seqs = ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=new, max_len=100)
+    ops.PagedAttention(kv, seqs, q, out)()
+    assert torch.equal(out.cpu(), want)
+    k = wide.as_strided((rows, KV, hd), (step, hd, 1), 8192)
+    k[:] = torch.randn(rows, KV, hd, device=GPU)
+    ops.PagedAppend(kv, seqs, k, k)()
+    b.k_pages = spread[0][far:].cpu()
+    assert torch.equal(b.cached(b.k_pages, 0)[-new:], k[:new].cpu()) and torch.equal(b.cached(b.k_pages, 1)[-1:], k[new:].cpu())
+    assert int((spread[0][far:] != last).any(-1).sum()) == rows * KV  # and nothing else
+    del spread, kv, wide, q, out, k
+
+    n = 2 * 64 + 5  # rows behind 4 GB and the first ones
+    wide = torch.empty((n - 1) * step + 16384, dtype=F16, device=GPU)
+    view = lambda heads, at: wide.as_strided((n, heads, hd), (step, hd, 1), at)  # noqa: E731
+    q, k, v, out = view(4, 0), view(2, 1024), view(2, 2048), view(4, 4096)
+    for x in (q, k, v):
+        x[:] = torch.randn(x.shape, device=GPU)
+    starts = torch.tensor([0, 70, n], dtype=torch.int32, device=GPU)
+    ops.PackedAttention(ops.Seqs(starts, max_new=70, max_len=70), q, k, v, out)()
+    for r in (slice(0, 70), slice(70, n)):
+        o, a, size = S.attend(q[r].cpu(), k[r].cpu(), v[r].cpu(), 0, 1 / 8)
+        assert bool(((out[r].cpu().double() - o).abs() <= S.tolerance(o, a, size, 70, hd, F16)).all())
+    x = wide.as_strided((n, 3001), (step, 1), 8192)
+    x[:] = torch.randn(x.shape, device=GPU)
+    check_logprobs(ops, x.cpu(), x, torch.arange(n, dtype=torch.int32), 5)
+
+
 # query heads of a KV head and new tokens: 16 rows (one block), 17 and up to 32 (two), 33 (tiles)
 ROWS = [(4, 4), (17, 1), (3, 6), (5, 6), (8, 4), (1, 32), (11, 3)]
 
