@@ -286,11 +286,14 @@ typedef struct rie_hip_attn {
 int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *seqs, int32_t src_ty, const void *k, const void *v,
                                int64_t row_stride, int64_t head_stride, void *stream, char *err, size_t err_len);
 /* Causal attention of every sequence's new tokens over its pages, which already hold them:
- * chunks of prompts and single tokens in one batch.  A token that sees nothing, or
- * nothing that scores above −inf, gets zeros.
- * An infinite or NaN key or value reaches only the tokens that see it (an infinite value as
- * that infinity).  Finite values have finite outputs (bf16: over up to 2^24 positions; bf16
- * values under 2^-94 may count as zeros). */
+ * chunks of prompts and single tokens in one batch.  A token that sees nothing, or nothing
+ * that scores above −inf, gets zeros.  An infinite or NaN key or value reaches only the
+ * tokens that see it (an infinite value as that infinity).  Finite values have finite
+ * outputs (bf16: over up to 2^24 positions; bf16 values under 2^-94 may count as zeros).
+ * Scores, the softmax's sums and the outputs are f32 sums.  With up to 32 query rows to a KV
+ * head (max_new * n_head / n_kv) only the output is rounded to the keys' type; with more, and
+ * in packed attention, so is each probability, once (2-norm against float64, bf16: 1.6e-3 and
+ * 2.0e-3 to 2.3e-3; f16: 2.0e-4 and 2.3e-4 to 2.8e-4). */
 size_t rie_hip_k_paged_attention_ws(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn);
 int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn, void *ws,
                                   size_t ws_bytes, void *stream, char *err, size_t err_len);

@@ -99,7 +99,8 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
 // Addresses in LDS as numbers: sums with constants become the instructions' offsets, where
 // generic pointers take a register for every one, 50 to 70 of them in the tile kernel, which
 // then holds all 256 (and one more is a spill whose reload waits for the copies: 219 to 272 us
-// for chunks in a batch of 13; 202 without a spill, 216 here with 209 registers; four prompts
+// for chunks in a batch of 13; 202 without a spill, 219 here with 209 vector registers; scalars,
+// 45 to 62 of them from head size 96 on, are kept in lanes of vector registers; four prompts
 // of 64-wide heads, 3 waves on a SIMD instead of 2: 187, with pointers 201).
 __device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)p; }
 __device__ __forceinline__ u32x4 lds_16(uint32_t at) { return *(__attribute__((address_space(3))) const u32x4 *)(uintptr_t)at; }
@@ -1167,7 +1168,8 @@ SplitPlan serve_attn_splits(const ServeAttnArgs &a) {
     // workgroups, 75.0 at 2048, 73.2 at 4096, 74.3 at 8192); a cache of under 512 positions is
     // not split, a second launch being longer than its loads.
     if (few) return split_plan(blocks * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
-    // Tiles: 2 us each with every slot taken (64 positions of 128 values), partials at 4.5 TB/s.
+    // Tiles: 2 us each with every slot taken (64 positions of 128 values, plain bf16: f16 takes 0 to 5 % more
+    // and a softcap 1.4 to 1.6 times it, which would split a little more), partials at 4.5 TB/s.
     // Chunks in a batch of 13 (488 workgroups): 208 us in one, 202 to 248 in 2 to 5 splits;
     // window prompts with 256-wide heads (123) 31.5 in one, 47.7 in 4; one long prompt is split.
     const double part_us = (double)a.b.n_rows * a.n_head * a.hd * 8 / 4.5e6;
