@@ -297,6 +297,36 @@ int32_t rie_hip_k_paged_append(const rie_hip_pages *pages, const rie_hip_seqs *s
 size_t rie_hip_k_paged_attention_ws(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn);
 int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs *seqs, const rie_hip_attn *attn, void *ws,
                                   size_t ws_bytes, void *stream, char *err, size_t err_len);
+/* The same cache in 8 bits: pages.ty is 24 (int8), pages.k and pages.v hold codes of −127..127,
+ * and a value is its code times the scale of its block: `block` positions of a page (a power of
+ * two, 16 to page_size) of one head, at page*scale_page_stride + (slot/block)*scale_block_stride
+ * + head*scale_head_stride of k_scale and of v_scale (f32).  Alignments and the limits of strides
+ * are those of bytes.  A scale is 0 (of zeros), NaN, or 2^-60 to 2^50; others count as the nearest
+ * of these bounds. */
+typedef struct rie_hip_pages8 {
+    rie_hip_pages pages;
+    float *k_scale, *v_scale;
+    int64_t scale_page_stride, scale_block_stride, scale_head_stride;
+    int32_t block;
+} rie_hip_pages8;
+
+/* Writes the new tokens' keys and values (src_ty: f32, f16 or bf16) to their pages.  A block's
+ * scale is the largest of its values / 127 (0 where that is under 2^-60: such values become
+ * zeros); where a call finds a block begun, the block keeps its scale s, or takes the new values'
+ * larger one s' and its codes become round(code * s/s'), which adds up to half a step of s' to
+ * their error each time a scale grows.  Codes are rounded to nearest, ties to even.  A block that
+ * is given an infinite or NaN value, or one over 127 * 2^50, has a NaN scale from then on, until
+ * a call brings its first position again.  A block that new tokens come to has to be one
+ * sequence's alone, and its earlier positions that sequence's own. */
+int32_t rie_hip_k_paged_append8(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t src_ty, const void *k, const void *v,
+                                int64_t row_stride, int64_t head_stride, void *stream, char *err, size_t err_len);
+/* Causal attention over such pages, of queries and to outputs of type ty (f16 or bf16).  A token
+ * that sees a position of a block whose scale is NaN gets NaN for the heads that read it.  With
+ * up to 32 query rows to a KV head only the output is rounded; with more, so is each
+ * probability, to f16 (2-norm against float64: see the rules for 16-bit pages, f16's for both types). */
+size_t rie_hip_k_paged_attention8_ws(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t ty, const rie_hip_attn *attn);
+int32_t rie_hip_k_paged_attention8(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t ty, const rie_hip_attn *attn, void *ws,
+                                   size_t ws_bytes, void *stream, char *err, size_t err_len);
 /* Causal attention within whole prompts packed one behind the other: keys and values are
  * rows beside the queries' (n_kv heads; slices of a fused projection, say). */
 size_t rie_hip_k_packed_attention_ws(const rie_hip_seqs *seqs, int32_t ty, int32_t head_dim, int32_t n_kv, const rie_hip_attn *attn);

@@ -41,6 +41,12 @@ class Pages(C.Structure):
         ("table", C.c_void_p), ("table_stride", C.c_int64)]
 
 
+class Pages8(C.Structure):
+    """rie_hip_pages8"""
+    _fields_ = [("pages", Pages), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("scale_page_stride", "scale_block_stride", "scale_head_stride")] + [("block", C.c_int32)]
+
+
 class Attn(C.Structure):
     """rie_hip_attn"""
     _fields_ = [("n_head", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float),
@@ -65,7 +71,7 @@ def lib():
     L = C.CDLL(LIB_PATH)
     P, S, I, F, D = C.c_void_p, C.c_size_t, C.c_int32, C.c_float, C.c_double
     CP, U8P = C.c_char_p, C.POINTER(C.POINTER(C.c_uint8))
-    I64, PG, SQ, AT = C.c_int64, C.POINTER(Pages), C.POINTER(Seqs), C.POINTER(Attn)
+    I64, PG, PG8, SQ, AT = C.c_int64, C.POINTER(Pages), C.POINTER(Pages8), C.POINTER(Seqs), C.POINTER(Attn)
     sig = {
         "rie_hip_default_config": (Config, []),
         "rie_hip_create": (P, [P, S, C.POINTER(Config), C.POINTER(I), CP, S]),
@@ -100,6 +106,9 @@ def lib():
         "rie_hip_k_paged_append": (I, [PG, SQ, I, P, P, I64, I64, P, CP, S]),
         "rie_hip_k_paged_attention_ws": (S, [PG, SQ, AT]),
         "rie_hip_k_paged_attention": (I, [PG, SQ, AT, P, S, P, CP, S]),
+        "rie_hip_k_paged_append8": (I, [PG8, SQ, I, P, P, I64, I64, P, CP, S]),
+        "rie_hip_k_paged_attention8_ws": (S, [PG8, SQ, I, AT]),
+        "rie_hip_k_paged_attention8": (I, [PG8, SQ, I, AT, P, S, P, CP, S]),
         "rie_hip_k_packed_attention_ws": (S, [SQ, I, I, I, AT]),
         "rie_hip_k_packed_attention": (I, [SQ, I, I, I, P, P, I64, I64, I64, I64, AT, P, S, P, CP, S]),
         "rie_hip_k_token_logprobs_ws": (S, [I, I]),

@@ -12,7 +12,7 @@ namespace rie {
 // ggml type ids (quant/mod.rs:34-51 in the reference)
 enum GgmlType : int {
     T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q4_1 = 3, T_Q5_0 = 6, T_Q5_1 = 7, T_Q8_0 = 8,
-    T_Q2_K = 10, T_Q3_K = 11, T_Q4_K = 12, T_Q5_K = 13, T_Q6_K = 14, T_BF16 = 30
+    T_Q2_K = 10, T_Q3_K = 11, T_Q4_K = 12, T_Q5_K = 13, T_Q6_K = 14, T_I8 = 24, T_BF16 = 30
 };
 
 // Error codes of the C ABI: one per variant of the reference's Error enum

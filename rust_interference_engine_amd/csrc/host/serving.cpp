@@ -1,131 +1,70 @@
 // serving.cpp — the C ABI of the batched serving operators (include/rie_hip.h): checks of
 // what the host can see, and the launches on the caller's stream.
-#include "../../../include/rie_hip.h"
+#include "serve_check.hpp"
 
-#include "../serve.hpp"
-#include "guard.hpp"
-
-#include <algorithm>
 #include <cmath>
-#include <string>
-
-using rie::Error;
-using rie::guarded;
 
 namespace {
 
-Error bad(const std::string &m) { return Error{rie::E_RUNTIME, m}; }
+using namespace rie;
 
-// The stream's device is the current one while this lives.
-class OnDevice {
-  public:
-    explicit OnDevice(hipStream_t st) {
-        RIE_HIP_CHECK(hipGetDevice(&was_));
-        device = was_;
-        if (st) {
-            hipDevice_t d;
-            RIE_HIP_CHECK(hipStreamGetDevice(st, &d));
-            device = (int)d;
-        }
-        if (device != was_) RIE_HIP_CHECK(hipSetDevice(device));
-    }
-    ~OnDevice() {
-        if (device != was_) (void)hipSetDevice(was_);
-    }
-    OnDevice(const OnDevice &) = delete;
-    OnDevice &operator=(const OnDevice &) = delete;
-
-    // p is memory that a kernel on this device may use
-    void check(const void *p, const char *what) const {
-        if (!p) throw bad(std::string(what) + " is NULL");
-        hipPointerAttribute_t a;
-        const hipError_t e = hipPointerGetAttributes(&a, p);
-        if (e != hipSuccess) (void)hipGetLastError();  // not an error of the launch
-        if (e != hipSuccess || (a.type != hipMemoryTypeDevice && a.type != hipMemoryTypeManaged))
-            throw bad(std::string(what) + " is not device memory");
-        if (a.type == hipMemoryTypeDevice && a.device != device)
-            throw bad(std::string(what) + " is on device " + std::to_string(a.device) + ", the stream on device " + std::to_string(device));
-    }
-
-    int device;
-
-  private:
-    int was_;
-};
-
-bool is16(int ty) { return ty == rie::T_F16 || ty == rie::T_BF16; }
-
-// A dimension of one entry is at 0, whatever its stride says (that of a tensor's is arbitrary)
-int64_t used(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
-
-// Rows of values of es bytes each start at p + any multiples of the strides: all 16-byte
-// aligned, and strides of 2^26 bytes at most, so that 16 rows stay within 31 bits
-void check_rows(const void *p, int64_t row, int64_t head, int es, const char *what) {
-    const int64_t a = 16 / es, most = ((int64_t)1 << 26) / es;
-    if ((uintptr_t)p % 16 || row % a || head % a) throw bad(std::string(what) + ": rows have to be 16-byte aligned");
-    if (row < 0 || row > most || head < 0 || head > most) throw bad(std::string(what) + ": strides have to lie in 0.." + std::to_string(most));
-}
-
-// Rows that are written, n of each dimension a stride apart: no two of them share a value.  Every
-// stride has to cover what the smaller ones span.
-struct Dim {
-    int64_t n, stride;
-};
-template <size_t N>
-void check_apart(Dim (&&dims)[N], int hd, const char *what) {
-    std::sort(dims, dims + N, [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
-    __int128 span = hd;  // strides of up to 2^40 by counts of up to 2^31
-    for (const Dim &d : dims) {
-        if (d.n <= 1) continue;
-        if (d.stride < span) throw bad(std::string(what) + ": strides below head_dim, or below what the smaller ones span, would make rows overlap");
-        span += (__int128)(d.n - 1) * d.stride;
-    }
-}
-
-constexpr int MOST = 1 << 30;  // positions
-constexpr int MOST_ROWS = (1 << 26) - 4;  // 4 to a workgroup of 256: a launch has under 2^32 threads
-
-rie::BatchView batch(const rie_hip_seqs *s, bool lens) {
-    if (!s) throw bad("seqs is NULL");
-    if (s->n_seq < 1 || s->n_rows < 1 || s->n_seq >= 1 << 24 || s->n_rows > MOST_ROWS) throw bad("n_seq has to lie in 1..2^24-1, n_rows in 1..2^26-4");
-    if (s->max_new < 1 || s->max_len < 1 || s->max_new > MOST || s->max_len > MOST) throw bad("max_new and max_len have to lie in 1..2^30");
-    rie::BatchView b;
-    b.starts = s->starts;
-    b.lens = lens ? s->lens : nullptr;
-    b.n_seq = s->n_seq;
-    b.n_rows = s->n_rows;
-    b.max_new = std::min(s->max_new, s->n_rows);
-    b.max_len = s->max_len;
-    return b;
-}
-
-void check_heads(int ty, int hd, int n_kv) {
-    if (!is16(ty)) throw Error{rie::E_UNSUPPORTED, "keys and values have to be f16 or bf16"};
+void check_head_dim(int hd, int n_kv) {
     if (!rie::serve_attn_head_dim_ok(hd)) throw Error{rie::E_UNSUPPORTED, "head_dim has to be 32, 64, 96, 128 or 256"};
     if (n_kv < 1 || n_kv > 4096) throw bad("n_kv has to lie in 1..4096");
 }
 
-rie::KvView pages_view(const rie_hip_pages *p) {
-    if (!p) throw bad("pages is NULL");
-    check_heads(p->ty, p->head_dim, p->n_kv);
+void check_heads(int ty, int hd, int n_kv) {
+    if (!is16(ty)) throw Error{rie::E_UNSUPPORTED, "keys and values have to be f16 or bf16"};
+    check_head_dim(hd, n_kv);
+}
+
+// pages of values of es bytes each
+rie::KvView view_pages(const rie_hip_pages *p, int es) {
     if (p->page_size < 16 || p->page_size > 4096 || (p->page_size & (p->page_size - 1)))
         throw Error{rie::E_UNSUPPORTED, "page_size has to be a power of two in 16..4096"};
     if (p->n_pages < 1 || p->table_cols < 1 || p->table_stride < 0) throw bad("n_pages and table_cols have to be positive");
     const int64_t head = used(p->n_kv, p->head_stride), page = used(p->n_pages, p->page_stride);
-    check_rows(p->k, p->slot_stride, head, 2, "pages");
-    check_rows(p->v, p->slot_stride, head, 2, "pages");
-    if (page < 0 || page % 8 || page > ((int64_t)1 << 40)) throw bad("pages: page_stride has to be a multiple of 8 in 0..2^40");
+    check_rows(p->k, p->slot_stride, head, es, "pages");
+    check_rows(p->v, p->slot_stride, head, es, "pages");
+    const int a = 16 / es;
+    if (page < 0 || page % a || page > ((int64_t)1 << 40)) throw bad("pages: page_stride has to be a multiple of " + std::to_string(a) + " in 0..2^40");
     rie::KvView v;
     v.k = (const uint8_t *)p->k;
     v.v = (const uint8_t *)p->v;
-    v.k_row = v.v_row = p->slot_stride * 2;
-    v.k_head = v.v_head = head * 2;
-    v.page = page * 2;
+    v.k_row = v.v_row = p->slot_stride * es;
+    v.k_head = v.v_head = head * es;
+    v.page = page * es;
     v.table = p->table;
     v.table_stride = p->table_stride;
     v.page_shift = __builtin_ctz((unsigned)p->page_size);
     v.n_pages = p->n_pages;
     v.cap = (int)std::min<int64_t>((int64_t)p->table_cols * p->page_size, MOST);
+    return v;
+}
+
+rie::KvView pages_view(const rie_hip_pages *p) {
+    if (!p) throw bad("pages is NULL");
+    check_heads(p->ty, p->head_dim, p->n_kv);
+    return view_pages(p, 2);
+}
+
+rie::KvView pages8_view(const rie_hip_pages8 *p, rie::Scales8 &s) {
+    if (!p) throw bad("pages is NULL");
+    const rie_hip_pages &g = p->pages;
+    if (g.ty != T_I8) throw Error{rie::E_UNSUPPORTED, "codes have to be int8"};
+    check_head_dim(g.head_dim, g.n_kv);
+    const rie::KvView v = view_pages(&g, 1);
+    if (p->block < 16 || p->block > g.page_size || (p->block & (p->block - 1)))
+        throw Error{rie::E_UNSUPPORTED, "block has to be a power of two in 16..page_size"};
+    s.k = p->k_scale;
+    s.v = p->v_scale;
+    s.page = used(g.n_pages, p->scale_page_stride);
+    s.block = used(g.page_size / p->block, p->scale_block_stride);
+    s.head = used(g.n_kv, p->scale_head_stride);
+    s.block_shift = __builtin_ctz((unsigned)p->block);
+    const int64_t most = (int64_t)1 << 40;
+    if (s.page < 0 || s.block < 0 || s.head < 0 || s.page > most || s.block > most || s.head > most) throw bad("scales: strides have to lie in 0..2^40");
+    if ((uintptr_t)s.k % 4 || (uintptr_t)s.v % 4) throw bad("scales have to be aligned to their type");
     return v;
 }
 
@@ -160,14 +99,16 @@ rie::ServeAttnArgs attention(const rie_hip_seqs *seqs, const rie_hip_attn *at, i
     return a;
 }
 
-void run_attention(const rie::ServeAttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
+// what an attention call reads and writes, as far as it can be seen without a device; need: its workspace
+void check_attention(const rie::ServeAttnArgs &a, const void *ws, size_t ws_bytes, size_t need) {
     check_rows(a.q, a.q_row / 2, a.q_head / 2, 2, "q");
     check_rows(a.out, a.o_row / 2, a.o_head / 2, 2, "out");
     check_apart({{a.b.n_rows, a.o_row / 2}, {a.n_head, a.o_head / 2}}, a.hd, "out");
-    const size_t need = rie::serve_attn_ws(a);
     if (ws_bytes < need) throw bad("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
     if ((uintptr_t)ws % 16) throw bad("ws has to be 16-byte aligned");
-    const OnDevice dev((hipStream_t)stream);
+}
+
+void check_attention(const rie::ServeAttnArgs &a, const OnDevice &dev, const void *ws, size_t need) {
     dev.check(a.q, "q");
     dev.check(a.out, "out");
     dev.check(a.kv.k, "k");
@@ -178,6 +119,13 @@ void run_attention(const rie::ServeAttnArgs &a, void *ws, size_t ws_bytes, void 
         dev.check(a.b.lens, "lens");
     }
     if (need) dev.check(ws, "ws");
+}
+
+void run_attention(const rie::ServeAttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
+    const size_t need = rie::serve_attn_ws(a);
+    check_attention(a, ws, ws_bytes, need);
+    const OnDevice dev((hipStream_t)stream);
+    check_attention(a, dev, ws, need);
     rie::launch_serve_attn(a, ws, (hipStream_t)stream);
     RIE_HIP_CHECK(hipGetLastError());
 }
@@ -255,6 +203,75 @@ int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs
         const rie::KvView kv = pages_view(pages);
         if (!kv.table) throw bad("table is NULL");
         run_attention(attention(seqs, attn, pages->ty, pages->head_dim, pages->n_kv, kv), ws, ws_bytes, stream);
+    });
+}
+
+int32_t rie_hip_k_paged_append8(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t src_ty, const void *k, const void *v,
+                                int64_t row_stride, int64_t head_stride, void *stream, char *err, size_t err_len) {
+    return guarded(err, err_len, [&] {
+        rie::PagedAppend8Args x;
+        rie::PagedAppendArgs &a = x.a;
+        a.kv = pages8_view(pages, x.s);
+        a.b = batch(seqs, true);
+        const rie_hip_pages &g = pages->pages;
+        if (src_ty != T_F32 && !is16(src_ty)) throw Error{rie::E_UNSUPPORTED, "new rows have to be f32, f16 or bf16"};
+        const int es = src_ty == T_F32 ? 4 : 2;
+        const int64_t row = used(a.b.n_rows, row_stride), head = used(g.n_kv, head_stride);
+        check_rows(k, row, head, es, "k");
+        check_rows(v, row, head, es, "v");
+        // keys and values too, which may lie between one another
+        const int64_t apart = (const uint8_t *)g.v - (const uint8_t *)g.k, scales_apart = x.s.v - x.s.k;
+        check_apart({{g.page_size, g.slot_stride}, {g.n_kv, g.head_stride}, {g.n_pages, g.page_stride}, {2, apart < 0 ? -apart : apart}}, g.head_dim, "pages");
+        check_apart({{g.page_size / pages->block, x.s.block}, {g.n_kv, x.s.head}, {g.n_pages, x.s.page}, {2, scales_apart < 0 ? -scales_apart : scales_apart}}, 1, "scales");
+        if (rie::append8_count(a.b.n_rows, a.b.n_seq, x.s.block_shift) * g.n_kv >= 1 << 25) throw bad("(n_rows/block + 2*n_seq)*n_kv has to stay under 2^25");  // 2^32 threads
+        a.k = (const uint8_t *)k;
+        a.v = (const uint8_t *)v;
+        a.k_row = a.v_row = row * es;
+        a.k_head = a.v_head = head * es;
+        a.n_kv = g.n_kv;
+        a.hd = g.head_dim;
+        a.src_ty = src_ty;
+        const OnDevice dev((hipStream_t)stream);
+        dev.check(a.kv.k, "pages");
+        dev.check(a.kv.v, "pages");
+        dev.check(x.s.k, "k_scale");
+        dev.check(x.s.v, "v_scale");
+        dev.check(a.kv.table, "table");
+        dev.check(a.b.starts, "starts");
+        dev.check(a.b.lens, "lens");
+        dev.check(k, "k");
+        dev.check(v, "v");
+        rie::launch_paged_append8(x, (hipStream_t)stream);
+        RIE_HIP_CHECK(hipGetLastError());
+    });
+}
+
+size_t rie_hip_k_paged_attention8_ws(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t ty, const rie_hip_attn *attn) {
+    size_t n = 0;
+    (void)guarded(nullptr, 0, [&] {
+        rie::Scales8 s;
+        const rie::KvView kv = pages8_view(pages, s);
+        n = rie::serve_attn8_ws(attention(seqs, attn, ty, pages->pages.head_dim, pages->pages.n_kv, kv));
+    });
+    return n;
+}
+
+int32_t rie_hip_k_paged_attention8(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t ty, const rie_hip_attn *attn, void *ws,
+                                   size_t ws_bytes, void *stream, char *err, size_t err_len) {
+    return guarded(err, err_len, [&] {
+        rie::ServeAttn8Args x;
+        const rie::KvView kv = pages8_view(pages, x.s);
+        if (!kv.table) throw bad("table is NULL");
+        if (!is16(ty)) throw Error{rie::E_UNSUPPORTED, "queries and outputs have to be f16 or bf16"};
+        x.a = attention(seqs, attn, ty, pages->pages.head_dim, pages->pages.n_kv, kv);
+        const size_t need = rie::serve_attn8_ws(x.a);
+        check_attention(x.a, ws, ws_bytes, need);
+        const OnDevice dev((hipStream_t)stream);
+        check_attention(x.a, dev, ws, need);
+        dev.check(x.s.k, "k_scale");
+        dev.check(x.s.v, "v_scale");
+        rie::launch_serve_attn8(x, ws, (hipStream_t)stream);
+        RIE_HIP_CHECK(hipGetLastError());
     });
 }
 

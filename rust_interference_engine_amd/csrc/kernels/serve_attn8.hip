@@ -1,0 +1,936 @@
+// serve_attn8.hip — the paged cache in 8 bits, and attention over it.  A value is a code of
+// −127..127 times a scale, which the values of one head at a block of 16, 32, … positions of a
+// page share:
+//
+//   append:     s' = max(s, max |x| / 127) over the block's new values x (s: 0 where the block
+//               holds no earlier position),  c = round(x / s'),  earlier codes c' = round(c · s / s')
+//   attention:  o_t = Σ_j softmax_j(s_tj) v_j  with  s_tj = scale · q_t·k_j  as over 16-bit pages
+//
+// Rounding.  Codes are small whole numbers, exact in any of the matrix units' types, and a scale
+// is the same for all values of a product's row, so it is applied to f32 sums: scores are
+// (q · codes) · s_k, and a value's scale goes into the exponent of its probability,
+// p · s_v = 2^(score + log2 s_v − m).  m is the maximum of these exponents, so that what is
+// multiplied with the codes stays in f16's range whatever the scales are; the sum of the
+// probabilities alone is formed in f32 as Σ (p · s_v) / s_v.  In the few-rows kernel queries are
+// three 8-bit parts of a whole number (23 bits, relative to a row's largest value), and p · s_v
+// two f16 parts; in the tile kernel queries are f16 as they are (bf16 ones with a row's power of
+// two taken out, exact but for values 2^28 times smaller than the row's largest), p · s_v one f16,
+// rounded to nearest.
+//
+// Infinite and NaN values cannot be codes: a block that was given one has a NaN scale, and the
+// tokens that see any of its positions get NaN.  Those that see none of it are unaffected: codes
+// are finite, and exponents are masked after the scales are in.
+#include "../common.hpp"
+#include "../serve_device.hpp"
+
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+namespace rie {
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// A scale as the kernels use it: that of a block of zeros, whose codes are zeros, is any number
+__device__ __forceinline__ float usable(float s) { return s == s ? fminf(fmaxf(s, SCALE8_MIN), SCALE8_MAX) : s; }
+
+// 4 codes in f16.  1024 + (code + 128) is f16's 0x6400 with the code, its sign bit turned over, as
+// the low byte; the difference is exact.
+__device__ __forceinline__ void halves4(uint32_t codes, uint32_t &lo, uint32_t &hi) {
+    const uint32_t u = codes ^ 0x80808080u;
+    const half2_t bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+}
+
+// 8 bytes of one column: lanes 2r and 2r + 1 of a group of 16 name the 16 bytes of row r, and
+// lane l gets rows 0..7 of column l
+__device__ __forceinline__ u32x2 read_tr8(uint32_t at) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(uintptr_t)at));
+}
+
+constexpr float P_SHIFT8 = 6.0f;  // p · s_v is 2^(exponent − m + P_SHIFT8): at most 2^14, and small ones are normal f16 numbers
+
+// ---- a sequence with at most 16·NB query rows: a tile of 32 positions per wave ----
+//
+// As over 16-bit pages (attn_few_kernel): each of the workgroup's 4 waves takes every fourth tile,
+// keys go from global memory to operand registers, values to the wave's own part of LDS, and the
+// waves' results are added up at the end.  Keys meet the query's 8-bit parts on integer matrix
+// instructions as they are; values are read transposed, 8 positions of a dim to a lane, and made
+// f16 there, 10 vector instructions for 8 values.
+constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT;
+template <int HD, int NB>
+constexpr int FEW8_WAVES = NB == 1 ? (HD <= 128 ? 4 : 2) : (HD <= 64 ? 3 : HD <= 128 ? 2 : 1);  // of a SIMD, as registers allow
+
+// A wave's values in LDS: it copies 1 KB at a time, RPI whole rows, by 16-byte chunk, then row
+template <int HD>
+struct Value8Lds {
+    static constexpr int HDP = HD <= 32 ? 32 : HD <= 64 ? 64 : HD <= 128 ? 128 : 256;
+    static constexpr int CPR = HDP / 16, RPI = 64 / CPR;
+    // a read takes 128 bytes of rows 0..7, say, and of rows 16..23: those lie in other banks
+    static constexpr int BLOCK = 1024 + (RPI == 8 ? 64 : RPI == 16 ? 128 : 0);
+    static __device__ __forceinline__ int at(int r, int chunk) { return r / RPI * BLOCK + chunk * (RPI * 16) + r % RPI * 16; }
+    static __device__ __forceinline__ int row(int lane) { return lane % RPI; }
+    static __device__ __forceinline__ int chunk(int lane) { return lane / RPI; }
+};
+
+template <int HD, bool BF, bool CAP, int NB>
+__global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(ServeAttn8Args x) {
+    using Lds = Value8Lds<HD>;
+    const ServeAttnArgs &a = x.a;
+    constexpr int KT = FEW8_KT, RPI = Lds::RPI, NLD = KT / RPI, DB = HD / 16;
+    constexpr int K64 = HD % 64 ? 0 : HD / 64, K32 = HD % 64 ? HD / 32 : 0, KS = K64 + K32;  // products of 64 or of 32 dims
+    constexpr int VB = NLD * Lds::BLOCK, OB = 16 * NB * HD * 4;  // a wave's values, and its outputs at the end
+    constexpr int WB = VB > OB ? VB : OB;
+    __shared__ __align__(16) uint8_t s_buf[4][WB];
+    __shared__ float s_ml[4][16 * NB][2];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
+    const int G = a.G, kvh = blockIdx.x % a.n_kv, si = blockIdx.x / a.n_kv;
+    const SeqView sv = view_of(a.b, a.kv, si);
+    const int n_rows = imin(sv.n_new * G, 16 * NB);
+    if (n_rows == 0) return;
+    const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.pos0();
+    const KeyRange kr = key_range(sv, 0, n_tok - 1, a.window);
+    const int hi = same(kr.hi), t0 = same(first_tile(kr, FEW8_STEP)), nt = same(tile_count(kr, FEW8_STEP)), ns = same(split_count(nt, a.C, a.S)), sp = blockIdx.y;
+    if (sp >= ns) return;
+    const int begin = (t0 + sp * a.C) * 4 + w, end = imin((sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * 4, (hi + KT - 1) / KT);
+
+    // Queries: a row's values are whole numbers of at most 2^22 times 2^(e − 22), in three 8-bit parts
+    int p_q[NB], lo_q[NB];
+    u32x4 qf[NB][KS][3];
+    float qs[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int row = b * 16 + col, tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
+        const bool live = row < n_rows;
+        p_q[b] = live ? imin(pos0 + tok, sv.len - 1) : -1;
+        lo_q[b] = before_window(pos0 + tok, a.window);
+        const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head;
+        u32x4 raw[KS][2];
+        float most = 0;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int d = K64 ? i * 64 + g * 16 : i * 32 + g * 8;
+#pragma unroll
+            for (int u = 0; u < (K64 ? 2 : 1); u++) {
+                raw[i][u] = live ? *(const u32x4 *)(qp + d * 2 + u * 16) : u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float f = fabsf(value16<BF>(raw[i][u][e / 2] >> (e & 1) * 16 & 0xFFFF));
+                    finite = finite && f <= FLT_MAX;
+                    most = fmaxf(most, f);
+                }
+            }
+        }
+        float a0, a1, b0, b1;
+        pair_f<16>(finite ? most : INFINITY, a0, a1);
+        pair_f<32>(fmaxf(a0, a1), b0, b1);
+        most = fmaxf(b0, b1);
+        const int ex = 22 - __builtin_amdgcn_frexp_expf(most);  // most < 2^(22 − ex)
+        qs[b] = most <= FLT_MAX ? __builtin_amdgcn_ldexpf(1.0f, -ex) : NAN;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            u32x4 part[3] = {};
+#pragma unroll
+            for (int u = 0; u < (K64 ? 2 : 1); u++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float f = value16<BF>(raw[i][u][e / 2] >> (e & 1) * 16 & 0xFFFF);
+                    const int n = __float2int_rn(__builtin_amdgcn_ldexpf(f, ex));
+                    const int lo = (int)(int8_t)n, n1 = (n - lo) >> 8, mid = (int)(int8_t)n1, top = (n1 - mid) >> 8;
+                    const int at = (u * 8 + e) / 4, sh = e % 4 * 8;
+                    part[0][at] |= (uint32_t)(lo & 255) << sh;
+                    part[1][at] |= (uint32_t)(mid & 255) << sh;
+                    part[2][at] |= (uint32_t)(top & 255) << sh;
+                }
+#pragma unroll
+            for (int k = 0; k < 3; k++) qf[b][i][k] = part[k];
+        }
+    }
+    const int all_hi = imin(pos0, sv.len - 1), all_lo = before_window(pos0 + n_tok - 1, a.window);
+
+    const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
+    const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
+    uint8_t *vt = s_buf[w];
+    const int k_row = (int)a.kv.k_row, v_row = (int)a.kv.v_row, page_mask = (1 << a.kv.page_shift) - 1;
+    const int v_r = Lds::row(lane), v_c = imin(Lds::chunk(lane), HD / 16 - 1) * 16;
+    // Page ids of a tile's two groups of 16 positions (even and odd lanes), requested a tile ahead.
+    // Positions behind the last one seen are read as copies of it.
+    auto first_of = [&](int t, int b) { return imin(t * KT + b * 16, (hi - 1) & ~15); };
+    auto request_pages = [&](int t) { return t < end ? trow[first_of(t, lane & 1) >> a.kv.page_shift] : 0; };
+    struct Pages {
+        int id, id0, id1, bad;  // the lane's; bad bit b: the page of group b is none (any that exists is read, and nobody sees it)
+    };
+    auto pages_of = [&](int ids) {
+        const bool ok = (unsigned)ids < (unsigned)a.kv.n_pages;
+        Pages p;
+        p.id = ok ? ids : 0;
+        p.bad = (int)(__ballot(!ok) & 3);
+        p.id0 = __builtin_amdgcn_readlane(p.id, 0);
+        p.id1 = __builtin_amdgcn_readlane(p.id, 1);
+        return p;
+    };
+    // lanes 0 and 1: the scales of the groups' keys; 2 and 3: of their values
+    auto request_scales = [&](int t, const Pages &pg) {
+        const int slot = first_of(t, lane & 1) & page_mask;
+        return ((lane & 2) ? x.s.v : x.s.k)[pg.id * x.s.page + (slot >> x.s.block_shift) * x.s.block + kvh * x.s.head];
+    };
+    u32x4 rk[2][KS];
+    auto load_keys = [&](int t, const Pages &pg) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int g0 = first_of(t, b), slot = g0 & page_mask;
+            const uint8_t *kp = kbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.k_row;
+            const int off = imin(col, hi - 1 - g0) * k_row;
+#pragma unroll
+            for (int i = 0; i < K64; i++) rk[b][i] = *(const u32x4 *)(kp + off + i * 64 + g * 16);
+#pragma unroll
+            for (int i = 0; i < K32; i++) {
+                const u32x2 y = *(const u32x2 *)(kp + off + i * 32 + g * 8);
+                rk[b][i] = u32x4{y[0], y[1], 0, 0};
+            }
+        }
+    };
+    auto copy_values = [&](int t, const Pages &pg) __attribute__((always_inline)) {
+        if constexpr (RPI <= 16) {
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const int g0 = first_of(t, b), slot = g0 & page_mask, last = hi - 1 - g0;
+                const uint8_t *vp = vbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.v_row;
+#pragma unroll
+                for (int i = 0; i < NLD / 2; i++) copy_lds(vp, imin(i * RPI + v_r, last) * v_row + v_c, vt + (b * (NLD / 2) + i) * Lds::BLOCK);
+            }
+        } else {  // both groups in one copy: their distance may pass 32 bits, so by way of registers
+            const int b = v_r >> 4, g0 = first_of(t, b), slot = g0 & page_mask;
+            const uint8_t *vp = vbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.v_row + imin(v_r & 15, hi - 1 - g0) * v_row + v_c;
+            *(u32x4 *)(vt + lane * 16) = *(const u32x4 *)vp;
+        }
+    };
+
+    f32x4 o[NB][DB];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        m[b] = -FLT_MAX;
+        l[b] = 0;
+#pragma unroll
+        for (int d = 0; d < DB; d++) o[b][d] = f32x4{};
+    }
+    const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
+    // where the lane reads values: positions 4 g … of both groups, 16 dims of a chunk
+    const int r8 = col >> 1, v_at = Lds::at((r8 & 3) + 4 * g + (r8 >> 2) * 16, 0) + (lane & 1) * 8;
+
+    Pages pg{};
+    int ids = 0;
+    float sc = 1;
+    if (begin < end) {
+        pg = pages_of(request_pages(begin));
+        sc = request_scales(begin, pg);
+        load_keys(begin, pg);
+        copy_values(begin, pg);
+        ids = request_pages(begin + 4);
+    }
+    for (int t = begin; t < end; t += 4) {
+        const int key0 = t * KT, bad = pg.bad;
+        const bool part = key0 + KT - 1 > all_hi || key0 <= all_lo || bad;  // some row does not see all of the tile
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const float us = usable(sc), lg = __builtin_amdgcn_logf(us), rc = us == us ? 1.0f / us : 1.0f;
+        float ks[2], lv[2], iv[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            ks[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(us), b));
+            lv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg), 2 + b));
+            iv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rc), 2 + b));
+        }
+        f32x4 s[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                i32x4 n[3] = {};
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        if constexpr (K64 > 0) {
+                            n[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, rk[kb][i]), __builtin_bit_cast(i32x4, qf[b][i][k]), n[k], 0, 0, 0);
+                        } else {
+                            const long kk = (long)((uint64_t)rk[kb][i][1] << 32 | rk[kb][i][0]), qq = (long)((uint64_t)qf[b][i][k][1] << 32 | qf[b][i][k][0]);
+                            n[k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(kk, qq, n[k], 0, 0, 0);
+                        }
+                    }
+                // |mid · 256 + lo| is under 2^31 for 256 dims
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[b][kb][e] = fmaf((float)n[2][e], 65536.0f, (float)(n[1][e] * 256 + n[0][e]));
+            }
+        if (t + 4 < end) {
+            pg = pages_of(ids);
+            sc = request_scales(t + 4, pg);
+            load_keys(t + 4, pg);
+            ids = request_pages(t + 8);
+        }
+        u32x4 pf[NB][2];  // probabilities times the values' scales, and what their rounding left
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                const float c = ks[kb] * (CAP ? 1.0f : a.scale * LOG2E_F) * qs[b];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float y = CAP ? cap_score<CAP>(s[b][kb][e] * c, cap) + lv[kb] : fmaf(s[b][kb][e], c, lv[kb]);
+                    if (part) {
+                        const int j = key0 + kb * 16 + 4 * g + e;
+                        y = (j > p_q[b]) | (j <= lo_q[b]) | (bad >> kb & 1) ? -INFINITY : y;
+                    }
+                    s[b][kb][e] = y;
+                    mx = fmaxf(mx, y);
+                }
+            }
+            if (__any(mx > m[b] + M_SLACK)) {
+                float x0, x1, y0, y1;
+                pair_f<16>(mx, x0, x1);
+                pair_f<32>(fmaxf(x0, x1), y0, y1);
+                const float mn = fmaxf(m[b], fmaxf(y0, y1)), al = exp2_hw(m[b] - mn);
+                m[b] = mn;
+                l[b] *= al;
+#pragma unroll
+                for (int d = 0; d < DB; d++) o[b][d] *= al;
+            }
+            const float ref = P_SHIFT8 - m[b];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p0 = exp2_hw(s[b][e / 2][2 * (e & 1)] + ref), p1 = exp2_hw(s[b][e / 2][2 * (e & 1) + 1] + ref);
+                const uint32_t near = pack2<false>(p0, p1);
+                pf[b][0][e] = near;
+                pf[b][1][e] = pack2<false>(p0 - h2f(near & 0xFFFF), p1 - h2f(near >> 16));
+                l[b] = fmaf(p0 + p1, iv[e / 2], l[b]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+            const u32x2 c = read_tr8(lds_at(vt) + v_at + Lds::at(0, d));
+            u32x4 vf;
+            uint32_t h0, h1;
+            halves4(c[0], h0, h1);
+            vf[0] = h0;
+            vf[1] = h1;
+            halves4(c[1], h0, h1);
+            vf[2] = h0;
+            vf[3] = h1;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                o[b][d] = mfma16<false>(vf, pf[b][1], o[b][d]);
+                o[b][d] = mfma16<false>(vf, pf[b][0], o[b][d]);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values have been read: their place is free
+        if (t + 4 < end) copy_values(t + 4, pg);
+    }
+
+    // the four waves' results
+    wave_sync();
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        float x0, x1, y0, y1;
+        pair_f<16>(l[b], x0, x1);
+        pair_f<32>(x0 + x1, y0, y1);
+        float *po = (float *)vt + (b * 16 + col) * HD + 4 * g;
+#pragma unroll
+        for (int d = 0; d < DB; d++) *(f32x4 *)(po + d * 16) = o[b][d];
+        if (g == 0) {
+            s_ml[w][b * 16 + col][0] = m[b];
+            s_ml[w][b * 16 + col][1] = y0 + y1;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_rows * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), d4 = i % (HD / 4), tok = r / G, head = kvh * G + r - tok * G;
+        float mm = s_ml[0][r][0];
+#pragma unroll
+        for (int k = 1; k < 4; k++) mm = fmaxf(mm, s_ml[k][r][0]);
+        f32x4 acc = f32x4{};
+        float L = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = exp2_hw(s_ml[k][r][0] - mm);
+            L = fmaf(f, s_ml[k][r][1], L);
+            const f32x4 y = *(const f32x4 *)((const float *)s_buf[k] + r * HD + d4 * 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] = fmaf(f, y[e], acc[e]);
+        }
+        if (ns == 1) {
+            const float inv = L > 0 || L != L ? 1.0f / L : 0.0f;
+            uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d4 * 8;
+            *(u32x2 *)op = u32x2{pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
+        } else {
+            const int64_t at = ((int64_t)(sv.row0 + tok) * a.n_head + head) * a.S + sp;
+            *(f32x4 *)(a.part + at * HD + d4 * 4) = acc;
+            if (d4 == 0) *(f32x2 *)(a.ml + at * 2) = f32x2{mm, L};
+        }
+    }
+}
+
+// ---- 128 query rows of a sequence and KV head, tiles of 64 (256-wide heads: 32) positions ----
+//
+// The schedule is that of the 16-bit tile kernel: a tile's work is cut into groups of 32
+// positions, and the probabilities of group h are made while the matrix units form the outputs of
+// h − 1 and the scores of h + 1.  A tile lies in LDS in f16, which its four waves share: codes come
+// to registers a tile ahead, each wave's 16 (8) rows, and are made f16 on their way to LDS (5
+// vector instructions for 4 values), in the place of a tile that has been read by then.
+template <int HD>
+constexpr int TILE8_KT = HD <= 128 ? 64 : 32;
+
+template <int HD, bool BF, bool CAP>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(ServeAttn8Args xa) {
+    const ServeAttnArgs &a = xa.a;
+    constexpr int KT = TILE8_KT<HD>, KB = KT / 32, RW = KT / 4, KS = HD / 16, DB = HD / 32;
+    using Lds = TileLds<HD>;
+    constexpr int RPI = Lds::RPI, KBYTES = KT / RPI * Lds::K_BLOCK, VBYTES = KT / RPI * Lds::V_BLOCK;
+    constexpr int NG = KT / 16;                                         // groups of 16 positions, which lie in one page and block
+    constexpr int CH = RW * (HD / 16), NCH = (CH + 63) / 64;            // 16-byte chunks of a wave's rows, and of a lane
+    __shared__ __align__(16) uint8_t s_k0[KBYTES], s_k1[KBYTES], s_v0[VBYTES], s_v1[VBYTES];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    // the splits of a block side by side, and a KV head's workgroups on one XCD where there are 8 of them
+    const int G = a.G, kvh = blockIdx.x % a.n_kv, sp = blockIdx.x / a.n_kv % a.S, blk = blockIdx.x / a.n_kv / a.S;
+    int si;
+    const SeqView sv = find_seq(a.b, a.kv, blk, si, [&](int s, int i) { return block_base(iclamp(s, 0, a.b.n_rows), i, G, TILE_M); });
+    const int n_rows = sv.n_new * G;
+    const int lb = (n_rows + TILE_M - 1) / TILE_M - 1 - (blk - block_base(sv.row0, si, G, TILE_M));  // a sequence's longest rows first
+    if (lb < 0 || lb >= (n_rows + TILE_M - 1) / TILE_M) return;
+    const int r0 = same(lb * TILE_M), r1 = same(imin(r0 + TILE_M, n_rows) - 1), tok0 = same(r0 / G), tok1 = same(r1 / G);
+    const int pos0 = sv.pos0();  // position of token 0
+    const KeyRange kr = key_range(sv, tok0, tok1, a.window);
+    const int hi = same(kr.hi), nt = same(tile_count(kr, KT)), ns = same(split_count(nt, a.C, a.S));
+    if (sp >= ns) return;
+    const int t_first = same(first_tile(kr, KT)), t_begin = t_first + sp * a.C, t_end = sp == ns - 1 ? t_first + nt : t_begin + a.C;
+
+    // this lane's query row, and what the rows of its wave see
+    const int row = r0 + w * 32 + (lane & 31);
+    const bool live = row < n_rows;
+    const int tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
+    const int p_q = live ? imin(pos0 + tok, sv.len - 1) : -1;
+    const int lo_q = before_window(pos0 + tok, a.window);  // sees j in (lo_q, p_q]
+    const bool wave_live = r0 + w * 32 <= r1;
+    const int w_t0 = same(imin(r0 + w * 32, r1) / G), w_t1 = same(imin(r0 + w * 32 + 31, r1) / G);
+    const int all_hi = imin(pos0 + w_t0, sv.len - 1), all_lo = before_window(pos0 + w_t1, a.window);  // every row of the wave sees (all_lo, all_hi]
+    u32x4 qf[KS];
+    {
+        const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + h * 16;
+#pragma unroll
+        for (int i = 0; i < KS; i++) qf[i] = live ? *(const u32x4 *)(qp + i * 32) : u32x4{0, 0, 0, 0};
+    }
+    float qs = 1;  // a row's power of two
+    if constexpr (BF) {
+        float most = 0;
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(value16<true>(qf[i][e / 2] >> (e & 1) * 16 & 0xFFFF)));
+        float a0, a1;
+        pair_f<32>(most, a0, a1);
+        const int ex = 14 - __builtin_amdgcn_frexp_expf(fminf(fmaxf(a0, a1), FLT_MAX));  // infinities stay what they are
+        qs = __builtin_amdgcn_ldexpf(1.0f, -ex);
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                qf[i][e] = pack2<false>(__builtin_amdgcn_ldexpf(value16<true>(qf[i][e] & 0xFFFF), ex), __builtin_amdgcn_ldexpf(value16<true>(qf[i][e] >> 16), ex));
+    }
+
+    // ---- codes: wave w's are rows w·RW .. of a tile, which lie in one page ----
+    const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
+    const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
+    const int k_row = (int)a.kv.k_row, v_row = (int)a.kv.v_row, page_mask = (1 << a.kv.page_shift) - 1;
+    // Of a tile: page ids of its groups of 16 positions, a lane each, and (lanes 0.. and 4..) their
+    // keys' and values' scales.  A page id that is none: any page that exists is read, and nobody
+    // sees its values.
+    auto group_at = [&](int t) { return imin(t * KT + (lane & (NG - 1)) * 16, (hi - 1) & ~15); };
+    auto request_pages = [&](int t) __attribute__((always_inline)) { return t < t_end ? trow[group_at(t) >> a.kv.page_shift] : -1; };
+    auto known = [&](int id) { return (unsigned)id < (unsigned)a.kv.n_pages ? id : 0; };
+    auto bad_of = [&](int ids) __attribute__((always_inline)) { return same((int)(__ballot((unsigned)ids >= (unsigned)a.kv.n_pages) & ((1u << NG) - 1))); };
+    auto request_scales = [&](int t, int ids) __attribute__((always_inline)) {
+        const int slot = group_at(t) & page_mask;
+        return ((lane & 4) ? xa.s.v : xa.s.k)[known(ids) * xa.s.page + (slot >> xa.s.block_shift) * xa.s.block + kvh * xa.s.head];
+    };
+    auto load = [&](const uint8_t *base, int rs, int t, int ids, u32x4 (&raw)[NCH]) __attribute__((always_inline)) {
+        const int g0 = imin(t * KT + w * RW, (hi - 1) & ~(RW - 1));  // rows behind the last one seen: copies of it
+        const int64_t page = __builtin_amdgcn_readlane(known(ids), w * RW / 16);
+        const uint8_t *src = base + page * a.kv.page + (int64_t)(g0 & page_mask) * rs;
+        const int last = hi - 1 - g0;
+#pragma unroll
+        for (int i = 0; i < NCH; i++) {
+            const int u = imin(i * 64 + lane, CH - 1), r = u % RW, c = u / RW;
+            raw[i] = *(const u32x4 *)(src + imin(r, last) * rs + c * 16);
+        }
+    };
+    auto store = [&](auto is_v, const u32x4 (&raw)[NCH], uint8_t *dst) __attribute__((always_inline)) {
+        constexpr bool V = decltype(is_v)::value;
+#pragma unroll
+        for (int i = 0; i < NCH; i++) {
+            const int u = i * 64 + lane, r = w * RW + u % RW, c = u / RW;
+            if (CH % 64 && u >= CH) continue;
+            u32x4 y[2];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t lo, hi2;
+                halves4(raw[i][k], lo, hi2);
+                y[k / 2][k % 2 * 2] = lo;
+                y[k / 2][k % 2 * 2 + 1] = hi2;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) *(u32x4 *)(dst + (V ? Lds::value(r, 2 * c + k) : Lds::key(r, 2 * c + k))) = y[k];
+        }
+    };
+    using K_ = std::false_type;
+    using V_ = std::true_type;
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x16{};
+    float m = -FLT_MAX, l = 0, ym0 = 0, ym1 = 0;  // ym: largest scores of either half of the group whose turn is next
+    const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
+    const float cq = CAP ? qs : a.scale * LOG2E_F;
+    // the lane's places in a tile: keys row-wise, values transposed
+    const int k_at = Lds::key(lane & 31, h), v_at = Lds::value(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
+
+    f32x16 s[2];
+    u32x4 pf[2][2];
+    struct GroupScales {  // of a group's halves: a score's factor, log2 of the values' scale and its inverse
+        float c[2], lv[2], iv[2];
+    };
+    auto scales_of = [&](float sc, int kb) __attribute__((always_inline)) {
+        const float us = usable(sc), lg = __builtin_amdgcn_logf(us), rc = us == us ? 1.0f / us : 1.0f;
+        GroupScales x;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            x.c[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(us), kb * 2 + b)) * cq;
+            if (BF && !CAP) x.c[b] *= qs;
+            x.lv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg), 4 + kb * 2 + b));
+            x.iv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rc), 4 + kb * 2 + b));
+        }
+        return x;
+    };
+    auto max8 = [&](const f32x16 &x, int at) __attribute__((always_inline)) {
+        float v = fmaxf(fmaxf(x[at], x[at + 1]), x[at + 2]);
+        v = fmaxf(fmaxf(v, x[at + 3]), x[at + 4]);
+        return fmaxf(fmaxf(fmaxf(v, x[at + 5]), x[at + 6]), x[at + 7]);
+    };
+    auto scores = [&](uint32_t kt, int kb, f32x16 &d) __attribute__((always_inline)) {
+        d = f32x16{};
+#pragma unroll
+        for (int i = 0; i < KS; i++) d = mfma32<false>(lds_16(kt + k_at + Lds::key(kb * 32, 2 * i)), qf[i], d);
+    };
+    auto outputs = [&](uint32_t vt, int kb, const u32x4 (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const uint32_t vp = vt + v_at + Lds::value(kb * 32 + st * 16, 4 * d);
+                const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
+                o[d] = mfma32<false>(u32x4{v0[0], v0[1], v1[0], v1[1]}, p[st], o[d]);
+            }
+    };
+    // group (t, kb): probabilities of its scores x → p; outputs of the group before from values
+    // (vt, vkb) and probabilities po; scores of the group behind from keys (kt, nkb) → y
+    auto group = [&](int key0, int bad2, const GroupScales &gs, f32x16 &x, u32x4 (&p)[2], const u32x4 (&po)[2], f32x16 &y, uint32_t vt, int vkb, uint32_t kt, int nkb) __attribute__((always_inline)) {
+        // positions of the lane's scores: key0 + 4 h + (8 (e / 4) + e % 4)
+        float c[2] = {gs.c[0], gs.c[1]}, lv[2] = {gs.lv[0], gs.lv[1]};
+        float mx = fmaxf(fmaf(ym0, c[0], lv[0]), fmaf(ym1, c[1], lv[1]));
+        const bool late = key0 + 31 > all_hi, early = key0 <= all_lo;
+        if (CAP || late || early || bad2) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = CAP ? cap_score<CAP>(x[e] * c[e / 8], cap) + lv[e / 8] : fmaf(x[e], c[e / 8], lv[e / 8]);
+            if (late) {
+                const int d = p_q - key0 - 4 * h;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 <= d ? x[e] : -INFINITY;
+            }
+            if (early) {
+                const int d = lo_q - key0 - 4 * h;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 8 * (e / 4) + e % 4 > d ? x[e] : -INFINITY;
+            }
+            if (bad2) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = bad2 >> (e / 8) & 1 ? -INFINITY : x[e];
+            }
+            c[0] = c[1] = 1;
+            lv[0] = lv[1] = 0;
+            mx = fmaxf(max8(x, 0), max8(x, 8));
+        }
+        const bool moved = __any(mx > m + M_SLACK);
+        float al = 1;
+        if (moved) {
+            float a0, a1;
+            pair_f<32>(mx, a0, a1);
+            const float mn = fmaxf(m, fmaxf(a0, a1));
+            al = exp2_hw(m - mn);
+            m = mn;
+            l *= al;
+        }
+        // Eight rounds of matrix products, first the scores', then the outputs', operands read three
+        // products ahead, with a share of the probabilities after each; the next group's maximum
+        // at the end, so that its own round begins with it.  The fences keep the order.
+        constexpr int NV = 2 * DB, NM = KS + NV;
+        y = f32x16{};
+        const float ref[2] = {P_SHIFT8 - m + lv[0], P_SHIFT8 - m + lv[1]};
+        u32x4 fr[NM];
+        auto read = [&](int u) __attribute__((always_inline)) {
+            if (u >= NM) return;
+            if (u < KS) {
+                fr[u] = lds_16(kt + k_at + Lds::key(nkb * 32, 2 * u));
+            } else {
+                const uint32_t vp = vt + v_at + Lds::value(vkb * 32 + (u - KS) / DB * 16, (u - KS) % DB * 4);
+                const u32x2 v0 = read_tr(vp), v1 = read_tr(vp + Lds::value(8, 0));
+                fr[u] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+            }
+        };
+        float ex[16], sum[2] = {0, 0};
+        auto exps = [&](int i) __attribute__((always_inline)) {
+            ex[2 * i] = exp2_hw(fmaf(x[2 * i], c[i / 4], ref[i / 4]));
+            ex[2 * i + 1] = exp2_hw(fmaf(x[2 * i + 1], c[i / 4], ref[i / 4]));
+        };
+        auto pack = [&](int i) __attribute__((always_inline)) {
+            p[i / 4][i % 4] = pack2<false>(ex[2 * i], ex[2 * i + 1]);
+            sum[i / 4] += ex[2 * i];
+            sum[i / 4] += ex[2 * i + 1];
+        };
+        auto product = [&](int u) __attribute__((always_inline)) {
+            if (u < KS) y = mfma32<false>(fr[u], qf[u], y);
+            else o[(u - KS) % DB] = mfma32<false>(fr[u], po[(u - KS) / DB], o[(u - KS) % DB]);
+        };
+        constexpr int AHEAD = 3;
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) read(u);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int u0 = i * NM / 8, u1 = (i + 1) * NM / 8;
+            if (u0 < u1) {
+                product(u0);
+                read(u0 + AHEAD);
+            }
+            exps(i);
+            if (u0 < u1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = u0 + 1; u < u1; u++) {
+                product(u);
+                read(u + AHEAD);
+                if (u < u1 - 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            pack(i);
+            if (u0 + 1 < u1) __builtin_amdgcn_sched_barrier(0);
+            if (i == 6) ym0 = max8(y, 0);
+            if (i == 7) ym1 = max8(y, 8);
+        }
+        l = fmaf(sum[1], gs.iv[1], fmaf(sum[0], gs.iv[0], l));
+        // all three belong into this block: the compiler would move the probabilities to where
+        // they are used, and make two copies of the block
+        asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l), "+v"(ym0), "+v"(ym1));
+        int after = __builtin_amdgcn_readfirstlane(moved);
+        asm volatile("" : "+s"(after));
+        if (after) {  // the outputs so far were formed with the maximum before
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= al;
+        }
+    };
+
+    if (t_begin < t_end) {
+        // page ids of tiles t .. t + 3, the scales of t and t + 1, codes of keys t + 2 and of values t + KB − 1
+        int id0 = request_pages(t_begin), id1 = request_pages(t_begin + 1), id2 = request_pages(t_begin + 2), id3 = request_pages(t_begin + 3);
+        float sc0 = request_scales(t_begin, id0), sc1 = request_scales(t_begin + 1, id1);
+        u32x4 rk[NCH], rv[NCH];
+        load(kbase, k_row, t_begin, id0, rk);
+        store(K_{}, rk, s_k0);
+        if (t_begin + 1 < t_end) {
+            load(kbase, k_row, t_begin + 1, id1, rk);
+            store(K_{}, rk, s_k1);
+        }
+        load(vbase, v_row, t_begin, id0, rv);
+        if constexpr (KB == 2) {
+            store(V_{}, rv, s_v0);
+            if (t_begin + 1 < t_end) load(vbase, v_row, t_begin + 1, id1, rv);
+        }
+        if (t_begin + 2 < t_end) load(kbase, k_row, t_begin + 2, id2, rk);
+        // the first group's outputs before it: zeros
+        for (int i = w; i < 32 / RPI; i += 4) *(u32x4 *)(s_v1 + Lds::value((KB - 1) * 32 + i * RPI, 0) + lane * 16) = u32x4{0, 0, 0, 0};
+        pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
+        lds_barrier();
+        if (wave_live) {
+            scores(lds_at(s_k0), 0, s[0]);
+            ym0 = max8(s[0], 0);
+            ym1 = max8(s[0], 8);
+        }
+        auto tile = [&](int t, uint8_t *k_t, uint8_t *k_n, uint8_t *v_t, uint8_t *v_n, f32x16 &x0, f32x16 &x1, u32x4 (&p0)[2], u32x4 (&p1)[2]) __attribute__((always_inline)) {
+            const int bad = bad_of(id0);
+            if constexpr (KB == 2)
+                if (wave_live) group(t * KT, bad & 3, scales_of(sc0, 0), x0, p0, p1, x1, lds_at(v_n), 1, lds_at(k_t), 1);
+            lds_barrier();
+            if (t + 2 < t_end) store(K_{}, rk, k_t);
+            if constexpr (KB == 2) {
+                if (t + 1 < t_end) store(V_{}, rv, v_n);
+                if (t + 2 < t_end) load(vbase, v_row, t + 2, id2, rv);
+            } else {
+                store(V_{}, rv, v_t);
+                if (t + 1 < t_end) load(vbase, v_row, t + 1, id1, rv);
+            }
+            if (t + 3 < t_end) load(kbase, k_row, t + 3, id3, rk);
+            const int id4 = request_pages(t + 4);
+            const float sc2 = request_scales(t + 2, id2);
+            if (wave_live) {
+                if constexpr (KB == 2) group(t * KT + 32, bad >> 2, scales_of(sc0, 1), x1, p1, p0, x0, lds_at(v_t), 0, lds_at(k_n), 0);
+                else group(t * KT, bad, scales_of(sc0, 0), x0, p0, p1, x1, lds_at(v_n), 0, lds_at(k_n), 0);
+            }
+            id0 = id1;
+            id1 = id2;
+            id2 = id3;
+            id3 = id4;
+            sc0 = sc1;
+            sc1 = sc2;
+        };
+        for (int t = t_begin; t < t_end; t += 2) {
+            tile(t, s_k0, s_k1, s_v0, s_v1, s[0], s[1], pf[0], pf[1]);
+            if (t + 1 >= t_end) break;
+            if constexpr (KB == 2) tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[0], s[1], pf[0], pf[1]);
+            else tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[1], s[0], pf[1], pf[0]);
+        }
+        // the last group's outputs
+        const bool odd = (t_end - t_begin) & 1;
+        if constexpr (KB == 1) lds_barrier();
+        if (wave_live) {
+            if (odd) outputs(lds_at(s_v0), KB - 1, pf[KB == 2 ? 1 : 0]);
+            else outputs(lds_at(s_v1), KB - 1, pf[1]);
+        }
+    }
+    if (!live) return;
+    float l0, l1;
+    pair_f<32>(l, l0, l1);
+    l = l0 + l1;
+    if (ns == 1) {
+        const float inv = l > 0 || l != l ? 1.0f / l : 0.0f;
+        uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + h * 8;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u32x2 v = {pack2<BF>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv), pack2<BF>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)};
+                *(u32x2 *)(op + d * 64 + e * 16) = v;
+            }
+    } else {
+        const int64_t at = ((int64_t)(sv.row0 + tok) * a.n_head + head) * a.S + sp;
+        float *pp = a.part + at * HD + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) *(f32x4 *)(pp + d * 32 + e * 8) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+        if (h == 0) *(f32x2 *)(a.ml + at * 2) = f32x2{m, l};
+    }
+}
+
+// ---- new rows into their pages ----
+//
+// A wave takes what a call brings to one block of positions, of one head's keys or values: the
+// rows' largest value, the block's new scale, the codes of earlier positions where it has grown,
+// and the new ones.  Codes are rounded from f64 quotients, so that they are those of the formula.
+// Blocks are numbered without a list: sequence i owns ids from ⌊start / block⌋ + 2 i on, which
+// are enough, since n new tokens touch at most ⌊n / block⌋ + 2 blocks.
+template <int SRC>  // ggml type
+__device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
+    if constexpr (SRC == T_F32) {
+        const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = a[e];
+            v[4 + e] = b[e];
+        }
+    } else {
+        const u32x4 a = *(const u32x4 *)p;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = value16<SRC == T_BF16>(a[e / 2] >> (e & 1) * 16 & 0xFFFF);
+    }
+}
+
+template <int HD, int SRC>
+__global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) {
+    const PagedAppendArgs &a = x.a;
+    constexpr int CPR = HD / 8, RP = 64 / CPR, NP = (16 + RP - 1) / RP;  // lanes of a row, rows of a pass, passes of 16 rows
+    constexpr int ES = SRC == T_F32 ? 4 : 2;
+    const int lane = threadIdx.x & 63, u = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = u / (2 * a.n_kv), h = u / 2 % a.n_kv;
+    const bool is_v = u & 1;
+    const int bs = x.s.block_shift, B = 1 << bs;
+    if (id >= append8_id(a.b.n_rows, a.b.n_seq, bs)) return;
+    int si;
+    const SeqView sv = find_seq(a.b, a.kv, id, si, [&](int s, int i) { return append8_id(iclamp(s, 0, a.b.n_rows), i, bs); });
+    const int pos0 = sv.pos0(), from = imax(pos0, 0), to = imin(pos0 + sv.n_new, sv.len);  // positions that are written
+    const int b0 = same(((from >> bs) + id - append8_id(sv.row0, si, bs)) << bs);          // the block's first position
+    if (b0 >= to) return;
+    int page;
+    if (!page_of(a.kv, a.kv.table + (int64_t)si * a.kv.table_stride, b0, page)) return;
+    page = same(page);
+    const int first = imax(b0, from), n = imin(b0 + B, to) - first, slot0 = b0 & ((1 << a.kv.page_shift) - 1);
+    if (n <= 0) return;
+    float *sp = (is_v ? x.s.v : x.s.k) + page * x.s.page + (slot0 >> bs) * x.s.block + h * x.s.head;
+    const float was = first > b0 ? *sp : 0.0f;
+    const uint8_t *src = (is_v ? a.v + h * a.v_head : a.k + h * a.k_head) + (int64_t)(sv.row0 + first - pos0) * (is_v ? a.v_row : a.k_row);
+    const int64_t src_row = is_v ? a.v_row : a.k_row, row = is_v ? a.kv.v_row : a.kv.k_row;
+    uint8_t *dst = const_cast<uint8_t *>(is_v ? a.kv.v + h * a.kv.v_head : a.kv.k + h * a.kv.k_head) + page * a.kv.page + slot0 * row;
+    const int r = lane / CPR, ch = lane % CPR;
+    const bool on = r < RP;
+
+    float v[NP][8];  // 16 rows at a time; those of a block of 16 stay
+    auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int q = r0 + i * RP + r;
+            if (on && i * RP + r < 16 && q < n) load8<SRC>(src + q * src_row + ch * (8 * ES), v[i]);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[i][e] = 0;
+        }
+    };
+    float most = 0;
+    bool fine = true;
+    for (int r0 = 0; r0 < n; r0 += 16) {
+        load(r0);
+#pragma unroll
+        for (int i = 0; i < NP; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                fine = fine && fabsf(v[i][e]) <= FLT_MAX;
+                most = fmaxf(most, fabsf(v[i][e]));
+            }
+    }
+    most = xmax_f<64>(most);
+    float now = (float)((double)most / 127.0);
+    if (now < SCALE8_MIN) now = 0;
+    if (__any(!fine) || now > SCALE8_MAX || !(was >= 0 && was <= SCALE8_MAX)) now = NAN;
+    else now = fmaxf(now, was);
+    if (lane == 0) *sp = now;
+    if (first > b0 && now > was) {  // codes of earlier positions
+        const double f = (double)was / (double)now;
+        for (int q = r; q < first - b0; q += RP) {
+            if (!on) break;
+            u32x2 *p = (u32x2 *)(dst + q * row + ch * 8);
+            u32x2 y = *p;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int c = (int)(int8_t)(y[e / 4] >> e % 4 * 8);
+                const uint32_t again = (uint32_t)__double2int_rn(c * f) & 255;
+                y[e / 4] = (y[e / 4] & ~(255u << e % 4 * 8)) | again << e % 4 * 8;
+            }
+            *p = y;
+        }
+    }
+    const double inv = now > 0 ? 1.0 / (double)now : 0.0;
+    for (int r0 = 0; r0 < n; r0 += 16) {
+        if (n > 16) load(r0);
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int q = r0 + i * RP + r;
+            if (!(on && i * RP + r < 16 && q < n)) continue;
+            u32x2 y = {0, 0};
+            if (inv > 0)
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e / 4] |= ((uint32_t)__double2int_rn((double)v[i][e] * inv) & 255) << e % 4 * 8;
+            *(u32x2 *)(dst + (first - b0 + q) * row + ch * 8) = y;
+        }
+    }
+}
+
+template <int HD, bool BF>
+void launch_hd(const ServeAttn8Args &x, hipStream_t st) {
+    const ServeAttnArgs &a = x.a;
+    const bool cap = a.softcap > 0;
+    const int few = few_row_blocks(true, a.b.max_new, a.G);
+    if (few) {
+        const dim3 grid(a.b.n_seq * a.n_kv, a.S);
+        if (few == 1) {
+            if (cap) attn8_few_kernel<HD, BF, true, 1><<<grid, 256, 0, st>>>(x);
+            else attn8_few_kernel<HD, BF, false, 1><<<grid, 256, 0, st>>>(x);
+        } else {
+            if (cap) attn8_few_kernel<HD, BF, true, 2><<<grid, 256, 0, st>>>(x);
+            else attn8_few_kernel<HD, BF, false, 2><<<grid, 256, 0, st>>>(x);
+        }
+    } else {
+        const int grid = a.n_blocks * a.n_kv * a.S;
+        if (cap) attn8_tile_kernel<HD, BF, true><<<grid, 256, 0, st>>>(x);
+        else attn8_tile_kernel<HD, BF, false><<<grid, 256, 0, st>>>(x);
+    }
+}
+
+template <bool BF>
+void launch_ty(const ServeAttn8Args &x, hipStream_t st) {
+    switch (x.a.hd) {
+    case 32: launch_hd<32, BF>(x, st); break;
+    case 64: launch_hd<64, BF>(x, st); break;
+    case 96: launch_hd<96, BF>(x, st); break;
+    case 128: launch_hd<128, BF>(x, st); break;
+    default: launch_hd<256, BF>(x, st); break;
+    }
+}
+
+template <int SRC>
+void launch_append(const PagedAppend8Args &x, int grid, hipStream_t st) {
+    switch (x.a.hd) {
+    case 32: paged_append8_kernel<32, SRC><<<grid, 256, 0, st>>>(x); break;
+    case 64: paged_append8_kernel<64, SRC><<<grid, 256, 0, st>>>(x); break;
+    case 96: paged_append8_kernel<96, SRC><<<grid, 256, 0, st>>>(x); break;
+    case 128: paged_append8_kernel<128, SRC><<<grid, 256, 0, st>>>(x); break;
+    default: paged_append8_kernel<256, SRC><<<grid, 256, 0, st>>>(x); break;
+    }
+}
+
+int tile8_kt(int hd) { return hd <= 128 ? TILE8_KT<128> : TILE8_KT<256>; }
+
+SplitPlan splits8(const ServeAttnArgs &a) {
+    const bool few = few_row_blocks(true, a.b.max_new, a.G) > 0;
+    const int KT = few ? FEW8_STEP : tile8_kt(a.hd);
+    const int64_t blocks = few ? a.b.n_seq : block_count(a.b.n_rows, a.b.n_seq, a.G, TILE_M);
+    // positions that a block's rows see, at most
+    int64_t span = a.b.max_len;
+    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? FEW_ROWS : TILE_M / a.G + 1) + KT);
+    const int tiles = (int)((span + KT - 1) / KT);
+    if (few) return split_plan(blocks * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
+    const double part_us = (double)a.b.n_rows * a.n_head * a.hd * 8 / 4.5e6;
+    return tile_plan(blocks * a.n_kv, a.hd <= 128 ? 512 : 256, tiles, 2.0 * KT * a.hd / (64 * 128), part_us, SERVE_MAX_SPLIT);
+}
+
+}  // namespace
+
+size_t serve_attn8_ws(const ServeAttnArgs &a) {
+    const SplitPlan p = splits8(a);
+    return p.S == 1 ? 0 : (size_t)a.b.n_rows * a.n_head * p.S * (a.hd + 2) * sizeof(float);
+}
+
+void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st) {
+    ServeAttnArgs &a = x.a;
+    const SplitPlan p = splits8(a);
+    const bool few = few_row_blocks(true, a.b.max_new, a.G) > 0;
+    a.C = p.C;
+    a.S = p.S;
+    a.part = (float *)ws;
+    a.ml = a.part + (size_t)a.b.n_rows * a.n_head * p.S * a.hd;
+    a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, TILE_M);
+    if (a.ty == T_BF16) launch_ty<true>(x, st);
+    else launch_ty<false>(x, st);
+    if (p.S > 1) launch_serve_combine(a, few ? FEW_ROWS : TILE_M, few ? FEW8_STEP : tile8_kt(a.hd), st);
+}
+
+void launch_paged_append8(const PagedAppend8Args &x, hipStream_t st) {
+    const int64_t waves = (int64_t)append8_count(x.a.b.n_rows, x.a.b.n_seq, x.s.block_shift) * x.a.n_kv * 2;
+    const int grid = (int)((waves + 3) / 4);
+    if (x.a.src_ty == T_F32) launch_append<T_F32>(x, grid, st);
+    else if (x.a.src_ty == T_BF16) launch_append<T_BF16>(x, grid, st);
+    else launch_append<T_F16>(x, grid, st);
+}
+
+}  // namespace rie

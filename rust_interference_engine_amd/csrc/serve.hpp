@@ -45,6 +45,24 @@ size_t serve_attn_ws(const ServeAttnArgs &a);
 bool serve_attn_head_dim_ok(int hd);
 void launch_serve_attn(ServeAttnArgs a, void *ws, hipStream_t st);
 
+// adds the splits of each (row, head) up: M rows per block and KT positions per tile are those of
+// the kernel that made the partials
+void launch_serve_combine(const ServeAttnArgs &a, int M, int KT, hipStream_t st);
+
+// Pages of 8 bits: a value is its code times the scale of its block of positions and head
+struct Scales8 {
+    float *k = nullptr, *v = nullptr;
+    int64_t page = 0, block = 0, head = 0;  // strides, values
+    int block_shift = 0;
+};
+constexpr float SCALE8_MIN = 0x1p-60f, SCALE8_MAX = 0x1p50f;  // of blocks that hold anything but zeros
+struct ServeAttn8Args {
+    ServeAttnArgs a;  // a.ty: type of queries and outputs
+    Scales8 s;
+};
+size_t serve_attn8_ws(const ServeAttnArgs &a);
+void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st);
+
 struct PagedAppendArgs {
     KvView kv;  // kv.k and kv.v are written
     BatchView b;
@@ -53,6 +71,11 @@ struct PagedAppendArgs {
     int n_kv = 0, hd = 0, ty = 0, src_ty = 0;
 };
 void launch_paged_append(const PagedAppendArgs &a, hipStream_t st);
+struct PagedAppend8Args {
+    PagedAppendArgs a;  // a.ty is not looked at
+    Scales8 s;
+};
+void launch_paged_append8(const PagedAppend8Args &x, hipStream_t st);
 
 struct LogprobArgs {
     const void *x = nullptr;

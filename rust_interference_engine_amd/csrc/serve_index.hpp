@@ -46,6 +46,11 @@ RIE_HD SeqView seq_view(int start, int end, int len, int n_rows, int cap) {
 RIE_HD int block_base(int start, int i, int G, int M) { return (int)((int64_t)start * G / M) + i; }
 inline int64_t block_count(int n_rows, int n_seq, int G, int M) { return (int64_t)n_rows * G / M + n_seq; }
 
+// The same for blocks of 2^shift positions of a cache of 8 bits that a sequence's new tokens are
+// written to: n of them touch at most ⌊n / 2^shift⌋ + 2 blocks, wherever the first one lies.
+RIE_HD int append8_id(int start, int i, int shift) { return (start >> shift) + 2 * i; }
+inline int64_t append8_count(int n_rows, int n_seq, int shift) { return ((int64_t)n_rows >> shift) + 2 * (int64_t)n_seq; }
+
 // the last position before the window of a token at position p (window 0: none), for any p and
 // any window of 31 bits
 RIE_HD int before_window(int p, int window) { return window > 0 ? imax(p, -1) - window : -1; }

@@ -28,6 +28,7 @@ from . import _lib
 from .backend import RieError
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml type ids
+_I8 = 24
 
 
 def _current_stream(device: int) -> int:
@@ -154,9 +155,14 @@ class Seqs:
 class PagedKv:
     """A layer's keys and values in pages: ``k`` and ``v`` [pages, page size, KV heads, head
     size] of the same type and strides (a transposed view of another order of the middle
-    two will do), ``table`` int32 [sequences, most pages of one]."""
+    two will do), ``table`` int32 [sequences, most pages of one].
 
-    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
+    In 8 bits: ``k`` and ``v`` are int8 codes, and ``k_scale`` and ``v_scale`` (f32 [pages,
+    blocks of a page, KV heads], of the same strides) what the codes of a block of page size /
+    blocks positions are multiplied by.  A block that new tokens come to is one sequence's alone."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, *, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None):
         _need(k.dim() == 4 and k.numel() > 0, f"pages have to be [pages, page size, KV heads, head size], got {tuple(k.shape)}")
         _need(k.shape == v.shape and k.dtype == v.dtype and _strides(k) == _strides(v), "k and v have to have one shape, type and strides")
         _need(k.shape[3] == 1 or k.stride(3) == 1, "pages: a row's values have to be consecutive")
@@ -165,8 +171,21 @@ class PagedKv:
         self.device = _device(k, v, table)
         self.k, self.v, self.table = k, v, table
         n_pages, page, n_kv, hd = k.shape
-        self._struct = _lib.Pages(_type(k, "pages"), hd, n_kv, n_pages, page, table.shape[1], k.data_ptr(), v.data_ptr(),
-                                  k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), table.stride(0))
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self.bits8 = k.dtype == torch.int8
+        _need((k_scale is not None) == (v_scale is not None) == self.bits8, "int8 pages, and no others, have k_scale and v_scale")
+        pages = _lib.Pages(_I8 if self.bits8 else _type(k, "pages"), hd, n_kv, n_pages, page, table.shape[1], k.data_ptr(), v.data_ptr(),
+                           k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), table.stride(0))
+        if not self.bits8:
+            self._struct = pages
+            return
+        _device(k, k_scale, v_scale)
+        blocks = k_scale.shape[1] if k_scale.dim() == 3 else 0
+        _need(k_scale.dtype == v_scale.dtype == torch.float32, f"scales are {k_scale.dtype} and {v_scale.dtype}: f32 is wanted")
+        _need(k_scale.shape == v_scale.shape == (n_pages, blocks, n_kv) and blocks > 0 and page % blocks == 0,
+              f"scales have to be [{n_pages} pages, blocks of a page, {n_kv} KV heads], got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
+        _need(_strides(k_scale) == _strides(v_scale), "k_scale and v_scale have to have the same strides")
+        self._struct = _lib.Pages8(pages, k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), k_scale.stride(1), k_scale.stride(2), page // blocks)
 
 
 def _check_seqs(seqs: Seqs, table: torch.Tensor | None) -> None:
@@ -176,8 +195,8 @@ def _check_seqs(seqs: Seqs, table: torch.Tensor | None) -> None:
 
 
 class PagedAppend(_Op):
-    """The new tokens' ``k`` and ``v`` [rows, KV heads, head size] (f32 or the pages' type,
-    one stride set) written to their pages."""
+    """The new tokens' ``k`` and ``v`` [rows, KV heads, head size] (f32 or the pages' type; to
+    8-bit pages f32, f16 or bf16; one stride set) written to their pages."""
 
     def __init__(self, kv: PagedKv, seqs: Seqs, k: torch.Tensor, v: torch.Tensor):
         hd = kv.k.shape[3]
@@ -186,9 +205,12 @@ class PagedAppend(_Op):
         _need(k.shape[1] == kv.k.shape[2], f"k has {k.shape[1]} heads, the pages {kv.k.shape[2]}")
         _check_seqs(seqs, kv.table)
         _written(kv.k, "pages")
+        if kv.bits8:
+            _written(kv.k_scale, "scales")
         dev = _device(kv.k, k, v, seqs.starts, seqs.lens)
         sq = seqs._struct(k.shape[0])
-        self._ready(_lib.lib().rie_hip_k_paged_append, [C.byref(kv._struct), C.byref(sq), _type(k, "k"), k.data_ptr(), v.data_ptr(),
+        L = _lib.lib()
+        self._ready(L.rie_hip_k_paged_append8 if kv.bits8 else L.rie_hip_k_paged_append, [C.byref(kv._struct), C.byref(sq), _type(k, "k"), k.data_ptr(), v.data_ptr(),
                     k.stride(0), k.stride(1)], dev, 0, None, (kv, seqs, sq, k, v))
 
 
@@ -203,17 +225,21 @@ def _attn(q: torch.Tensor, out: torch.Tensor, n_kv: int, ty: torch.dtype, hd: in
 
 class PagedAttention(_Op):
     """Causal attention of every sequence's new tokens ``q`` [rows, heads, head size] over
-    its pages, which hold them already, to ``out``."""
+    its pages, which hold them already, to ``out``, both of the pages' type (over 8-bit pages
+    f16 or bf16)."""
 
     def __init__(self, kv: PagedKv, seqs: Seqs, q: torch.Tensor, out: torch.Tensor, *, scale: float | None = None, window: int = 0,
                  softcap: float = 0.0):
         _check_seqs(seqs, kv.table)
-        at = _attn(q, out, kv.k.shape[2], kv.k.dtype, kv.k.shape[3], scale, window, softcap)
+        at = _attn(q, out, kv.k.shape[2], q.dtype if kv.bits8 else kv.k.dtype, kv.k.shape[3], scale, window, softcap)
         dev = _device(kv.k, q, out, seqs.starts, seqs.lens)
         sq = seqs._struct(q.shape[0])
-        args = [C.byref(kv._struct), C.byref(sq), C.byref(at)]
-        self._ready(_lib.lib().rie_hip_k_paged_attention, args, dev, _lib.lib().rie_hip_k_paged_attention_ws(*args), 3,
-                    (kv, seqs, sq, at, q, out))
+        L = _lib.lib()
+        if kv.bits8:
+            fn, ws, args = L.rie_hip_k_paged_attention8, L.rie_hip_k_paged_attention8_ws, [C.byref(kv._struct), C.byref(sq), _type(q, "q"), C.byref(at)]
+        else:
+            fn, ws, args = L.rie_hip_k_paged_attention, L.rie_hip_k_paged_attention_ws, [C.byref(kv._struct), C.byref(sq), C.byref(at)]
+        self._ready(fn, args, dev, ws(*args), len(args), (kv, seqs, sq, at, q, out))
 
 
 class PackedAttention(_Op):
