@@ -218,7 +218,7 @@ int32_t rie_hip_k_argmax(const float *x, int32_t n, uint32_t *out_idx);
 int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, void *stream, char *err, size_t err_len);
 
 /* ---- batched serving: a cache of pages, attention over it and over packed prompts,
- * token log probabilities.  No counterpart in the reference, whose backends hold one
+ * token log probabilities, rotary positions, beam selection, pools of pages.  No counterpart in the reference, whose backends hold one
  * sequence each.  Everything but the structs themselves is device memory; nothing of it
  * is read by the host, so a call can be captured into a graph and replayed over new
  * contents.
@@ -345,6 +345,87 @@ size_t rie_hip_k_token_logprobs_ws(int32_t n, int32_t n_vocab);
 int32_t rie_hip_k_token_logprobs(int32_t ty, const void *logits, int32_t n, int32_t n_vocab, int64_t row_stride,
                                  const int32_t *targets, float *logprob, float *entropy, int32_t n_top, int32_t *top_ids,
                                  float *top_logprobs, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len);
+
+/* Rotary positions.  Of the first `dims` values of a head, pair i (values i and i + dims/2, or,
+ * interleaved, 2i and 2i + 1) is turned by position * freqs[i] (radians, f64) and multiplied by
+ * magnitude; the values behind are copied.  Row r's position is positions[r], or, with seqs, that
+ * of its token (rows outside the sequences are neither read nor written).  Any 32-bit position;
+ * angles keep their digits.  n_q heads of q and n_k of k, of src_ty to dst_ty (f32, f16 or bf16,
+ * rounded to nearest once); q_out may be q and k_out k, of the same strides and type.  head_dim: 2
+ * to 1024; rows of any alignment of their type (16-byte aligned ones, with dims a multiple of 16
+ * and head_dim of 8, are read faster).  Strides up to 2^40. */
+typedef struct rie_hip_rotary {
+    int32_t n_rows, head_dim, dims, n_q, n_k, interleaved, src_ty, dst_ty;
+    float magnitude;
+    const double *freqs; /* [dims / 2] */
+    const int32_t *positions;
+    const void *q;
+    int64_t q_row_stride, q_head_stride;
+    void *q_out;
+    int64_t q_out_row_stride, q_out_head_stride;
+    const void *k;
+    int64_t k_row_stride, k_head_stride;
+    void *k_out;
+    int64_t k_out_row_stride, k_out_head_stride;
+} rie_hip_rotary;
+int32_t rie_hip_k_rotary(const rie_hip_rotary *rotary, const rie_hip_seqs *seqs, void *stream, char *err, size_t err_len);
+
+/* Beam search's selection: n requests of n_beams beams, whose logits are rows request*n_beams +
+ * beam (row_stride elements apart, any alignment of their type).  Of a request's candidates,
+ * scores[row] + ln p_row(token), the n_out best in order: their sums (next_scores), the rows that
+ * they go on from (parents) and their tokens, each [n][n_out].  Among equals the lowest beam comes
+ * first, then the larger logit, then the lowest token.  Sums are compared in f64 (ln of an f32
+ * sum) and rounded once.  A beam with finished[row] != 0 (finished may be NULL) goes on as it is:
+ * its one candidate is the token pad with its own score.  A beam whose score is not finite, or
+ * whose row has a NaN or +inf logit or nothing above −inf, offers nothing; where a request has too
+ * few candidates the sums of the others are −inf.  n_beams ≤ 64, n_out ≤ 128, n_vocab ≤ 2^21. */
+size_t rie_hip_k_beam_select_ws(int32_t n, int32_t n_beams, int32_t n_vocab, int32_t n_out);
+int32_t rie_hip_k_beam_select(int32_t ty, const void *logits, int32_t n, int32_t n_beams, int32_t n_vocab, int64_t row_stride,
+                              const float *scores, const int32_t *finished, int32_t pad, int32_t n_out, float *next_scores,
+                              int32_t *parents, int32_t *tokens, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len);
+
+/* A pool of pages and the sequences that hold them, all in device memory (int32): row i of the
+ * table holds the pages of sequence i, held[i] of them, for lens[i] positions of page_size each;
+ * refs[p] is how many rows hold page p, 0 for a free one.  Calls that need pages take the free
+ * ones with the lowest numbers, row by row.  counts[0]: how many pages the last reserve or fork
+ * lacked; counts[1]: pages in use after the last compact.  A table's entries behind held are −1
+ * where a call has written them.  The calls keep this in order for the caches that it describes;
+ * what else a program shares (a page in two rows) it counts in refs itself.  n_seq ≤ 4096. */
+typedef struct rie_hip_pool {
+    int32_t n_seq, n_pages, table_cols, page_size;
+    int32_t *table;
+    int64_t table_stride;
+    int32_t *lens, *held, *refs, *counts;
+} rie_hip_pool;
+/* A cache whose page p is the page_bytes bytes at base + p*page_stride (multiples of 4; keys,
+ * values and scales of a layer are three or four of them). */
+typedef struct rie_hip_page_buf {
+    void *base;
+    int64_t page_stride, page_bytes;
+} rie_hip_page_buf;
+/* workspace of any of the calls below */
+size_t rie_hip_k_page_ws(const rie_hip_pool *pool);
+/* Pages for the positions of every sequence: rows that hold fewer than lens needs get more.
+ * Where the pool runs out, later rows get fewer. */
+int32_t rie_hip_k_page_reserve(const rie_hip_pool *pool, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len);
+/* Row i becomes what row src[i] was (all at once; several rows may take one, and a row whose src
+ * is none, a number outside 0..n_seq-1, becomes empty).  Pages that are full are shared.  A source's
+ * partial last page, and what it holds behind that, stays with the row itself if it goes on (src[i]
+ * = i), else with the first that takes it; the others get a new page, which the call fills from the
+ * n_bufs caches, or −1 where the pool has none (new pages are those that were free before the
+ * call).  Pages that no row holds any more become free. */
+int32_t rie_hip_k_page_fork(const rie_hip_pool *pool, const int32_t *src, const rie_hip_page_buf *bufs, int32_t n_bufs, void *ws,
+                            size_t ws_bytes, void *stream, char *err, size_t err_len);
+/* Rows with which[i] != 0 give up their pages and positions. */
+int32_t rie_hip_k_page_free(const rie_hip_pool *pool, const int32_t *which, void *stream, char *err, size_t err_len);
+/* With n pages in use: those numbered n and up move, in order, to the free ones below n, in the
+ * tables, in refs and in the n_bufs caches, so that pages from n on are free. */
+int32_t rie_hip_k_page_compact(const rie_hip_pool *pool, const rie_hip_page_buf *bufs, int32_t n_bufs, void *ws, size_t ws_bytes,
+                               void *stream, char *err, size_t err_len);
+/* Page src[i] of every cache to page dst[i], i < n; pairs with a number outside 0..n_pages-1 are
+ * left out.  No page may be written that another pair reads or writes. */
+int32_t rie_hip_k_page_copy(const rie_hip_page_buf *bufs, int32_t n_bufs, int32_t n_pages, const int32_t *src, const int32_t *dst,
+                            int32_t n, void *stream, char *err, size_t err_len);
 
 #ifdef __cplusplus
 }

@@ -54,6 +54,24 @@ class Attn(C.Structure):
                 ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64)]
 
 
+class Rotary(C.Structure):
+    """rie_hip_rotary"""
+    _fields_ = [(n, C.c_int32) for n in ("n_rows", "head_dim", "dims", "n_q", "n_k", "interleaved", "src_ty", "dst_ty")] + [
+        ("magnitude", C.c_float), ("freqs", C.c_void_p), ("positions", C.c_void_p)] + [
+        f for x in ("q", "q_out", "k", "k_out") for f in ((x, C.c_void_p), (x + "_row_stride", C.c_int64), (x + "_head_stride", C.c_int64))]
+
+
+class Pool(C.Structure):
+    """rie_hip_pool"""
+    _fields_ = [(n, C.c_int32) for n in ("n_seq", "n_pages", "table_cols", "page_size")] + [("table", C.c_void_p), ("table_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("lens", "held", "refs", "counts")]
+
+
+class PageBuf(C.Structure):
+    """rie_hip_page_buf"""
+    _fields_ = [("base", C.c_void_p), ("page_stride", C.c_int64), ("page_bytes", C.c_int64)]
+
+
 def build(jobs: int = 8) -> None:
     """Compile librie_hip.so for gfx950 (hipcc cross-compiles without a GPU)."""
     subprocess.run(["make", "-s", f"-j{jobs}", "-C", os.path.join(PKG, "csrc")], check=True)
@@ -72,6 +90,7 @@ def lib():
     P, S, I, F, D = C.c_void_p, C.c_size_t, C.c_int32, C.c_float, C.c_double
     CP, U8P = C.c_char_p, C.POINTER(C.POINTER(C.c_uint8))
     I64, PG, PG8, SQ, AT = C.c_int64, C.POINTER(Pages), C.POINTER(Pages8), C.POINTER(Seqs), C.POINTER(Attn)
+    RO, PO, PB = C.POINTER(Rotary), C.POINTER(Pool), C.POINTER(PageBuf)
     sig = {
         "rie_hip_default_config": (Config, []),
         "rie_hip_create": (P, [P, S, C.POINTER(Config), C.POINTER(I), CP, S]),
@@ -111,6 +130,15 @@ def lib():
         "rie_hip_k_paged_attention8": (I, [PG8, SQ, I, AT, P, S, P, CP, S]),
         "rie_hip_k_packed_attention_ws": (S, [SQ, I, I, I, AT]),
         "rie_hip_k_packed_attention": (I, [SQ, I, I, I, P, P, I64, I64, I64, I64, AT, P, S, P, CP, S]),
+        "rie_hip_k_rotary": (I, [RO, SQ, P, CP, S]),
+        "rie_hip_k_beam_select_ws": (S, [I, I, I, I]),
+        "rie_hip_k_beam_select": (I, [I, P, I, I, I, I64, P, P, I, I, P, P, P, P, S, P, CP, S]),
+        "rie_hip_k_page_ws": (S, [PO]),
+        "rie_hip_k_page_reserve": (I, [PO, P, S, P, CP, S]),
+        "rie_hip_k_page_fork": (I, [PO, P, PB, I, P, S, P, CP, S]),
+        "rie_hip_k_page_free": (I, [PO, P, P, CP, S]),
+        "rie_hip_k_page_compact": (I, [PO, PB, I, P, S, P, CP, S]),
+        "rie_hip_k_page_copy": (I, [PB, I, I, P, P, I, P, CP, S]),
         "rie_hip_k_token_logprobs_ws": (S, [I, I]),
         "rie_hip_k_token_logprobs": (I, [I, P, I, I, I64, P, P, P, I, P, P, P, S, P, CP, S]),
     }

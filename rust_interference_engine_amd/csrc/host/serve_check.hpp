@@ -11,9 +11,7 @@
 
 namespace rie {
 
-namespace {
-
-Error bad(const std::string &m) { return Error{E_RUNTIME, m}; }
+inline Error bad(const std::string &m) { return Error{E_RUNTIME, m}; }
 
 // The stream's device is the current one while this lives.
 class OnDevice {
@@ -52,14 +50,14 @@ class OnDevice {
     int was_;
 };
 
-bool is16(int ty) { return ty == T_F16 || ty == T_BF16; }
+inline bool is16(int ty) { return ty == T_F16 || ty == T_BF16; }
 
 // A dimension of one entry is at 0, whatever its stride says (that of a tensor's is arbitrary)
-int64_t used(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
+inline int64_t used(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
 
 // Rows of values of es bytes each start at p + any multiples of the strides: all 16-byte
 // aligned, and strides of 2^26 bytes at most, so that 16 rows stay within 31 bits
-void check_rows(const void *p, int64_t row, int64_t head, int es, const char *what) {
+inline void check_rows(const void *p, int64_t row, int64_t head, int es, const char *what) {
     const int64_t a = 16 / es, most = ((int64_t)1 << 26) / es;
     if ((uintptr_t)p % 16 || row % a || head % a) throw bad(std::string(what) + ": rows have to be 16-byte aligned");
     if (row < 0 || row > most || head < 0 || head > most) throw bad(std::string(what) + ": strides have to lie in 0.." + std::to_string(most));
@@ -84,7 +82,7 @@ void check_apart(Dim (&&dims)[N], int hd, const char *what) {
 constexpr int MOST = 1 << 30;  // positions
 constexpr int MOST_ROWS = (1 << 26) - 4;  // 4 to a workgroup of 256: a launch has under 2^32 threads
 
-BatchView batch(const rie_hip_seqs *s, bool lens) {
+inline BatchView batch(const rie_hip_seqs *s, bool lens) {
     if (!s) throw bad("seqs is NULL");
     if (s->n_seq < 1 || s->n_rows < 1 || s->n_seq >= 1 << 24 || s->n_rows > MOST_ROWS) throw bad("n_seq has to lie in 1..2^24-1, n_rows in 1..2^26-4");
     if (s->max_new < 1 || s->max_len < 1 || s->max_new > MOST || s->max_len > MOST) throw bad("max_new and max_len have to lie in 1..2^30");
@@ -97,7 +95,5 @@ BatchView batch(const rie_hip_seqs *s, bool lens) {
     b.max_len = s->max_len;
     return b;
 }
-
-}  // namespace
 
 }  // namespace rie

@@ -1,0 +1,426 @@
+// pages.hip — a pool of pages whose bookkeeping stays on the device: pages given to sequences
+// that grow, sequences forked and reordered (the beams of a search), freed, and a pool's pages
+// moved together.
+//
+// refs[p] is the number of table rows that hold page p, and a page with none is free; nothing else
+// says so, and a call that needs pages takes the free ones with the lowest numbers.  All choices
+// go by row and page number, so that a call's results do not depend on timing: references change
+// by integer additions, which may come in any order.
+//
+// Everything read from device memory is clamped before it is an index.
+//
+// The planning of a call is one workgroup's: it counts what is needed, finds pages by counting
+// through refs 16 to a thread (16384 to a round), and leaves lists in the workspace.  Tables and
+// pages are changed by a second and third launch over the whole card.
+//
+// Bound: for many or large pages HBM, every moved byte read and written once; else the launches.
+#include "../common.hpp"
+#include "../device.hpp"
+#include "../serve.hpp"
+
+#include <algorithm>
+
+namespace rie {
+
+namespace {
+
+constexpr int PLAN = 1024;       // threads of a planning workgroup
+constexpr int PER = 16;          // references of a thread in a round
+constexpr int MAX_BUFS = 64;     // buffers of a launch
+constexpr int PIECE = 256 * 16;  // bytes that a workgroup copies at a time
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// x of the threads before this one, and of all of them; s: 17 words.  All threads call this.
+__device__ __forceinline__ int scan(int x, int *s, int &total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int y = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int z = __shfl_up(y, o);
+        if (lane >= o) y += z;
+    }
+    __syncthreads();
+    if (lane == 63) s[w] = y;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < PLAN / 64; i++) {
+        before += i < w ? s[i] : 0;
+        all += s[i];
+    }
+    total = all;
+    return before + y - x;
+}
+
+// Bit i: page p0 + i is free.  Behind the last page none is.
+__device__ __forceinline__ uint32_t free_of(const int *refs, int p0, int n_pages) {
+    uint32_t bits = 0;
+    if (p0 + PER <= n_pages) {
+        typedef i32x4 i32x4_a4 __attribute__((aligned(4)));
+        i32x4 r[PER / 4];
+#pragma unroll
+        for (int i = 0; i < PER / 4; i++) r[i] = *(const i32x4_a4 *)(refs + p0 + 4 * i);
+#pragma unroll
+        for (int i = 0; i < PER; i++) bits |= r[i / 4][i % 4] == 0 ? 1u << i : 0;
+    } else {
+        for (int i = 0; i < PER; i++) bits |= p0 + i < n_pages && refs[p0 + i] == 0 ? 1u << i : 0;
+    }
+    return bits;
+}
+
+// The free pages with the lowest numbers, up to `want`, in order into list; how many there are.  All threads call this.
+__device__ int find_free(const PoolView &p, int want, int *list, int *s) {
+    int found = 0;
+    for (int p0 = 0; p0 < p.n_pages && found < want; p0 += PLAN * PER) {
+        const int mine = p0 + (int)threadIdx.x * PER;
+        uint32_t bits = mine < p.n_pages ? free_of(p.refs, mine, p.n_pages) : 0;
+        int total, at = found + scan(__popc(bits), s, total);
+        for (; bits && at < want; bits &= bits - 1) list[at++] = mine + __builtin_ctz(bits);
+        found += total;
+    }
+    return min(found, want);
+}
+
+struct Seq {  // of a row: pages that its positions fill, pages that they touch, and pages that it holds
+    int full, touched, held;
+};
+__device__ __forceinline__ Seq seq_of(const PoolView &p, int i) {
+    const int page = 1 << p.page_shift, len = (int)min((int64_t)max(p.lens[i], 0), (int64_t)p.cols << p.page_shift);
+    return Seq{len >> p.page_shift, (len >> p.page_shift) + ((len & (page - 1)) != 0), min(max(p.held[i], 0), p.cols)};
+}
+
+// ---- pages for the positions that sequences have: row by row, the lowest free pages ----
+__global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
+    __shared__ int s[PLAN / 64];
+    __shared__ int s_at[POOL_MAX_SEQ + 1];  // pages that the rows before need, up to all there are
+    int64_t want = 0;
+    for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
+        const int i = i0 + (int)threadIdx.x;
+        int need = 0, total;
+        if (i < p.n_seq) {
+            const Seq q = seq_of(p, i);
+            need = max(q.touched - q.held, 0);
+        }
+        const int before = scan(need, s, total);
+        if (i < p.n_seq) s_at[i] = (int)min(want + before, (int64_t)p.n_pages);
+        want += total;
+    }
+    const int most = (int)min(want, (int64_t)p.n_pages);
+    if (threadIdx.x == 0) s_at[p.n_seq] = most;
+    const int found = find_free(p, most, list, s);
+    __syncthreads();
+    for (int j = threadIdx.x; j < found; j += PLAN) {
+        int lo = 0, hi = p.n_seq;  // the last row that begins at or before j
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (s_at[mid] <= j) lo = mid;
+            else hi = mid;
+        }
+        const int page = list[j];
+        p.table[lo * p.table_stride + seq_of(p, lo).held + (j - s_at[lo])] = page;
+        p.refs[page] = 1;
+    }
+    __syncthreads();
+    // a row gets what there is, from its first missing page on
+    for (int i = threadIdx.x; i < p.n_seq; i += PLAN) {
+        const Seq q = seq_of(p, i);
+        const int got = max(min(s_at[i + 1], found) - s_at[i], 0);
+        if (got) p.held[i] = q.held + got;
+    }
+    if (threadIdx.x == 0) p.counts[0] = (int)min(want - found, (int64_t)INT32_MAX);
+}
+
+// ---- fork ----
+struct Child {  // what becomes of a row
+    int src, keep, held, old_held, len, fresh;  // keep: it takes the source's pages as they are; fresh: the page in the place of the source's partial one, or −1
+    int at;                                     // that place (−1: none)
+};
+struct Lists {
+    int n;  // pages to copy
+    int pad[3];
+};
+
+__global__ __launch_bounds__(PLAN) void fork_plan_kernel(PoolView p, const int *src, Lists *lists, Child *child, int *children, int *from, int *to, int *list) {
+    extern __shared__ int s_row[];  // children of a row, and which of them inherits its partial page
+    __shared__ int s[PLAN / 64];
+    int *count = s_row, *heir = s_row + p.n_seq;
+    for (int i = threadIdx.x; i < p.n_seq; i += PLAN) {
+        count[i] = 0;
+        heir[i] = INT32_MAX;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.n_seq; i += PLAN) {
+        const int r = src[i];
+        if ((unsigned)r >= (unsigned)p.n_seq) continue;
+        atomicAdd(count + r, 1);
+        atomicMin(heir + r, r == i ? -1 : i);  // the row itself, or its first child
+    }
+    __syncthreads();
+    int want = 0;
+    for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
+        const int i = i0 + (int)threadIdx.x;
+        int need = 0, total;
+        if (i < p.n_seq) {
+            const int r = src[i];
+            Child c;
+            c.src = (unsigned)r < (unsigned)p.n_seq ? r : -1;
+            c.keep = c.src >= 0 && (r == i || heir[r] == i);
+            c.old_held = seq_of(p, i).held;
+            c.fresh = c.at = -1;
+            c.held = c.len = 0;
+            if (c.src >= 0) {
+                const Seq q = seq_of(p, r);
+                c.held = c.keep ? q.held : min(q.touched, q.held);
+                c.len = p.lens[r];
+                if (!c.keep && q.touched > q.full && q.held > q.full) c.at = q.full;
+            }
+            need = c.at >= 0;
+            child[i] = c;
+            children[i] = count[i];
+        }
+        scan(need, s, total);
+        want += total;
+    }
+    const int found = find_free(p, want, list, s);
+    __syncthreads();
+    int at = 0, copies = 0;
+    for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
+        const int i = i0 + (int)threadIdx.x;
+        const int place = i < p.n_seq ? child[i].at : -1;
+        int total;
+        const int mine = at + scan(place >= 0, s, total);
+        bool copy = false;
+        int page = -1, old = -1;
+        if (place >= 0 && mine < found) {
+            page = list[mine];
+            old = p.table[child[i].src * p.table_stride + place];
+            copy = (unsigned)old < (unsigned)p.n_pages;
+            child[i].fresh = page;
+            p.refs[page] = 1;
+        }
+        at += total;
+        const int c = copies + scan(copy, s, total);
+        if (copy) {
+            from[c] = old;
+            to[c] = page;
+        }
+        copies += total;
+    }
+    if (threadIdx.x == 0) {
+        lists->n = copies;
+        p.counts[0] = want - found;
+    }
+}
+
+// The old rows' references, and the rows that others go on from into `rows`
+__global__ __launch_bounds__(256) void fork_refs_kernel(PoolView p, const int *src, const int *children, int *rows) {
+    const int r = blockIdx.x, n = children[r];
+    const bool stays = (unsigned)src[r] < (unsigned)p.n_seq && src[r] == r;
+    if (n == 1 && stays) return;
+    const Seq q = seq_of(p, r);
+    const int *t = p.table + r * p.table_stride;
+    for (int c = threadIdx.x; c < q.held; c += 256) {
+        const int page = t[c], change = c < q.full ? n - 1 : n == 0 ? -1 : 0;
+        if (n) rows[(int64_t)r * p.cols + c] = page;
+        if (change && (unsigned)page < (unsigned)p.n_pages) atomicAdd(p.refs + page, change);
+    }
+}
+
+struct Bufs {
+    PageBuf b[MAX_BUFS];
+    int first[MAX_BUFS + 1];  // pieces of a page before buffer i
+    int n;
+};
+
+// Copies pages: workgroup g of n takes every n-th piece of every page in the lists
+__device__ void copy_pages(const Bufs &bufs, int g, int n, const int *from, const int *to, int n_copies, int n_pages) {
+    const int per = bufs.first[bufs.n];
+    for (int64_t i = g; i < (int64_t)n_copies * per; i += n) {
+        const int j = (int)(i / per), piece = (int)(i - (int64_t)j * per);
+        int b = 0;
+        while (piece >= bufs.first[b + 1]) b++;
+        const PageBuf &buf = bufs.b[b];
+        const int f = from[j], t = to[j];
+        if ((unsigned)f >= (unsigned)n_pages || (unsigned)t >= (unsigned)n_pages) continue;
+        const int64_t at = (int64_t)(piece - bufs.first[b]) * PIECE;
+        const uint8_t *x = buf.base + f * buf.stride + at;
+        uint8_t *y = buf.base + t * buf.stride + at;
+        const int len = (int)min((int64_t)PIECE, buf.bytes - at);
+        if ((((uintptr_t)x | (uintptr_t)y | (unsigned)len) & 15) == 0) {
+            const int o = threadIdx.x * 16;
+            if (o < len) *(u32x4 *)(y + o) = *(const u32x4 *)(x + o);
+        } else {
+            for (int o = threadIdx.x * 4; o < len; o += 256 * 4) *(uint32_t *)(y + o) = *(const uint32_t *)(x + o);
+        }
+    }
+}
+
+// The new rows, a workgroup each, and the copies
+__global__ __launch_bounds__(256) void fork_rows_kernel(PoolView p, Bufs bufs, int row_wgs, const Lists *lists, const Child *child, const int *from, const int *to, const int *rows) {
+    if ((int)blockIdx.x >= row_wgs) {
+        copy_pages(bufs, blockIdx.x - row_wgs, gridDim.x - row_wgs, from, to, lists->n, p.n_pages);
+        return;
+    }
+    const int i = blockIdx.x;
+    const Child c = child[i];
+    if (c.src == i) return;  // and keeps its pages
+    int *t = p.table + i * p.table_stride;
+    const int *r = rows + (int64_t)max(c.src, 0) * p.cols;
+    for (int k = threadIdx.x; k < max(c.held, c.old_held); k += 256) t[k] = k >= c.held ? -1 : k == c.at ? c.fresh : r[k];
+    if (threadIdx.x == 0) {
+        p.lens[i] = c.len;
+        p.held[i] = c.held;
+    }
+}
+
+// ---- free: a workgroup per row ----
+__global__ __launch_bounds__(256) void free_kernel(PoolView p, const int *which) {
+    const int i = blockIdx.x;
+    if (!which[i]) return;
+    const int held = seq_of(p, i).held;
+    int *t = p.table + i * p.table_stride;
+    for (int c = threadIdx.x; c < held; c += 256) {
+        const int page = t[c];
+        if ((unsigned)page < (unsigned)p.n_pages) atomicSub(p.refs + page, 1);
+        t[c] = -1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.held[i] = p.lens[i] = 0;
+}
+
+// ---- compact: of n pages in use, those from number n on go to the free ones below it, in order ----
+__global__ __launch_bounds__(PLAN) void compact_plan_kernel(PoolView p, Lists *lists, int *from, int *to, int *goes) {
+    __shared__ int s[PLAN / 64];
+    int used = 0;
+    for (int p0 = 0; p0 < p.n_pages; p0 += PLAN * PER) {
+        const int mine = p0 + (int)threadIdx.x * PER, n = min(max(p.n_pages - mine, 0), PER);
+        int total;
+        scan(n ? n - __popc(free_of(p.refs, mine, p.n_pages)) : 0, s, total);
+        used += total;
+    }
+    int n_from = 0, n_to = 0;
+    for (int p0 = 0; p0 < p.n_pages; p0 += PLAN * PER) {
+        const int mine = p0 + (int)threadIdx.x * PER, n = min(max(p.n_pages - mine, 0), PER);
+        const uint32_t all = (1u << n) - 1, low = mine >= used ? 0 : used - mine >= PER ? all : all & ((1u << (used - mine)) - 1);
+        const uint32_t f = n ? free_of(p.refs, mine, p.n_pages) : 0;
+        uint32_t a = ~f & all & ~low, b = f & low;
+        for (uint32_t c = f & ~low; c; c &= c - 1) goes[mine + __builtin_ctz(c)] = mine + __builtin_ctz(c);
+        int total;
+        int at = n_from + scan(__popc(a), s, total);
+        n_from += total;
+        for (; a; a &= a - 1) from[at++] = mine + __builtin_ctz(a);
+        at = n_to + scan(__popc(b), s, total);
+        n_to += total;
+        for (; b; b &= b - 1) to[at++] = mine + __builtin_ctz(b);
+    }
+    __syncthreads();
+    const int n = min(n_from, n_to);  // the same
+    for (int j = threadIdx.x; j < n; j += PLAN) {
+        const int f = from[j], t = to[j];
+        goes[f] = t;
+        p.refs[t] = p.refs[f];
+        p.refs[f] = 0;
+    }
+    if (threadIdx.x == 0) {
+        lists->n = n;
+        p.counts[1] = used;
+    }
+}
+
+__global__ __launch_bounds__(256) void compact_rows_kernel(PoolView p, Bufs bufs, int row_wgs, const Lists *lists, const int *from, const int *to, const int *goes) {
+    if ((int)blockIdx.x >= row_wgs) {
+        copy_pages(bufs, blockIdx.x - row_wgs, gridDim.x - row_wgs, from, to, lists->n, p.n_pages);
+        return;
+    }
+    const int i = blockIdx.x, used = p.counts[1];
+    const Seq q = seq_of(p, i);
+    int *t = p.table + i * p.table_stride;
+    for (int c = threadIdx.x; c < q.held; c += 256) {
+        const int page = t[c];
+        if (page >= used && page < p.n_pages) t[c] = goes[page];
+    }
+}
+
+__global__ __launch_bounds__(256) void copy_kernel(Bufs bufs, const int *from, const int *to, int n, int n_pages) {
+    copy_pages(bufs, blockIdx.x, gridDim.x, from, to, n, n_pages);
+}
+
+Bufs bufs_of(const PageBuf *b, int n) {
+    Bufs x;
+    x.n = n;
+    x.first[0] = 0;
+    for (int i = 0; i < n; i++) {
+        x.b[i] = b[i];
+        x.first[i + 1] = x.first[i] + (int)((b[i].bytes + PIECE - 1) / PIECE);
+    }
+    return x;
+}
+
+constexpr int COPY_WGS = 2048;  // 8 to a CU
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+}  // namespace
+
+size_t page_reserve_ws(const PoolView &p) { return up16((size_t)p.n_pages * sizeof(int)); }
+
+size_t page_fork_ws(const PoolView &p) {
+    return sizeof(Lists) + up16(p.n_seq * sizeof(Child)) + 4 * up16(p.n_seq * sizeof(int)) + up16((size_t)p.n_seq * p.cols * sizeof(int));
+}
+
+size_t page_compact_ws(const PoolView &p) { return sizeof(Lists) + 3 * up16((size_t)p.n_pages * sizeof(int)); }
+
+void launch_page_reserve(const PoolView &p, void *ws, hipStream_t st) { reserve_kernel<<<1, PLAN, 0, st>>>(p, (int *)ws); }
+
+void launch_page_fork(const PoolView &p, const int *src, const PageBuf *bufs, int n_bufs, void *ws, hipStream_t st) {
+    uint8_t *w = (uint8_t *)ws;
+    Lists *lists = (Lists *)w;
+    w += sizeof(Lists);
+    Child *child = (Child *)w;
+    w += up16(p.n_seq * sizeof(Child));
+    int *ints[4];  // children, pages copied from and to, free ones
+    for (int *&x : ints) {
+        x = (int *)w;
+        w += up16(p.n_seq * sizeof(int));
+    }
+    int *rows = (int *)w;
+    fork_plan_kernel<<<1, PLAN, 2 * p.n_seq * sizeof(int), st>>>(p, src, lists, child, ints[0], ints[1], ints[2], ints[3]);
+    fork_refs_kernel<<<p.n_seq, 256, 0, st>>>(p, src, ints[0], rows);
+    int done = 0;
+    do {
+        const int n = std::min(n_bufs - done, MAX_BUFS), row_wgs = done ? 0 : p.n_seq;
+        fork_rows_kernel<<<row_wgs + (n ? COPY_WGS : 0), 256, 0, st>>>(p, bufs_of(bufs + done, n), row_wgs, lists, child, ints[1], ints[2], rows);
+        done += n;
+    } while (done < n_bufs);
+}
+
+void launch_page_free(const PoolView &p, const int *which, hipStream_t st) { free_kernel<<<p.n_seq, 256, 0, st>>>(p, which); }
+
+void launch_page_compact(const PoolView &p, const PageBuf *bufs, int n_bufs, void *ws, hipStream_t st) {
+    uint8_t *w = (uint8_t *)ws;
+    Lists *lists = (Lists *)w;
+    w += sizeof(Lists);
+    int *ints[3];  // pages moved from and to; where a page goes
+    for (int *&x : ints) {
+        x = (int *)w;
+        w += up16((size_t)p.n_pages * sizeof(int));
+    }
+    compact_plan_kernel<<<1, PLAN, 0, st>>>(p, lists, ints[0], ints[1], ints[2]);
+    int done = 0;
+    do {
+        const int n = std::min(n_bufs - done, MAX_BUFS), row_wgs = done ? 0 : p.n_seq;
+        compact_rows_kernel<<<row_wgs + (n ? COPY_WGS : 0), 256, 0, st>>>(p, bufs_of(bufs + done, n), row_wgs, lists, ints[0], ints[1], ints[2]);
+        done += n;
+    } while (done < n_bufs);
+}
+
+void launch_page_copy(const PageBuf *bufs, int n_bufs, int n_pages, const int *src, const int *dst, int n, hipStream_t st) {
+    for (int done = 0; done < n_bufs;) {
+        const int m = std::min(n_bufs - done, MAX_BUFS);
+        copy_kernel<<<COPY_WGS, 256, 0, st>>>(bufs_of(bufs + done, m), src, dst, n, n_pages);
+        done += m;
+    }
+}
+
+}  // namespace rie

@@ -77,6 +77,58 @@ struct PagedAppend8Args {
 };
 void launch_paged_append8(const PagedAppend8Args &x, hipStream_t st);
 
+// Rows of queries and keys turned by their positions: those given, or those of the batch's rows
+struct RotaryArgs {
+    BatchView b;
+    KvView kv;  // kv.table is not read; it says that positions go by lens
+    const int *positions = nullptr;
+    const double *freqs = nullptr;  // [dims / 2]
+    float magnitude = 1;
+    int hd = 0, dims = 0, n_q = 0, n_k = 0, src_ty = 0, dst_ty = 0;
+    bool interleaved = false, in_place = false, wide = false;  // wide: rows and halves are 16-byte aligned
+    const uint8_t *q = nullptr, *k = nullptr;
+    uint8_t *q_out = nullptr, *k_out = nullptr;
+    int64_t q_row = 0, q_head = 0, k_row = 0, k_head = 0, qo_row = 0, qo_head = 0, ko_row = 0, ko_head = 0;  // bytes
+};
+constexpr int ROTARY_MAX_HD = 1024;
+void launch_rotary(const RotaryArgs &a, hipStream_t st);
+
+// The n_out best (beam, token) candidates of each of n requests of n_beams beams, a row of logits each
+struct BeamArgs {
+    const void *x = nullptr;
+    int ty = 0, n = 0, n_beams = 0, V = 0, n_out = 0, pad = 0;
+    int64_t ld = 0;  // elements between rows
+    const float *scores = nullptr;
+    const int *finished = nullptr;
+    float *next = nullptr;
+    int *parents = nullptr, *tokens = nullptr;
+};
+constexpr int BEAM_MAX_BEAMS = 64, BEAM_MAX_OUT = 128, BEAM_MAX_V = 1 << 21;
+size_t beam_ws(int n, int n_beams, int V, int n_out);
+void launch_beam(const BeamArgs &a, void *ws, hipStream_t st);
+
+// A pool of pages: the table rows of n_seq sequences, how many pages each holds and how many
+// positions it has, the rows that hold each page (0: free), and what calls count
+struct PoolView {
+    int n_seq = 0, n_pages = 0, cols = 0, page_shift = 0;
+    int *table = nullptr, *lens = nullptr, *held = nullptr, *refs = nullptr, *counts = nullptr;
+    int64_t table_stride = 0;
+};
+// Memory that is divided into pages as the caches are; all of a page's bytes lie together
+struct PageBuf {
+    uint8_t *base;
+    int64_t stride, bytes;
+};
+constexpr int POOL_MAX_SEQ = 4096, POOL_MAX_PAGES = 1 << 24, POOL_MAX_COLS = 1 << 20;
+size_t page_reserve_ws(const PoolView &p);
+size_t page_fork_ws(const PoolView &p);
+size_t page_compact_ws(const PoolView &p);
+void launch_page_reserve(const PoolView &p, void *ws, hipStream_t st);
+void launch_page_fork(const PoolView &p, const int *src, const PageBuf *bufs, int n_bufs, void *ws, hipStream_t st);
+void launch_page_free(const PoolView &p, const int *which, hipStream_t st);
+void launch_page_compact(const PoolView &p, const PageBuf *bufs, int n_bufs, void *ws, hipStream_t st);
+void launch_page_copy(const PageBuf *bufs, int n_bufs, int n_pages, const int *src, const int *dst, int n, hipStream_t st);
+
 struct LogprobArgs {
     const void *x = nullptr;
     int ty = 0, n = 0, V = 0;

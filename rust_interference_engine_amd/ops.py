@@ -1,6 +1,7 @@
 """The batched serving operators of librie_hip.so on torch tensors: rows appended to a
-cache of pages, attention of new tokens over it, attention over packed prompts, and
-token log probabilities (include/rie_hip.h has their rules).
+cache of pages (of 16 or 8 bits), attention of new tokens over it, attention over packed
+prompts, token log probabilities, rotary positions, beam search's selection, and pools of
+pages (include/rie_hip.h has their rules).
 
 Each operator is an object that is made once over the tensors it works on, which checks
 them, holds them and takes its workspace, and is then called as often as wanted: a call
@@ -16,6 +17,14 @@ capture belongs to that graph.  There are no gradients.
     append = ops.PagedAppend(kv, seqs, k, v)
     attend = ops.PagedAttention(kv, seqs, q, out)
     append(); attend()
+
+A search with beams over a pool, after the step's logits:
+
+    pool = ops.PagePool.empty(n_pages, n_seq, most_pages_of_one, page_size, device)
+    select = ops.BeamSelect(logits, scores, next_scores, parents, tokens)
+    fork = ops.PageFork(pool, parents.view(-1), [k_pages, v_pages])
+    reserve = ops.PageReserve(pool)
+    select(); fork(); pool.lens += 1; reserve()
 """
 from __future__ import annotations
 
@@ -286,3 +295,203 @@ class TokenLogprobs(_Op):
         ptr = [None if t is None or not t.numel() else t.data_ptr() for t in (targets, logprob, entropy, top_ids, top_logprobs)]
         self._ready(_lib.lib().rie_hip_k_token_logprobs, [_type(logits, "logits"), logits.data_ptr(), n, n_vocab, logits.stride(0),
                     ptr[0], ptr[1], ptr[2], top, ptr[3], ptr[4]], dev, _lib.lib().rie_hip_k_token_logprobs_ws(n, n_vocab), 11, (logits, given))
+
+
+def rotary_frequencies(dims: int, base: float = 10000.0, *, factors=None, linear: float = 1.0, parts: tuple | None = None):
+    """The angles per position of ``dims`` / 2 pairs, base^(-2i / dims), as f64 on the host, and the factor of the
+    rotated values.  For contexts beyond those trained on: ``factors`` divides each pair's angle by its own number (as
+    ``rope_freqs.weight`` does), ``linear`` all of them by one; ``parts`` = (factor, original context) divides the
+    slow ones by factor and leaves the fast ones, with a ramp between those that turn once and 32 times within the
+    original context, and multiplies the rotated values by 0.1 ln(factor) + 1 (YaRN, arXiv 2309.00071)."""
+    _need(dims >= 2 and dims % 2 == 0, f"dims has to be even and positive, got {dims}")
+    _need(base > 0 and linear > 0, "base and linear have to be positive")
+    f = base ** (-2 * torch.arange(dims // 2, dtype=torch.float64) / dims) / linear
+    magnitude = 1.0
+    if factors is not None:
+        factors = torch.as_tensor(factors, dtype=torch.float64, device="cpu")
+        _need(factors.shape == f.shape, f"{tuple(factors.shape)} factors for {dims // 2} pairs")
+        f = f / factors
+    if parts is not None:
+        factor, original = parts
+        _need(factor >= 1 and original > 0 and base > 1, "parts has to be (a factor of 1 or more, the original context), of a base above 1")
+
+        def pair(turns):  # that turns so often within the original context
+            return dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low, high = max(math.floor(pair(32)), 0), min(math.ceil(pair(1)), dims - 1)
+        ramp = ((torch.arange(dims // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        f = f / factor * ramp + f * (1 - ramp)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    return f, magnitude
+
+
+class Rotary(_Op):
+    """Queries ``q`` and keys ``k`` [rows, heads, head size] turned by their positions, to
+    ``q_out`` and ``k_out`` (of any of the types; ``q`` and ``k`` themselves will do).
+    ``frequencies`` f64 [dims / 2] on the GPU: angles per position of the first dims values
+    of a head.  Positions: int32 ``positions`` [rows], or those of the tokens of ``seqs``.
+    ``k`` and ``k_out`` may be None."""
+
+    def __init__(self, frequencies: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, q_out: torch.Tensor, k_out: torch.Tensor | None, *,
+                 positions: torch.Tensor | None = None, seqs: Seqs | None = None, interleaved: bool = False, magnitude: float = 1.0):
+        _need(frequencies.dtype == torch.float64 and frequencies.dim() == 1 and frequencies.is_contiguous() and frequencies.numel() > 0,
+              f"frequencies have to be contiguous f64 [dims / 2], got {frequencies.dtype} {tuple(frequencies.shape)}")
+        _need((positions is None) != (seqs is None), "positions or seqs has to be given, not both")
+        _need((k is None) == (k_out is None), "k and k_out have to be given together")
+        hd = _rows(q, "q").shape[2]
+        pairs = [(q, q_out, "q")] + ([(k, k_out, "k")] if k is not None else [])
+        n = _int(q.shape[0], "rows", 1, (1 << 26) - 4)
+        x = _lib.Rotary(n, hd, 2 * frequencies.numel(), 0, 0, int(interleaved), _type(q, "q"), _type(q_out, "q_out"), magnitude, frequencies.data_ptr(),
+                        positions.data_ptr() if positions is not None else None)
+        for t, out, what in pairs:
+            _rows(t, what, hd), _rows(out, what + "_out", hd)
+            _need(t.shape == out.shape and t.shape[0] == n, f"{what} and {what}_out have to have one shape, and q's rows")
+            _need(t.dtype == q.dtype and out.dtype == q_out.dtype, "q and k, and q_out and k_out, have to have one type")
+            _written(out, what + "_out")
+            setattr(x, "n_" + what, t.shape[1])
+            for name, y in ((what, t), (what + "_out", out)):
+                setattr(x, name, y.data_ptr())
+                setattr(x, name + "_row_stride", y.stride(0))
+                setattr(x, name + "_head_stride", y.stride(1))
+        _need(2 * frequencies.numel() <= hd, f"{2 * frequencies.numel()} dims of heads of {hd}")
+        tensors = [frequencies] + [t for p in pairs for t in p[:2]]
+        sq = None
+        if positions is not None:
+            _ints(positions, "positions", 1)
+            _need(positions.numel() == n, f"{positions.numel()} positions for {n} rows")
+            tensors.append(positions)
+        else:
+            _need(seqs.lens is not None, "seqs has no lens")
+            sq = seqs._struct(n)
+            tensors += [seqs.starts, seqs.lens]
+        dev = _device(*tensors)
+        self._ready(_lib.lib().rie_hip_k_rotary, [C.byref(x), C.byref(sq) if sq else None], dev, 0, None, (x, sq, seqs, tensors))
+
+
+class BeamSelect(_Op):
+    """Of ``logits`` [requests * beams, vocabulary] and the beams' sums ``scores`` f32
+    [requests, beams]: the best continuations of every request, in order, to ``next_scores``
+    (f32), ``parents`` (int32: rows of logits) and ``tokens`` (int32), all [requests, number
+    wanted].  Beams with ``finished`` (int32 [requests, beams]) other than 0 go on with the
+    token ``pad`` and their own sum."""
+
+    def __init__(self, logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, *,
+                 finished: torch.Tensor | None = None, pad: int = 0):
+        _need(logits.dim() == 2 and logits.numel() > 0, f"logits have to be [requests * beams, vocabulary], got {tuple(logits.shape)}")
+        _need(logits.shape[1] == 1 or logits.stride(1) == 1, "a row's logits have to be consecutive")
+        _need(scores.dim() == 2 and scores.numel() == logits.shape[0], f"scores have to be [requests, beams] of {logits.shape[0]} rows, got {tuple(scores.shape)}")
+        n, beams = scores.shape
+        _need(next_scores.dim() == 2 and next_scores.shape[0] == n and next_scores.shape == parents.shape == tokens.shape,
+              "next_scores, parents and tokens have to be [requests, number wanted]")
+        for t, what, dtype in ((scores, "scores", torch.float32), (next_scores, "next_scores", torch.float32), (parents, "parents", torch.int32),
+                               (tokens, "tokens", torch.int32), (finished, "finished", torch.int32)):
+            _need(t is None or t.dtype == dtype and t.is_contiguous(), f"{what} has to be contiguous {dtype}")
+        _need(finished is None or finished.shape == scores.shape, "finished has to have the shape of scores")
+        n_vocab, keep = _int(logits.shape[1], "vocabulary", 1, 1 << 21), next_scores.shape[1]
+        given = [scores, next_scores, parents, tokens] + ([finished] if finished is not None else [])
+        dev = _device(logits, *given)
+        L = _lib.lib()
+        self._ready(L.rie_hip_k_beam_select, [_type(logits, "logits"), logits.data_ptr(), n, beams, n_vocab, logits.stride(0), scores.data_ptr(),
+                    finished.data_ptr() if finished is not None else None, _int(pad, "pad", 0, n_vocab - 1), keep, next_scores.data_ptr(), parents.data_ptr(),
+                    tokens.data_ptr()], dev, L.rie_hip_k_beam_select_ws(n, beams, n_vocab, keep), 13, (logits, given))
+
+
+class PagePool:
+    """The pages of a cache and the sequences that hold them, all int32 on the GPU: ``table``
+    [sequences, most pages of one], the positions ``lens`` and the number of pages ``held`` of
+    each, ``refs`` [pages], how many rows hold a page (0: free), and ``counts`` [2], how many
+    pages the last reserve or fork lacked and how many the last compact found in use."""
+
+    def __init__(self, table: torch.Tensor, lens: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, counts: torch.Tensor, *, page_size: int):
+        _ints(table, "table", 2)
+        for t, what in ((lens, "lens"), (held, "held"), (refs, "refs"), (counts, "counts")):
+            _ints(t, what, 1)
+        n = table.shape[0]
+        _need(lens.numel() == held.numel() == n, f"{lens.numel()} lens and {held.numel()} held for {n} sequences")
+        _need(counts.numel() == 2, "counts has to hold two numbers")
+        _written(table, "table")
+        self.device = _device(table, lens, held, refs, counts)
+        self.table, self.lens, self.held, self.refs, self.counts, self.page_size = table, lens, held, refs, counts, page_size
+        self._struct = _lib.Pool(_int(n, "sequences", 1, 4096), _int(refs.numel(), "pages", 1, 1 << 24), _int(table.shape[1], "columns", 1, 1 << 20),
+                                 _int(page_size, "page_size", 1, 4096), table.data_ptr(), table.stride(0), lens.data_ptr(), held.data_ptr(), refs.data_ptr(),
+                                 counts.data_ptr())
+
+    @classmethod
+    def empty(cls, n_pages: int, n_seq: int, cols: int, page_size: int, device) -> "PagePool":
+        """A pool of free pages and sequences without any."""
+        def zeros(*shape):
+            return torch.zeros(*shape, dtype=torch.int32, device=device)
+
+        return cls(zeros(n_seq, cols) - 1, zeros(n_seq), zeros(n_seq), zeros(n_pages), zeros(2), page_size=page_size)
+
+    def _workspace(self) -> int:
+        return _lib.lib().rie_hip_k_page_ws(C.byref(self._struct))
+
+
+def _page_bufs(caches, n_pages: int):
+    """caches [pages, ...] as the library takes them: a page's values lie together, in any order"""
+    caches = list(caches)
+    bufs = (_lib.PageBuf * max(len(caches), 1))()
+    for b, t in zip(bufs, caches):
+        _need(t.dim() >= 2 and t.shape[0] == n_pages and t.numel() > 0, f"a cache has to be [{n_pages} pages, ...], got {tuple(t.shape)}")
+        span = 1
+        for st, n in sorted((st, n) for n, st in zip(t.shape[1:], t.stride()[1:]) if n > 1):
+            _need(st == span, "a page's values have to lie together")
+            span *= n
+        b.base, b.page_stride, b.page_bytes = t.data_ptr(), t.stride(0) * t.element_size(), span * t.element_size()
+    return caches, bufs
+
+
+class PageReserve(_Op):
+    """Pages for the positions that ``pool.lens`` says: the lowest free ones, row by row."""
+
+    def __init__(self, pool: PagePool):
+        self._ready(_lib.lib().rie_hip_k_page_reserve, [C.byref(pool._struct)], pool.device, pool._workspace(), 1, (pool,))
+
+
+class PageFork(_Op):
+    """Row i of the pool becomes what row ``src[i]`` (int32 [sequences], on the GPU) was, all at
+    once: full pages are shared, a partial last one is copied for all but one of the rows that
+    take it, in the pages of all ``caches`` [pages, ...].  A row whose src is none becomes empty."""
+
+    def __init__(self, pool: PagePool, src: torch.Tensor, caches=()):
+        _ints(src, "src", 1)
+        _need(src.numel() == pool.table.shape[0], f"{src.numel()} src for {pool.table.shape[0]} sequences")
+        caches, bufs = _page_bufs(caches, pool.refs.numel())
+        dev = _device(pool.table, src, *caches)
+        self._ready(_lib.lib().rie_hip_k_page_fork, [C.byref(pool._struct), src.data_ptr(), bufs, len(caches)], dev, pool._workspace(), 4, (pool, src, caches, bufs))
+
+
+class PageFree(_Op):
+    """Sequences whose ``which`` (int32 [sequences], on the GPU) is not 0 give up their pages."""
+
+    def __init__(self, pool: PagePool, which: torch.Tensor):
+        _ints(which, "which", 1)
+        _need(which.numel() == pool.table.shape[0], f"{which.numel()} which for {pool.table.shape[0]} sequences")
+        dev = _device(pool.table, which)
+        self._ready(_lib.lib().rie_hip_k_page_free, [C.byref(pool._struct), which.data_ptr()], dev, 0, None, (pool, which))
+
+
+class PageCompact(_Op):
+    """The pool's n pages in use become pages 0..n-1: those numbered n and up move, with their
+    contents in all ``caches`` [pages, ...]."""
+
+    def __init__(self, pool: PagePool, caches=()):
+        caches, bufs = _page_bufs(caches, pool.refs.numel())
+        dev = _device(pool.table, *caches)
+        self._ready(_lib.lib().rie_hip_k_page_compact, [C.byref(pool._struct), bufs, len(caches)], dev, pool._workspace(), 3, (pool, caches, bufs))
+
+
+class PageCopy(_Op):
+    """Page ``src[i]`` of every one of ``caches`` [pages, ...] to page ``dst[i]`` (int32, on the
+    GPU).  No page may be written that another pair reads or writes."""
+
+    def __init__(self, caches, src: torch.Tensor, dst: torch.Tensor):
+        caches = list(caches)
+        _need(len(caches) > 0, "no caches")
+        _ints(src, "src", 1), _ints(dst, "dst", 1)
+        _need(src.numel() == dst.numel() > 0, f"{src.numel()} src and {dst.numel()} dst")
+        n_pages = caches[0].shape[0]
+        caches, bufs = _page_bufs(caches, n_pages)
+        dev = _device(src, dst, *caches)
+        self._ready(_lib.lib().rie_hip_k_page_copy, [bufs, len(caches), n_pages, src.data_ptr(), dst.data_ptr(), src.numel()], dev, 0, None, (caches, src, dst, bufs))
