@@ -300,8 +300,8 @@ int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs
 /* The same cache in 8 bits: pages.ty is 24 (int8), pages.k and pages.v hold codes of −127..127,
  * and a value is its code times the scale of its block: `block` positions of a page (a power of
  * two, 16 to page_size) of one head, at page*scale_page_stride + (slot/block)*scale_block_stride
- * + head*scale_head_stride of k_scale and of v_scale (f32).  Alignments and the limits of strides
- * are those of bytes.  A scale is 0 (of zeros), NaN, or 2^-60 to 2^50; others count as the nearest
+ * + head*scale_head_stride of k_scale and of v_scale (f32; strides up to 2^31-1).  Alignments and
+ * the limits of the codes' strides are those of bytes.  A scale is 0 (of zeros), NaN, or 2^-60 to 2^50; others count as the nearest
  * of these bounds. */
 typedef struct rie_hip_pages8 {
     rie_hip_pages pages;

@@ -58,12 +58,12 @@ rie::KvView pages8_view(const rie_hip_pages8 *p, rie::Scales8 &s) {
         throw Error{rie::E_UNSUPPORTED, "block has to be a power of two in 16..page_size"};
     s.k = p->k_scale;
     s.v = p->v_scale;
-    s.page = used(g.n_pages, p->scale_page_stride);
-    s.block = used(g.page_size / p->block, p->scale_block_stride);
-    s.head = used(g.n_kv, p->scale_head_stride);
+    const int64_t page = used(g.n_pages, p->scale_page_stride), block = used(g.page_size / p->block, p->scale_block_stride), head = used(g.n_kv, p->scale_head_stride);
     s.block_shift = __builtin_ctz((unsigned)p->block);
-    const int64_t most = (int64_t)1 << 40;
-    if (s.page < 0 || s.block < 0 || s.head < 0 || s.page > most || s.block > most || s.head > most) throw bad("scales: strides have to lie in 0..2^40");
+    if (page < 0 || block < 0 || head < 0 || page > INT32_MAX || block > INT32_MAX || head > INT32_MAX) throw bad("scales: strides have to lie in 0..2^31-1");
+    s.page = (uint32_t)page;
+    s.block = (uint32_t)block;
+    s.head = (uint32_t)head;
     if ((uintptr_t)s.k % 4 || (uintptr_t)s.v % 4) throw bad("scales have to be aligned to their type");
     return v;
 }

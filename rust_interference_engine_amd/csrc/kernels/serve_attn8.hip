@@ -176,9 +176,10 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
         return p;
     };
     // lanes 0 and 1: the scales of the groups' keys; 2 and 3: of their values
+    const float *sbase = ((lane & 2) ? x.s.v : x.s.k) + (int64_t)kvh * x.s.head;
     auto request_scales = [&](int t, const Pages &pg) {
         const int slot = first_of(t, lane & 1) & page_mask;
-        return ((lane & 2) ? x.s.v : x.s.k)[pg.id * x.s.page + (slot >> x.s.block_shift) * x.s.block + kvh * x.s.head];
+        return sbase[(uint64_t)(uint32_t)pg.id * x.s.page + (uint64_t)(uint32_t)(slot >> x.s.block_shift) * x.s.block];
     };
     u32x4 rk[2][KS];
     auto load_keys = [&](int t, const Pages &pg) __attribute__((always_inline)) {
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
     }
 }
 
-// ---- 128 query rows of a sequence and KV head, tiles of 64 (256-wide heads: 32) positions ----
+// ---- 32·NW query rows of a sequence and KV head, tiles of 64 (256-wide heads: 32) positions ----
 //
 // The schedule is that of the 16-bit tile kernel: a tile's work is cut into groups of 32
 // positions, and the probabilities of group h are made while the matrix units form the outputs of
@@ -386,15 +387,16 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
 template <int HD>
 constexpr int TILE8_KT = HD <= 128 ? 64 : 32;
 
-template <int HD, bool BF, bool CAP>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(ServeAttn8Args xa) {
+template <int HD, bool BF, bool CAP, int NW>
+__global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_kernel(ServeAttn8Args xa) {
     const ServeAttnArgs &a = xa.a;
-    constexpr int KT = TILE8_KT<HD>, KB = KT / 32, RW = KT / 4, KS = HD / 16, DB = HD / 32;
+    constexpr int TILE_M = 32 * NW;
+    constexpr int KT = TILE8_KT<HD>, KB = KT / 32, RW = KT / NW, KS = HD / 16, DB = HD / 32;
     using Lds = TileLds<HD>;
     constexpr int RPI = Lds::RPI, KBYTES = KT / RPI * Lds::K_BLOCK, VBYTES = KT / RPI * Lds::V_BLOCK;
     constexpr int NG = KT / 16;                                         // groups of 16 positions, which lie in one page and block
     constexpr int CH = RW * (HD / 16), NCH = (CH + 63) / 64;            // 16-byte chunks of a wave's rows, and of a lane
-    __shared__ __align__(16) uint8_t s_k0[KBYTES], s_k1[KBYTES], s_v0[VBYTES], s_v1[VBYTES];
+    __shared__ __align__(16) uint8_t s_tiles[2 * KBYTES + 2 * VBYTES];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     // the splits of a block side by side, and a KV head's workgroups on one XCD where there are 8 of them
     const int G = a.G, kvh = blockIdx.x % a.n_kv, sp = blockIdx.x / a.n_kv % a.S, blk = blockIdx.x / a.n_kv / a.S;
@@ -450,31 +452,64 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(Serv
     // Of a tile: page ids of its groups of 16 positions, a lane each, and (lanes 0.. and 4..) their
     // keys' and values' scales.  A page id that is none: any page that exists is read, and nobody
     // sees its values.
+    const float *sbase = ((lane & 4) ? xa.s.v : xa.s.k) + (int64_t)kvh * xa.s.head;
     auto group_at = [&](int t) { return imin(t * KT + (lane & (NG - 1)) * 16, (hi - 1) & ~15); };
-    auto request_pages = [&](int t) __attribute__((always_inline)) { return t < t_end ? trow[group_at(t) >> a.kv.page_shift] : -1; };
+    auto request_pages = [&](int t) __attribute__((always_inline)) { return trow[group_at(t) >> a.kv.page_shift]; };
     auto known = [&](int id) { return (unsigned)id < (unsigned)a.kv.n_pages ? id : 0; };
     auto bad_of = [&](int ids) __attribute__((always_inline)) { return same((int)(__ballot((unsigned)ids >= (unsigned)a.kv.n_pages) & ((1u << NG) - 1))); };
     auto request_scales = [&](int t, int ids) __attribute__((always_inline)) {
         const int slot = group_at(t) & page_mask;
-        return ((lane & 4) ? xa.s.v : xa.s.k)[known(ids) * xa.s.page + (slot >> xa.s.block_shift) * xa.s.block + kvh * xa.s.head];
+        return sbase[(uint64_t)(uint32_t)known(ids) * xa.s.page + (uint64_t)(uint32_t)(slot >> xa.s.block_shift) * xa.s.block];
     };
-    auto load = [&](const uint8_t *base, int rs, int t, int ids, u32x4 (&raw)[NCH]) __attribute__((always_inline)) {
+    // Which of its wave's rows and codes' chunks a lane takes, so that 8 lanes' places in LDS lie in
+    // other banks: of keys, a column of rows; of values, two chunks of a row, which follow each other
+    // there, the pairs of every other two rows the other way round (chunks of 13 sequences up to 8200:
+    // 281 us with columns of values, 264 without the turn).
+    auto place = [&](auto is_v, int i, int &r, int &c) __attribute__((always_inline)) {
+        const int u = CH % 64 ? imin(i * 64 + lane, CH - 1) : i * 64 + lane;
+        if constexpr (decltype(is_v)::value) {
+            r = u / 2 % RW;
+            c = u / (2 * RW) * 2 + u % 2;
+        } else {
+            r = u % RW;
+            c = u / RW;
+        }
+    };
+    int k_off[NCH], v_off[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; i++) {
+        int r, c;
+        place(std::false_type{}, i, r, c);
+        k_off[i] = r * k_row + c * 16;
+        place(std::true_type{}, i, r, c);
+        v_off[i] = r * v_row + c * 16;
+    }
+    auto load = [&](auto is_v, int t, int ids, u32x4 (&raw)[NCH]) __attribute__((always_inline)) {
+        constexpr bool V = decltype(is_v)::value;
+        const int rs = V ? v_row : k_row;
         const int g0 = imin(t * KT + w * RW, (hi - 1) & ~(RW - 1));  // rows behind the last one seen: copies of it
         const int64_t page = __builtin_amdgcn_readlane(known(ids), w * RW / 16);
-        const uint8_t *src = base + page * a.kv.page + (int64_t)(g0 & page_mask) * rs;
+        const uint8_t *src = (V ? vbase : kbase) + page * a.kv.page + (int64_t)(g0 & page_mask) * rs;
         const int last = hi - 1 - g0;
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
-            const int u = imin(i * 64 + lane, CH - 1), r = u % RW, c = u / RW;
-            raw[i] = *(const u32x4 *)(src + imin(r, last) * rs + c * 16);
+            int off = V ? v_off[i] : k_off[i];
+            if (last < RW - 1) {
+                int r, c;
+                place(is_v, i, r, c);
+                off = imin(r, last) * rs + c * 16;
+            }
+            raw[i] = *(const u32x4 *)(src + off);
         }
     };
-    auto store = [&](auto is_v, const u32x4 (&raw)[NCH], uint8_t *dst) __attribute__((always_inline)) {
+    auto store = [&](auto is_v, const u32x4 (&raw)[NCH], uint32_t dst) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
-            const int u = i * 64 + lane, r = w * RW + u % RW, c = u / RW;
-            if (CH % 64 && u >= CH) continue;
+            if (CH % 64 && i * 64 + lane >= CH) continue;
+            int r, c;
+            place(is_v, i, r, c);
+            r += w * RW;
             u32x4 y[2];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -484,7 +519,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(Serv
                 y[k / 2][k % 2 * 2 + 1] = hi2;
             }
 #pragma unroll
-            for (int k = 0; k < 2; k++) *(u32x4 *)(dst + (V ? Lds::value(r, 2 * c + k) : Lds::key(r, 2 * c + k))) = y[k];
+            for (int k = 0; k < 2; k++) *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(dst + (V ? Lds::value(r, (2 * c + k) ^ ((r >> 1) & 1)) : Lds::key(r, 2 * c + k))) = y[k];
         }
     };
     using K_ = std::false_type;
@@ -495,24 +530,30 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(Serv
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
     float m = -FLT_MAX, l = 0, ym0 = 0, ym1 = 0;  // ym: largest scores of either half of the group whose turn is next
     const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
-    const float cq = CAP ? qs : a.scale * LOG2E_F;
+    const float cq = CAP ? qs : a.scale * LOG2E_F * qs;
     // the lane's places in a tile: keys row-wise, values transposed
-    const int k_at = Lds::key(lane & 31, h), v_at = Lds::value(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
+    const int k_at = Lds::key(lane & 31, h), v_at = Lds::value(4 * h + ((lane & 15) >> 2), (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ ((lane >> 3) & 1)) + (lane & 1) * 8;
 
     f32x16 s[2];
     u32x4 pf[2][2];
     struct GroupScales {  // of a group's halves: a score's factor, log2 of the values' scale and its inverse
         float c[2], lv[2], iv[2];
     };
-    auto scales_of = [&](float sc, int kb) __attribute__((always_inline)) {
-        const float us = usable(sc), lg = __builtin_amdgcn_logf(us), rc = us == us ? 1.0f / us : 1.0f;
+    struct TileScales {  // by lane: a scale, its log2, its inverse
+        float s, lg, inv;
+    };
+    auto tile_scales = [&](float sc) __attribute__((always_inline)) {
+        const float us = usable(sc);
+        return TileScales{us, __builtin_amdgcn_logf(us), us == us ? __builtin_amdgcn_rcpf(us) : 1.0f};
+    };
+    auto scales_of = [&](const TileScales &t, int kb) __attribute__((always_inline)) {
+        auto lane_of = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
         GroupScales x;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            x.c[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(us), kb * 2 + b)) * cq;
-            if (BF && !CAP) x.c[b] *= qs;
-            x.lv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg), 4 + kb * 2 + b));
-            x.iv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rc), 4 + kb * 2 + b));
+            x.c[b] = lane_of(t.s, kb * 2 + b) * cq;
+            x.lv[b] = lane_of(t.lg, 4 + kb * 2 + b);
+            x.iv[b] = lane_of(t.inv, 4 + kb * 2 + b);
         }
         return x;
     };
@@ -598,8 +639,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(Serv
         };
         auto pack = [&](int i) __attribute__((always_inline)) {
             p[i / 4][i % 4] = pack2<false>(ex[2 * i], ex[2 * i + 1]);
-            sum[i / 4] += ex[2 * i];
-            sum[i / 4] += ex[2 * i + 1];
+            sum[i / 4] += ex[2 * i] + ex[2 * i + 1];
         };
         auto product = [&](int u) __attribute__((always_inline)) {
             if (u < KS) y = mfma32<false>(fr[u], qf[u], y);
@@ -644,70 +684,82 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn8_tile_kernel(Serv
     };
 
     if (t_begin < t_end) {
-        // page ids of tiles t .. t + 3, the scales of t and t + 1, codes of keys t + 2 and of values t + KB − 1
-        int id0 = request_pages(t_begin), id1 = request_pages(t_begin + 1), id2 = request_pages(t_begin + 2), id3 = request_pages(t_begin + 3);
-        float sc0 = request_scales(t_begin, id0), sc1 = request_scales(t_begin + 1, id1);
+        // What is on its way, of a tile t: page ids of t + 3, scales of t + 1, codes of keys t + 2 and of
+        // values t + KB − 1, requested in this order at t − 1, so that the codes' arrival is all that is
+        // waited for.  All of it is requested whatever t, behind the last tile for its rows again: where
+        // a register may or may not have been loaded, the compiler copies it, and waits for all loads
+        // to do so.
+        int id0 = request_pages(t_begin), id1 = request_pages(t_begin + 1), id2 = request_pages(t_begin + 2), ids = request_pages(t_begin + 3);
+        float sc0 = request_scales(t_begin, id0), sc = request_scales(t_begin + 1, id1);
+        int bad0 = bad_of(id0);
         u32x4 rk[NCH], rv[NCH];
-        load(kbase, k_row, t_begin, id0, rk);
+        const uint32_t s_k0 = lds_at(s_tiles), s_k1 = s_k0 + KBYTES, s_v0 = s_k1 + KBYTES, s_v1 = s_v0 + VBYTES;
+        load(K_{}, t_begin, id0, rk);
         store(K_{}, rk, s_k0);
-        if (t_begin + 1 < t_end) {
-            load(kbase, k_row, t_begin + 1, id1, rk);
-            store(K_{}, rk, s_k1);
-        }
-        load(vbase, v_row, t_begin, id0, rv);
+        load(K_{}, t_begin + 1, id1, rk);
+        store(K_{}, rk, s_k1);
+        load(V_{}, t_begin, id0, rv);
         if constexpr (KB == 2) {
             store(V_{}, rv, s_v0);
-            if (t_begin + 1 < t_end) load(vbase, v_row, t_begin + 1, id1, rv);
+            load(V_{}, t_begin + 1, id1, rv);
         }
-        if (t_begin + 2 < t_end) load(kbase, k_row, t_begin + 2, id2, rk);
+        load(K_{}, t_begin + 2, id2, rk);
         // the first group's outputs before it: zeros
-        for (int i = w; i < 32 / RPI; i += 4) *(u32x4 *)(s_v1 + Lds::value((KB - 1) * 32 + i * RPI, 0) + lane * 16) = u32x4{0, 0, 0, 0};
+        for (int i = w; i < 32 / RPI; i += NW) *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(s_v1 + Lds::value((KB - 1) * 32 + i * RPI, 0) + lane * 16) = u32x4{0, 0, 0, 0};
         pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
         lds_barrier();
         if (wave_live) {
-            scores(lds_at(s_k0), 0, s[0]);
+            scores(s_k0, 0, s[0]);
             ym0 = max8(s[0], 0);
             ym1 = max8(s[0], 8);
         }
-        auto tile = [&](int t, uint8_t *k_t, uint8_t *k_n, uint8_t *v_t, uint8_t *v_n, f32x16 &x0, f32x16 &x1, u32x4 (&p0)[2], u32x4 (&p1)[2]) __attribute__((always_inline)) {
-            const int bad = bad_of(id0);
+        TileScales ts = tile_scales(sc0);
+        auto tile = [&](int t, uint32_t k_t, uint32_t k_n, uint32_t v_t, uint32_t v_n, f32x16 &x0, f32x16 &x1, u32x4 (&p0)[2], u32x4 (&p1)[2]) __attribute__((always_inline)) {
+            const int bad = bad0;
             if constexpr (KB == 2)
-                if (wave_live) group(t * KT, bad & 3, scales_of(sc0, 0), x0, p0, p1, x1, lds_at(v_n), 1, lds_at(k_t), 1);
+                if (wave_live) group(t * KT, bad & 3, scales_of(ts, 0), x0, p0, p1, x1, v_n, 1, k_t, 1);
             lds_barrier();
-            if (t + 2 < t_end) store(K_{}, rk, k_t);
-            if constexpr (KB == 2) {
-                if (t + 1 < t_end) store(V_{}, rv, v_n);
-                if (t + 2 < t_end) load(vbase, v_row, t + 2, id2, rv);
-            } else {
-                store(V_{}, rv, v_t);
-                if (t + 1 < t_end) load(vbase, v_row, t + 1, id1, rv);
-            }
-            if (t + 3 < t_end) load(kbase, k_row, t + 3, id3, rk);
-            const int id4 = request_pages(t + 4);
-            const float sc2 = request_scales(t + 2, id2);
-            if (wave_live) {
-                if constexpr (KB == 2) group(t * KT + 32, bad >> 2, scales_of(sc0, 1), x1, p1, p0, x0, lds_at(v_t), 0, lds_at(k_n), 0);
-                else group(t * KT, bad, scales_of(sc0, 0), x0, p0, p1, x1, lds_at(v_n), 0, lds_at(k_n), 0);
-            }
-            id0 = id1;
+            store(K_{}, rk, k_t);
+            store(V_{}, rv, KB == 2 ? v_n : v_t);
+            const GroupScales gs = scales_of(ts, KB - 1);
+            ts = tile_scales(sc);
+            bad0 = bad_of(id1);
+            const int id3 = ids;
+            ids = request_pages(t + 4);
+            sc = request_scales(t + 2, id2);
+            load(V_{}, t + KB, KB == 2 ? id2 : id1, rv);
+            load(K_{}, t + 3, id3, rk);
             id1 = id2;
             id2 = id3;
-            id3 = id4;
-            sc0 = sc1;
-            sc1 = sc2;
+            if (wave_live) {
+                if constexpr (KB == 2) group(t * KT + 32, bad >> 2, gs, x1, p1, p0, x0, v_t, 0, k_n, 0);
+                else group(t * KT, bad, gs, x0, p0, p1, x1, v_n, 0, k_n, 0);
+            }
         };
-        for (int t = t_begin; t < t_end; t += 2) {
-            tile(t, s_k0, s_k1, s_v0, s_v1, s[0], s[1], pf[0], pf[1]);
-            if (t + 1 >= t_end) break;
-            if constexpr (KB == 2) tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[0], s[1], pf[0], pf[1]);
-            else tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[1], s[0], pf[1], pf[0]);
+        if constexpr (KB == 2) {
+            // one tile to a turn, so that the registers that are on their way are the same in every turn
+            uint32_t kt = s_k0, kn = s_k1, vt = s_v0, vn = s_v1;
+            for (int t = t_begin; t < t_end; t++) {
+                tile(t, kt, kn, vt, vn, s[0], s[1], pf[0], pf[1]);
+                const uint32_t k = kt, v = vt;
+                kt = kn;
+                kn = k;
+                vt = vn;
+                vn = v;
+            }
+        } else {
+            for (int t = t_begin; t < t_end; t += 2) {
+                tile(t, s_k0, s_k1, s_v0, s_v1, s[0], s[1], pf[0], pf[1]);
+                if (t + 1 >= t_end) break;
+                tile(t + 1, s_k1, s_k0, s_v1, s_v0, s[1], s[0], pf[1], pf[0]);
+            }
         }
         // the last group's outputs
         const bool odd = (t_end - t_begin) & 1;
         if constexpr (KB == 1) lds_barrier();
         if (wave_live) {
-            if (odd) outputs(lds_at(s_v0), KB - 1, pf[KB == 2 ? 1 : 0]);
-            else outputs(lds_at(s_v1), KB - 1, pf[1]);
+            if (odd) outputs(s_v0, KB - 1, pf[KB == 2 ? 1 : 0]);
+            else outputs(s_v1, KB - 1, pf[1]);
         }
     }
     if (!live) return;
@@ -778,7 +830,7 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     page = same(page);
     const int first = imax(b0, from), n = imin(b0 + B, to) - first, slot0 = b0 & ((1 << a.kv.page_shift) - 1);
     if (n <= 0) return;
-    float *sp = (is_v ? x.s.v : x.s.k) + page * x.s.page + (slot0 >> bs) * x.s.block + h * x.s.head;
+    float *sp = (is_v ? x.s.v : x.s.k) + (int64_t)page * x.s.page + (int64_t)(slot0 >> bs) * x.s.block + (int64_t)h * x.s.head;
     const float was = first > b0 ? *sp : 0.0f;
     const uint8_t *src = (is_v ? a.v + h * a.v_head : a.k + h * a.k_head) + (int64_t)(sv.row0 + first - pos0) * (is_v ? a.v_row : a.k_row);
     const int64_t src_row = is_v ? a.v_row : a.k_row, row = is_v ? a.kv.v_row : a.kv.k_row;
@@ -846,6 +898,9 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     }
 }
 
+int tile8_waves(const ServeAttnArgs &a) { return a.hd <= 128 && (int64_t)a.b.max_new * a.G > 128 ? 8 : 4; }
+int tile8_m(const ServeAttnArgs &a) { return 32 * tile8_waves(a); }
+
 template <int HD, bool BF>
 void launch_hd(const ServeAttn8Args &x, hipStream_t st) {
     const ServeAttnArgs &a = x.a;
@@ -862,8 +917,17 @@ void launch_hd(const ServeAttn8Args &x, hipStream_t st) {
         }
     } else {
         const int grid = a.n_blocks * a.n_kv * a.S;
-        if (cap) attn8_tile_kernel<HD, BF, true><<<grid, 256, 0, st>>>(x);
-        else attn8_tile_kernel<HD, BF, false><<<grid, 256, 0, st>>>(x);
+        bool wide = false;
+        if constexpr (HD <= 128) wide = tile8_waves(a) == 8;
+        if (wide) {
+            if constexpr (HD <= 128) {
+                if (cap) attn8_tile_kernel<HD, BF, true, 8><<<grid, 512, 0, st>>>(x);
+                else attn8_tile_kernel<HD, BF, false, 8><<<grid, 512, 0, st>>>(x);
+            }
+        } else {
+            if (cap) attn8_tile_kernel<HD, BF, true, 4><<<grid, 256, 0, st>>>(x);
+            else attn8_tile_kernel<HD, BF, false, 4><<<grid, 256, 0, st>>>(x);
+        }
     }
 }
 
@@ -894,14 +958,14 @@ int tile8_kt(int hd) { return hd <= 128 ? TILE8_KT<128> : TILE8_KT<256>; }
 SplitPlan splits8(const ServeAttnArgs &a) {
     const bool few = few_row_blocks(true, a.b.max_new, a.G) > 0;
     const int KT = few ? FEW8_STEP : tile8_kt(a.hd);
-    const int64_t blocks = few ? a.b.n_seq : block_count(a.b.n_rows, a.b.n_seq, a.G, TILE_M);
+    const int64_t blocks = few ? a.b.n_seq : block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
     // positions that a block's rows see, at most
     int64_t span = a.b.max_len;
-    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? FEW_ROWS : TILE_M / a.G + 1) + KT);
+    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? FEW_ROWS : tile8_m(a) / a.G + 1) + KT);
     const int tiles = (int)((span + KT - 1) / KT);
     if (few) return split_plan(blocks * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
     const double part_us = (double)a.b.n_rows * a.n_head * a.hd * 8 / 4.5e6;
-    return tile_plan(blocks * a.n_kv, a.hd <= 128 ? 512 : 256, tiles, 2.0 * KT * a.hd / (64 * 128), part_us, SERVE_MAX_SPLIT);
+    return tile_plan(blocks * a.n_kv, (a.hd <= 128 ? 2048 : 1024) / tile8_waves(a), tiles, 2.0 * KT * a.hd / (64 * 128), part_us, SERVE_MAX_SPLIT);
 }
 
 }  // namespace
@@ -919,10 +983,10 @@ void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st) {
     a.S = p.S;
     a.part = (float *)ws;
     a.ml = a.part + (size_t)a.b.n_rows * a.n_head * p.S * a.hd;
-    a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, TILE_M);
+    a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
     if (a.ty == T_BF16) launch_ty<true>(x, st);
     else launch_ty<false>(x, st);
-    if (p.S > 1) launch_serve_combine(a, few ? FEW_ROWS : TILE_M, few ? FEW8_STEP : tile8_kt(a.hd), st);
+    if (p.S > 1) launch_serve_combine(a, few ? FEW_ROWS : tile8_m(a), few ? FEW8_STEP : tile8_kt(a.hd), st);
 }
 
 void launch_paged_append8(const PagedAppend8Args &x, hipStream_t st) {

@@ -52,7 +52,7 @@ void launch_serve_combine(const ServeAttnArgs &a, int M, int KT, hipStream_t st)
 // Pages of 8 bits: a value is its code times the scale of its block of positions and head
 struct Scales8 {
     float *k = nullptr, *v = nullptr;
-    int64_t page = 0, block = 0, head = 0;  // strides, values
+    uint32_t page = 0, block = 0, head = 0;  // strides, values
     int block_shift = 0;
 };
 constexpr float SCALE8_MIN = 0x1p-60f, SCALE8_MAX = 0x1p50f;  // of blocks that hold anything but zeros
