@@ -387,30 +387,28 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
 template <int HD>
 constexpr int TILE8_KT = HD <= 128 ? 64 : 32;
 
+template <int HD>
+constexpr int TILE8_KBYTES = TILE8_KT<HD> / TileLds<HD>::RPI * TileLds<HD>::K_BLOCK;
+template <int HD>
+constexpr int TILE8_VBYTES = TILE8_KT<HD> / TileLds<HD>::RPI * TileLds<HD>::V_BLOCK;
+
+// Tiles [from, to) of block lb of sequence si: to the outputs, or (part given) unnormalised to part,
+// as they lie in the waves' registers, with the rows' maxima and sums behind
 template <int HD, bool BF, bool CAP, int NW>
-__global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_kernel(ServeAttn8Args xa) {
+__device__ __forceinline__ void tile8_piece(const ServeAttn8Args &xa, uint8_t *s_tiles, int kvh, int si, const SeqView &sv, int lb, int from, int to, float *part) {
     const ServeAttnArgs &a = xa.a;
     constexpr int TILE_M = 32 * NW;
     constexpr int KT = TILE8_KT<HD>, KB = KT / 32, RW = KT / NW, KS = HD / 16, DB = HD / 32;
     using Lds = TileLds<HD>;
-    constexpr int RPI = Lds::RPI, KBYTES = KT / RPI * Lds::K_BLOCK, VBYTES = KT / RPI * Lds::V_BLOCK;
+    constexpr int RPI = Lds::RPI, KBYTES = TILE8_KBYTES<HD>, VBYTES = TILE8_VBYTES<HD>;
     constexpr int NG = KT / 16;                                         // groups of 16 positions, which lie in one page and block
     constexpr int CH = RW * (HD / 16), NCH = (CH + 63) / 64;            // 16-byte chunks of a wave's rows, and of a lane
-    __shared__ __align__(16) uint8_t s_tiles[2 * KBYTES + 2 * VBYTES];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-    // the splits of a block side by side, and a KV head's workgroups on one XCD where there are 8 of them
-    const int G = a.G, kvh = blockIdx.x % a.n_kv, sp = blockIdx.x / a.n_kv % a.S, blk = blockIdx.x / a.n_kv / a.S;
-    int si;
-    const SeqView sv = find_seq(a.b, a.kv, blk, si, [&](int s, int i) { return block_base(iclamp(s, 0, a.b.n_rows), i, G, TILE_M); });
-    const int n_rows = sv.n_new * G;
-    const int lb = (n_rows + TILE_M - 1) / TILE_M - 1 - (blk - block_base(sv.row0, si, G, TILE_M));  // a sequence's longest rows first
-    if (lb < 0 || lb >= (n_rows + TILE_M - 1) / TILE_M) return;
+    const int G = a.G, n_rows = sv.n_new * G;
     const int r0 = same(lb * TILE_M), r1 = same(imin(r0 + TILE_M, n_rows) - 1), tok0 = same(r0 / G), tok1 = same(r1 / G);
     const int pos0 = sv.pos0();  // position of token 0
     const KeyRange kr = key_range(sv, tok0, tok1, a.window);
-    const int hi = same(kr.hi), nt = same(tile_count(kr, KT)), ns = same(split_count(nt, a.C, a.S));
-    if (sp >= ns) return;
-    const int t_first = same(first_tile(kr, KT)), t_begin = t_first + sp * a.C, t_end = sp == ns - 1 ? t_first + nt : t_begin + a.C;
+    const int hi = same(kr.hi), t_first = same(first_tile(kr, KT)), nt = same(tile_count(kr, KT)), t_begin = same(t_first + imin(from, nt)), t_end = same(t_first + imin(to, nt));
 
     // this lane's query row, and what the rows of its wave see
     const int row = r0 + w * 32 + (lane & 31);
@@ -422,28 +420,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_ke
     const int w_t0 = same(imin(r0 + w * 32, r1) / G), w_t1 = same(imin(r0 + w * 32 + 31, r1) / G);
     const int all_hi = imin(pos0 + w_t0, sv.len - 1), all_lo = before_window(pos0 + w_t1, a.window);  // every row of the wave sees (all_lo, all_hi]
     u32x4 qf[KS];
-    {
-        const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + h * 16;
-#pragma unroll
-        for (int i = 0; i < KS; i++) qf[i] = live ? *(const u32x4 *)(qp + i * 32) : u32x4{0, 0, 0, 0};
-    }
-    float qs = 1;  // a row's power of two
-    if constexpr (BF) {
-        float most = 0;
-#pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(value16<true>(qf[i][e / 2] >> (e & 1) * 16 & 0xFFFF)));
-        float a0, a1;
-        pair_f<32>(most, a0, a1);
-        const int ex = 14 - __builtin_amdgcn_frexp_expf(fminf(fmaxf(a0, a1), FLT_MAX));  // infinities stay what they are
-        qs = __builtin_amdgcn_ldexpf(1.0f, -ex);
-#pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                qf[i][e] = pack2<false>(__builtin_amdgcn_ldexpf(value16<true>(qf[i][e] & 0xFFFF), ex), __builtin_amdgcn_ldexpf(value16<true>(qf[i][e] >> 16), ex));
-    }
+    float qs = 1, cq = 0;  // a row's power of two, and a score's factor but for its keys' scale
 
     // ---- codes: wave w's are rows w·RW .. of a tile, which lie in one page ----
     const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
@@ -530,7 +507,6 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_ke
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
     float m = -FLT_MAX, l = 0, ym0 = 0, ym1 = 0;  // ym: largest scores of either half of the group whose turn is next
     const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
-    const float cq = CAP ? qs : a.scale * LOG2E_F * qs;
     // the lane's places in a tile: keys row-wise, values transposed
     const int k_at = Lds::key(lane & 31, h), v_at = Lds::value(4 * h + ((lane & 15) >> 2), (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ ((lane >> 3) & 1)) + (lane & 1) * 8;
 
@@ -689,21 +665,50 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_ke
         // waited for.  All of it is requested whatever t, behind the last tile for its rows again: where
         // a register may or may not have been loaded, the compiler copies it, and waits for all loads
         // to do so.
-        int id0 = request_pages(t_begin), id1 = request_pages(t_begin + 1), id2 = request_pages(t_begin + 2), ids = request_pages(t_begin + 3);
-        float sc0 = request_scales(t_begin, id0), sc = request_scales(t_begin + 1, id1);
-        int bad0 = bad_of(id0);
+        int id1, id2, ids, bad0;
+        float sc0, sc;
         u32x4 rk[NCH], rv[NCH];
         const uint32_t s_k0 = lds_at(s_tiles), s_k1 = s_k0 + KBYTES, s_v0 = s_k1 + KBYTES, s_v1 = s_v0 + VBYTES;
-        load(K_{}, t_begin, id0, rk);
-        store(K_{}, rk, s_k0);
-        load(K_{}, t_begin + 1, id1, rk);
-        store(K_{}, rk, s_k1);
-        load(V_{}, t_begin, id0, rv);
-        if constexpr (KB == 2) {
-            store(V_{}, rv, s_v0);
-            load(V_{}, t_begin + 1, id1, rv);
+        {
+            const int id0 = request_pages(t_begin);
+            id1 = request_pages(t_begin + 1);
+            id2 = request_pages(t_begin + 2);
+            ids = request_pages(t_begin + 3);
+            sc0 = request_scales(t_begin, id0);
+            sc = request_scales(t_begin + 1, id1);
+            {
+                const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head + h * 16;
+#pragma unroll
+                for (int i = 0; i < KS; i++) qf[i] = live ? *(const u32x4 *)(qp + i * 32) : u32x4{0, 0, 0, 0};
+            }
+            bad0 = bad_of(id0);
+            u32x4 k0[NCH], k1[NCH], v0[NCH];  // the first tiles, all requested at once, and the queries before them
+            load(K_{}, t_begin, id0, k0);
+            load(K_{}, t_begin + 1, id1, k1);
+            load(V_{}, t_begin, id0, KB == 2 ? v0 : rv);
+            if constexpr (KB == 2) load(V_{}, t_begin + 1, id1, rv);
+            load(K_{}, t_begin + 2, id2, rk);
+            if constexpr (BF) {
+                float most = 0;
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(value16<true>(qf[i][e / 2] >> (e & 1) * 16 & 0xFFFF)));
+                float a0, a1;
+                pair_f<32>(most, a0, a1);
+                const int ex = 14 - __builtin_amdgcn_frexp_expf(fminf(fmaxf(a0, a1), FLT_MAX));  // infinities stay what they are
+                qs = __builtin_amdgcn_ldexpf(1.0f, -ex);
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        qf[i][e] = pack2<false>(__builtin_amdgcn_ldexpf(value16<true>(qf[i][e] & 0xFFFF), ex), __builtin_amdgcn_ldexpf(value16<true>(qf[i][e] >> 16), ex));
+            }
+            cq = CAP ? qs : a.scale * LOG2E_F * qs;
+            store(K_{}, k0, s_k0);
+            store(K_{}, k1, s_k1);
+            if constexpr (KB == 2) store(V_{}, v0, s_v0);
         }
-        load(K_{}, t_begin + 2, id2, rk);
         // the first group's outputs before it: zeros
         for (int i = w; i < 32 / RPI; i += NW) *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(s_v1 + Lds::value((KB - 1) * 32 + i * RPI, 0) + lane * 16) = u32x4{0, 0, 0, 0};
         pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
@@ -766,7 +771,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_ke
     float l0, l1;
     pair_f<32>(l, l0, l1);
     l = l0 + l1;
-    if (ns == 1) {
+    if (!part) {
         const float inv = l > 0 || l != l ? 1.0f / l : 0.0f;
         uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + h * 8;
 #pragma unroll
@@ -777,14 +782,211 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_ke
                 *(u32x2 *)(op + d * 64 + e * 16) = v;
             }
     } else {
-        const int64_t at = ((int64_t)(sv.row0 + tok) * a.n_head + head) * a.S + sp;
-        float *pp = a.part + at * HD + 4 * h;
+        float *pp = part + w * (32 * HD) + lane * 4;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) *(f32x4 *)(pp + d * 32 + e * 8) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
-        if (h == 0) *(f32x2 *)(a.ml + at * 2) = f32x2{m, l};
+            for (int e = 0; e < 4; e++) *(f32x4 *)(pp + (d * 4 + e) * 256) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+        if (h == 0) *(f32x2 *)(part + TILE_M * HD + (w * 32 + (lane & 31)) * 2) = f32x2{m, l};
     }
+}
+
+// The work of a launch, divided evenly: the blocks of all sequences in a row, each as long as its
+// tiles take, are cut into as many pieces as workgroups run at a time (per KV head), wherever the
+// cuts fall.  A workgroup goes through the blocks of its piece; one that it has all of goes to the
+// outputs, and at most two (its first, its last) to partial results, which tile8_join_kernel adds
+// up.  With a workgroup for each block, the longest sequence's ran on while the others' were done:
+// chunks of 13 sequences up to 8200 258 us; in pieces 185, of which 175 the tiles (at the 2.1 GHz
+// that the card keeps with all matrix units busy), 5 the plan and 8 the join.
+struct Tile8Plan {
+    int64_t total;  // what the tiles of all blocks take
+    int n, pad;     // blocks
+};
+struct Tile8Item {
+    int64_t before;  // what the blocks ahead take
+    int si, lb;      // sequence, and block of its rows
+    int row0, n_new, len, over;
+};
+constexpr int TILE8_FULL = 16, TILE8_BEGIN = 72, TILE8_LEAST = 10;  // a full tile's time, that until a block's first tile; tiles that a piece is worth
+struct Tile8Share {
+    int64_t total;
+    int P;
+    __device__ __forceinline__ int64_t begin(int j) const { return (total * j + P - 1) / P; }  // of piece j
+    __device__ __forceinline__ int owner(int64_t x) const { return (int)(x * P / total); }
+};
+__device__ __forceinline__ Tile8Share tile8_share(int64_t total, int P) {
+    return Tile8Share{total, (int)imax(1, (int)min((int64_t)P, total / (TILE8_LEAST * TILE8_FULL)))};
+}
+struct Tile8Block {
+    int rows, nt, cost;  // rows, tiles, and what one takes: waves without rows help to make it
+    __device__ __forceinline__ int units() const { return TILE8_BEGIN + imax(nt, 1) * cost; }
+    // tiles that begin in the block's first x units
+    __device__ __forceinline__ int upto(int64_t x) const { return (int)min((int64_t)imax(nt, 1), (max(x - TILE8_BEGIN, (int64_t)0) + cost - 1) / cost); }
+};
+template <int M>
+__device__ __forceinline__ Tile8Block tile8_block(const ServeAttnArgs &a, const SeqView &sv, int lb, int KT) {
+    const int n_rows = sv.n_new * a.G, r0 = lb * M, r1 = imin(r0 + M, n_rows) - 1;
+    return Tile8Block{r1 - r0 + 1, tile_count(key_range(sv, r0 / a.G, r1 / a.G, a.window), KT), 11 + 5 * ((r1 - r0) / 32 + 1) * 32 / M};
+}
+__device__ __forceinline__ SeqView tile8_seq(const Tile8Item &it) { return uniform(SeqView{it.row0, it.n_new, it.len, it.over}); }
+
+// items, and (first) the item with which each piece begins
+template <int M>
+__global__ __launch_bounds__(1024) void tile8_plan_kernel(ServeAttnArgs a, int KT, Tile8Plan *plan, Tile8Item *items, int *first, int P) {
+    __shared__ int64_t s_sum[16];
+    __shared__ int s_n[16];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int64_t before = 0;
+    int n = 0;
+    for (int b0 = 0; b0 < a.n_blocks; b0 += 1024) {
+        const int id = b0 + tid;
+        int64_t units = 0;
+        Tile8Item it{};
+        if (id < a.n_blocks) {
+            int lo = 0, hi = a.b.n_seq;  // the last sequence whose first id is at or before this one
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (block_base(iclamp(a.b.starts[mid], 0, a.b.n_rows), mid, a.G, M) <= id) lo = mid;
+                else hi = mid;
+            }
+            const SeqView sv = seq_view(a.b.starts[lo], a.b.starts[lo + 1], a.b.lens[lo], a.b.n_rows, a.kv.cap);
+            it = Tile8Item{0, lo, id - block_base(sv.row0, lo, a.G, M), sv.row0, sv.n_new, sv.len, sv.over};
+            // blocks whose rows see nothing, too: their zeros are written
+            if (it.lb >= 0 && it.lb < (sv.n_new * a.G + M - 1) / M) units = tile8_block<M>(a, sv, it.lb, KT).units();
+        }
+        int64_t x = units;
+        int c = units > 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up(x, o);
+            const int d = __shfl_up(c, o);
+            if (lane >= o) {
+                x += y;
+                c += d;
+            }
+        }
+        __syncthreads();
+        if (lane == 63) {
+            s_sum[w] = x;
+            s_n[w] = c;
+        }
+        __syncthreads();
+        it.before = before + x - units;
+        int place = n + c - (units > 0);
+        for (int i = 0; i < 16; i++) {
+            if (i < w) {
+                it.before += s_sum[i];
+                place += s_n[i];
+            }
+            before += s_sum[i];
+            n += s_n[i];
+        }
+        if (units) items[place] = it;
+    }
+    if (tid == 0) *plan = Tile8Plan{before, n, 0};
+    __syncthreads();
+    const Tile8Share share = tile8_share(before, P);
+    for (int j = tid; j < share.P && n; j += 1024) {
+        const int64_t begin = share.begin(j);
+        int lo = 0, hi = n;  // the last block that begins at or before it
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (items[mid].before <= begin) lo = mid;
+            else hi = mid;
+        }
+        first[j] = lo;
+    }
+}
+
+template <int HD, bool BF, bool CAP, int NW>
+__global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : NW / 4) void attn8_tile_kernel(ServeAttn8Args x, const Tile8Plan *plan, const Tile8Item *items, const int *first, int P, float *parts) {
+    constexpr int M = 32 * NW, KT = TILE8_KT<HD>;
+    __shared__ __align__(16) uint8_t s_tiles[2 * TILE8_KBYTES<HD> + 2 * TILE8_VBYTES<HD>];
+    const ServeAttnArgs &a = x.a;
+    // a KV head's workgroups on one XCD where there are 8 of them
+    const int kvh = blockIdx.x % a.n_kv, j = blockIdx.x / a.n_kv;
+    int i = 0, n = 1;
+    int64_t begin = 0, end = 0;
+    Tile8Item it{};
+    if (plan) {
+        i = first[j];  // there for every j
+        n = same(plan->n);
+        if (n == 0) return;
+        const Tile8Share share = tile8_share(plan->total, P);
+        if (j >= share.P) return;
+        i = same(i);
+        it = items[i];
+        begin = share.begin(j);
+        end = share.begin(j + 1);
+    } else {  // a workgroup for each block
+        const SeqView sv = find_seq(a.b, a.kv, j, it.si, [&](int s, int q) { return block_base(iclamp(s, 0, a.b.n_rows), q, a.G, M); });
+        const int blocks = (sv.n_new * a.G + M - 1) / M;
+        it.lb = blocks - 1 - (j - block_base(sv.row0, it.si, a.G, M));  // a sequence's longest rows first
+        if (it.lb < 0 || it.lb >= blocks) return;
+        it.row0 = sv.row0;
+        it.n_new = sv.n_new;
+        it.len = sv.len;
+        it.over = sv.over;
+    }
+    for (;;) {
+        const SeqView sv = tile8_seq(it);
+        const int si = same(it.si), lb = same(it.lb);
+        int from = 0, to = INT32_MAX;
+        float *part = nullptr;
+        bool more = false;
+        if (plan) {
+            const int64_t before = it.before;
+            const Tile8Block k = tile8_block<M>(a, sv, lb, KT);
+            from = k.upto(begin - before);
+            to = k.upto(end - before);
+            if (from > 0 || to < imax(k.nt, 1)) part = parts + (((int64_t)kvh * P + j) * 2 + (begin >= before ? 0 : 1)) * (M * (HD + 2));
+            more = ++i < n && before + k.units() < end;
+            if (more) it = items[i];
+            lds_barrier();  // the tiles of the piece before have been read
+        }
+        if (from < to) tile8_piece<HD, BF, CAP, NW>(x, s_tiles, kvh, si, sv, lb, from, to, part);
+        if (!more) break;
+    }
+}
+
+// Blocks whose tiles several workgroups took, a workgroup for each of their waves' parts
+template <int HD, bool BF, int M>
+__global__ __launch_bounds__(256) void tile8_join_kernel(ServeAttnArgs a, int KT, const Tile8Plan *plan, const Tile8Item *items, int P, const float *parts) {
+    const int kvh = blockIdx.x % a.n_kv, i = blockIdx.x / a.n_kv, w = blockIdx.y;
+    if (i >= plan->n) return;
+    const Tile8Share share = tile8_share(plan->total, P);
+    const Tile8Item it = items[i];
+    const SeqView sv = tile8_seq(it);
+    const Tile8Block k = tile8_block<M>(a, sv, it.lb, KT);
+    if (w * 32 >= k.rows) return;
+    const int j0 = share.owner(it.before + TILE8_BEGIN), j1 = share.owner(it.before + TILE8_BEGIN + (int64_t)(imax(k.nt, 1) - 1) * k.cost);
+    if (j0 == j1) return;
+    const int lane = threadIdx.x & 63, r = w * 32 + (lane & 31);
+    if (r >= k.rows) return;
+    constexpr int N = HD / 32;  // 16-byte pieces of a lane: (d, e) = threadIdx.x / 64 + 4 u
+    float m = -FLT_MAX, l = 0;
+    f32x4 o[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) o[u] = f32x4{0, 0, 0, 0};
+    for (int j = j0; j <= j1; j++) {
+        const float *p = parts + (((int64_t)kvh * P + j) * 2 + (share.begin(j) >= it.before ? 0 : 1)) * (M * (HD + 2));
+        const f32x2 ml = *(const f32x2 *)(p + M * HD + r * 2);
+        f32x4 y[N];
+#pragma unroll
+        for (int u = 0; u < N; u++) y[u] = *(const f32x4 *)(p + w * (32 * HD) + (threadIdx.x / 64 + 4 * u) * 256 + lane * 4);
+        const float mn = fmaxf(m, ml[0]), f = exp2_hw(m - mn), e = exp2_hw(ml[0] - mn);
+        m = mn;
+        l = fmaf(l, f, ml[1] * e);
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) o[u][q] = fmaf(o[u][q], f, y[u][q] * e);
+    }
+    const float inv = l > 0 || l != l ? 1.0f / l : 0.0f;
+    const int row = it.lb * M + r, tok = row / a.G, head = kvh * a.G + row - tok * a.G;
+    uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + (lane >> 5) * 8;
+#pragma unroll
+    for (int u = 0; u < N; u++) *(u32x2 *)(op + (threadIdx.x / 64 + 4 * u) * 16) = u32x2{pack2<BF>(o[u][0] * inv, o[u][1] * inv), pack2<BF>(o[u][2] * inv, o[u][3] * inv)};
 }
 
 // ---- new rows into their pages ----
@@ -900,9 +1102,54 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
 
 int tile8_waves(const ServeAttnArgs &a) { return a.hd <= 128 && (int64_t)a.b.max_new * a.G > 128 ? 8 : 4; }
 int tile8_m(const ServeAttnArgs &a) { return 32 * tile8_waves(a); }
+int tile8_kt(int hd) { return hd <= 128 ? TILE8_KT<128> : TILE8_KT<256>; }
+
+// positions that a block's rows see, at most
+int64_t span8(const ServeAttnArgs &a, int tokens, int KT) {
+    return a.window > 0 ? std::min<int64_t>(a.b.max_len, (int64_t)a.window + std::min(a.b.max_new, tokens) + KT) : a.b.max_len;
+}
+
+// Pieces per KV head that a launch of the tile kernel is divided into, or 0: a workgroup for each
+// block, where the longest is too short to be cut.
+int tile8_pieces(const ServeAttnArgs &a) {
+    const int KT = tile8_kt(a.hd), M = tile8_m(a);
+    const int64_t tiles = (span8(a, M / a.G + 1, KT) + KT - 1) / KT, blocks = block_count(a.b.n_rows, a.b.n_seq, a.G, M);
+    if (tiles < 2 * TILE8_LEAST) return 0;
+    const int slots = (a.hd <= 32 ? 3 : a.hd <= 128 ? 2 : 1) * 1024 / tile8_waves(a) / a.n_kv;
+    return (int)std::clamp<int64_t>(blocks * tiles / TILE8_LEAST, 1, std::max(slots, 1));
+}
+
+struct Tile8Ws {
+    size_t first, parts, bytes;  // where they begin, behind the plan and its items
+};
+Tile8Ws tile8_ws(const ServeAttnArgs &a) {
+    const size_t P = tile8_pieces(a), blocks = block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
+    if (!P) return Tile8Ws{0, 0, 0};
+    Tile8Ws w;
+    w.first = sizeof(Tile8Plan) + blocks * sizeof(Tile8Item);
+    w.parts = w.first + (P + 3) / 4 * 16;
+    w.bytes = w.parts + a.n_kv * P * 2 * tile8_m(a) * (a.hd + 2) * sizeof(float);
+    return w;
+}
+
+template <int HD, bool BF, int NW>
+void launch_tile(const ServeAttn8Args &x, void *ws, hipStream_t st) {
+    constexpr int M = 32 * NW;
+    const ServeAttnArgs &a = x.a;
+    const int P = tile8_pieces(a), grid = (P ? P : a.n_blocks) * a.n_kv;
+    const Tile8Ws w = tile8_ws(a);
+    Tile8Plan *plan = P ? (Tile8Plan *)ws : nullptr;
+    Tile8Item *items = (Tile8Item *)(plan + 1);
+    int *first = (int *)((uint8_t *)ws + w.first);
+    float *parts = (float *)((uint8_t *)ws + w.parts);
+    if (P) tile8_plan_kernel<M><<<1, 1024, 0, st>>>(a, TILE8_KT<HD>, plan, items, first, P);
+    if (a.softcap > 0) attn8_tile_kernel<HD, BF, true, NW><<<grid, 64 * NW, 0, st>>>(x, plan, items, first, P, parts);
+    else attn8_tile_kernel<HD, BF, false, NW><<<grid, 64 * NW, 0, st>>>(x, plan, items, first, P, parts);
+    if (P) tile8_join_kernel<HD, BF, M><<<dim3(a.n_blocks * a.n_kv, NW), 256, 0, st>>>(a, TILE8_KT<HD>, plan, items, P, parts);
+}
 
 template <int HD, bool BF>
-void launch_hd(const ServeAttn8Args &x, hipStream_t st) {
+void launch_hd(const ServeAttn8Args &x, void *ws, hipStream_t st) {
     const ServeAttnArgs &a = x.a;
     const bool cap = a.softcap > 0;
     const int few = few_row_blocks(true, a.b.max_new, a.G);
@@ -915,30 +1162,22 @@ void launch_hd(const ServeAttn8Args &x, hipStream_t st) {
             if (cap) attn8_few_kernel<HD, BF, true, 2><<<grid, 256, 0, st>>>(x);
             else attn8_few_kernel<HD, BF, false, 2><<<grid, 256, 0, st>>>(x);
         }
-    } else {
-        const int grid = a.n_blocks * a.n_kv * a.S;
-        bool wide = false;
-        if constexpr (HD <= 128) wide = tile8_waves(a) == 8;
-        if (wide) {
-            if constexpr (HD <= 128) {
-                if (cap) attn8_tile_kernel<HD, BF, true, 8><<<grid, 512, 0, st>>>(x);
-                else attn8_tile_kernel<HD, BF, false, 8><<<grid, 512, 0, st>>>(x);
-            }
-        } else {
-            if (cap) attn8_tile_kernel<HD, BF, true, 4><<<grid, 256, 0, st>>>(x);
-            else attn8_tile_kernel<HD, BF, false, 4><<<grid, 256, 0, st>>>(x);
-        }
+        return;
     }
+    if constexpr (HD <= 128) {
+        if (tile8_waves(a) == 8) return launch_tile<HD, BF, 8>(x, ws, st);
+    }
+    launch_tile<HD, BF, 4>(x, ws, st);
 }
 
 template <bool BF>
-void launch_ty(const ServeAttn8Args &x, hipStream_t st) {
+void launch_ty(const ServeAttn8Args &x, void *ws, hipStream_t st) {
     switch (x.a.hd) {
-    case 32: launch_hd<32, BF>(x, st); break;
-    case 64: launch_hd<64, BF>(x, st); break;
-    case 96: launch_hd<96, BF>(x, st); break;
-    case 128: launch_hd<128, BF>(x, st); break;
-    default: launch_hd<256, BF>(x, st); break;
+    case 32: launch_hd<32, BF>(x, ws, st); break;
+    case 64: launch_hd<64, BF>(x, ws, st); break;
+    case 96: launch_hd<96, BF>(x, ws, st); break;
+    case 128: launch_hd<128, BF>(x, ws, st); break;
+    default: launch_hd<256, BF>(x, ws, st); break;
     }
 }
 
@@ -953,40 +1192,39 @@ void launch_append(const PagedAppend8Args &x, int grid, hipStream_t st) {
     }
 }
 
-int tile8_kt(int hd) { return hd <= 128 ? TILE8_KT<128> : TILE8_KT<256>; }
+bool few8(const ServeAttnArgs &a) { return few_row_blocks(true, a.b.max_new, a.G) > 0; }
 
+// how the few-rows kernel divides the positions
 SplitPlan splits8(const ServeAttnArgs &a) {
-    const bool few = few_row_blocks(true, a.b.max_new, a.G) > 0;
-    const int KT = few ? FEW8_STEP : tile8_kt(a.hd);
-    const int64_t blocks = few ? a.b.n_seq : block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
-    // positions that a block's rows see, at most
-    int64_t span = a.b.max_len;
-    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + std::min<int64_t>(a.b.max_new, few ? FEW_ROWS : tile8_m(a) / a.G + 1) + KT);
-    const int tiles = (int)((span + KT - 1) / KT);
-    if (few) return split_plan(blocks * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
-    const double part_us = (double)a.b.n_rows * a.n_head * a.hd * 8 / 4.5e6;
-    return tile_plan(blocks * a.n_kv, (a.hd <= 128 ? 2048 : 1024) / tile8_waves(a), tiles, 2.0 * KT * a.hd / (64 * 128), part_us, SERVE_MAX_SPLIT);
+    const int tiles = (int)((span8(a, FEW_ROWS, FEW8_STEP) + FEW8_STEP - 1) / FEW8_STEP);
+    return split_plan((int64_t)a.b.n_seq * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
 }
 
 }  // namespace
 
 size_t serve_attn8_ws(const ServeAttnArgs &a) {
+    if (!few8(a)) {
+        return tile8_ws(a).bytes;
+    }
     const SplitPlan p = splits8(a);
     return p.S == 1 ? 0 : (size_t)a.b.n_rows * a.n_head * p.S * (a.hd + 2) * sizeof(float);
 }
 
 void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st) {
     ServeAttnArgs &a = x.a;
-    const SplitPlan p = splits8(a);
-    const bool few = few_row_blocks(true, a.b.max_new, a.G) > 0;
-    a.C = p.C;
-    a.S = p.S;
-    a.part = (float *)ws;
-    a.ml = a.part + (size_t)a.b.n_rows * a.n_head * p.S * a.hd;
-    a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
-    if (a.ty == T_BF16) launch_ty<true>(x, st);
-    else launch_ty<false>(x, st);
-    if (p.S > 1) launch_serve_combine(a, few ? FEW_ROWS : tile8_m(a), few ? FEW8_STEP : tile8_kt(a.hd), st);
+    const bool few = few8(a);
+    if (few) {
+        const SplitPlan p = splits8(a);
+        a.C = p.C;
+        a.S = p.S;
+        a.part = (float *)ws;
+        a.ml = a.part + (size_t)a.b.n_rows * a.n_head * p.S * a.hd;
+    } else {
+        a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
+    }
+    if (a.ty == T_BF16) launch_ty<true>(x, ws, st);
+    else launch_ty<false>(x, ws, st);
+    if (few && a.S > 1) launch_serve_combine(a, FEW_ROWS, FEW8_STEP, st);
 }
 
 void launch_paged_append8(const PagedAppend8Args &x, hipStream_t st) {
