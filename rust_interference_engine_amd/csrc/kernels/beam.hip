@@ -8,12 +8,15 @@
 // of groups, with the run's maximum and sum, and keeps every group's maximum.  beam_row_kernel
 // joins a row's runs and finds its own best n_out tokens: they lie in the n_out groups with the
 // largest maxima (by value, then by place: a group ahead of theirs holds a logit ahead of them),
-// so only those are read again.  beam_join_kernel merges the rows of a request.
+// so only those are read again.  The workgroup of a request that is done last merges its rows.
 //
 // Beams are compared by sums in f64: in f32 the candidates of two beams would be equal to the last
 // bit too often, and their order that of the roundings.  ln Σ is f64 of an f32 sum (2^-22 of it).
 //
-// Bound: HBM, rows · V values, and for a few rows the three launches.
+// Bound: HBM, rows · V values, for the first launch, latency for the second.  192 rows of 128256
+// bf16 logits, 16 wanted: 12.1 us (4.1 TB/s) + 15.8 us, of which 3 us are T, 4 us the groups' loads
+// and their candidates, 3.4 us the merge; 4 rows of 151936 f32 logits, 8 wanted: 3.4 + 8.6 us.  The
+// merge in a launch of its own: 5.5 us more.
 #include "../common.hpp"
 #include "../device.hpp"
 #include "../serve.hpp"
@@ -27,6 +30,7 @@ namespace {
 
 constexpr int R = 16, STEP = 64 * R;  // logits of a lane and of a wave at a time
 constexpr int MAX_GROUPS = 512;       // of a row: groups of 1024, 2048 or 4096 logits
+constexpr float FAST_M = 1 << 20;     // size of a maximum below which an exponent is one fma
 
 typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
@@ -82,13 +86,22 @@ __device__ __forceinline__ Run join(const Run &a, const Run &b) {
 }
 
 template <int TY>
-__global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int n_groups, int steps, int per, int n_parts, float *gmax, Run *runs) {
+__global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int n_groups, int steps, int per, int n_parts, float *gmax, Run *runs, int *arrived) {
     const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = id / n_parts, part = id - row * n_parts;
     if (row >= a.n * a.n_beams) return;
     const void *x = (const uint8_t *)a.x + row * a.ld * (TY == T_F32 ? 4 : 2);
     const int g0 = part * per, g1 = min(g0 + per, n_groups), u1 = min(g1 * steps, (a.V + STEP - 1) / STEP);
-    float M = -FLT_MAX, s = 0;  // the wave's maximum so far, and the lane's sum
+    // M is the wave's maximum so far, s the lane's sum.  fs is the sum of the steps since M moved, in
+    // log2 units against −c, where c = −M · log2 e rounded: one fma forms an exponent, and the rounding
+    // of c, r = M · log2 e + c exactly, is taken out of the sum when M moves or at the end (it holds
+    // 2^r times its own).  From |M| = 2^20 on, r could pass 2^-4: those take a subtraction.
+    float M = -FLT_MAX, s = 0, fs = 0, c = 0;
+    bool plain = true;
+    auto settle = [&] {
+        s = fmaf(fs, plain ? 1.0f : exp2_hw(-fmaf(M, LOG2E_F, c)), s);
+        fs = 0;
+    };
     float v[R], nx[R], g = -INFINITY;
     load_step<TY>(x, g0 * steps * STEP, a.V, lane, v);
     for (int u = g0 * steps; u < u1; u++) {
@@ -105,126 +118,244 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int n_groups
             g = -INFINITY;
         }
         if (mx > M) {
+            settle();
             s *= exp2_hw((M - mx) * LOG2E_F);
             M = mx;
+            plain = !(fabsf(M) < FAST_M);
+            c = plain ? 0.0f : -(M * LOG2E_F);
+        }
+        float e[R];
+        if (!plain) {
+#pragma unroll
+            for (int j = 0; j < R; j++) e[j] = exp2_hw(fmaf(v[j], LOG2E_F, c));
+        } else {
+#pragma unroll
+            for (int j = 0; j < R; j++) e[j] = exp2_hw((v[j] - M) * LOG2E_F);
         }
 #pragma unroll
-        for (int j = 0; j < R; j++) s += exp2_hw((v[j] - M) * LOG2E_F);
+        for (int o = R / 2; o; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < o; j++) e[j] += e[j + o];
+        fs += e[0];
 #pragma unroll
         for (int j = 0; j < R; j++) v[j] = nx[j];
     }
+    settle();
     s = xsum_f<64>(s);
     if (lane == 0) runs[(int64_t)row * n_parts + part] = Run{M, s};
+    if (part == 0 && lane == 0 && row % a.n_beams == 0) arrived[row / a.n_beams] = 0;
 }
 
 constexpr int CAND = 1024;  // logits that are ranked at once
 
-// A row's best k = min(n_out, V) tokens in order, with their sums: key[row][k], id[row][k]
+// Stores and loads that other XCDs' workgroups see, and are seen by
+__device__ __forceinline__ void put(double *p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Numbers in the order of the values, equal ones' lower index first
+__device__ __forceinline__ uint64_t ordered(float v, int index) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ int64_t ordered(double v) {
+    const int64_t b = __double_as_longlong(v + 0.0);
+    return b < 0 ? b ^ INT64_MAX : b;
+}
+
+// A row's best k = min(n_out, V) tokens in order, with their sums: key[row][k], id[row][k].
+//
+// A few thousand cycles of one workgroup, so what counts is what waits for what: all loads are
+// requested before anything is waited for; each wave finds the groups for itself, without a
+// barrier; barriers are LDS's only, so that loads pass them; and ranks are counted with one
+// comparison of whole numbers and an addition with its carry (masks of two comparisons joined in
+// scalar registers took 75 cycles a candidate).
 template <int TY>
-__global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a, int n_groups, int steps, int n_parts, const float *gmax, const Run *runs, double *key, int *id) {
+__device__ void best_of_row(const BeamArgs &a, int row, int n_groups, int steps, int n_parts, const float *gmax, const Run *runs, double *key, int *id) {
     __shared__ Run s_run[4];
-    __shared__ float s_val[CAND];
-    __shared__ int s_idx[CAND];
-    __shared__ float s_gmax[MAX_GROUPS];
-    __shared__ int s_group[BEAM_MAX_OUT];
-    __shared__ int s_n;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x;
+    __shared__ uint64_t s_cand[CAND];
+    __shared__ int s_group[4][BEAM_MAX_OUT];
+    __shared__ int s_n[4];  // candidates of each wave, in its quarter of the list
+    __shared__ float s_mine[256];
+    __shared__ float s_thr;
+    constexpr int PART = CAND / 4;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint64_t before = (1ull << lane) - 1;
     const void *x = (const uint8_t *)a.x + row * a.ld * (TY == T_F32 ? 4 : 2);
     const int k = min(a.n_out, a.V), kg = min(k, n_groups);
     key += (int64_t)row * k;
     id += (int64_t)row * k;
-    const float score = a.scores[row];
-    if (a.finished && a.finished[row]) {  // goes on as it is
-        for (int i = tid; i < k; i += 256) {
-            key[i] = i == 0 && fabsf(score) <= FLT_MAX ? (double)score : -INFINITY;
-            id[i] = a.pad;
-        }
-        return;
-    }
+    constexpr int NG = MAX_GROUPS / 64;
+    float own[NG];
+#pragma unroll
+    for (int i = 0; i < NG; i++) own[i] = lane + 64 * i < n_groups ? fmaxf(gmax[(int64_t)row * n_groups + lane + 64 * i], -INFINITY) : NAN;
     Run p{-FLT_MAX, 0};
     for (int i = tid; i < n_parts; i += 256) p = join(p, runs[(int64_t)row * n_parts + i]);
-    for (int i = tid; i < n_groups; i += 256) s_gmax[i] = gmax[(int64_t)row * n_groups + i];
+    const float score = a.scores[row];
+    const int finished = a.finished ? a.finished[row] : 0;
+
+    // T, the kg-th largest maximum: one value after the other, the largest first (NaN: no group)
+    float T = INFINITY;
+    for (int n = 0; n < kg;) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+            if (64 * i >= n_groups) break;
+            m = n == 0 || own[i] < T ? fmaxf(m, own[i]) : m;
+        }
+        T = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(xmax_f<64>(m))));
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+            if (64 * i >= n_groups) break;
+            n += (int)__popcll(__ballot(own[i] == T));
+        }
+    }
+    // the groups above it, and of those that equal it the first
+    int n_above = 0, n_equal = 0;
+#pragma unroll
+    for (int i = 0; i < NG; i++) {
+        if (64 * i >= n_groups) break;
+        n_above += (int)__popcll(__ballot(own[i] > T));
+    }
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < NG; i++) {
+        if (64 * i >= n_groups) break;
+        const uint64_t above = __ballot(own[i] > T), equal = __ballot(own[i] == T);
+        const int pa = at + (int)__popcll(above & before), pe = n_above + n_equal + (int)__popcll(equal & before);
+        if (own[i] > T) s_group[w][pa] = i * 64 + lane;
+        else if (own[i] == T && pe < kg) s_group[w][pe] = i * 64 + lane;
+        at += (int)__popcll(above);
+        n_equal += (int)__popcll(equal);
+    }
+    wave_sync();
+    // The logits of these from T on may be among the first k.  More than fit (few groups, or equal
+    // logits): those from the k-th largest of the threads' own maxima on.
+    constexpr int AT_ONCE = 4;  // steps that a wave reads at once
+    float v[AT_ONCE][R];
+    const int n_steps = kg * steps;
+    auto first_of = [&](int u) { return (s_group[w][u / steps] * steps + u % steps) * STEP; };
+    auto read = [&](int u0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < AT_ONCE; q++)
+            if (u0 + 4 * q < n_steps) load_step<TY>(x, first_of(u0 + 4 * q), a.V, lane, v[q]);
+    };
+    read(w);
+    // the row's sum meanwhile
 #pragma unroll
     for (int o = 32; o; o >>= 1) p = join(p, Run{__shfl_xor(p.m, o), __shfl_xor(p.s, o)});
     if (lane == 0) s_run[w] = p;
-    if (tid == 0) s_n = 0;
-    __syncthreads();
+    lds_barrier();
     p = join(join(s_run[0], s_run[1]), join(s_run[2], s_run[3]));
+    if (finished) {  // goes on as it is
+        for (int i = tid; i < k; i += 256) {
+            put(key + i, i == 0 && fabsf(score) <= FLT_MAX ? (double)score : -INFINITY);
+            put(id + i, a.pad);
+        }
+        return;
+    }
     if (!(p.s > 0) || !(p.m <= FLT_MAX) || !(fabsf(score) <= FLT_MAX)) {  // offers nothing
         for (int i = tid; i < k; i += 256) {
-            key[i] = -INFINITY;
-            id[i] = i;
+            put(key + i, -INFINITY);
+            put(id + i, i);
         }
         return;
     }
     const double log_s = log((double)p.s);
-    // the groups with the largest maxima, by counting those ahead of each
-    for (int i = tid; i < n_groups; i += 256) {
-        const float v = s_gmax[i];
-        int ahead = 0;
-#pragma unroll 8
-        for (int j = 0; j < n_groups; j++) ahead += (s_gmax[j] > v) | ((s_gmax[j] == v) & (j < i));
-        if (ahead < kg) s_group[ahead] = i;
-    }
-    __syncthreads();
-    // Their logits from the k-th largest group maximum on may be among the first k.  More than fit
-    // (few groups, or equal logits): those from the k-th largest of the threads' own maxima on.
-    float thr = kg < k ? -INFINITY : s_gmax[s_group[kg - 1]], mine = -INFINITY;
+    float thr = kg < k ? -FLT_MAX : fmaxf(T, -FLT_MAX), mine = -INFINITY;  // not those of −inf, nor what lies behind the row's end
+    int n = 0;
     for (int attempt = 0; attempt < 2; attempt++) {
-        for (int u = w; u < kg * steps; u += 4) {
-            float v[R];
-            const int e0 = (s_group[u / steps] * steps + u % steps) * STEP;
-            if (e0 >= a.V) continue;
-            load_step<TY>(x, e0, a.V, lane, v);
+        int found = 0;
+        for (int u0 = w; u0 < n_steps; u0 += 4 * AT_ONCE) {
+            if (attempt || u0 > w) read(u0);
+            uint64_t hits = 0;
 #pragma unroll
-            for (int j = 0; j < R; j++) {
-                mine = fmaxf(mine, v[j]);
-                if (!(v[j] >= thr) || v[j] == -INFINITY) continue;
-                const int c = atomicAdd(&s_n, 1);
-                if (c < CAND) {
-                    s_val[c] = v[j];
-                    s_idx[c] = e0 + place<TY>(lane, j);
+            for (int q = 0; q < AT_ONCE; q++) {
+                uint32_t h = 0;
+                if (u0 + 4 * q < n_steps) {
+#pragma unroll
+                    for (int j = 0; j < R; j++) {
+                        mine = fmaxf(mine, v[q][j]);
+                        h |= v[q][j] >= thr ? 1u << j : 0;
+                    }
                 }
+                hits |= (uint64_t)h << (16 * q);
+            }
+            while (__any(hits != 0)) {
+                const uint64_t some = __ballot(hits != 0);
+                const int c = found + (int)__popcll(some & before);
+                if (hits) {
+                    const int b = __builtin_ctzll(hits);
+                    if (c < PART) s_cand[w * PART + c] = (uint32_t)(first_of(u0 + b / 16 * 4) + place<TY>(lane, b % 16));
+                    hits &= hits - 1;
+                }
+                found += (int)__popcll(some);
             }
         }
-        __syncthreads();
-        if (s_n <= CAND || attempt) break;
-        __syncthreads();
-        s_val[tid] = mine;
-        if (tid == 0) s_n = 0;
-        __syncthreads();
+        if (lane == 0) s_n[w] = found;
+        lds_barrier();
+        n = s_n[0] + s_n[1] + s_n[2] + s_n[3];
+        if (max(max(s_n[0], s_n[1]), max(s_n[2], s_n[3])) > PART) n = CAND + 1;
+        if (n <= CAND || attempt) break;
+        s_mine[tid] = mine;
+        lds_barrier();
         int ahead = 0;
-        for (int j = 0; j < 256; j++) ahead += (s_val[j] > mine) | ((s_val[j] == mine) & (j < tid));
-        if (ahead == k - 1) s_val[256] = mine;
-        __syncthreads();
-        thr = s_val[256];
-        __syncthreads();
+        for (int j = 0; j < 256; j++) ahead += (s_mine[j] > mine) | ((s_mine[j] == mine) & (j < tid));
+        if (ahead == k - 1) s_thr = mine;
+        lds_barrier();
+        thr = fmaxf(s_thr, -FLT_MAX);
     }
-    const int n = s_n;
     if (n <= CAND) {
-        for (int i = tid; i < n; i += 256) {
-            const float v = s_val[i];
-            const int e = s_idx[i];
+        // candidates by number: the i-th lies in the wave's quarter that holds it
+        auto slot = [&](int i) {
+            int g = 0;
+            while (i >= s_n[g]) i -= s_n[g++];
+            return g * PART + i;
+        };
+        float mine_v[CAND / 256];
+        int mine_s[CAND / 256], mine_e[CAND / 256];
+#pragma unroll
+        for (int u = 0; u < CAND / 256; u++) {
+            const int i = tid + 256 * u;
+            mine_s[u] = mine_e[u] = 0;
+            if (i >= n) continue;
+            mine_s[u] = slot(i);
+            mine_e[u] = (int)(uint32_t)s_cand[mine_s[u]];
+            mine_v[u] = logit<TY>(x, mine_e[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < CAND / 256; u++) {
+            if (tid + 256 * u >= n) continue;
+            s_cand[mine_s[u]] = ordered(mine_v[u], mine_e[u]);
+        }
+        lds_barrier();
+#pragma unroll
+        for (int u = 0; u < CAND / 256; u++) {
+            if (256 * u >= n) break;
+            const bool on = tid + 256 * u < n;
+            const uint64_t me = on ? s_cand[mine_s[u]] : 0;
             int ahead = 0;
-#pragma unroll 8
-            for (int j = 0; j < n; j++) ahead += (s_val[j] > v) | ((s_val[j] == v) & (s_idx[j] < e));
-            if (ahead < k) {
-                key[ahead] = (double)score + (((double)v - (double)p.m) - log_s);
-                id[ahead] = e;
+            for (int g = 0; g < 4; g++) {
+                const int m = s_n[g];
+#pragma unroll 4
+                for (int j = 0; j < m; j++) ahead += s_cand[g * PART + j] > me;
+            }
+            if (on && ahead < k) {
+                put(key + ahead, (double)score + (((double)mine_v[u] - (double)p.m) - log_s));
+                put(id + ahead, mine_e[u]);
             }
         }
         if (n >= k) return;
         // the first of the logits of −inf: under k of the row's are none, so they lie in its first 2 k
         const bool out = tid < a.V && logit<TY>(x, tid) == -INFINITY;
         const uint64_t m = __ballot(out);
-        __syncthreads();
-        if (lane == 0) s_idx[w] = (int)__popcll(m);
-        __syncthreads();
-        int at = n + (int)__popcll(m & ((1ull << lane) - 1));
-        for (int i = 0; i < w; i++) at += s_idx[i];
-        if (out && at < k) {
-            key[at] = -INFINITY;
-            id[at] = tid;
+        lds_barrier();
+        if (lane == 0) s_n[w] = (int)__popcll(m);
+        lds_barrier();
+        int place_of = n + (int)__popcll(m & before);
+        for (int i = 0; i < w; i++) place_of += s_n[i];
+        if (out && place_of < k) {
+            put(key + place_of, -INFINITY);
+            put(id + place_of, tid);
         }
         return;
     }
@@ -235,7 +366,7 @@ __global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a, int n_groups,
         float bv = -INFINITY;
         int be = INT32_MAX;
         for (int i = tid; i < kg * steps * STEP; i += 256) {
-            const int e = s_group[i / (steps * STEP)] * steps * STEP + i % (steps * STEP);
+            const int e = s_group[w][i / (steps * STEP)] * steps * STEP + i % (steps * STEP);
             if (e >= a.V) continue;
             const float v = logit<TY>(x, e);
             if ((v < last || (v == last && e > last_e)) && (v > bv || (v == bv && e < be))) {
@@ -254,32 +385,72 @@ __global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a, int n_groups,
         }
         __syncthreads();
         if (lane == 0) {
-            s_val[w] = bv;
-            s_idx[w] = be;
+            s_mine[w] = bv;
+            s_n[w] = be;
         }
         __syncthreads();
         for (int i = 0; i < 4; i++)
-            if (s_val[i] > bv || (s_val[i] == bv && s_idx[i] < be)) {
-                bv = s_val[i];
-                be = s_idx[i];
+            if (s_mine[i] > bv || (s_mine[i] == bv && s_n[i] < be)) {
+                bv = s_mine[i];
+                be = s_n[i];
             }
         last = bv;
         last_e = be;
         if (tid == 0) {
-            key[r] = (double)score + (((double)bv - (double)p.m) - log_s);
-            id[r] = be;
+            put(key + r, (double)score + (((double)bv - (double)p.m) - log_s));
+            put(id + r, be);
         }
     }
 }
 
 // The rows of a request merged.  Each row's candidates are in order, so what is ahead of one in
 // another row is found by halving.
-__global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a, const double *key, const int *id) {
-    extern __shared__ double s_key[];
-    const int W = a.n_beams, k = min(a.n_out, a.V), n = W * k, req = blockIdx.x;
+__device__ void merge_rows(const BeamArgs &a, int req, const double *key, const int *id, double *s_key) {
+    const int W = a.n_beams, k = min(a.n_out, a.V), n = W * k;
     key += (int64_t)req * n;
     id += (int64_t)req * n;
-    for (int i = threadIdx.x; i < n; i += 256) s_key[i] = key[i];
+    auto chosen = [&](int i, int ahead, double v, int token) {
+        if (ahead >= a.n_out) return;
+        const int64_t o = (int64_t)req * a.n_out + ahead;
+        a.next[o] = (float)v;
+        a.parents[o] = req * W + i / k;
+        a.tokens[o] = token;
+    };
+    constexpr int FEW = 256;  // that are ranked by counting (24 requests of 8 beams and 16 candidates: by halving 4.7 us)
+    if (n <= FEW) {
+        __shared__ int s_ahead[FEW], s_at[BEAM_MAX_OUT], s_tie;
+        int64_t *s_ord = (int64_t *)s_key;
+        const int i = threadIdx.x, at = i < n ? i : 0;
+        const double v = __hip_atomic_load(key + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int token = __hip_atomic_load(id + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_ahead[i] = 0;
+        if (i < n) s_ord[i] = ordered(v);
+        if (i == 0) s_tie = 0;
+        lds_barrier();
+        // as many threads to a candidate as there are, each with a share of the others
+        const int per = n <= FEW / 4 ? 4 : n <= FEW / 2 ? 2 : 1, c = i / per, share = (n + per - 1) / per, from = i % per * share, to = min(from + share, n);
+        if (c < n) {
+            const int64_t me = s_ord[c];
+            int ahead = 0;
+#pragma unroll 4
+            for (int j = from; j < to; j++) ahead += s_ord[j] > me;
+            atomicAdd(s_ahead + c, ahead);
+        }
+        lds_barrier();
+        // equal ones have one place: their order is that of the candidates
+        int ahead = i < n ? s_ahead[i] : a.n_out;
+        if (ahead < a.n_out) s_at[ahead] = i;
+        lds_barrier();
+        if (ahead < a.n_out && s_at[ahead] != i) s_tie = 1;
+        lds_barrier();
+        if (s_tie && i < n) {
+            const int64_t me = s_ord[i];
+            for (int j = 0; j < i; j++) ahead += s_ord[j] == me;
+        }
+        if (i < n) chosen(i, ahead, v, token);
+        return;
+    }
+    for (int i = threadIdx.x; i < n; i += 256) s_key[i] = __hip_atomic_load(key + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += 256) {
         const int b = i / k;
@@ -296,12 +467,23 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a, const double
             }
             ahead += lo;
         }
-        if (ahead >= a.n_out) continue;
-        const int64_t o = (int64_t)req * a.n_out + ahead;
-        a.next[o] = (float)v;
-        a.parents[o] = req * W + b;
-        a.tokens[o] = id[i];
+        chosen(i, ahead, v, __hip_atomic_load(id + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     }
+}
+
+// A workgroup for each row; the one of a request that is done last merges them.  Rows are passed on
+// through atomic stores and loads, and counted when their stores have completed.
+template <int TY>
+__global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a, int n_groups, int steps, int n_parts, const float *gmax, const Run *runs, double *key, int *id, int *arrived) {
+    extern __shared__ double s_key[];
+    __shared__ int s_last;
+    const int row = blockIdx.x, req = row / a.n_beams;
+    best_of_row<TY>(a, row, n_groups, steps, n_parts, gmax, runs, key, id);
+    wait_vmem();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = __hip_atomic_fetch_add(arrived + req, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.n_beams - 1;
+    __syncthreads();
+    if (s_last) merge_rows(a, req, key, id, s_key);
 }
 
 struct BeamPlan {
@@ -313,7 +495,7 @@ BeamPlan beam_plan(int rows, int V) {
     p.steps = (n + MAX_GROUPS - 1) / MAX_GROUPS;
     p.n_groups = (n + p.steps - 1) / p.steps;
     // groups per wave: enough waves to fill the card, and long runs beyond that
-    p.per = (int)std::clamp<int64_t>((int64_t)rows * p.n_groups / 8192, 1, 32);
+    p.per = (int)std::clamp<int64_t>(((int64_t)rows * p.n_groups + 8191) / 8192, 1, 32);
     p.n_parts = (p.n_groups + p.per - 1) / p.per;
     return p;
 }
@@ -332,9 +514,10 @@ void launch_ty(const BeamArgs &a, void *ws, hipStream_t st) {
     Run *runs = (Run *)w;
     w += up16((size_t)rows * p.n_parts * sizeof(Run));
     float *gmax = (float *)w;
-    beam_part_kernel<TY><<<(int)(((int64_t)rows * p.n_parts + 3) / 4), 256, 0, st>>>(a, p.n_groups, p.steps, p.per, p.n_parts, gmax, runs);
-    beam_row_kernel<TY><<<rows, 256, 0, st>>>(a, p.n_groups, p.steps, p.n_parts, gmax, runs, key, id);
-    beam_join_kernel<<<a.n, 256, (size_t)a.n_beams * k * sizeof(double), st>>>(a, key, id);
+    w += up16((size_t)rows * p.n_groups * sizeof(float));
+    int *arrived = (int *)w;
+    beam_part_kernel<TY><<<(int)(((int64_t)rows * p.n_parts + 3) / 4), 256, 0, st>>>(a, p.n_groups, p.steps, p.per, p.n_parts, gmax, runs, arrived);
+    beam_row_kernel<TY><<<rows, 256, (size_t)a.n_beams * k * sizeof(double), st>>>(a, p.n_groups, p.steps, p.n_parts, gmax, runs, key, id, arrived);
 }
 
 }  // namespace
@@ -343,7 +526,7 @@ size_t beam_ws(int n, int n_beams, int V, int n_out) {
     const int64_t rows = (int64_t)n * n_beams;
     const int k = std::min(n_out, V);
     const BeamPlan p = beam_plan((int)rows, V);
-    return up16(rows * k * sizeof(double)) + up16(rows * k * sizeof(int)) + up16(rows * p.n_parts * sizeof(Run)) + up16(rows * p.n_groups * sizeof(float));
+    return up16(rows * k * sizeof(double)) + up16(rows * k * sizeof(int)) + up16(rows * p.n_parts * sizeof(Run)) + up16(rows * p.n_groups * sizeof(float)) + up16(n * sizeof(int));
 }
 
 void launch_beam(const BeamArgs &a, void *ws, hipStream_t st) {

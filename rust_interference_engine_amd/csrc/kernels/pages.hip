@@ -13,7 +13,11 @@
 // through refs 16 to a thread (16384 to a round), and leaves lists in the workspace.  Tables and
 // pages are changed by a second and third launch over the whole card.
 //
-// Bound: for many or large pages HBM, every moved byte read and written once; else the launches.
+// Bound: for many or large pages HBM, every moved byte read and written once; else the launches
+// and what the planning workgroup waits for.  24 searches of 8 beams forked, 44 MB read and written:
+// 6.9 us to plan (loads requested before anything waits; state kept in registers over the steps;
+// 9.5 before), 10 us for references and copies in one launch (13 in two), 3 us for the rows.  A pool
+// of 120000 positions compacted, 430 MB read and written: 7 + 90 us (4.8 TB/s).
 #include "../common.hpp"
 #include "../device.hpp"
 #include "../serve.hpp"
@@ -69,12 +73,17 @@ __device__ __forceinline__ uint32_t free_of(const int *refs, int p0, int n_pages
     return bits;
 }
 
-// The free pages with the lowest numbers, up to `want`, in order into list; how many there are.  All threads call this.
-__device__ int find_free(const PoolView &p, int want, int *list, int *s) {
+// The free pages with the lowest numbers, up to `want`, in order into list; how many there are.  All
+// threads call this; bits0: of the first round, which callers read while they find out what they want.
+__device__ __forceinline__ uint32_t free_in_round(const PoolView &p, int p0) {
+    const int mine = p0 + (int)threadIdx.x * PER;
+    return mine < p.n_pages ? free_of(p.refs, mine, p.n_pages) : 0;
+}
+__device__ __forceinline__ int find_free(const PoolView &p, uint32_t bits0, int want, int *list, int *s) {
     int found = 0;
     for (int p0 = 0; p0 < p.n_pages && found < want; p0 += PLAN * PER) {
         const int mine = p0 + (int)threadIdx.x * PER;
-        uint32_t bits = mine < p.n_pages ? free_of(p.refs, mine, p.n_pages) : 0;
+        uint32_t bits = p0 ? free_in_round(p, p0) : bits0;
         int total, at = found + scan(__popc(bits), s, total);
         for (; bits && at < want; bits &= bits - 1) list[at++] = mine + __builtin_ctz(bits);
         found += total;
@@ -94,6 +103,7 @@ __device__ __forceinline__ Seq seq_of(const PoolView &p, int i) {
 __global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
     __shared__ int s[PLAN / 64];
     __shared__ int s_at[POOL_MAX_SEQ + 1];  // pages that the rows before need, up to all there are
+    const uint32_t bits0 = free_in_round(p, 0);
     int64_t want = 0;
     for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
         const int i = i0 + (int)threadIdx.x;
@@ -108,7 +118,7 @@ __global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
     }
     const int most = (int)min(want, (int64_t)p.n_pages);
     if (threadIdx.x == 0) s_at[p.n_seq] = most;
-    const int found = find_free(p, most, list, s);
+    const int found = find_free(p, bits0, most, list, s);
     __syncthreads();
     for (int j = threadIdx.x; j < found; j += PLAN) {
         int lo = 0, hi = p.n_seq;  // the last row that begins at or before j
@@ -133,8 +143,8 @@ __global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
 
 // ---- fork ----
 struct Child {  // what becomes of a row
-    int src, keep, held, old_held, len, fresh;  // keep: it takes the source's pages as they are; fresh: the page in the place of the source's partial one, or −1
-    int at;                                     // that place (−1: none)
+    int src, held, old_held, len;
+    int at, fresh;  // place of the source's partial page where the row gets a copy of it (−1: none), and that copy (−1: the pool has none)
 };
 struct Lists {
     int n;  // pages to copy
@@ -142,88 +152,78 @@ struct Lists {
 };
 
 __global__ __launch_bounds__(PLAN) void fork_plan_kernel(PoolView p, const int *src, Lists *lists, Child *child, int *children, int *from, int *to, int *list) {
-    extern __shared__ int s_row[];  // children of a row, and which of them inherits its partial page
+    __shared__ int s_count[POOL_MAX_SEQ], s_heir[POOL_MAX_SEQ];  // children of a row, and which of them inherits its partial page
     __shared__ int s[PLAN / 64];
-    int *count = s_row, *heir = s_row + p.n_seq;
-    for (int i = threadIdx.x; i < p.n_seq; i += PLAN) {
-        count[i] = 0;
-        heir[i] = INT32_MAX;
+    constexpr int ROUNDS = POOL_MAX_SEQ / PLAN;
+    const uint32_t bits0 = free_in_round(p, 0);
+    int r[ROUNDS];
+#pragma unroll
+    for (int u = 0; u < ROUNDS; u++) {
+        const int i = u * PLAN + (int)threadIdx.x;
+        r[u] = i < p.n_seq ? src[i] : -1;
+        r[u] = (unsigned)r[u] < (unsigned)p.n_seq ? r[u] : -1;
+        s_count[i] = 0;
+        s_heir[i] = INT32_MAX;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.n_seq; i += PLAN) {
-        const int r = src[i];
-        if ((unsigned)r >= (unsigned)p.n_seq) continue;
-        atomicAdd(count + r, 1);
-        atomicMin(heir + r, r == i ? -1 : i);  // the row itself, or its first child
+#pragma unroll
+    for (int u = 0; u < ROUNDS; u++) {
+        const int i = u * PLAN + (int)threadIdx.x;
+        if (r[u] < 0) continue;
+        atomicAdd(s_count + r[u], 1);
+        atomicMin(s_heir + r[u], r[u] == i ? -1 : i);  // the row itself, or its first child
     }
     __syncthreads();
-    int want = 0;
-    for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
-        const int i = i0 + (int)threadIdx.x;
-        int need = 0, total;
+    int want = 0, copies = 0;
+    Child c[ROUNDS];
+    int old[ROUNDS], mine[ROUNDS];  // the source's partial page; which of the new ones goes in its place
+#pragma unroll
+    for (int u = 0; u < ROUNDS; u++) {
+        const int i = u * PLAN + (int)threadIdx.x;
+        c[u] = Child{r[u], 0, 0, 0, -1, -1};
+        old[u] = -1;
+        if (u * PLAN >= p.n_seq) continue;
         if (i < p.n_seq) {
-            const int r = src[i];
-            Child c;
-            c.src = (unsigned)r < (unsigned)p.n_seq ? r : -1;
-            c.keep = c.src >= 0 && (r == i || heir[r] == i);
-            c.old_held = seq_of(p, i).held;
-            c.fresh = c.at = -1;
-            c.held = c.len = 0;
-            if (c.src >= 0) {
-                const Seq q = seq_of(p, r);
-                c.held = c.keep ? q.held : min(q.touched, q.held);
-                c.len = p.lens[r];
-                if (!c.keep && q.touched > q.full && q.held > q.full) c.at = q.full;
-            }
-            need = c.at >= 0;
-            child[i] = c;
-            children[i] = count[i];
+            children[i] = s_count[i];
+            c[u].old_held = seq_of(p, i).held;
         }
-        scan(need, s, total);
+        if (r[u] >= 0) {
+            const Seq q = seq_of(p, r[u]);
+            const bool keep = r[u] == i || s_heir[r[u]] == i;  // it takes the source's pages as they are
+            c[u].held = keep ? q.held : min(q.touched, q.held);
+            c[u].len = p.lens[r[u]];
+            if (!keep && q.touched > q.full && q.held > q.full) {
+                c[u].at = q.full;
+                old[u] = p.table[r[u] * p.table_stride + q.full];
+            }
+        }
+        int total;
+        mine[u] = want + scan(c[u].at >= 0, s, total);
         want += total;
     }
-    const int found = find_free(p, want, list, s);
+    const int found = find_free(p, bits0, want, list, s);
     __syncthreads();
-    int at = 0, copies = 0;
-    for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
-        const int i = i0 + (int)threadIdx.x;
-        const int place = i < p.n_seq ? child[i].at : -1;
-        int total;
-        const int mine = at + scan(place >= 0, s, total);
-        bool copy = false;
-        int page = -1, old = -1;
-        if (place >= 0 && mine < found) {
-            page = list[mine];
-            old = p.table[child[i].src * p.table_stride + place];
-            copy = (unsigned)old < (unsigned)p.n_pages;
-            child[i].fresh = page;
-            p.refs[page] = 1;
+#pragma unroll
+    for (int u = 0; u < ROUNDS; u++) {
+        const int i = u * PLAN + (int)threadIdx.x;
+        if (u * PLAN >= p.n_seq) break;
+        if (c[u].at >= 0 && mine[u] < found) {
+            c[u].fresh = list[mine[u]];
+            p.refs[c[u].fresh] = 1;
         }
-        at += total;
-        const int c = copies + scan(copy, s, total);
+        const bool copy = c[u].fresh >= 0 && (unsigned)old[u] < (unsigned)p.n_pages;
+        int total;
+        const int k = copies + scan(copy, s, total);
         if (copy) {
-            from[c] = old;
-            to[c] = page;
+            from[k] = old[u];
+            to[k] = c[u].fresh;
         }
         copies += total;
+        if (i < p.n_seq) child[i] = c[u];
     }
     if (threadIdx.x == 0) {
         lists->n = copies;
         p.counts[0] = want - found;
-    }
-}
-
-// The old rows' references, and the rows that others go on from into `rows`
-__global__ __launch_bounds__(256) void fork_refs_kernel(PoolView p, const int *src, const int *children, int *rows) {
-    const int r = blockIdx.x, n = children[r];
-    const bool stays = (unsigned)src[r] < (unsigned)p.n_seq && src[r] == r;
-    if (n == 1 && stays) return;
-    const Seq q = seq_of(p, r);
-    const int *t = p.table + r * p.table_stride;
-    for (int c = threadIdx.x; c < q.held; c += 256) {
-        const int page = t[c], change = c < q.full ? n - 1 : n == 0 ? -1 : 0;
-        if (n) rows[(int64_t)r * p.cols + c] = page;
-        if (change && (unsigned)page < (unsigned)p.n_pages) atomicAdd(p.refs + page, change);
     }
 }
 
@@ -256,12 +256,26 @@ __device__ void copy_pages(const Bufs &bufs, int g, int n, const int *from, cons
     }
 }
 
-// The new rows, a workgroup each, and the copies
-__global__ __launch_bounds__(256) void fork_rows_kernel(PoolView p, Bufs bufs, int row_wgs, const Lists *lists, const Child *child, const int *from, const int *to, const int *rows) {
+// The old rows' references, and the rows that others go on from into `rows`, a workgroup each; and the copies
+__global__ __launch_bounds__(256) void fork_refs_kernel(PoolView p, Bufs bufs, int row_wgs, const Lists *lists, const int *src, const int *children, const int *from, const int *to, int *rows) {
     if ((int)blockIdx.x >= row_wgs) {
         copy_pages(bufs, blockIdx.x - row_wgs, gridDim.x - row_wgs, from, to, lists->n, p.n_pages);
         return;
     }
+    const int r = blockIdx.x, n = children[r];
+    const bool stays = (unsigned)src[r] < (unsigned)p.n_seq && src[r] == r;
+    if (n == 1 && stays) return;
+    const Seq q = seq_of(p, r);
+    const int *t = p.table + r * p.table_stride;
+    for (int c = threadIdx.x; c < q.held; c += 256) {
+        const int page = t[c], change = c < q.full ? n - 1 : n == 0 ? -1 : 0;
+        if (n) rows[(int64_t)r * p.cols + c] = page;
+        if (change && (unsigned)page < (unsigned)p.n_pages) atomicAdd(p.refs + page, change);
+    }
+}
+
+// The new rows, a workgroup each
+__global__ __launch_bounds__(256) void fork_rows_kernel(PoolView p, const Child *child, const int *rows) {
     const int i = blockIdx.x;
     const Child c = child[i];
     if (c.src == i) return;  // and keeps its pages
@@ -385,14 +399,14 @@ void launch_page_fork(const PoolView &p, const int *src, const PageBuf *bufs, in
         w += up16(p.n_seq * sizeof(int));
     }
     int *rows = (int *)w;
-    fork_plan_kernel<<<1, PLAN, 2 * p.n_seq * sizeof(int), st>>>(p, src, lists, child, ints[0], ints[1], ints[2], ints[3]);
-    fork_refs_kernel<<<p.n_seq, 256, 0, st>>>(p, src, ints[0], rows);
+    fork_plan_kernel<<<1, PLAN, 0, st>>>(p, src, lists, child, ints[0], ints[1], ints[2], ints[3]);
     int done = 0;
     do {
         const int n = std::min(n_bufs - done, MAX_BUFS), row_wgs = done ? 0 : p.n_seq;
-        fork_rows_kernel<<<row_wgs + (n ? COPY_WGS : 0), 256, 0, st>>>(p, bufs_of(bufs + done, n), row_wgs, lists, child, ints[1], ints[2], rows);
+        fork_refs_kernel<<<row_wgs + (n ? COPY_WGS : 0), 256, 0, st>>>(p, bufs_of(bufs + done, n), row_wgs, lists, src, ints[0], ints[1], ints[2], rows);
         done += n;
     } while (done < n_bufs);
+    fork_rows_kernel<<<p.n_seq, 256, 0, st>>>(p, child, rows);
 }
 
 void launch_page_free(const PoolView &p, const int *which, hipStream_t st) { free_kernel<<<p.n_seq, 256, 0, st>>>(p, which); }
