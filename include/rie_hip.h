@@ -218,8 +218,8 @@ int32_t rie_hip_k_argmax(const float *x, int32_t n, uint32_t *out_idx);
 int32_t rie_hip_k_argmax_noalloc(const float *x, int32_t n, uint32_t *out_idx, void *stream, char *err, size_t err_len);
 
 /* ---- batched serving: a cache of pages, attention over it and over packed prompts,
- * token log probabilities, rotary positions, beam selection, pools of pages.  No counterpart in the reference, whose backends hold one
- * sequence each.  Everything but the structs themselves is device memory; nothing of it
+ * token log probabilities, rotary positions, beam selection, pools of pages.  No counterpart
+ * in the reference, whose backends hold one sequence each.  Everything but the structs themselves is device memory; nothing of it
  * is read by the host, so a call can be captured into a graph and replayed over new
  * contents.
  *
@@ -301,8 +301,8 @@ int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs
  * and a value is its code times the scale of its block: `block` positions of a page (a power of
  * two, 16 to page_size) of one head, at page*scale_page_stride + (slot/block)*scale_block_stride
  * + head*scale_head_stride of k_scale and of v_scale (f32; strides up to 2^31-1).  Alignments and
- * the limits of the codes' strides are those of bytes.  A scale is 0 (of zeros), NaN, or 2^-60 to 2^50; others count as the nearest
- * of these bounds. */
+ * the limits of the codes' strides are those of bytes.  A scale is 0 (of zeros), NaN, or 2^-60 to
+ * 2^50; others count as the nearest of these bounds. */
 typedef struct rie_hip_pages8 {
     rie_hip_pages pages;
     float *k_scale, *v_scale;
@@ -323,7 +323,8 @@ int32_t rie_hip_k_paged_append8(const rie_hip_pages8 *pages, const rie_hip_seqs 
 /* Causal attention over such pages, of queries and to outputs of type ty (f16 or bf16).  A token
  * that sees a position of a block whose scale is NaN gets NaN for the heads that read it.  With
  * up to 32 query rows to a KV head only the output is rounded; with more, so is each
- * probability, to f16 (2-norm against float64: see the rules for 16-bit pages, f16's for both types). */
+ * probability, to f16 (2-norm against float64: see the rules for 16-bit pages, f16's for both
+ * types). */
 size_t rie_hip_k_paged_attention8_ws(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t ty, const rie_hip_attn *attn);
 int32_t rie_hip_k_paged_attention8(const rie_hip_pages8 *pages, const rie_hip_seqs *seqs, int32_t ty, const rie_hip_attn *attn, void *ws,
                                    size_t ws_bytes, void *stream, char *err, size_t err_len);
@@ -351,7 +352,8 @@ int32_t rie_hip_k_token_logprobs(int32_t ty, const void *logits, int32_t n, int3
  * magnitude; the values behind are copied.  Row r's position is positions[r], or, with seqs, that
  * of its token (rows outside the sequences are neither read nor written).  Any 32-bit position;
  * angles keep their digits.  n_q heads of q and n_k of k, of src_ty to dst_ty (f32, f16 or bf16,
- * rounded to nearest once); q_out may be q and k_out k, of the same strides and type.  head_dim: 2
+ * rounded to nearest once); q_out may be q and k_out k, of the same strides and type, and outputs
+ * overlap nothing else.  head_dim: 2
  * to 1024; rows of any alignment of their type (16-byte aligned ones, with dims a multiple of 16
  * and head_dim of 8, are read faster).  Strides up to 2^40. */
 typedef struct rie_hip_rotary {
@@ -378,7 +380,8 @@ int32_t rie_hip_k_rotary(const rie_hip_rotary *rotary, const rie_hip_seqs *seqs,
  * sum) and rounded once.  A beam with finished[row] != 0 (finished may be NULL) goes on as it is:
  * its one candidate is the token pad with its own score.  A beam whose score is not finite, or
  * whose row has a NaN or +inf logit or nothing above −inf, offers nothing; where a request has too
- * few candidates the sums of the others are −inf.  n_beams ≤ 64, n_out ≤ 128, n_vocab ≤ 2^21. */
+ * few candidates the sums of the others are −inf.  No output may overlap an input.  n_beams ≤ 64,
+ * n_out ≤ 128, n_vocab ≤ 2^21. */
 size_t rie_hip_k_beam_select_ws(int32_t n, int32_t n_beams, int32_t n_vocab, int32_t n_out);
 int32_t rie_hip_k_beam_select(int32_t ty, const void *logits, int32_t n, int32_t n_beams, int32_t n_vocab, int64_t row_stride,
                               const float *scores, const int32_t *finished, int32_t pad, int32_t n_out, float *next_scores,

@@ -177,24 +177,22 @@ class PagedKv:
         _need(k.shape[3] == 1 or k.stride(3) == 1, "pages: a row's values have to be consecutive")
         _ints(table, "table", 2)
         _need(table.numel() > 0, "table is empty")
-        self.device = _device(k, v, table)
-        self.k, self.v, self.table = k, v, table
         n_pages, page, n_kv, hd = k.shape
-        self.k_scale, self.v_scale = k_scale, v_scale
         self.bits8 = k.dtype == torch.int8
-        _need((k_scale is not None) == (v_scale is not None) == self.bits8, "int8 pages, and no others, have k_scale and v_scale")
+        scales = [s for s in (k_scale, v_scale) if s is not None]
+        _need(len(scales) == 2 * self.bits8, "int8 pages, and no others, have k_scale and v_scale")
+        blocks = 0
+        if self.bits8:
+            blocks = k_scale.shape[1] if k_scale.dim() == 3 else 0
+            _need(k_scale.dtype == v_scale.dtype == torch.float32, f"scales are {k_scale.dtype} and {v_scale.dtype}: f32 is wanted")
+            _need(k_scale.shape == v_scale.shape == (n_pages, blocks, n_kv) and blocks > 0 and page % blocks == 0,
+                  f"scales have to be [{n_pages} pages, blocks of a page, {n_kv} KV heads], got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
+            _need(_strides(k_scale) == _strides(v_scale), "k_scale and v_scale have to have the same strides")
+        self.device = _device(k, v, table, *scales)
+        self.k, self.v, self.table, self.k_scale, self.v_scale = k, v, table, k_scale, v_scale
         pages = _lib.Pages(_I8 if self.bits8 else _type(k, "pages"), hd, n_kv, n_pages, page, table.shape[1], k.data_ptr(), v.data_ptr(),
                            k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), table.stride(0))
-        if not self.bits8:
-            self._struct = pages
-            return
-        _device(k, k_scale, v_scale)
-        blocks = k_scale.shape[1] if k_scale.dim() == 3 else 0
-        _need(k_scale.dtype == v_scale.dtype == torch.float32, f"scales are {k_scale.dtype} and {v_scale.dtype}: f32 is wanted")
-        _need(k_scale.shape == v_scale.shape == (n_pages, blocks, n_kv) and blocks > 0 and page % blocks == 0,
-              f"scales have to be [{n_pages} pages, blocks of a page, {n_kv} KV heads], got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
-        _need(_strides(k_scale) == _strides(v_scale), "k_scale and v_scale have to have the same strides")
-        self._struct = _lib.Pages8(pages, k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), k_scale.stride(1), k_scale.stride(2), page // blocks)
+        self._struct = _lib.Pages8(pages, k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), page // blocks) if self.bits8 else pages
 
 
 def _check_seqs(seqs: Seqs, table: torch.Tensor | None) -> None:
