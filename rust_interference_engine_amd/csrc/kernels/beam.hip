@@ -14,9 +14,9 @@
 // bit too often, and their order that of the roundings.  ln Σ is f64 of an f32 sum (2^-22 of it).
 //
 // Bound: HBM, rows · V values, for the first launch, latency for the second.  192 rows of 128256
-// bf16 logits, 16 wanted: 12.1 us (4.1 TB/s) + 15.8 us, of which 3 us are T, 4 us the groups' loads
-// and their candidates, 3.4 us the merge; 4 rows of 151936 f32 logits, 8 wanted: 3.4 + 8.6 us.  The
-// merge in a launch of its own: 5.5 us more.
+// bf16 logits, 16 wanted: 12.1 us (4.1 TB/s) + 14.7 us, of which 2.5 us wait for the groups'
+// maxima, 4 us are the groups' loads and their candidates, 3.4 us the merge; 4 rows of 151936 f32
+// logits, 8 wanted: 3.3 + 8.3 us.  The merge in a launch of its own: 5.5 us more.
 #include "../common.hpp"
 #include "../device.hpp"
 #include "../serve.hpp"
@@ -193,20 +193,44 @@ __device__ void best_of_row(const BeamArgs &a, int row, int n_groups, int steps,
     const float score = a.scores[row];
     const int finished = a.finished ? a.finished[row] : 0;
 
-    // T, the kg-th largest maximum: one value after the other, the largest first (NaN: no group)
-    float T = INFINITY;
-    for (int n = 0; n < kg;) {
-        float m = -INFINITY;
+    // T, from which on a group is taken: at most the kg-th largest maximum, so that at least kg are.
+    // That of the lanes' own largest maxima, found by counting; with more to come, or too many equal
+    // ones, the kg-th largest maximum itself, one value after the other, the largest first (16 of
+    // them 2.4 us, the counts 0.5).  NaN: no group.
+    float T = -INFINITY;
+    int sel = MAX_GROUPS;
+    if (kg <= 64) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NG; i++) most = fmaxf(most, own[i]);
+        int ahead = 0;
+#pragma unroll
+        for (int j = 0; j < 64; j++) ahead += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(most), j)) > most;
+        T = -xmax_f<64>(ahead < kg ? -most : -INFINITY);
+        T = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(T)));
+        sel = 0;
 #pragma unroll
         for (int i = 0; i < NG; i++) {
             if (64 * i >= n_groups) break;
-            m = n == 0 || own[i] < T ? fmaxf(m, own[i]) : m;
+            sel += (int)__popcll(__ballot(own[i] >= T));
         }
-        T = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(xmax_f<64>(m))));
+    }
+    if (sel > BEAM_MAX_OUT) {
+        sel = kg;
+        T = INFINITY;
+        for (int n = 0; n < kg;) {
+            float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NG; i++) {
-            if (64 * i >= n_groups) break;
-            n += (int)__popcll(__ballot(own[i] == T));
+            for (int i = 0; i < NG; i++) {
+                if (64 * i >= n_groups) break;
+                m = n == 0 || own[i] < T ? fmaxf(m, own[i]) : m;
+            }
+            T = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(xmax_f<64>(m))));
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                if (64 * i >= n_groups) break;
+                n += (int)__popcll(__ballot(own[i] == T));
+            }
         }
     }
     // the groups above it, and of those that equal it the first
@@ -223,7 +247,7 @@ __device__ void best_of_row(const BeamArgs &a, int row, int n_groups, int steps,
         const uint64_t above = __ballot(own[i] > T), equal = __ballot(own[i] == T);
         const int pa = at + (int)__popcll(above & before), pe = n_above + n_equal + (int)__popcll(equal & before);
         if (own[i] > T) s_group[w][pa] = i * 64 + lane;
-        else if (own[i] == T && pe < kg) s_group[w][pe] = i * 64 + lane;
+        else if (own[i] == T && pe < sel) s_group[w][pe] = i * 64 + lane;
         at += (int)__popcll(above);
         n_equal += (int)__popcll(equal);
     }
@@ -232,7 +256,7 @@ __device__ void best_of_row(const BeamArgs &a, int row, int n_groups, int steps,
     // logits): those from the k-th largest of the threads' own maxima on.
     constexpr int AT_ONCE = 4;  // steps that a wave reads at once
     float v[AT_ONCE][R];
-    const int n_steps = kg * steps;
+    const int n_steps = sel * steps;
     auto first_of = [&](int u) { return (s_group[w][u / steps] * steps + u % steps) * STEP; };
     auto read = [&](int u0) __attribute__((always_inline)) {
 #pragma unroll
@@ -365,7 +389,7 @@ __device__ void best_of_row(const BeamArgs &a, int row, int n_groups, int steps,
     for (int r = 0; r < k; r++) {
         float bv = -INFINITY;
         int be = INT32_MAX;
-        for (int i = tid; i < kg * steps * STEP; i += 256) {
+        for (int i = tid; i < sel * steps * STEP; i += 256) {
             const int e = s_group[w][i / (steps * STEP)] * steps * STEP + i % (steps * STEP);
             if (e >= a.V) continue;
             const float v = logit<TY>(x, e);
