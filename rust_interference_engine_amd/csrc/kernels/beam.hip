@@ -16,7 +16,7 @@
 // Bound: HBM, rows · V values, for the first launch, latency for the second.  192 rows of 128256
 // bf16 logits, 16 wanted: 12.1 us (4.1 TB/s) + 14.7 us, of which 2.5 us wait for the groups'
 // maxima, 4 us are the groups' loads and their candidates, 3.4 us the merge; 4 rows of 151936 f32
-// logits, 8 wanted: 3.3 + 8.3 us.  The merge in a launch of its own: 5.5 us more.
+// logits, 4 wanted: 3.3 + 8.3 us.  The merge in a launch of its own: 5.5 us more.
 #include "../common.hpp"
 #include "../device.hpp"
 #include "../serve.hpp"

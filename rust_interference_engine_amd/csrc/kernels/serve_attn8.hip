@@ -62,6 +62,13 @@ constexpr float P_SHIFT8 = 6.0f;  // p · s_v is 2^(exponent − m + P_SHIFT8): 
 // waves' results are added up at the end.  Keys meet the query's 8-bit parts on integer matrix
 // instructions as they are; values are read transposed, 8 positions of a dim to a lane, and made
 // f16 there, 10 vector instructions for 8 values.
+//
+// Bound: HBM while all workgroups stream (6.4 TB/s by timestamps), and their beginnings: starts,
+// page ids, scales and the first tile lie behind one another, 8 us until a workgroup's first tile
+// is there.  So the positions are divided into about four rounds of workgroups, whose beginnings
+// pass while others stream.  48 tokens over up to 4000 positions, 32/8 heads of 128 (149 MB) 41 us
+// (3.6 TB/s) and 7 for the join, 1 over 100003 positions, 32/4 of 128 (103 MB) 22 and 5.5; in equal
+// pieces, as many as workgroups run at a time, 43.5 and 5.9, 29 and 8.7: all begin at once.
 constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT;
 template <int HD, int NB>
 constexpr int FEW8_WAVES = NB == 1 ? (HD <= 128 ? 4 : 2) : (HD <= 64 ? 3 : HD <= 128 ? 2 : 1);  // of a SIMD, as registers allow
@@ -381,9 +388,14 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
 //
 // The schedule is that of the 16-bit tile kernel: a tile's work is cut into groups of 32
 // positions, and the probabilities of group h are made while the matrix units form the outputs of
-// h − 1 and the scores of h + 1.  A tile lies in LDS in f16, which its four waves share: codes come
+// h − 1 and the scores of h + 1.  A tile lies in LDS in f16, which its waves share: codes come
 // to registers a tile ahead, each wave's 16 (8) rows, and are made f16 on their way to LDS (5
 // vector instructions for 4 values), in the place of a tile that has been read by then.
+//
+// Bound: a SIMD's matrix and vector instructions, which hardly overlap: of a wave's tile of 64
+// positions, head size 128, 1024 cycles are matrix products and about 1100 vector work (exponentials
+// alone 512, codes 160).  Eight waves to a tile (256 rows) where there are so many, since then
+// each makes half as many codes: 215 us with four, 185 with eight (13 sequences, see below).
 template <int HD>
 constexpr int TILE8_KT = HD <= 128 ? 64 : 32;
 
@@ -996,6 +1008,11 @@ __global__ __launch_bounds__(256) void tile8_join_kernel(ServeAttnArgs a, int KT
 // and the new ones.  Codes are rounded from f64 quotients, so that they are those of the formula.
 // Blocks are numbered without a list: sequence i owns ids from ⌊start / block⌋ + 2 i on, which
 // are enough, since n new tokens touch at most ⌊n / block⌋ + 2 blocks.
+//
+// Bound: loads behind one another (the sequence, the rows, the page and scale meanwhile), and for
+// long prompts the second reading of blocks over 16 positions, from L2.  61 tokens for 4 heads of
+// 128 4.0 us; 2854 rows for 8 heads, f32, blocks of 32 (29 MB) 10.9 us.  32 rows kept in registers
+// 4.8 and 10.0: steps of single tokens are what a server makes most of.
 template <int SRC>  // ggml type
 __device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
     if constexpr (SRC == T_F32) {
@@ -1015,7 +1032,7 @@ __device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
 template <int HD, int SRC>
 __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) {
     const PagedAppendArgs &a = x.a;
-    constexpr int CPR = HD / 8, RP = 64 / CPR, NP = (16 + RP - 1) / RP;  // lanes of a row, rows of a pass, passes of 16 rows
+    constexpr int CPR = HD / 8, RP = 64 / CPR, ROWS = 16, NP = (ROWS + RP - 1) / RP;  // lanes of a row, rows of a pass, rows and passes at a time
     constexpr int ES = SRC == T_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, u = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = u / (2 * a.n_kv), h = u / 2 % a.n_kv;
@@ -1027,16 +1044,10 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     const int pos0 = sv.pos0(), from = imax(pos0, 0), to = imin(pos0 + sv.n_new, sv.len);  // positions that are written
     const int b0 = same(((from >> bs) + id - append8_id(sv.row0, si, bs)) << bs);          // the block's first position
     if (b0 >= to) return;
-    int page;
-    if (!page_of(a.kv, a.kv.table + (int64_t)si * a.kv.table_stride, b0, page)) return;
-    page = same(page);
     const int first = imax(b0, from), n = imin(b0 + B, to) - first, slot0 = b0 & ((1 << a.kv.page_shift) - 1);
     if (n <= 0) return;
-    float *sp = (is_v ? x.s.v : x.s.k) + (int64_t)page * x.s.page + (int64_t)(slot0 >> bs) * x.s.block + (int64_t)h * x.s.head;
-    const float was = first > b0 ? *sp : 0.0f;
     const uint8_t *src = (is_v ? a.v + h * a.v_head : a.k + h * a.k_head) + (int64_t)(sv.row0 + first - pos0) * (is_v ? a.v_row : a.k_row);
     const int64_t src_row = is_v ? a.v_row : a.k_row, row = is_v ? a.kv.v_row : a.kv.k_row;
-    uint8_t *dst = const_cast<uint8_t *>(is_v ? a.kv.v + h * a.kv.v_head : a.kv.k + h * a.kv.k_head) + page * a.kv.page + slot0 * row;
     const int r = lane / CPR, ch = lane % CPR;
     const bool on = r < RP;
 
@@ -1045,16 +1056,23 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int q = r0 + i * RP + r;
-            if (on && i * RP + r < 16 && q < n) load8<SRC>(src + q * src_row + ch * (8 * ES), v[i]);
+            if (on && i * RP + r < ROWS && q < n) load8<SRC>(src + q * src_row + ch * (8 * ES), v[i]);
             else
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[i][e] = 0;
         }
     };
+    load(0);
+    int page;
+    if (!page_of(a.kv, a.kv.table + (int64_t)si * a.kv.table_stride, b0, page)) return;
+    page = same(page);
+    float *sp = (is_v ? x.s.v : x.s.k) + (int64_t)page * x.s.page + (int64_t)(slot0 >> bs) * x.s.block + (int64_t)h * x.s.head;
+    const float was = first > b0 ? *sp : 0.0f;
+    uint8_t *dst = const_cast<uint8_t *>(is_v ? a.kv.v + h * a.kv.v_head : a.kv.k + h * a.kv.k_head) + page * a.kv.page + slot0 * row;
     float most = 0;
     bool fine = true;
-    for (int r0 = 0; r0 < n; r0 += 16) {
-        load(r0);
+    for (int r0 = 0; r0 < n; r0 += ROWS) {
+        if (r0) load(r0);
 #pragma unroll
         for (int i = 0; i < NP; i++)
 #pragma unroll
@@ -1085,12 +1103,12 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
         }
     }
     const double inv = now > 0 ? 1.0 / (double)now : 0.0;
-    for (int r0 = 0; r0 < n; r0 += 16) {
-        if (n > 16) load(r0);
+    for (int r0 = 0; r0 < n; r0 += ROWS) {
+        if (n > ROWS) load(r0);
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int q = r0 + i * RP + r;
-            if (!(on && i * RP + r < 16 && q < n)) continue;
+            if (!(on && i * RP + r < ROWS && q < n)) continue;
             u32x2 y = {0, 0};
             if (inv > 0)
 #pragma unroll
