@@ -395,7 +395,8 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
 // Bound: a SIMD's matrix and vector instructions, which hardly overlap: of a wave's tile of 64
 // positions, head size 128, 1024 cycles are matrix products and about 1100 vector work (exponentials
 // alone 512, codes 160).  Eight waves to a tile (256 rows) where there are so many, since then
-// each makes half as many codes: 215 us with four, 185 with eight (13 sequences, see below).
+// each makes half as many codes: 13 sequences as below, both under a profiler, 215 us with four
+// and 200 with eight.
 template <int HD>
 constexpr int TILE8_KT = HD <= 128 ? 64 : 32;
 
