@@ -1020,18 +1020,16 @@ void launch_serve_attn(ServeAttnArgs a, void *ws, hipStream_t st) {
     const bool bf = a.ty == T_BF16;
     if (bf) launch_ty<true>(a, st);
     else launch_ty<false>(a, st);
-    if (p.S > 1) launch_serve_combine(a, few ? FEW_ROWS : TILE_M, few ? FEW_STEP : tile_kt(a.hd), st);
-}
-
-void launch_serve_combine(const ServeAttnArgs &a, int M, int KT, hipStream_t st) {
-    const bool bf = a.ty == T_BF16;
-    const int64_t n = (int64_t)a.b.n_rows * a.n_head;
-    if (n <= COMBINE_FEW) {
-        if (bf) serve_combine_kernel<true, 4><<<n, 256, 0, st>>>(a, M, KT);
-        else serve_combine_kernel<false, 4><<<n, 256, 0, st>>>(a, M, KT);
-    } else {
-        if (bf) serve_combine_kernel<true, 1><<<(n + 3) / 4, 256, 0, st>>>(a, M, KT);
-        else serve_combine_kernel<false, 1><<<(n + 3) / 4, 256, 0, st>>>(a, M, KT);
+    if (p.S > 1) {
+        const int M = few ? FEW_ROWS : TILE_M, KT = few ? FEW_STEP : tile_kt(a.hd);
+        const int64_t n = (int64_t)a.b.n_rows * a.n_head;
+        if (n <= COMBINE_FEW) {
+            if (bf) serve_combine_kernel<true, 4><<<n, 256, 0, st>>>(a, M, KT);
+            else serve_combine_kernel<false, 4><<<n, 256, 0, st>>>(a, M, KT);
+        } else {
+            if (bf) serve_combine_kernel<true, 1><<<(n + 3) / 4, 256, 0, st>>>(a, M, KT);
+            else serve_combine_kernel<false, 1><<<(n + 3) / 4, 256, 0, st>>>(a, M, KT);
+        }
     }
 }
 

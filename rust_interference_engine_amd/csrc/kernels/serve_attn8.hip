@@ -63,15 +63,37 @@ constexpr float P_SHIFT8 = 6.0f;  // p · s_v is 2^(exponent − m + P_SHIFT8): 
 // instructions as they are; values are read transposed, 8 positions of a dim to a lane, and made
 // f16 there, 10 vector instructions for 8 values.
 //
-// Bound: HBM while all workgroups stream (6.4 TB/s by timestamps), and their beginnings: starts,
-// page ids, scales and the first tile lie behind one another, 8 us until a workgroup's first tile
-// is there.  So the positions are divided into about four rounds of workgroups, whose beginnings
-// pass while others stream.  48 tokens over up to 4000 positions, 32/8 heads of 128 (149 MB) 41 us
-// (3.6 TB/s) and 7 for the join, 1 over 100003 positions, 32/4 of 128 (103 MB) 22 and 5.5; in equal
-// pieces, as many as workgroups run at a time, 43.5 and 5.9, 29 and 8.7: all begin at once.
-constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT;
-template <int HD, int NB>
-constexpr int FEW8_WAVES = NB == 1 ? (HD <= 128 ? 4 : 2) : (HD <= 64 ? 3 : HD <= 128 ? 2 : 1);  // of a SIMD, as registers allow
+// Bound: HBM while all workgroups stream (6.4 TB/s by timestamps), and their beginning: starts,
+// page ids, scales and the first tile lie behind one another.  48 tokens over up to 4000
+// positions, 32/8 heads of 128 (149 MB) 35 us (4.3 TB/s) and 6 for the join, 1 over 100003
+// positions, 32/4 of 128 (103 MB) 22.7 and 6.
+constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT, FEW8_LEAST = 4, FEW8_BEGIN = 1;  // positions of a wave's tile and of a step; steps that a piece is worth, and those that a sequence's beginning takes
+constexpr int few8_waves(int hd, int nb) { return nb == 2 && hd > 128 ? 1 : 2; }  // of a SIMD: more are no faster, and have fewer registers
+
+// The steps of all sequences in a row are cut into P equal pieces, two workgroups to a CU (per KV
+// head), wherever the cuts fall.  A workgroup goes through the sequences of its piece; one that it
+// has all of goes to the outputs, and at most two (its first, its last) to partial results, which
+// few8_join_kernel adds up.  Everyone finds the cuts from the lengths.  Splits of three steps of
+// each sequence, about four rounds of workgroups: 48 tokens 42 and 7 us, 1 token 22 and 5.5; the
+// whole call 50.7 for 43 and 29 for 30.  Pieces for one workgroup to a CU: 53 and 35; for four,
+// which spill registers, 52 and 39.
+__device__ __forceinline__ SeqView few8_view(const ServeAttnArgs &a, int i) {
+    return i < a.b.n_seq ? seq_view(a.b.starts[i], a.b.starts[i + 1], a.b.lens[i], a.b.n_rows, a.kv.cap) : SeqView{0, 0, 0};
+}
+template <int M>  // rows of a sequence, at most
+__device__ __forceinline__ int few8_steps(const ServeAttnArgs &a, const SeqView &v) {
+    if (v.n_new == 0) return 0;
+    return imax(tile_count(key_range(v, 0, imin(v.n_new, (M + a.G - 1) / a.G) - 1, a.window), FEW8_STEP), 1) + FEW8_BEGIN;
+}
+// Steps of a piece.  A sequence has under 2^24 and a call under 2^12 sequences, so a sum of 64 of
+// them fits 32 bits, that of all may not; P is no less than a sixteenth of the sequences, so a piece does.
+__device__ __forceinline__ int few8_per(int64_t total, int P) {
+    return imax(total >> 31 ? (int)((total + P - 1) / P) : (int)(((uint32_t)total + (uint32_t)P - 1) / (uint32_t)P), FEW8_LEAST);
+}
+template <int HD, int M>
+__device__ __forceinline__ int64_t few8_part(int kvh, int P, int piece, bool begins) {  // begins: with the sequence's first step
+    return (((int64_t)kvh * P + piece) * 2 + begins) * (M * (HD + 2));
+}
 
 // A wave's values in LDS: it copies 1 KB at a time, RPI whole rows, by 16-byte chunk, then row
 template <int HD>
@@ -86,7 +108,7 @@ struct Value8Lds {
 };
 
 template <int HD, bool BF, bool CAP, int NB>
-__global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(ServeAttn8Args x) {
+__global__ __launch_bounds__(256, few8_waves(HD, NB)) void attn8_few_kernel(ServeAttn8Args x, int P, float *parts) {
     using Lds = Value8Lds<HD>;
     const ServeAttnArgs &a = x.a;
     constexpr int KT = FEW8_KT, RPI = Lds::RPI, NLD = KT / RPI, DB = HD / 16;
@@ -95,293 +117,414 @@ __global__ __launch_bounds__(256, (FEW8_WAVES<HD, NB>)) void attn8_few_kernel(Se
     constexpr int WB = VB > OB ? VB : OB;
     __shared__ __align__(16) uint8_t s_buf[4][WB];
     __shared__ float s_ml[4][16 * NB][2];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
-    const int G = a.G, kvh = blockIdx.x % a.n_kv, si = blockIdx.x / a.n_kv;
-    const SeqView sv = view_of(a.b, a.kv, si);
-    const int n_rows = imin(sv.n_new * G, 16 * NB);
-    if (n_rows == 0) return;
-    const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.pos0();
-    const KeyRange kr = key_range(sv, 0, n_tok - 1, a.window);
-    const int hi = same(kr.hi), t0 = same(first_tile(kr, FEW8_STEP)), nt = same(tile_count(kr, FEW8_STEP)), ns = same(split_count(nt, a.C, a.S)), sp = blockIdx.y;
-    if (sp >= ns) return;
-    const int begin = (t0 + sp * a.C) * 4 + w, end = imin((sp == ns - 1 ? t0 + nt : t0 + (sp + 1) * a.C) * 4, (hi + KT - 1) / KT);
+    __shared__ int s_seq[4][6][64];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.G, kvh = blockIdx.x % a.n_kv, piece = blockIdx.x / a.n_kv;
 
-    // Queries: a row's values are whole numbers of at most 2^22 times 2^(e − 22), in three 8-bit parts
-    int p_q[NB], lo_q[NB];
-    u32x4 qf[NB][KS][3];
-    float qs[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-        const int row = b * 16 + col, tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
-        const bool live = row < n_rows;
-        p_q[b] = live ? imin(pos0 + tok, sv.len - 1) : -1;
-        lo_q[b] = before_window(pos0 + tok, a.window);
-        const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head;
-        u32x4 raw[KS][2];
-        float most = 0;
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const int d = K64 ? i * 64 + g * 16 : i * 32 + g * 8;
-#pragma unroll
-            for (int u = 0; u < (K64 ? 2 : 1); u++) {
-                raw[i][u] = live ? *(const u32x4 *)(qp + d * 2 + u * 16) : u32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float f = fabsf(value16<BF>(raw[i][u][e / 2] >> (e & 1) * 16 & 0xFFFF));
-                    finite = finite && f <= FLT_MAX;
-                    most = fmaxf(most, f);
-                }
-            }
-        }
-        float a0, a1, b0, b1;
-        pair_f<16>(finite ? most : INFINITY, a0, a1);
-        pair_f<32>(fmaxf(a0, a1), b0, b1);
-        most = fmaxf(b0, b1);
-        const int ex = 22 - __builtin_amdgcn_frexp_expf(most);  // most < 2^(22 − ex)
-        qs[b] = most <= FLT_MAX ? __builtin_amdgcn_ldexpf(1.0f, -ex) : NAN;
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-            u32x4 part[3] = {};
-#pragma unroll
-            for (int u = 0; u < (K64 ? 2 : 1); u++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float f = value16<BF>(raw[i][u][e / 2] >> (e & 1) * 16 & 0xFFFF);
-                    const int n = __float2int_rn(__builtin_amdgcn_ldexpf(f, ex));
-                    const int lo = (int)(int8_t)n, n1 = (n - lo) >> 8, mid = (int)(int8_t)n1, top = (n1 - mid) >> 8;
-                    const int at = (u * 8 + e) / 4, sh = e % 4 * 8;
-                    part[0][at] |= (uint32_t)(lo & 255) << sh;
-                    part[1][at] |= (uint32_t)(mid & 255) << sh;
-                    part[2][at] |= (uint32_t)(top & 255) << sh;
-                }
-#pragma unroll
-            for (int k = 0; k < 3; k++) qf[b][i][k] = part[k];
-        }
-    }
-    const int all_hi = imin(pos0, sv.len - 1), all_lo = before_window(pos0 + n_tok - 1, a.window);
+    // what the piece, `per` steps, has of the n of sequence si, the first of which is the piece's number base
+    auto sequence = [&](int si, const SeqView &sv, int per, int base, int n) __attribute__((always_inline)) {
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));  // nothing of it is kept in registers from one sequence to the next
+        const int g = lane >> 4, col = lane & 15;
+        const int n_rows = imin(sv.n_new * G, 16 * NB);
+        const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.pos0();
+        const KeyRange kr = key_range(sv, 0, n_tok - 1, a.window);
+        const int hi = same(kr.hi), t0 = same(first_tile(kr, FEW8_STEP)), nt = same(tile_count(kr, FEW8_STEP));
+        const int s0 = imax(-base, 0), s1 = imin(per - base, nt);
+        const bool whole = base >= 0 && per - base >= n;
+        const int begin = (t0 + s0) * 4 + w, end = imin((t0 + s1) * 4, (hi + KT - 1) / KT);
 
-    const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
-    const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
-    uint8_t *vt = s_buf[w];
-    const int k_row = (int)a.kv.k_row, v_row = (int)a.kv.v_row, page_mask = (1 << a.kv.page_shift) - 1;
-    const int v_r = Lds::row(lane), v_c = imin(Lds::chunk(lane), HD / 16 - 1) * 16;
-    // Page ids of a tile's two groups of 16 positions (even and odd lanes), requested a tile ahead.
-    // Positions behind the last one seen are read as copies of it.
-    auto first_of = [&](int t, int b) { return imin(t * KT + b * 16, (hi - 1) & ~15); };
-    auto request_pages = [&](int t) { return t < end ? trow[first_of(t, lane & 1) >> a.kv.page_shift] : 0; };
-    struct Pages {
-        int id, id0, id1, bad;  // the lane's; bad bit b: the page of group b is none (any that exists is read, and nobody sees it)
-    };
-    auto pages_of = [&](int ids) {
-        const bool ok = (unsigned)ids < (unsigned)a.kv.n_pages;
-        Pages p;
-        p.id = ok ? ids : 0;
-        p.bad = (int)(__ballot(!ok) & 3);
-        p.id0 = __builtin_amdgcn_readlane(p.id, 0);
-        p.id1 = __builtin_amdgcn_readlane(p.id, 1);
-        return p;
-    };
-    // lanes 0 and 1: the scales of the groups' keys; 2 and 3: of their values
-    const float *sbase = ((lane & 2) ? x.s.v : x.s.k) + (int64_t)kvh * x.s.head;
-    auto request_scales = [&](int t, const Pages &pg) {
-        const int slot = first_of(t, lane & 1) & page_mask;
-        return sbase[(uint64_t)(uint32_t)pg.id * x.s.page + (uint64_t)(uint32_t)(slot >> x.s.block_shift) * x.s.block];
-    };
-    u32x4 rk[2][KS];
-    auto load_keys = [&](int t, const Pages &pg) __attribute__((always_inline)) {
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-            const int g0 = first_of(t, b), slot = g0 & page_mask;
-            const uint8_t *kp = kbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.k_row;
-            const int off = imin(col, hi - 1 - g0) * k_row;
-#pragma unroll
-            for (int i = 0; i < K64; i++) rk[b][i] = *(const u32x4 *)(kp + off + i * 64 + g * 16);
-#pragma unroll
-            for (int i = 0; i < K32; i++) {
-                const u32x2 y = *(const u32x2 *)(kp + off + i * 32 + g * 8);
-                rk[b][i] = u32x4{y[0], y[1], 0, 0};
-            }
-        }
-    };
-    auto copy_values = [&](int t, const Pages &pg) __attribute__((always_inline)) {
-        if constexpr (RPI <= 16) {
+        int p_q[NB], lo_q[NB];
+        const int all_hi = imin(pos0, sv.len - 1), all_lo = before_window(pos0 + n_tok - 1, a.window);
+
+        const int *trow = a.kv.table + (int64_t)si * a.kv.table_stride;
+        const uint8_t *kbase = a.kv.k + kvh * a.kv.k_head, *vbase = a.kv.v + kvh * a.kv.v_head;
+        uint8_t *vt = s_buf[w];
+        const int k_row = (int)a.kv.k_row, v_row = (int)a.kv.v_row, page_mask = (1 << a.kv.page_shift) - 1;
+        const int v_r = Lds::row(lane), v_c = imin(Lds::chunk(lane), HD / 16 - 1) * 16;
+        // Page ids of a tile's two groups of 16 positions (even and odd lanes), requested a tile ahead.
+        // Positions behind the last one seen are read as copies of it.
+        auto first_of = [&](int t, int b) { return imin(t * KT + b * 16, (hi - 1) & ~15); };
+        auto request_pages = [&](int t) { return t < end ? trow[first_of(t, lane & 1) >> a.kv.page_shift] : 0; };
+        struct Pages {
+            int id, id0, id1, bad;  // the lane's; bad bit b: the page of group b is none (any that exists is read, and nobody sees it)
+        };
+        auto pages_of = [&](int ids) {
+            const bool ok = (unsigned)ids < (unsigned)a.kv.n_pages;
+            Pages p;
+            p.id = ok ? ids : 0;
+            p.bad = (int)(__ballot(!ok) & 3);
+            p.id0 = __builtin_amdgcn_readlane(p.id, 0);
+            p.id1 = __builtin_amdgcn_readlane(p.id, 1);
+            return p;
+        };
+        // lanes 0 and 1: the scales of the groups' keys; 2 and 3: of their values
+        const float *sbase = ((lane & 2) ? x.s.v : x.s.k) + (int64_t)kvh * x.s.head;
+        auto request_scales = [&](int t, const Pages &pg) {
+            const int slot = first_of(t, lane & 1) & page_mask;
+            return sbase[(uint64_t)(uint32_t)pg.id * x.s.page + (uint64_t)(uint32_t)(slot >> x.s.block_shift) * x.s.block];
+        };
+        u32x4 rk[2][KS];
+        auto load_keys = [&](int t, const Pages &pg) __attribute__((always_inline)) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
-                const int g0 = first_of(t, b), slot = g0 & page_mask, last = hi - 1 - g0;
-                const uint8_t *vp = vbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.v_row;
+                const int g0 = first_of(t, b), slot = g0 & page_mask;
+                const uint8_t *kp = kbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.k_row;
+                const int off = imin(col, hi - 1 - g0) * k_row;
 #pragma unroll
-                for (int i = 0; i < NLD / 2; i++) copy_lds(vp, imin(i * RPI + v_r, last) * v_row + v_c, vt + (b * (NLD / 2) + i) * Lds::BLOCK);
+                for (int i = 0; i < K64; i++) rk[b][i] = *(const u32x4 *)(kp + off + i * 64 + g * 16);
+#pragma unroll
+                for (int i = 0; i < K32; i++) {
+                    const u32x2 y = *(const u32x2 *)(kp + off + i * 32 + g * 8);
+                    rk[b][i] = u32x4{y[0], y[1], 0, 0};
+                }
             }
-        } else {  // both groups in one copy: their distance may pass 32 bits, so by way of registers
-            const int b = v_r >> 4, g0 = first_of(t, b), slot = g0 & page_mask;
-            const uint8_t *vp = vbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.v_row + imin(v_r & 15, hi - 1 - g0) * v_row + v_c;
-            *(u32x4 *)(vt + lane * 16) = *(const u32x4 *)vp;
+        };
+        auto copy_values = [&](int t, const Pages &pg) __attribute__((always_inline)) {
+            if constexpr (RPI <= 16) {
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int g0 = first_of(t, b), slot = g0 & page_mask, last = hi - 1 - g0;
+                    const uint8_t *vp = vbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.v_row;
+#pragma unroll
+                    for (int i = 0; i < NLD / 2; i++) copy_lds(vp, imin(i * RPI + v_r, last) * v_row + v_c, vt + (b * (NLD / 2) + i) * Lds::BLOCK);
+                }
+            } else {  // both groups in one copy: their distance may pass 32 bits, so by way of registers
+                const int b = v_r >> 4, g0 = first_of(t, b), slot = g0 & page_mask;
+                const uint8_t *vp = vbase + (b ? pg.id1 : pg.id0) * a.kv.page + slot * a.kv.v_row + imin(v_r & 15, hi - 1 - g0) * v_row + v_c;
+                *(u32x4 *)(vt + lane * 16) = *(const u32x4 *)vp;
+            }
+        };
+
+        // the first tile is on its way before the queries are made ready
+        int ids = request_pages(begin);
+        u32x4 raw[NB][KS][2];
+        bool live[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const int row = b * 16 + col, tok = imin(row, n_rows - 1) / G, head = kvh * G + imin(row, n_rows - 1) - tok * G;
+            live[b] = row < n_rows;
+            p_q[b] = live[b] ? imin(pos0 + tok, sv.len - 1) : -1;
+            lo_q[b] = before_window(pos0 + tok, a.window);
+            const uint8_t *qp = a.q + (int64_t)(sv.row0 + tok) * a.q_row + head * a.q_head;
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int u = 0; u < (K64 ? 2 : 1); u++) raw[b][i][u] = *(const u32x4 *)(qp + (K64 ? i * 64 + g * 16 : i * 32 + g * 8) * 2 + u * 16);
+        }
+        Pages pg{};
+        float sc = 1;
+        if (begin < end) {
+            pg = pages_of(ids);
+            sc = request_scales(begin, pg);
+            load_keys(begin, pg);
+            copy_values(begin, pg);
+            ids = request_pages(begin + 4);
+        }
+
+        // Queries: a row's values are whole numbers of at most 2^22 times 2^(e − 22), in three 8-bit parts
+        u32x4 qf[NB][KS][3];
+        float qs[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float most = 0;
+            bool finite = true;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+#pragma unroll
+                for (int u = 0; u < (K64 ? 2 : 1); u++) {
+                    if (!live[b]) raw[b][i][u] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float f = fabsf(value16<BF>(raw[b][i][u][e / 2] >> (e & 1) * 16 & 0xFFFF));
+                        finite = finite && f <= FLT_MAX;
+                        most = fmaxf(most, f);
+                    }
+                }
+            }
+            float a0, a1, b0, b1;
+            pair_f<16>(finite ? most : INFINITY, a0, a1);
+            pair_f<32>(fmaxf(a0, a1), b0, b1);
+            most = fmaxf(b0, b1);
+            const int ex = 22 - __builtin_amdgcn_frexp_expf(most);  // most < 2^(22 − ex)
+            qs[b] = most <= FLT_MAX ? __builtin_amdgcn_ldexpf(1.0f, -ex) : NAN;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                u32x4 part[3] = {};
+#pragma unroll
+                for (int u = 0; u < (K64 ? 2 : 1); u++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float f = value16<BF>(raw[b][i][u][e / 2] >> (e & 1) * 16 & 0xFFFF);
+                        const int n = __float2int_rn(__builtin_amdgcn_ldexpf(f, ex));
+                        const int lo = (int)(int8_t)n, n1 = (n - lo) >> 8, mid = (int)(int8_t)n1, top = (n1 - mid) >> 8;
+                        const int at = (u * 8 + e) / 4, sh = e % 4 * 8;
+                        part[0][at] |= (uint32_t)(lo & 255) << sh;
+                        part[1][at] |= (uint32_t)(mid & 255) << sh;
+                        part[2][at] |= (uint32_t)(top & 255) << sh;
+                    }
+#pragma unroll
+                for (int k = 0; k < 3; k++) qf[b][i][k] = part[k];
+            }
+        }
+        f32x4 o[NB][DB];
+        float m[NB], l[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            m[b] = -FLT_MAX;
+            l[b] = 0;
+#pragma unroll
+            for (int d = 0; d < DB; d++) o[b][d] = f32x4{};
+        }
+        const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
+        // where the lane reads values: positions 4 g … of both groups, 16 dims of a chunk
+        const int r8 = col >> 1, v_at = Lds::at((r8 & 3) + 4 * g + (r8 >> 2) * 16, 0) + (lane & 1) * 8;
+
+        for (int t = begin; t < end; t += 4) {
+            const int key0 = t * KT, bad = pg.bad;
+            const bool part = key0 + KT - 1 > all_hi || key0 <= all_lo || bad;  // some row does not see all of the tile
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const float us = usable(sc), lg = __builtin_amdgcn_logf(us), rc = us == us ? 1.0f / us : 1.0f;
+            float ks[2], lv[2], iv[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                ks[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(us), b));
+                lv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg), 2 + b));
+                iv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rc), 2 + b));
+            }
+            f32x4 s[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) {
+                    i32x4 n[3] = {};
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+#pragma unroll
+                        for (int i = 0; i < KS; i++) {
+                            if constexpr (K64 > 0) {
+                                n[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, rk[kb][i]), __builtin_bit_cast(i32x4, qf[b][i][k]), n[k], 0, 0, 0);
+                            } else {
+                                const long kk = (long)((uint64_t)rk[kb][i][1] << 32 | rk[kb][i][0]), qq = (long)((uint64_t)qf[b][i][k][1] << 32 | qf[b][i][k][0]);
+                                n[k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(kk, qq, n[k], 0, 0, 0);
+                            }
+                        }
+                    // |mid · 256 + lo| is under 2^31 for 256 dims
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[b][kb][e] = fmaf((float)n[2][e], 65536.0f, (float)(n[1][e] * 256 + n[0][e]));
+                }
+            if (t + 4 < end) {
+                pg = pages_of(ids);
+                sc = request_scales(t + 4, pg);
+                load_keys(t + 4, pg);
+                ids = request_pages(t + 8);
+            }
+            u32x4 pf[NB][2];  // probabilities times the values' scales, and what their rounding left
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) {
+                    const float c = ks[kb] * (CAP ? 1.0f : a.scale * LOG2E_F) * qs[b];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float y = CAP ? cap_score<CAP>(s[b][kb][e] * c, cap) + lv[kb] : fmaf(s[b][kb][e], c, lv[kb]);
+                        if (part) {
+                            const int j = key0 + kb * 16 + 4 * g + e;
+                            y = (j > p_q[b]) | (j <= lo_q[b]) | (bad >> kb & 1) ? -INFINITY : y;
+                        }
+                        s[b][kb][e] = y;
+                        mx = fmaxf(mx, y);
+                    }
+                }
+                if (__any(mx > m[b] + M_SLACK)) {
+                    float x0, x1, y0, y1;
+                    pair_f<16>(mx, x0, x1);
+                    pair_f<32>(fmaxf(x0, x1), y0, y1);
+                    const float mn = fmaxf(m[b], fmaxf(y0, y1)), al = exp2_hw(m[b] - mn);
+                    m[b] = mn;
+                    l[b] *= al;
+#pragma unroll
+                    for (int d = 0; d < DB; d++) o[b][d] *= al;
+                }
+                const float ref = P_SHIFT8 - m[b];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p0 = exp2_hw(s[b][e / 2][2 * (e & 1)] + ref), p1 = exp2_hw(s[b][e / 2][2 * (e & 1) + 1] + ref);
+                    const uint32_t near = pack2<false>(p0, p1);
+                    pf[b][0][e] = near;
+                    pf[b][1][e] = pack2<false>(p0 - h2f(near & 0xFFFF), p1 - h2f(near >> 16));
+                    l[b] = fmaf(p0 + p1, iv[e / 2], l[b]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const u32x2 c = read_tr8(lds_at(vt) + v_at + Lds::at(0, d));
+                u32x4 vf;
+                uint32_t h0, h1;
+                halves4(c[0], h0, h1);
+                vf[0] = h0;
+                vf[1] = h1;
+                halves4(c[1], h0, h1);
+                vf[2] = h0;
+                vf[3] = h1;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    o[b][d] = mfma16<false>(vf, pf[b][1], o[b][d]);
+                    o[b][d] = mfma16<false>(vf, pf[b][0], o[b][d]);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values have been read: their place is free
+            if (t + 4 < end) copy_values(t + 4, pg);
+        }
+
+        // the four waves' results
+        wave_sync();
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float x0, x1, y0, y1;
+            pair_f<16>(l[b], x0, x1);
+            pair_f<32>(x0 + x1, y0, y1);
+            float *po = (float *)vt + (b * 16 + col) * HD + 4 * g;
+#pragma unroll
+            for (int d = 0; d < DB; d++) *(f32x4 *)(po + d * 16) = o[b][d];
+            if (g == 0) {
+                s_ml[w][b * 16 + col][0] = m[b];
+                s_ml[w][b * 16 + col][1] = y0 + y1;
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_rows * (HD / 4); i += 256) {
+            const int r = i / (HD / 4), d4 = i % (HD / 4), tok = r / G, head = kvh * G + r - tok * G;
+            float mm = s_ml[0][r][0];
+#pragma unroll
+            for (int k = 1; k < 4; k++) mm = fmaxf(mm, s_ml[k][r][0]);
+            f32x4 acc = f32x4{};
+            float L = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f = exp2_hw(s_ml[k][r][0] - mm);
+                L = fmaf(f, s_ml[k][r][1], L);
+                const f32x4 y = *(const f32x4 *)((const float *)s_buf[k] + r * HD + d4 * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] = fmaf(f, y[e], acc[e]);
+            }
+            if (whole) {
+                const float inv = L > 0 || L != L ? 1.0f / L : 0.0f;
+                uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d4 * 8;
+                *(u32x2 *)op = u32x2{pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
+            } else {
+                float *pp = parts + few8_part<HD, 16 * NB>(kvh, P, piece, base >= 0);
+                *(f32x4 *)(pp + r * HD + d4 * 4) = acc;
+                if (d4 == 0) *(f32x2 *)(pp + 16 * NB * HD + r * 2) = f32x2{mm, L};
+            }
         }
     };
 
-    f32x4 o[NB][DB];
-    float m[NB], l[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-        m[b] = -FLT_MAX;
-        l[b] = 0;
-#pragma unroll
-        for (int d = 0; d < DB; d++) o[b][d] = f32x4{};
+    constexpr int M = 16 * NB;
+    const int lane = threadIdx.x & 63;
+    SeqView view = few8_view(a, P ? lane : piece);
+    int i0 = P ? 0 : piece, per = INT32_MAX, first = lane == 0 && view.n_new > 0 ? 1 + FEW8_BEGIN : 0;  // P = 0: a workgroup for each
+    int64_t before = 0;  // steps before the chunk's sequences, from the piece's first on
+    if (P) {
+        first = few8_steps<M>(a, view);
+        int64_t total = a.b.n_seq > 1 ? same(xsum_i<64>(first)) : same(first);
+        for (int i = 64; i < a.b.n_seq; i += 64) total += same(xsum_i<64>(few8_steps<M>(a, few8_view(a, i + lane))));
+        per = same(few8_per(total, P));
+        before = -(int64_t)piece * per;
     }
-    const SoftCap cap = CAP ? soft_cap(a) : SoftCap{};
-    // where the lane reads values: positions 4 g … of both groups, 16 dims of a chunk
-    const int r8 = col >> 1, v_at = Lds::at((r8 & 3) + 4 * g + (r8 >> 2) * 16, 0) + (lane & 1) * 8;
+    const int i_first = i0;
+    bool again = false;
+    for (; i0 < a.b.n_seq && before < per; i0 += P ? 64 : a.b.n_seq) {
+        int n = first;
+        if (i0 != i_first) {
+            view = few8_view(a, i0 + lane);
+            n = few8_steps<M>(a, view);
+        }
+        int upto = n;
+        if (P && a.b.n_seq > 1) {
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(upto, o);
+                if (lane >= o) upto += y;
+            }
+        }
+        const int sum = __builtin_amdgcn_readlane(upto, P && a.b.n_seq > 1 ? 63 : 0);
+        if (before + sum > 0) {
+            const int base = (int)before + upto - n + FEW8_BEGIN;
+            const int mine_of[6] = {base, n - FEW8_BEGIN, view.row0, view.n_new, view.len, view.over};
+#pragma unroll
+            for (int i = 0; i < 6; i++) s_seq[w][i][lane] = mine_of[i];
+            for (uint64_t mine = __ballot(n > 0 && base < per && base - FEW8_BEGIN + n > 0); mine; mine &= mine - 1) {
+                const int j = __builtin_ctzll(mine);
+                if (again) __syncthreads();  // the one before has been read
+                again = true;
+                auto of = [&](int i) { return same(s_seq[w][i][j]); };
+                sequence(i0 + j, SeqView{of(2), of(3), of(4), of(5)}, per, of(0), of(1));
+            }
+        }
+        before += sum;
+    }
+}
 
-    Pages pg{};
-    int ids = 0;
-    float sc = 1;
-    if (begin < end) {
-        pg = pages_of(request_pages(begin));
-        sc = request_scales(begin, pg);
-        load_keys(begin, pg);
-        copy_values(begin, pg);
-        ids = request_pages(begin + 4);
+// Sequences that several pieces have a part of: a workgroup for each row
+template <int HD, bool BF, int M>
+__global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, int P, const float *parts) {
+    __shared__ f32x4 s_o[256];
+    const int lane = threadIdx.x & 63, kvh = blockIdx.x % a.n_kv, si = blockIdx.x / a.n_kv, r = blockIdx.y;
+    int64_t total = 0, base = FEW8_BEGIN;
+    for (int i0 = 0; i0 < a.b.n_seq; i0 += 64) {
+        const int n = few8_steps<M>(a, few8_view(a, i0 + lane));
+        total += same(xsum_i<64>(n));
+        base += same(xsum_i<64>(i0 + lane < si ? n : 0));
     }
-    for (int t = begin; t < end; t += 4) {
-        const int key0 = t * KT, bad = pg.bad;
-        const bool part = key0 + KT - 1 > all_hi || key0 <= all_lo || bad;  // some row does not see all of the tile
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const float us = usable(sc), lg = __builtin_amdgcn_logf(us), rc = us == us ? 1.0f / us : 1.0f;
-        float ks[2], lv[2], iv[2];
+    const SeqView sv = view_of(a.b, a.kv, si);
+    const int n = same(few8_steps<M>(a, sv)) - FEW8_BEGIN, per = same(few8_per(total, P));
+    if (r >= imin(sv.n_new, M) * a.G || r >= M) return;
+    const int j0 = base >> 31 ? (int)(base / per) : (int)((uint32_t)base / (uint32_t)per), ns = ((int)(base - (int64_t)j0 * per) + n - 1) / per + 1;
+    if (ns == 1) return;
+    constexpr int LPR = HD / 4, AT_ONCE = 256 / LPR;  // lanes of a part's row, parts at a time
+    auto part = [&](int s) { return parts + few8_part<HD, M>(kvh, P, j0 + s, s == 0); };
+    const int g = threadIdx.x / LPR, d = threadIdx.x % LPR;
+    const bool in = g < AT_ONCE;
+    constexpr int FIRST = 16;  // requested before their weights are known
+    f32x4 y[FIRST];
+    float my[FIRST];
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            ks[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(us), b));
-            lv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg), 2 + b));
-            iv[b] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rc), 2 + b));
-        }
-        f32x4 s[NB][2];
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int kb = 0; kb < 2; kb++) {
-                i32x4 n[3] = {};
-#pragma unroll
-                for (int k = 0; k < 3; k++)
-#pragma unroll
-                    for (int i = 0; i < KS; i++) {
-                        if constexpr (K64 > 0) {
-                            n[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, rk[kb][i]), __builtin_bit_cast(i32x4, qf[b][i][k]), n[k], 0, 0, 0);
-                        } else {
-                            const long kk = (long)((uint64_t)rk[kb][i][1] << 32 | rk[kb][i][0]), qq = (long)((uint64_t)qf[b][i][k][1] << 32 | qf[b][i][k][0]);
-                            n[k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(kk, qq, n[k], 0, 0, 0);
-                        }
-                    }
-                // |mid · 256 + lo| is under 2^31 for 256 dims
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[b][kb][e] = fmaf((float)n[2][e], 65536.0f, (float)(n[1][e] * 256 + n[0][e]));
-            }
-        if (t + 4 < end) {
-            pg = pages_of(ids);
-            sc = request_scales(t + 4, pg);
-            load_keys(t + 4, pg);
-            ids = request_pages(t + 8);
-        }
-        u32x4 pf[NB][2];  // probabilities times the values' scales, and what their rounding left
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < 2; kb++) {
-                const float c = ks[kb] * (CAP ? 1.0f : a.scale * LOG2E_F) * qs[b];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float y = CAP ? cap_score<CAP>(s[b][kb][e] * c, cap) + lv[kb] : fmaf(s[b][kb][e], c, lv[kb]);
-                    if (part) {
-                        const int j = key0 + kb * 16 + 4 * g + e;
-                        y = (j > p_q[b]) | (j <= lo_q[b]) | (bad >> kb & 1) ? -INFINITY : y;
-                    }
-                    s[b][kb][e] = y;
-                    mx = fmaxf(mx, y);
-                }
-            }
-            if (__any(mx > m[b] + M_SLACK)) {
-                float x0, x1, y0, y1;
-                pair_f<16>(mx, x0, x1);
-                pair_f<32>(fmaxf(x0, x1), y0, y1);
-                const float mn = fmaxf(m[b], fmaxf(y0, y1)), al = exp2_hw(m[b] - mn);
-                m[b] = mn;
-                l[b] *= al;
-#pragma unroll
-                for (int d = 0; d < DB; d++) o[b][d] *= al;
-            }
-            const float ref = P_SHIFT8 - m[b];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p0 = exp2_hw(s[b][e / 2][2 * (e & 1)] + ref), p1 = exp2_hw(s[b][e / 2][2 * (e & 1) + 1] + ref);
-                const uint32_t near = pack2<false>(p0, p1);
-                pf[b][0][e] = near;
-                pf[b][1][e] = pack2<false>(p0 - h2f(near & 0xFFFF), p1 - h2f(near >> 16));
-                l[b] = fmaf(p0 + p1, iv[e / 2], l[b]);
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < DB; d++) {
-            const u32x2 c = read_tr8(lds_at(vt) + v_at + Lds::at(0, d));
-            u32x4 vf;
-            uint32_t h0, h1;
-            halves4(c[0], h0, h1);
-            vf[0] = h0;
-            vf[1] = h1;
-            halves4(c[1], h0, h1);
-            vf[2] = h0;
-            vf[3] = h1;
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                o[b][d] = mfma16<false>(vf, pf[b][1], o[b][d]);
-                o[b][d] = mfma16<false>(vf, pf[b][0], o[b][d]);
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values have been read: their place is free
-        if (t + 4 < end) copy_values(t + 4, pg);
+    for (int k = 0; k < FIRST; k++) {
+        if (k * AT_ONCE >= ns) break;
+        const float *p = part(imin(g + k * AT_ONCE, ns - 1));
+        y[k] = *(const f32x4 *)(p + r * HD + d * 4);
+        my[k] = p[M * HD + r * 2];
     }
-
-    // the four waves' results
-    wave_sync();
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-        float x0, x1, y0, y1;
-        pair_f<16>(l[b], x0, x1);
-        pair_f<32>(x0 + x1, y0, y1);
-        float *po = (float *)vt + (b * 16 + col) * HD + 4 * g;
-#pragma unroll
-        for (int d = 0; d < DB; d++) *(f32x4 *)(po + d * 16) = o[b][d];
-        if (g == 0) {
-            s_ml[w][b * 16 + col][0] = m[b];
-            s_ml[w][b * 16 + col][1] = y0 + y1;
-        }
+    float m = -FLT_MAX, l = 0;
+#pragma unroll 2
+    for (int s = lane; s < ns; s += 64) {
+        const f32x2 ml = *(const f32x2 *)(part(s) + M * HD + r * 2);
+        const float mn = fmaxf(m, ml[0]);
+        l = fmaf(l, exp2_hw(m - mn), ml[1] * exp2_hw(ml[0] - mn));
+        m = mn;
     }
+    const float mm = xmax_f<64>(m), L = xsum_f<64>(l * exp2_hw(m - mm)), inv = L > 0 || L != L ? 1.0f / L : 0.0f;
+    f32x4 acc = f32x4{};
+    auto add = [&](float ms, const f32x4 &v) {
+        const float f = exp2_hw(ms - mm);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = fmaf(f, v[e], acc[e]);
+    };
+#pragma unroll
+    for (int k = 0; k < FIRST; k++) {
+        if (k * AT_ONCE >= ns) break;
+        if (in && g + k * AT_ONCE < ns) add(my[k], y[k]);
+    }
+#pragma unroll 4
+    for (int s = in ? g + FIRST * AT_ONCE : ns; s < ns; s += AT_ONCE) add(part(s)[M * HD + r * 2], *(const f32x4 *)(part(s) + r * HD + d * 4));
+    s_o[threadIdx.x] = acc;
     __syncthreads();
-    for (int i = threadIdx.x; i < n_rows * (HD / 4); i += 256) {
-        const int r = i / (HD / 4), d4 = i % (HD / 4), tok = r / G, head = kvh * G + r - tok * G;
-        float mm = s_ml[0][r][0];
-#pragma unroll
-        for (int k = 1; k < 4; k++) mm = fmaxf(mm, s_ml[k][r][0]);
-        f32x4 acc = f32x4{};
-        float L = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float f = exp2_hw(s_ml[k][r][0] - mm);
-            L = fmaf(f, s_ml[k][r][1], L);
-            const f32x4 y = *(const f32x4 *)((const float *)s_buf[k] + r * HD + d4 * 4);
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[e] = fmaf(f, y[e], acc[e]);
-        }
-        if (ns == 1) {
-            const float inv = L > 0 || L != L ? 1.0f / L : 0.0f;
-            uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d4 * 8;
-            *(u32x2 *)op = u32x2{pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
-        } else {
-            const int64_t at = ((int64_t)(sv.row0 + tok) * a.n_head + head) * a.S + sp;
-            *(f32x4 *)(a.part + at * HD + d4 * 4) = acc;
-            if (d4 == 0) *(f32x2 *)(a.ml + at * 2) = f32x2{mm, L};
-        }
-    }
+    if (threadIdx.x >= LPR) return;
+    const int used = imin(AT_ONCE, ns);
+    for (int k = 1; k < used; k++) acc += s_o[k * LPR + d];
+    const int tok = r / a.G, head = kvh * a.G + r - tok * a.G;
+    *(u32x2 *)(a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d * 8) = u32x2{pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
 }
 
 // ---- 32·NW query rows of a sequence and KV head, tiles of 64 (256-wide heads: 32) positions ----
@@ -1128,6 +1271,17 @@ int64_t span8(const ServeAttnArgs &a, int tokens, int KT) {
     return a.window > 0 ? std::min<int64_t>(a.b.max_len, (int64_t)a.window + std::min(a.b.max_new, tokens) + KT) : a.b.max_len;
 }
 
+bool few8(const ServeAttnArgs &a) { return few_row_blocks(true, a.b.max_new, a.G) > 0; }
+
+// Pieces per KV head that a launch of the few-rows kernel is divided into, or 0: a workgroup for
+// each sequence, where these are short or enough to fill the card several times.
+int few8_pieces(const ServeAttnArgs &a) {
+    const int64_t steps = (span8(a, FEW_ROWS, FEW8_STEP) + FEW8_STEP - 1) / FEW8_STEP, seqs = a.b.n_seq;
+    if (steps < 4 || seqs * a.n_kv >= 4096) return 0;
+    const int slots = 256 * few8_waves(a.hd, few_row_blocks(true, a.b.max_new, a.G)) / a.n_kv;
+    return (int)std::min<int64_t>(seqs * steps / FEW8_LEAST, std::max(slots, 1));
+}
+
 // Pieces per KV head that a launch of the tile kernel is divided into, or 0: a workgroup for each
 // block, where the longest is too short to be cut.
 int tile8_pieces(const ServeAttnArgs &a) {
@@ -1167,22 +1321,21 @@ void launch_tile(const ServeAttn8Args &x, void *ws, hipStream_t st) {
     if (P) tile8_join_kernel<HD, BF, M><<<dim3(a.n_blocks * a.n_kv, NW), 256, 0, st>>>(a, TILE8_KT<HD>, plan, items, P, parts);
 }
 
+template <int HD, bool BF, int NB>
+void launch_few(const ServeAttn8Args &x, void *ws, hipStream_t st) {
+    const ServeAttnArgs &a = x.a;
+    const int P = few8_pieces(a), grid = (P ? P : a.b.n_seq) * a.n_kv;
+    if (a.softcap > 0) attn8_few_kernel<HD, BF, true, NB><<<grid, 256, 0, st>>>(x, P, (float *)ws);
+    else attn8_few_kernel<HD, BF, false, NB><<<grid, 256, 0, st>>>(x, P, (float *)ws);
+    if (P) few8_join_kernel<HD, BF, 16 * NB><<<dim3(a.b.n_seq * a.n_kv, std::min(a.b.max_new * a.G, 16 * NB)), 256, 0, st>>>(a, P, (const float *)ws);
+}
+
 template <int HD, bool BF>
 void launch_hd(const ServeAttn8Args &x, void *ws, hipStream_t st) {
     const ServeAttnArgs &a = x.a;
-    const bool cap = a.softcap > 0;
     const int few = few_row_blocks(true, a.b.max_new, a.G);
-    if (few) {
-        const dim3 grid(a.b.n_seq * a.n_kv, a.S);
-        if (few == 1) {
-            if (cap) attn8_few_kernel<HD, BF, true, 1><<<grid, 256, 0, st>>>(x);
-            else attn8_few_kernel<HD, BF, false, 1><<<grid, 256, 0, st>>>(x);
-        } else {
-            if (cap) attn8_few_kernel<HD, BF, true, 2><<<grid, 256, 0, st>>>(x);
-            else attn8_few_kernel<HD, BF, false, 2><<<grid, 256, 0, st>>>(x);
-        }
-        return;
-    }
+    if (few == 1) return launch_few<HD, BF, 1>(x, ws, st);
+    if (few == 2) return launch_few<HD, BF, 2>(x, ws, st);
     if constexpr (HD <= 128) {
         if (tile8_waves(a) == 8) return launch_tile<HD, BF, 8>(x, ws, st);
     }
@@ -1211,39 +1364,18 @@ void launch_append(const PagedAppend8Args &x, int grid, hipStream_t st) {
     }
 }
 
-bool few8(const ServeAttnArgs &a) { return few_row_blocks(true, a.b.max_new, a.G) > 0; }
-
-// how the few-rows kernel divides the positions
-SplitPlan splits8(const ServeAttnArgs &a) {
-    const int tiles = (int)((span8(a, FEW_ROWS, FEW8_STEP) + FEW8_STEP - 1) / FEW8_STEP);
-    return split_plan((int64_t)a.b.n_seq * a.n_kv, tiles, 4096, 2, SERVE_MAX_SPLIT);
-}
-
 }  // namespace
 
 size_t serve_attn8_ws(const ServeAttnArgs &a) {
-    if (!few8(a)) {
-        return tile8_ws(a).bytes;
-    }
-    const SplitPlan p = splits8(a);
-    return p.S == 1 ? 0 : (size_t)a.b.n_rows * a.n_head * p.S * (a.hd + 2) * sizeof(float);
+    if (!few8(a)) return tile8_ws(a).bytes;
+    return (size_t)few8_pieces(a) * a.n_kv * 2 * 16 * few_row_blocks(true, a.b.max_new, a.G) * (a.hd + 2) * sizeof(float);
 }
 
 void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st) {
     ServeAttnArgs &a = x.a;
-    const bool few = few8(a);
-    if (few) {
-        const SplitPlan p = splits8(a);
-        a.C = p.C;
-        a.S = p.S;
-        a.part = (float *)ws;
-        a.ml = a.part + (size_t)a.b.n_rows * a.n_head * p.S * a.hd;
-    } else {
-        a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
-    }
+    if (!few8(a)) a.n_blocks = (int)block_count(a.b.n_rows, a.b.n_seq, a.G, tile8_m(a));
     if (a.ty == T_BF16) launch_ty<true>(x, ws, st);
     else launch_ty<false>(x, ws, st);
-    if (few && a.S > 1) launch_serve_combine(a, FEW_ROWS, FEW8_STEP, st);
 }
 
 void launch_paged_append8(const PagedAppend8Args &x, hipStream_t st) {

@@ -45,10 +45,6 @@ size_t serve_attn_ws(const ServeAttnArgs &a);
 bool serve_attn_head_dim_ok(int hd);
 void launch_serve_attn(ServeAttnArgs a, void *ws, hipStream_t st);
 
-// adds the splits of each (row, head) up: M rows per block and KT positions per tile are those of
-// the kernel that made the partials
-void launch_serve_combine(const ServeAttnArgs &a, int M, int KT, hipStream_t st);
-
 // Pages of 8 bits: a value is its code times the scale of its block of positions and head
 struct Scales8 {
     float *k = nullptr, *v = nullptr;

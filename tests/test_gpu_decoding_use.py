@@ -7,8 +7,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-import decoding_ref as D  # noqa: E402
 import serving8_ref as R  # noqa: E402
+import serving_ref as S  # noqa: E402
 from test_gpu_decoding import Both, chosen, near, random_rows  # noqa: E402
 from test_gpu_serving8 import check, paged  # noqa: E402
 
@@ -284,3 +284,49 @@ def test_numbers_that_are_none_stay_in_bounds(ops):
         torch.cuda.synchronize()
         assert torch.equal(whole[0], before[0]) and torch.equal(whole[7], before[7]) and torch.equal(whole[:, 6:], before[:, 6:])
         assert bool((guard == 9).all())
+
+
+# ---- single tokens in pieces ----
+
+@pytest.mark.parametrize("H,KV,hd,page,dtype", [(4, 1, 32, 16, F16), (8, 2, 64, 64, BF16), (6, 3, 96, 32, F16), (8, 2, 128, 128, BF16), (32, 1, 128, 16, F16), (4, 1, 256, 32, BF16), (9, 9, 64, 16, F16)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (700, 0.0), (0, 3.0)])
+def test_few_rows_that_several_workgroups_share(ops, H, KV, hd, page, dtype, window, softcap):
+    G = H // KV
+    some = max(1, 32 // G)
+    b = R.Batch8([(1, 9), (some, 2900), (0, 50), (1, 5000), (1, 1), (some, some), (1, 1700), (1, 0), (1, 128), (1, 129)], H, KV, hd, page=page, dtype=dtype, seed=51, extra_rows=5)
+    check(b, paged(ops, b, window, softcap), window, softcap)
+
+
+@pytest.mark.parametrize("n_seq", [2, 64, 65, 200, 700])
+def test_pieces_of_many_sequences(ops, n_seq):
+    """more sequences than a wave scans at once; lengths from none to many pieces, under a loose bound"""
+    rng = random.Random(n_seq)
+    lens = [(rng.choice([0, 1, 1, 2]), rng.choice([0, 1, 60, 127, 128, 300, 900])) for _ in range(n_seq)]
+    lens = [(min(n, x), x) for n, x in lens]
+    lens[-1], lens[n_seq // 2] = (1, 6000), (2, 3500)
+    b = R.Batch8(lens, 4, 2, 64, page=32, block=32, dtype=F16, seed=52)
+    check(b, paged(ops, b, max_len=20000))
+    check(b, paged(ops, b, window=200, max_len=20000), window=200)
+
+
+def test_lengths_beyond_the_bound_stay_in_bounds(ops):
+    """lengths that pass max_len, up to all that a table addresses, over pages used again and again: every call ends, what it
+    should not write stays, and a sequence that passes the bound is whole all the same"""
+    n_pages, KV, hd, page, cols = 9, 2, 64, 4096, 2000
+    codes = torch.randint(-127, 128, (2, n_pages, KV, page, hd), dtype=torch.int8, generator=torch.Generator().manual_seed(53))
+    scale = torch.full((2, n_pages, 1, KV), 0.01)
+    table = (torch.arange(40 * cols, dtype=torch.int32) % n_pages).view(40, cols)
+    dev, s = codes.to(GPU), scale.to(GPU)
+    kv = ops.PagedKv(*dev.transpose(2, 3), table.to(GPU), k_scale=s[0], v_scale=s[1])
+    starts = torch.arange(41, dtype=torch.int32, device=GPU)
+    lens = torch.full((40,), 1000, dtype=torch.int32, device=GPU)
+    lens[3], lens[7], lens[20] = 2 ** 31 - 1, 30000, -5
+    out = torch.full((44, 4, hd), 7.0, dtype=F16, device=GPU)
+    q = (torch.randn(44, 4, hd, generator=torch.Generator().manual_seed(54)) * 8).half()  # few positions count, so that a missing part shows
+    ops.PagedAttention(kv, ops.Seqs(starts, lens, max_new=1, max_len=1000), q.to(GPU), out)()
+    torch.cuda.synchronize()
+    assert bool((out[40:] == 7.0).all()) and bool(out[:40].isfinite().all()) and bool((out[20] == 0).all())
+    k, v = ((codes[i][table[7, :8].long()].double() * scale[i, 0, 0, 0].double()).transpose(1, 2).reshape(-1, KV, hd)[:30000] for i in range(2))
+    o, a, size = S.attend(q[7:8], k, v, 29999, hd ** -0.5)
+    tol = R.tolerance(o, a, q[7:8], k, v, hd ** -0.5, 30000, hd, F16, size)
+    assert bool(((out[7:8].cpu().double() - o).abs() <= tol).all())
