@@ -65,34 +65,52 @@ constexpr float P_SHIFT8 = 6.0f;  // p · s_v is 2^(exponent − m + P_SHIFT8): 
 //
 // Bound: HBM while all workgroups stream (6.4 TB/s by timestamps), and their beginning: starts,
 // page ids, scales and the first tile lie behind one another.  48 tokens over up to 4000
-// positions, 32/8 heads of 128 (149 MB) 35 us (4.3 TB/s) and 6 for the join, 1 over 100003
-// positions, 32/4 of 128 (103 MB) 22.7 and 6.
-constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT, FEW8_LEAST = 4, FEW8_BEGIN = 1;  // positions of a wave's tile and of a step; steps that a piece is worth, and those that a sequence's beginning takes
-constexpr int few8_waves(int hd, int nb) { return nb == 2 && hd > 128 ? 1 : 2; }  // of a SIMD: more are no faster, and have fewer registers
+// positions, 32/8 heads of 128 (149 MB) 34 us (4.4 TB/s) and 6 for the join, 1 over 100003
+// positions, 32/4 of 128 (103 MB) 21.8 (4.7 TB/s) and 5.2.
+constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT;          // positions of a wave's tile and of a step
+constexpr int FEW8_LEAST = 2, FEW8_BEGIN = 1, FEW8_SEQS = 64;  // steps that a piece is worth, those that a sequence's beginning takes; sequences that are cut in pieces
+// of a SIMD: with splits as many as registers allow, with pieces two, which have all that they need
+constexpr int few8_waves(int hd, int nb, bool pieces) {
+    return nb == 1 ? (hd <= 128 && !pieces ? 4 : 2) : hd <= 64 && !pieces ? 3 : hd <= 128 ? 2 : 1;
+}
 
-// The steps of all sequences in a row are cut into P equal pieces, two workgroups to a CU (per KV
-// head), wherever the cuts fall.  A workgroup goes through the sequences of its piece; one that it
-// has all of goes to the outputs, and at most two (its first, its last) to partial results, which
-// few8_join_kernel adds up.  Everyone finds the cuts from the lengths.  Splits of three steps of
-// each sequence, about four rounds of workgroups: 48 tokens 42 and 7 us, 1 token 22 and 5.5; the
-// whole call 50.7 for 43 and 29 for 30.  Pieces for one workgroup to a CU: 53 and 35; for four,
-// which spill registers, 52 and 39.
+// How the positions are divided.  Pieces (S = 0): the steps of all sequences in a row are cut into
+// P equal pieces, two workgroups to a CU (per KV head), wherever the cuts fall.  A workgroup goes
+// through the sequences of its piece; one that it has all of goes to the outputs, and at most two
+// (its first, its last) to partial results, which few8_join_kernel adds up.  Everyone finds the
+// cuts from the lengths, a lane for each sequence.  Splits: S for each sequence, of C steps, the
+// last of all that are left; P = S times the sequences, split by split.
+//
+// Pieces are for lengths that differ, of few sequences: 48 tokens over up to 4000 positions, 32/8
+// heads of 128, 43 us (splits 50.7), 32 over up to 8000, 32/4 heads, 31.3 (39).  One sequence is
+// faster in splits (100003 positions 27.8, in pieces 29.7), which take nothing to find, and so are
+// sequences that pieces hold several of, whose beginnings then lie behind one another (500 of up
+// to 1500, 32/4 heads of 128, 168 us; whole 87).  Pieces for one workgroup to a CU: 53 for 43; for
+// four, which spill registers, 52.
+struct Few8Cut {
+    int P, S, C;
+};
 __device__ __forceinline__ SeqView few8_view(const ServeAttnArgs &a, int i) {
     return i < a.b.n_seq ? seq_view(a.b.starts[i], a.b.starts[i + 1], a.b.lens[i], a.b.n_rows, a.kv.cap) : SeqView{0, 0, 0};
 }
-template <int M>  // rows of a sequence, at most
-__device__ __forceinline__ int few8_steps(const ServeAttnArgs &a, const SeqView &v) {
+// Rows of a sequence, at most
+template <int M>
+__device__ __forceinline__ int few8_rows(const ServeAttnArgs &a) { return imin(imin(a.b.max_new, M) * a.G, M); }
+__device__ __forceinline__ int few8_steps(const ServeAttnArgs &a, const SeqView &v, int R) {
     if (v.n_new == 0) return 0;
-    return imax(tile_count(key_range(v, 0, imin(v.n_new, (M + a.G - 1) / a.G) - 1, a.window), FEW8_STEP), 1) + FEW8_BEGIN;
+    return imax(tile_count(key_range(v, 0, imin(v.n_new, (R + a.G - 1) / a.G) - 1, a.window), FEW8_STEP), 1);
 }
-// Steps of a piece.  A sequence has under 2^24 and a call under 2^12 sequences, so a sum of 64 of
-// them fits 32 bits, that of all may not; P is no less than a sixteenth of the sequences, so a piece does.
-__device__ __forceinline__ int few8_per(int64_t total, int P) {
-    return imax(total >> 31 ? (int)((total + P - 1) / P) : (int)(((uint32_t)total + (uint32_t)P - 1) / (uint32_t)P), FEW8_LEAST);
+// A lane's sequence among those of pieces: its steps and its beginning
+__device__ __forceinline__ int few8_units(const ServeAttnArgs &a, const SeqView &v, int R) {
+    const int n = few8_steps(a, v, R);
+    return n ? n + FEW8_BEGIN : 0;
 }
-template <int HD, int M>
-__device__ __forceinline__ int64_t few8_part(int kvh, int P, int piece, bool begins) {  // begins: with the sequence's first step
-    return (((int64_t)kvh * P + piece) * 2 + begins) * (M * (HD + 2));
+// Units of a piece.  A sequence has at most 2^23 and a few, and pieces hold FEW8_SEQS sequences at most: sums fit 31 bits
+__device__ __forceinline__ int few8_per(int total, int P) { return imax((total + P - 1) / P, FEW8_LEAST); }
+// begins: of a piece, whether it has the sequence's first step
+template <int HD>
+__device__ __forceinline__ int64_t few8_part(const Few8Cut &cut, int kvh, int piece, bool begins, int R) {
+    return (((int64_t)kvh * cut.P + piece) * (cut.S ? 1 : 2) + (cut.S ? 0 : begins)) * (R * (HD + 2));
 }
 
 // A wave's values in LDS: it copies 1 KB at a time, RPI whole rows, by 16-byte chunk, then row
@@ -107,8 +125,8 @@ struct Value8Lds {
     static __device__ __forceinline__ int chunk(int lane) { return lane / RPI; }
 };
 
-template <int HD, bool BF, bool CAP, int NB>
-__global__ __launch_bounds__(256, few8_waves(HD, NB)) void attn8_few_kernel(ServeAttn8Args x, int P, float *parts) {
+template <int HD, bool BF, bool CAP, int NB, bool PIECES>
+__global__ __launch_bounds__(256, few8_waves(HD, NB, PIECES)) void attn8_few_kernel(ServeAttn8Args x, Few8Cut cut, float *parts) {
     using Lds = Value8Lds<HD>;
     const ServeAttnArgs &a = x.a;
     constexpr int KT = FEW8_KT, RPI = Lds::RPI, NLD = KT / RPI, DB = HD / 16;
@@ -117,15 +135,14 @@ __global__ __launch_bounds__(256, few8_waves(HD, NB)) void attn8_few_kernel(Serv
     constexpr int WB = VB > OB ? VB : OB;
     __shared__ __align__(16) uint8_t s_buf[4][WB];
     __shared__ float s_ml[4][16 * NB][2];
-    __shared__ int s_seq[4][6][64];
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.G, kvh = blockIdx.x % a.n_kv, piece = blockIdx.x / a.n_kv;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.G, R = few8_rows<16 * NB>(a), kvh = blockIdx.x % a.n_kv, piece = blockIdx.x / a.n_kv;
 
-    // what the piece, `per` steps, has of the n of sequence si, the first of which is the piece's number base
+    // what a piece of `per` steps has of the n of sequence si, the first of which is the piece's number base
     auto sequence = [&](int si, const SeqView &sv, int per, int base, int n) __attribute__((always_inline)) {
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));  // nothing of it is kept in registers from one sequence to the next
         const int g = lane >> 4, col = lane & 15;
-        const int n_rows = imin(sv.n_new * G, 16 * NB);
+        const int n_rows = imin(imin(sv.n_new, 16 * NB) * G, R);
         const int n_tok = same((n_rows + G - 1) / G), pos0 = sv.pos0();
         const KeyRange kr = key_range(sv, 0, n_tok - 1, a.window);
         const int hi = same(kr.hi), t0 = same(first_tile(kr, FEW8_STEP)), nt = same(tile_count(kr, FEW8_STEP));
@@ -413,77 +430,65 @@ __global__ __launch_bounds__(256, few8_waves(HD, NB)) void attn8_few_kernel(Serv
                 uint8_t *op = a.out + (int64_t)(sv.row0 + tok) * a.o_row + head * a.o_head + d4 * 8;
                 *(u32x2 *)op = u32x2{pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
             } else {
-                float *pp = parts + few8_part<HD, 16 * NB>(kvh, P, piece, base >= 0);
+                float *pp = parts + few8_part<HD>(cut, kvh, piece, base >= 0, R);
                 *(f32x4 *)(pp + r * HD + d4 * 4) = acc;
-                if (d4 == 0) *(f32x2 *)(pp + 16 * NB * HD + r * 2) = f32x2{mm, L};
+                if (d4 == 0) *(f32x2 *)(pp + R * HD + r * 2) = f32x2{mm, L};
             }
         }
     };
 
-    constexpr int M = 16 * NB;
-    const int lane = threadIdx.x & 63;
-    SeqView view = few8_view(a, P ? lane : piece);
-    int i0 = P ? 0 : piece, per = INT32_MAX, first = lane == 0 && view.n_new > 0 ? 1 + FEW8_BEGIN : 0;  // P = 0: a workgroup for each
-    int64_t before = 0;  // steps before the chunk's sequences, from the piece's first on
-    if (P) {
-        first = few8_steps<M>(a, view);
-        int64_t total = a.b.n_seq > 1 ? same(xsum_i<64>(first)) : same(first);
-        for (int i = 64; i < a.b.n_seq; i += 64) total += same(xsum_i<64>(few8_steps<M>(a, few8_view(a, i + lane))));
-        per = same(few8_per(total, P));
-        before = -(int64_t)piece * per;
-    }
-    const int i_first = i0;
-    bool again = false;
-    for (; i0 < a.b.n_seq && before < per; i0 += P ? 64 : a.b.n_seq) {
-        int n = first;
-        if (i0 != i_first) {
-            view = few8_view(a, i0 + lane);
-            n = few8_steps<M>(a, view);
-        }
+    if constexpr (PIECES) {
+        __shared__ int s_seq[4][6][64];
+        const int lane = threadIdx.x & 63;
+        const SeqView view = few8_view(a, lane);
+        const int n = few8_units(a, view, R);
         int upto = n;
-        if (P && a.b.n_seq > 1) {
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(upto, o);
-                if (lane >= o) upto += y;
-            }
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o);
+            if (lane >= o) upto += y;
         }
-        const int sum = __builtin_amdgcn_readlane(upto, P && a.b.n_seq > 1 ? 63 : 0);
-        if (before + sum > 0) {
-            const int base = (int)before + upto - n + FEW8_BEGIN;
-            const int mine_of[6] = {base, n - FEW8_BEGIN, view.row0, view.n_new, view.len, view.over};
+        const int per = same(few8_per(__builtin_amdgcn_readlane(upto, 63), cut.P));
+        const int base = (int)(upto - n + FEW8_BEGIN - min((int64_t)piece * per, (int64_t)1 << 30));
+        const int mine_of[6] = {base, n - FEW8_BEGIN, view.row0, view.n_new, view.len, view.over};
 #pragma unroll
-            for (int i = 0; i < 6; i++) s_seq[w][i][lane] = mine_of[i];
-            for (uint64_t mine = __ballot(n > 0 && base < per && base - FEW8_BEGIN + n > 0); mine; mine &= mine - 1) {
-                const int j = __builtin_ctzll(mine);
-                if (again) __syncthreads();  // the one before has been read
-                again = true;
-                auto of = [&](int i) { return same(s_seq[w][i][j]); };
-                sequence(i0 + j, SeqView{of(2), of(3), of(4), of(5)}, per, of(0), of(1));
-            }
+        for (int i = 0; i < 6; i++) s_seq[w][i][lane] = mine_of[i];
+        bool again = false;
+        for (uint64_t mine = __ballot(n > 0 && base < per && base - FEW8_BEGIN + n > 0); mine; mine &= mine - 1) {
+            const int j = __builtin_ctzll(mine);
+            if (again) __syncthreads();  // the one before has been read
+            again = true;
+            auto of = [&](int i) { return same(s_seq[w][i][j]); };
+            sequence(j, SeqView{of(2), of(3), of(4), of(5)}, per, of(0), of(1));
         }
-        before += sum;
+    } else {
+        const int split = piece / a.b.n_seq, si = piece - split * a.b.n_seq;
+        const SeqView sv = view_of(a.b, a.kv, si);
+        const int n = same(few8_steps(a, sv, R));
+        if (n > split * cut.C) sequence(si, sv, split == cut.S - 1 ? 1 << 30 : cut.C, -split * cut.C, n);
     }
 }
 
-// Sequences that several pieces have a part of: a workgroup for each row
+// Sequences that several pieces or splits have a part of: a workgroup for each row
 template <int HD, bool BF, int M>
-__global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, int P, const float *parts) {
+__global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, Few8Cut cut, const float *parts) {
     __shared__ f32x4 s_o[256];
-    const int lane = threadIdx.x & 63, kvh = blockIdx.x % a.n_kv, si = blockIdx.x / a.n_kv, r = blockIdx.y;
-    int64_t total = 0, base = FEW8_BEGIN;
-    for (int i0 = 0; i0 < a.b.n_seq; i0 += 64) {
-        const int n = few8_steps<M>(a, few8_view(a, i0 + lane));
-        total += same(xsum_i<64>(n));
-        base += same(xsum_i<64>(i0 + lane < si ? n : 0));
-    }
+    const int lane = threadIdx.x & 63, kvh = blockIdx.x % a.n_kv, si = blockIdx.x / a.n_kv, r = blockIdx.y, R = few8_rows<M>(a);
     const SeqView sv = view_of(a.b, a.kv, si);
-    const int n = same(few8_steps<M>(a, sv)) - FEW8_BEGIN, per = same(few8_per(total, P));
-    if (r >= imin(sv.n_new, M) * a.G || r >= M) return;
-    const int j0 = base >> 31 ? (int)(base / per) : (int)((uint32_t)base / (uint32_t)per), ns = ((int)(base - (int64_t)j0 * per) + n - 1) / per + 1;
+    const int n = same(few8_steps(a, sv, R));
+    if (r >= imin(imin(sv.n_new, M) * a.G, R)) return;
+    int j0 = 0, ns;
+    if (cut.S) {
+        ns = split_count(n, cut.C, cut.S);
+    } else {
+        const int units = few8_units(a, few8_view(a, lane), R);
+        const int per = same(few8_per(xsum_i<64>(units), cut.P)), base = same(xsum_i<64>(lane < si ? units : 0)) + FEW8_BEGIN;
+        j0 = base / per;
+        ns = (base - j0 * per + n - 1) / per + 1;
+    }
     if (ns == 1) return;
     constexpr int LPR = HD / 4, AT_ONCE = 256 / LPR;  // lanes of a part's row, parts at a time
-    auto part = [&](int s) { return parts + few8_part<HD, M>(kvh, P, j0 + s, s == 0); };
+    auto part = [&](int s) { return parts + few8_part<HD>(cut, kvh, cut.S ? s * a.b.n_seq + si : j0 + s, s == 0, R); };
     const int g = threadIdx.x / LPR, d = threadIdx.x % LPR;
     const bool in = g < AT_ONCE;
     constexpr int FIRST = 16;  // requested before their weights are known
@@ -494,12 +499,12 @@ __global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, int P, 
         if (k * AT_ONCE >= ns) break;
         const float *p = part(imin(g + k * AT_ONCE, ns - 1));
         y[k] = *(const f32x4 *)(p + r * HD + d * 4);
-        my[k] = p[M * HD + r * 2];
+        my[k] = p[R * HD + r * 2];
     }
     float m = -FLT_MAX, l = 0;
 #pragma unroll 2
     for (int s = lane; s < ns; s += 64) {
-        const f32x2 ml = *(const f32x2 *)(part(s) + M * HD + r * 2);
+        const f32x2 ml = *(const f32x2 *)(part(s) + R * HD + r * 2);
         const float mn = fmaxf(m, ml[0]);
         l = fmaf(l, exp2_hw(m - mn), ml[1] * exp2_hw(ml[0] - mn));
         m = mn;
@@ -517,7 +522,7 @@ __global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, int P, 
         if (in && g + k * AT_ONCE < ns) add(my[k], y[k]);
     }
 #pragma unroll 4
-    for (int s = in ? g + FIRST * AT_ONCE : ns; s < ns; s += AT_ONCE) add(part(s)[M * HD + r * 2], *(const f32x4 *)(part(s) + r * HD + d * 4));
+    for (int s = in ? g + FIRST * AT_ONCE : ns; s < ns; s += AT_ONCE) add(part(s)[R * HD + r * 2], *(const f32x4 *)(part(s) + r * HD + d * 4));
     s_o[threadIdx.x] = acc;
     __syncthreads();
     if (threadIdx.x >= LPR) return;
@@ -1273,13 +1278,16 @@ int64_t span8(const ServeAttnArgs &a, int tokens, int KT) {
 
 bool few8(const ServeAttnArgs &a) { return few_row_blocks(true, a.b.max_new, a.G) > 0; }
 
-// Pieces per KV head that a launch of the few-rows kernel is divided into, or 0: a workgroup for
-// each sequence, where these are short or enough to fill the card several times.
-int few8_pieces(const ServeAttnArgs &a) {
-    const int64_t steps = (span8(a, FEW_ROWS, FEW8_STEP) + FEW8_STEP - 1) / FEW8_STEP, seqs = a.b.n_seq;
-    if (steps < 4 || seqs * a.n_kv >= 4096) return 0;
-    const int slots = 256 * few8_waves(a.hd, few_row_blocks(true, a.b.max_new, a.G)) / a.n_kv;
-    return (int)std::min<int64_t>(seqs * steps / FEW8_LEAST, std::max(slots, 1));
+int few8_rows_most(const ServeAttnArgs &a) { return (int)std::min<int64_t>((int64_t)a.b.max_new * a.G, 16 * few_row_blocks(true, a.b.max_new, a.G)); }
+Few8Cut few8_cut(const ServeAttnArgs &a) {
+    const int steps = (int)((span8(a, FEW_ROWS, FEW8_STEP) + FEW8_STEP - 1) / FEW8_STEP), slots = 256 * few8_waves(a.hd, few_row_blocks(true, a.b.max_new, a.G), true);
+    const int64_t wgs = (int64_t)a.b.n_seq * a.n_kv;
+    if (steps >= 2 * FEW8_LEAST && a.b.n_seq > 1 && a.b.n_seq <= FEW8_SEQS && wgs <= slots)
+        return Few8Cut{(int)std::min<int64_t>((int64_t)a.b.n_seq * steps / FEW8_LEAST, slots / a.n_kv), 0, 0};
+    // splits of two steps where workgroups are few; where they fill the card, of twelve (500 sequences
+    // of up to 1500, 32/4 heads of 128, 111 us with two, 87 whole; 128 of up to 8000, 202 and 242)
+    const SplitPlan p = split_plan(wgs, steps, 4096, wgs < 512 ? FEW8_LEAST : 12, SERVE_MAX_SPLIT);
+    return Few8Cut{a.b.n_seq * p.S, p.S, p.C};
 }
 
 // Pieces per KV head that a launch of the tile kernel is divided into, or 0: a workgroup for each
@@ -1324,10 +1332,16 @@ void launch_tile(const ServeAttn8Args &x, void *ws, hipStream_t st) {
 template <int HD, bool BF, int NB>
 void launch_few(const ServeAttn8Args &x, void *ws, hipStream_t st) {
     const ServeAttnArgs &a = x.a;
-    const int P = few8_pieces(a), grid = (P ? P : a.b.n_seq) * a.n_kv;
-    if (a.softcap > 0) attn8_few_kernel<HD, BF, true, NB><<<grid, 256, 0, st>>>(x, P, (float *)ws);
-    else attn8_few_kernel<HD, BF, false, NB><<<grid, 256, 0, st>>>(x, P, (float *)ws);
-    if (P) few8_join_kernel<HD, BF, 16 * NB><<<dim3(a.b.n_seq * a.n_kv, std::min(a.b.max_new * a.G, 16 * NB)), 256, 0, st>>>(a, P, (const float *)ws);
+    const Few8Cut cut = few8_cut(a);
+    const int64_t grid = (int64_t)cut.P * a.n_kv;
+    if (cut.S) {
+        if (a.softcap > 0) attn8_few_kernel<HD, BF, true, NB, false><<<grid, 256, 0, st>>>(x, cut, (float *)ws);
+        else attn8_few_kernel<HD, BF, false, NB, false><<<grid, 256, 0, st>>>(x, cut, (float *)ws);
+    } else {
+        if (a.softcap > 0) attn8_few_kernel<HD, BF, true, NB, true><<<grid, 256, 0, st>>>(x, cut, (float *)ws);
+        else attn8_few_kernel<HD, BF, false, NB, true><<<grid, 256, 0, st>>>(x, cut, (float *)ws);
+    }
+    if (cut.S != 1) few8_join_kernel<HD, BF, 16 * NB><<<dim3(a.b.n_seq * a.n_kv, few8_rows_most(a)), 256, 0, st>>>(a, cut, (const float *)ws);
 }
 
 template <int HD, bool BF>
@@ -1368,7 +1382,8 @@ void launch_append(const PagedAppend8Args &x, int grid, hipStream_t st) {
 
 size_t serve_attn8_ws(const ServeAttnArgs &a) {
     if (!few8(a)) return tile8_ws(a).bytes;
-    return (size_t)few8_pieces(a) * a.n_kv * 2 * 16 * few_row_blocks(true, a.b.max_new, a.G) * (a.hd + 2) * sizeof(float);
+    const Few8Cut cut = few8_cut(a);
+    return cut.S == 1 ? 0 : (size_t)cut.P * a.n_kv * (cut.S ? 1 : 2) * few8_rows_most(a) * (a.hd + 2) * sizeof(float);
 }
 
 void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st) {
