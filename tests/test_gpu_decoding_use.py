@@ -330,3 +330,49 @@ def test_lengths_beyond_the_bound_stay_in_bounds(ops):
     o, a, size = S.attend(q[7:8], k, v, 29999, hd ** -0.5)
     tol = R.tolerance(o, a, q[7:8], k, v, hd ** -0.5, 30000, hd, F16, size)
     assert bool(((out[7:8].cpu().double() - o).abs() <= tol).all())
+
+
+def test_single_tokens_captured_and_replayed_over_other_lengths(ops):
+    """the cuts move with the lengths; two graphs with a workspace each, replayed in turn"""
+    b = R.Batch8([(1, 4000)] * 5, 8, 2, 64, page=64, block=64, dtype=F16, seed=55)
+    kv = ops.PagedKv(b.paged(b.k_pages.to(GPU)), b.paged(b.v_pages.to(GPU)), b.table.to(GPU), k_scale=b.k_scale.to(GPU), v_scale=b.v_scale.to(GPU))
+    starts, lens, q = b.starts.to(GPU), b.L.to(GPU), b.q.to(GPU)
+    out = [torch.empty_like(q) for _ in range(2)]
+    calls = [ops.PagedAttention(kv, ops.Seqs(starts, lens, max_new=3, max_len=4000), q, o) for o in out]
+    graphs = []
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call()
+    for new, length in (((1, 1, 1, 1, 1), (4000, 1, 128, 129, 0)), ((0, 3, 0, 2, 0), (9, 4000, 0, 3999, 4000)), ((0, 0, 0, 0, 1), (0, 0, 0, 0, 4000)), ((1, 1, 1, 1, 1), (1, 1, 1, 1, 1)), ((1, 1, 1, 1, 1), (4000,) * 5)):
+        b.lens = list(zip(new, length))
+        b.starts = torch.tensor([sum(new[:i]) for i in range(6)], dtype=torch.int32)
+        starts.copy_(b.starts)
+        lens.copy_(torch.tensor(length, dtype=torch.int32))
+        for graph, o in zip(graphs, out):
+            o.fill_(7.0)
+            graph.replay()
+        for o in out:
+            check(b, o.cpu())
+        settle()
+
+
+def test_two_batches_of_single_tokens_at_once_on_two_streams(ops):
+    b = R.Batch8([(1, 5000), (1, 100), (1, 3000), (1, 1)], 8, 2, 128, page=64, block=32, dtype=BF16, seed=56)
+    kv = ops.PagedKv(b.paged(b.k_pages.to(GPU)), b.paged(b.v_pages.to(GPU)), b.table.to(GPU), k_scale=b.k_scale.to(GPU), v_scale=b.v_scale.to(GPU))
+    seqs = ops.Seqs(b.starts.to(GPU), b.L.to(GPU), max_new=1, max_len=5000)
+    q = [b.q.to(GPU), -b.q.to(GPU)]
+    out = [torch.empty_like(x) for x in q]
+    calls = [ops.PagedAttention(kv, seqs, x, o) for x, o in zip(q, out)]
+    for c in calls:
+        c()
+    want = [o.cpu() for o in out]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, s in zip(calls, streams):
+            c(stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o.cpu(), w) for o, w in zip(out, want))
