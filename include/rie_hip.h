@@ -416,7 +416,11 @@ int32_t rie_hip_k_page_reserve(const rie_hip_pool *pool, void *ws, size_t ws_byt
  * partial last page, and what it holds behind that, stays with the row itself if it goes on (src[i]
  * = i), else with the first that takes it; the others get a new page, which the call fills from the
  * n_bufs caches, or −1 where the pool has none (new pages are those that were free before the
- * call).  Pages that no row holds any more become free. */
+ * call).  Where refs says that the partial page has more than one holder before the call (a row was
+ * cut back into pages that it shared), nobody keeps it and all get new ones, and of the pages
+ * behind, those before the first such one stay: after a fork no row holds a page from its last
+ * position's on that another row holds too.
+ * Pages that no row holds any more become free. */
 int32_t rie_hip_k_page_fork(const rie_hip_pool *pool, const int32_t *src, const rie_hip_page_buf *bufs, int32_t n_bufs, void *ws,
                             size_t ws_bytes, void *stream, char *err, size_t err_len);
 /* Rows with which[i] != 0 give up their pages and positions. */

@@ -142,6 +142,13 @@ __global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
 }
 
 // ---- fork ----
+//
+// Of those that take a row, its keeper (the row itself, or the first of them) goes on with what that
+// row may write next: its partial last page, and the pages held behind it.  Others may hold these
+// too, where a row has been cut back into pages that it shared.  Then no row goes on with them: a
+// partial page that another row holds is copied for the keeper as well, even where all that hold it
+// are in this call (one page more than it would take, but no choice among them), and of the pages
+// behind, the keeper gets those before the first that another row holds.
 struct Child {  // what becomes of a row
     int src, held, old_held, len;
     int at, fresh;  // place of the source's partial page where the row gets a copy of it (−1: none), and that copy (−1: the pool has none)
@@ -151,7 +158,19 @@ struct Lists {
     int pad[3];
 };
 
-__global__ __launch_bounds__(PLAN) void fork_plan_kernel(PoolView p, const int *src, Lists *lists, Child *child, int *children, int *from, int *to, int *list) {
+// The first of row r's pages [from, to) that more than one row holds, or to: 64 at a time, with the same
+// arguments in all of a wave's lanes
+__device__ __forceinline__ int first_shared(const PoolView &p, int r, int from, int to) {
+    const int lane = threadIdx.x & 63;
+    for (int k = from; k < to; k += 64) {
+        const int page = k + lane < to ? p.table[r * p.table_stride + k + lane] : -1;
+        const uint64_t shared = __ballot((unsigned)page < (unsigned)p.n_pages && p.refs[page] > 1);
+        if (shared) return k + __builtin_ctzll(shared);
+    }
+    return to;
+}
+
+__global__ __launch_bounds__(PLAN) void fork_plan_kernel(PoolView p, const int *src, Lists *lists, Child *child, int *children, int *kept, int *from, int *to, int *list) {
     __shared__ int s_count[POOL_MAX_SEQ], s_heir[POOL_MAX_SEQ];  // children of a row, and which of them inherits its partial page
     __shared__ int s[PLAN / 64];
     constexpr int ROUNDS = POOL_MAX_SEQ / PLAN;
@@ -182,6 +201,8 @@ __global__ __launch_bounds__(PLAN) void fork_plan_kernel(PoolView p, const int *
         const int i = u * PLAN + (int)threadIdx.x;
         c[u] = Child{r[u], 0, 0, 0, -1, -1};
         old[u] = -1;
+        int ahead = -1;  // of a keeper with pages behind its last position, the first of them
+        bool keeps = false, shared = false;
         if (u * PLAN >= p.n_seq) continue;
         if (i < p.n_seq) {
             children[i] = s_count[i];
@@ -192,11 +213,19 @@ __global__ __launch_bounds__(PLAN) void fork_plan_kernel(PoolView p, const int *
             const bool keep = r[u] == i || s_heir[r[u]] == i;  // it takes the source's pages as they are
             c[u].held = keep ? q.held : min(q.touched, q.held);
             c[u].len = p.lens[r[u]];
-            if (!keep && q.touched > q.full && q.held > q.full) {
-                c[u].at = q.full;
+            if (q.touched > q.full && q.held > q.full) {
                 old[u] = p.table[r[u] * p.table_stride + q.full];
+                shared = keep && (unsigned)old[u] < (unsigned)p.n_pages && p.refs[old[u]] > 1;
+                if (!keep || shared) c[u].at = q.full;
             }
+            keeps = keep;
+            ahead = keep && q.held > q.touched ? q.touched : -1;
         }
+        for (uint64_t m = __ballot(ahead >= 0); m; m &= m - 1) {
+            const int j = __builtin_ctzll(m), first = first_shared(p, __shfl(r[u], j), __shfl(ahead, j), __shfl(c[u].held, j));
+            if ((int)(threadIdx.x & 63) == j) c[u].held = first;
+        }
+        if (keeps) kept[r[u]] = shared ? ~c[u].held : c[u].held;
         int total;
         mine[u] = want + scan(c[u].at >= 0, s, total);
         want += total;
@@ -257,18 +286,20 @@ __device__ void copy_pages(const Bufs &bufs, int g, int n, const int *from, cons
 }
 
 // The old rows' references, and the rows that others go on from into `rows`, a workgroup each; and the copies
-__global__ __launch_bounds__(256) void fork_refs_kernel(PoolView p, Bufs bufs, int row_wgs, const Lists *lists, const int *src, const int *children, const int *from, const int *to, int *rows) {
+__global__ __launch_bounds__(256) void fork_refs_kernel(PoolView p, Bufs bufs, int row_wgs, const Lists *lists, const int *src, const int *children, const int *kept, const int *from, const int *to, int *rows) {
     if ((int)blockIdx.x >= row_wgs) {
         copy_pages(bufs, blockIdx.x - row_wgs, gridDim.x - row_wgs, from, to, lists->n, p.n_pages);
         return;
     }
     const int r = blockIdx.x, n = children[r];
     const bool stays = (unsigned)src[r] < (unsigned)p.n_seq && src[r] == r;
-    if (n == 1 && stays) return;
     const Seq q = seq_of(p, r);
+    // pages before this one stay with the keeper; negative: ~ it, and the partial one does not
+    const int k = n ? kept[r] : 0, stay = k < 0 ? ~k : k;
+    if (n == 1 && stays && k == q.held) return;
     const int *t = p.table + r * p.table_stride;
     for (int c = threadIdx.x; c < q.held; c += 256) {
-        const int page = t[c], change = c < q.full ? n - 1 : n == 0 ? -1 : 0;
+        const int page = t[c], change = c < q.full ? n - 1 : c >= stay || (k < 0 && c == q.full) ? -1 : 0;
         if (n) rows[(int64_t)r * p.cols + c] = page;
         if (change && (unsigned)page < (unsigned)p.n_pages) atomicAdd(p.refs + page, change);
     }
@@ -278,7 +309,7 @@ __global__ __launch_bounds__(256) void fork_refs_kernel(PoolView p, Bufs bufs, i
 __global__ __launch_bounds__(256) void fork_rows_kernel(PoolView p, const Child *child, const int *rows) {
     const int i = blockIdx.x;
     const Child c = child[i];
-    if (c.src == i) return;  // and keeps its pages
+    if (c.src == i && c.at < 0 && c.held == c.old_held) return;  // and keeps its pages
     int *t = p.table + i * p.table_stride;
     const int *r = rows + (int64_t)max(c.src, 0) * p.cols;
     for (int k = threadIdx.x; k < max(c.held, c.old_held); k += 256) t[k] = k >= c.held ? -1 : k == c.at ? c.fresh : r[k];
@@ -380,7 +411,7 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t page_reserve_ws(const PoolView &p) { return up16((size_t)p.n_pages * sizeof(int)); }
 
 size_t page_fork_ws(const PoolView &p) {
-    return sizeof(Lists) + up16(p.n_seq * sizeof(Child)) + 4 * up16(p.n_seq * sizeof(int)) + up16((size_t)p.n_seq * p.cols * sizeof(int));
+    return sizeof(Lists) + up16(p.n_seq * sizeof(Child)) + 5 * up16(p.n_seq * sizeof(int)) + up16((size_t)p.n_seq * p.cols * sizeof(int));
 }
 
 size_t page_compact_ws(const PoolView &p) { return sizeof(Lists) + 3 * up16((size_t)p.n_pages * sizeof(int)); }
@@ -393,17 +424,17 @@ void launch_page_fork(const PoolView &p, const int *src, const PageBuf *bufs, in
     w += sizeof(Lists);
     Child *child = (Child *)w;
     w += up16(p.n_seq * sizeof(Child));
-    int *ints[4];  // children, pages copied from and to, free ones
+    int *ints[5];  // children, pages that their keepers keep, pages copied from and to, free ones
     for (int *&x : ints) {
         x = (int *)w;
         w += up16(p.n_seq * sizeof(int));
     }
     int *rows = (int *)w;
-    fork_plan_kernel<<<1, PLAN, 0, st>>>(p, src, lists, child, ints[0], ints[1], ints[2], ints[3]);
+    fork_plan_kernel<<<1, PLAN, 0, st>>>(p, src, lists, child, ints[0], ints[1], ints[2], ints[3], ints[4]);
     int done = 0;
     do {
         const int n = std::min(n_bufs - done, MAX_BUFS), row_wgs = done ? 0 : p.n_seq;
-        fork_refs_kernel<<<row_wgs + (n ? COPY_WGS : 0), 256, 0, st>>>(p, bufs_of(bufs + done, n), row_wgs, lists, src, ints[0], ints[1], ints[2], rows);
+        fork_refs_kernel<<<row_wgs + (n ? COPY_WGS : 0), 256, 0, st>>>(p, bufs_of(bufs + done, n), row_wgs, lists, src, ints[0], ints[1], ints[2], ints[3], rows);
         done += n;
     } while (done < n_bufs);
     fork_rows_kernel<<<p.n_seq, 256, 0, st>>>(p, child, rows);
