@@ -409,7 +409,8 @@ typedef struct rie_hip_page_buf {
 /* workspace of any of the calls below */
 size_t rie_hip_k_page_ws(const rie_hip_pool *pool);
 /* Pages for the positions of every sequence: rows that hold fewer than lens needs get more.
- * Where the pool runs out, later rows get fewer. */
+ * Where the pool runs out, later rows get fewer.  Pages for positions behind table_cols pages,
+ * which a row has no room for, are counted as lacking too (counts[0] is 2^31-1 at most). */
 int32_t rie_hip_k_page_reserve(const rie_hip_pool *pool, void *ws, size_t ws_bytes, void *stream, char *err, size_t err_len);
 /* Row i becomes what row src[i] was (all at once; several rows may take one, and a row whose src
  * is none, a number outside 0..n_seq-1, becomes empty).  Pages that are full are shared.  A source's

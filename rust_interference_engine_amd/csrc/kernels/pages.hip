@@ -103,16 +103,21 @@ __device__ __forceinline__ Seq seq_of(const PoolView &p, int i) {
 __global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
     __shared__ int s[PLAN / 64];
     __shared__ int s_at[POOL_MAX_SEQ + 1];  // pages that the rows before need, up to all there are
+    __shared__ unsigned long long s_beyond;  // those that positions behind the columns need: lacking, whatever the pool has
     const uint32_t bits0 = free_in_round(p, 0);
     int64_t want = 0;
+    if (threadIdx.x == 0) s_beyond = 0;
     for (int i0 = 0; i0 < p.n_seq; i0 += PLAN) {
         const int i = i0 + (int)threadIdx.x;
-        int need = 0, total;
+        int need = 0, beyond = 0, total;
         if (i < p.n_seq) {
             const Seq q = seq_of(p, i);
             need = max(q.touched - q.held, 0);
+            const int len = max(p.lens[i], 0);
+            beyond = max((len >> p.page_shift) + ((len & ((1 << p.page_shift) - 1)) != 0) - p.cols, 0);
         }
         const int before = scan(need, s, total);
+        if (beyond) atomicAdd(&s_beyond, (unsigned long long)beyond);
         if (i < p.n_seq) s_at[i] = (int)min(want + before, (int64_t)p.n_pages);
         want += total;
     }
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(PLAN) void reserve_kernel(PoolView p, int *list) {
         const int got = max(min(s_at[i + 1], found) - s_at[i], 0);
         if (got) p.held[i] = q.held + got;
     }
-    if (threadIdx.x == 0) p.counts[0] = (int)min(want - found, (int64_t)INT32_MAX);
+    if (threadIdx.x == 0) p.counts[0] = (int)min(want - found + (int64_t)s_beyond, (int64_t)INT32_MAX);
 }
 
 // ---- fork ----

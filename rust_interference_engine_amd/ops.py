@@ -441,7 +441,8 @@ def _page_bufs(caches, n_pages: int):
 
 
 class PageReserve(_Op):
-    """Pages for the positions that ``pool.lens`` says: the lowest free ones, row by row."""
+    """Pages for the positions that ``pool.lens`` says: the lowest free ones, row by row.  What the pool lacks is counted in
+    ``pool.counts[0]``, and what a row of the table has no room for."""
 
     def __init__(self, pool: PagePool):
         self._ready(_lib.lib().rie_hip_k_page_reserve, [C.byref(pool._struct)], pool.device, pool._workspace(), 1, (pool,))

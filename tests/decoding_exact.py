@@ -42,3 +42,7 @@ class SharedPool(D.Pool):
             for a, b in copies:
                 c[b] = c[a]
         self.rows, self.lens, self.counts[0] = rows, lens, lacked
+
+    def reserve(self):
+        super().reserve()
+        self.counts[0] += sum(max(0, -(-x // self.page) - self.cols) for x in self.lens)

@@ -1,4 +1,4 @@
-"""Pools of pages on the GPU where rows have been cut back into pages that other rows hold."""
+"""Pools of pages on the GPU where rows have been cut back into pages that other rows hold, and where they outgrow their table."""
 import random
 
 import pytest
@@ -143,3 +143,29 @@ def test_what_a_cut_sequence_appends_leaves_the_other_as_it_was(ops):
     ops.PagedAppend(kv, seqs, x[:, :KV], x[:, KV:])()
     assert torch.equal(codes[:, held].cpu(), before[0]) and torch.equal(scales[:, held].cpu(), before[1])
     assert torch.equal(pool.table[1, :3].long(), held)
+
+
+# ---- rows that outgrow their table ----
+
+def test_reserve_counts_the_pages_that_a_table_has_no_room_for(ops):
+    b = Both(ops, [[], [2], [5, 6]], [100, 200, 17], 30, 4, 16)
+    reserve = ops.PageReserve(b.pool)
+    reserve()
+    b.ref.reserve()
+    b.check()
+    assert b.pool.counts.tolist()[0] == 3 + 9
+    b.shorten([64, 64, 64])
+    reserve()
+    b.ref.reserve()
+    b.check()
+    assert b.pool.counts.tolist()[0] == 0
+    b.shorten([2 ** 31 - 1, 2 ** 31 - 1, -5])
+    reserve()
+    assert b.pool.counts.tolist()[0] == 2 * (2 ** 31 // 16 - 4)
+
+
+def test_reserve_counts_beyond_31_bits_as_the_largest_number(ops):
+    pool = ops.PagePool.empty(9, 3000, 2, 1, GPU)
+    pool.lens.fill_(2 ** 31 - 1)
+    ops.PageReserve(pool)()
+    assert pool.counts.tolist()[0] == 2 ** 31 - 1 and pool.held.tolist() == [2] * 4 + [1] + [0] * 2995
