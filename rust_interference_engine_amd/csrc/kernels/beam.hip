@@ -526,6 +526,8 @@ BeamPlan beam_plan(int rows, int V) {
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
+constexpr size_t LDS_UNASKED = 32 << 10;  // dynamic LDS that, with what the kernel has itself, is under the 64 KiB that need not be asked for
+
 template <int TY>
 void launch_ty(const BeamArgs &a, void *ws, hipStream_t st) {
     const int rows = a.n * a.n_beams, k = std::min(a.n_out, a.V);
@@ -541,7 +543,10 @@ void launch_ty(const BeamArgs &a, void *ws, hipStream_t st) {
     w += up16((size_t)rows * p.n_groups * sizeof(float));
     int *arrived = (int *)w;
     beam_part_kernel<TY><<<(int)(((int64_t)rows * p.n_parts + 3) / 4), 256, 0, st>>>(a, p.n_groups, p.steps, p.per, p.n_parts, gmax, runs, arrived);
-    beam_row_kernel<TY><<<rows, 256, (size_t)a.n_beams * k * sizeof(double), st>>>(a, p.n_groups, p.steps, p.n_parts, gmax, runs, key, id, arrived);
+    // the merge's sums: up to 64 KiB (64 beams of 128), beside 13 KiB that the rows take
+    const size_t lds = (size_t)a.n_beams * k * sizeof(double);
+    if (lds > LDS_UNASKED) RIE_HIP_CHECK(hipFuncSetAttribute((const void *)beam_row_kernel<TY>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    beam_row_kernel<TY><<<rows, 256, lds, st>>>(a, p.n_groups, p.steps, p.n_parts, gmax, runs, key, id, arrived);
 }
 
 }  // namespace
