@@ -1154,7 +1154,7 @@ __global__ __launch_bounds__(256) void tile8_join_kernel(ServeAttnArgs a, int KT
 //
 // A wave takes what a call brings to one block of positions, of one head's keys or values: the
 // rows' largest value, the block's new scale, the codes of earlier positions where it has grown,
-// and the new ones.  Codes are rounded from f64 quotients, so that they are those of the formula.
+// and the new ones.  Codes are those of the formula, ties to even (codes8).
 // Blocks are numbered without a list: sequence i owns ids from ⌊start / block⌋ + 2 i on, which
 // are enough, since n new tokens touch at most ⌊n / block⌋ + 2 blocks.
 //
@@ -1176,6 +1176,37 @@ __device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = value16<SRC == T_BF16>(a[e / 2] >> (e & 1) * 16 & 0xFFFF);
     }
+}
+
+// 8 codes x / s, to the nearest whole number, ties to even; inv: 1 / s in f64.  In f32 a quotient is
+// off by under 2^-15 (three roundings of numbers up to 128), so what is 2^-14 or more away from half
+// way between two numbers goes the right way.  The others are formed in f64 (prompts 12.2 us with all
+// of them so): x and s have at most 32 bits, so a quotient that is not half way itself is 2^-34 of
+// its size away, and x · inv, good to 2^-52, goes the right way.  One that is may go either way; what
+// is left then is s / 2 exactly, in the fma as in truth.
+template <class F>
+__device__ __forceinline__ u32x2 codes8(F x, double inv, float s) {
+    const float inv_f = (float)inv;
+    int c[8];
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float t = (float)x(e) * inv_f, q = rintf(t);
+        near = near || fabsf(t - q) > 0.5f - 0x1p-14f;
+        c[e] = (int)q;
+    }
+    if (near) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double y = x(e), q = rint(y * inv), left = fma(-q, (double)s, y);
+            c[e] = (int)q;
+            if (fabs(left) == 0.5 * s && (c[e] & 1)) c[e] += left > 0 ? 1 : -1;
+        }
+    }
+    u32x2 y = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e / 4] |= ((uint32_t)c[e] & 255) << e % 4 * 8;
+    return y;
 }
 
 template <int HD, int SRC>
@@ -1236,33 +1267,22 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     if (__any(!fine) || now > SCALE8_MAX || !(was >= 0 && was <= SCALE8_MAX)) now = NAN;
     else now = fmaxf(now, was);
     if (lane == 0) *sp = now;
+    const double inv = now > 0 ? 1.0 / (double)now : 0.0;
     if (first > b0 && now > was) {  // codes of earlier positions
-        const double f = (double)was / (double)now;
         for (int q = r; q < first - b0; q += RP) {
             if (!on) break;
             u32x2 *p = (u32x2 *)(dst + q * row + ch * 8);
-            u32x2 y = *p;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = (int)(int8_t)(y[e / 4] >> e % 4 * 8);
-                const uint32_t again = (uint32_t)__double2int_rn(c * f) & 255;
-                y[e / 4] = (y[e / 4] & ~(255u << e % 4 * 8)) | again << e % 4 * 8;
-            }
-            *p = y;
+            const u32x2 y = *p;
+            *p = codes8([&](int e) { return (double)(int8_t)(y[e / 4] >> e % 4 * 8) * (double)was; }, inv, now);
         }
     }
-    const double inv = now > 0 ? 1.0 / (double)now : 0.0;
     for (int r0 = 0; r0 < n; r0 += ROWS) {
         if (n > ROWS) load(r0);
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int q = r0 + i * RP + r;
             if (!(on && i * RP + r < ROWS && q < n)) continue;
-            u32x2 y = {0, 0};
-            if (inv > 0)
-#pragma unroll
-                for (int e = 0; e < 8; e++) y[e / 4] |= ((uint32_t)__double2int_rn((double)v[i][e] * inv) & 255) << e % 4 * 8;
-            *(u32x2 *)(dst + (first - b0 + q) * row + ch * 8) = y;
+            *(u32x2 *)(dst + (first - b0 + q) * row + ch * 8) = inv > 0 ? codes8([&](int e) { return v[i][e]; }, inv, now) : u32x2{0, 0};
         }
     }
 }

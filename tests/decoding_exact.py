@@ -1,5 +1,12 @@
 """Plain forms of what the batched decoding operators do at their edges, from the header's words."""
+import math
+
+import torch
+
 import decoding_ref as D
+import serving8_ref as R8
+
+MIN, MAX = R8.MIN, R8.MAX
 
 
 class SharedPool(D.Pool):
@@ -46,3 +53,29 @@ class SharedPool(D.Pool):
     def reserve(self):
         super().reserve()
         self.counts[0] += sum(max(0, -(-x // self.page) - self.cols) for x in self.lens)
+
+
+def append(codes, scale, table, page, block, first, x):
+    """serving8_ref.append with quotients that are rounded once, and scales as the header reads them.  Quotients of f64 numbers of at most 32 bits are next to a
+    half only where they are one (they differ from it by 2^-34 at least), so f64 division finds every tie."""
+    x = x.double()
+    p, L = first, first + x.shape[0]
+    while p < L:
+        b0 = p // block * block
+        e = min(b0 + block, L)
+        pg, slot, nb = int(table[p // page]), b0 % page, b0 % page // block
+        y = x[p - first:e - first]
+        if 0 <= pg < codes.shape[0]:
+            for h in range(x.shape[1]):
+                was = float(scale[pg, nb, h]) if p > b0 else 0.0
+                was = math.nan if not 0 <= was <= MAX else was
+                now = float((y[:, h].abs().max() / 127).float())
+                now = 0.0 if now < MIN else now
+                now = math.nan if not bool(torch.isfinite(y[:, h]).all()) or now > MAX or was != was else max(now, was)
+                scale[pg, nb, h] = now
+                if now > was and p > b0:
+                    old = codes[pg, slot:slot + p - b0, h]
+                    codes[pg, slot:slot + p - b0, h] = (old.double() * was / now).round().to(torch.int8)
+                at = slice(slot + p - b0, slot + e - b0)
+                codes[pg, at, h] = (y[:, h] / now).round().to(torch.int8) if now > 0 else 0
+        p = e

@@ -1,0 +1,77 @@
+"""Pages in 8 bits on the GPU where append and attention can go wrong: values half way between two codes."""
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import decoding_exact as X  # noqa: E402
+import serving8_ref as R8  # noqa: E402
+import test_gpu_serving8 as T8  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+GPU = "cuda:0"
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "needs the MI355X"
+    from rust_interference_engine_amd import ops
+    return ops
+
+
+def appended_like(ops, b, x, KV):
+    """append to the GPU and to the plain form; both results"""
+    want = []
+    for codes, scale, y in ((b.k_pages, b.k_scale, x[:, :KV]), (b.v_pages, b.v_scale, x[:, KV:])):
+        c, s = b.paged(codes).clone(), scale.clone()
+        for i, (n, L) in enumerate(b.lens):
+            r = int(b.starts[i])
+            X.append(c, s, b.table[i], b.page, b.block, L - n, y[r:r + n])
+        want.append((c, s))
+    return T8.appended(ops, b, x[:, :KV], x[:, KV:]), [want[0][0], want[1][0], want[0][1], want[1][1]]
+
+
+def test_ties_of_codes_go_to_even(ops):
+    """values that lie half way between two codes, of scales whose inverse is no f64 number: 73.5 / 49 is 1.5"""
+    n, hd, KV = 60, 64, 2
+    b = R8.Batch8([(1, 1)] * n, KV, KV, hd, page=16, block=16, dtype=F16, seed=31)
+    x = torch.zeros(n, 2 * KV, hd)
+    for i in range(n):
+        for h in range(2 * KV):
+            s = 2 * (i * 2 * KV + h) + 3  # odd, so a half of it is a value
+            x[i, h, 0] = 127 * s
+            x[i, h, 1:] = (torch.arange(hd - 1) * 2 - 63 + (i % 2) * 62) / 2 * s
+    x[0, 0, 0], x[0, 0, 1] = 6223, 73.5
+    got, want = appended_like(ops, b, x, KV)
+    T8.same(got, want)
+    assert int(got[0][int(b.table[0, 0]), 0, 0, 1]) == 2
+
+
+@pytest.mark.parametrize("block", [16, 64])
+def test_ties_of_earlier_codes_go_to_even(ops, block):
+    """a block whose scale grows from s to s': code * s / s', where that is half way; 47 * 3 / 94 is 1.5"""
+    pairs = [(s, t) for s in range(1, 64) for t in range(s + 1, 200) if any((2 * c * s) % t == 0 and (2 * c * s) // t % 2 for c in range(-127, 128))]
+    pairs = [(3, 94)] + random.Random(3).sample(pairs, 399)
+    n, hd, KV = len(pairs) // 4, 256, 2
+    b = R8.Batch8([(1, 2)] * n, KV, KV, hd, page=64, block=block, dtype=F16, seed=32)
+    x = torch.zeros(n, 2 * KV, hd)
+    for i in range(n):
+        for h in range(2 * KV):
+            s, t = pairs[4 * i + h]
+            pg = int(b.table[i, 0])
+            codes, scale = (b.paged(b.k_pages), b.k_scale) if h < KV else (b.paged(b.v_pages), b.v_scale)
+            codes[pg, 0, h % KV, :255] = torch.arange(-127, 128, dtype=torch.int8)
+            scale[pg, 0, h % KV] = s
+            x[i, h, 5] = -127.0 * t
+    got, want = appended_like(ops, b, x, KV)
+    T8.same(got, want)
+    assert int(got[0][int(b.table[0, 0]), 0, 0, 127 + 47]) == 2
+
+
+def test_append_of_random_rows_to_the_bit(ops):
+    b = R8.Batch8([(1, 20), (40, 90), (3, 3), (17, 33)], 2, 2, 128, page=64, block=32, dtype=F16, seed=33)
+    for ty in (F32, F16, BF16):
+        x = (torch.randn(b.rows, 4, 128, generator=torch.Generator().manual_seed(2)) * 40).round().to(ty)  # whole numbers: many ties
+        T8.same(*appended_like(ops, b, x, 2))
