@@ -302,7 +302,7 @@ int32_t rie_hip_k_paged_attention(const rie_hip_pages *pages, const rie_hip_seqs
  * two, 16 to page_size) of one head, at page*scale_page_stride + (slot/block)*scale_block_stride
  * + head*scale_head_stride of k_scale and of v_scale (f32; strides up to 2^31-1).  Alignments and
  * the limits of the codes' strides are those of bytes.  A scale is 0 (of zeros), NaN, or 2^-60 to
- * 2^50; others count as the nearest of these bounds. */
+ * 2^50; one between 0 and 2^-60 counts as 2^-60, a negative one or one over 2^50 as NaN. */
 typedef struct rie_hip_pages8 {
     rie_hip_pages pages;
     float *k_scale, *v_scale;

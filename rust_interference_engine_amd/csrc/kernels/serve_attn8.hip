@@ -33,8 +33,9 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// A scale as the kernels use it: that of a block of zeros, whose codes are zeros, is any number
-__device__ __forceinline__ float usable(float s) { return s == s ? fminf(fmaxf(s, SCALE8_MIN), SCALE8_MAX) : s; }
+// A scale as the kernels use it: NaN where it is negative or too large, as append takes it.  That of a
+// block of zeros, whose codes are zeros, is any number.
+__device__ __forceinline__ float usable(float s) { return s >= 0 && s <= SCALE8_MAX ? fmaxf(s, SCALE8_MIN) : NAN; }
 
 // 4 codes in f16.  1024 + (code + 128) is f16's 0x6400 with the code, its sign bit turned over, as
 // the low byte; the difference is exact.
@@ -1247,7 +1248,7 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     if (!page_of(a.kv, a.kv.table + (int64_t)si * a.kv.table_stride, b0, page)) return;
     page = same(page);
     float *sp = (is_v ? x.s.v : x.s.k) + (int64_t)page * x.s.page + (int64_t)(slot0 >> bs) * x.s.block + (int64_t)h * x.s.head;
-    const float was = first > b0 ? *sp : 0.0f;
+    float was = first > b0 ? *sp : 0.0f;
     uint8_t *dst = const_cast<uint8_t *>(is_v ? a.kv.v + h * a.kv.v_head : a.kv.k + h * a.kv.k_head) + page * a.kv.page + slot0 * row;
     float most = 0;
     bool fine = true;
@@ -1261,10 +1262,11 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
                 most = fmaxf(most, fabsf(v[i][e]));
             }
     }
+    was = was != 0 ? usable(was) : 0.0f;
     most = xmax_f<64>(most);
     float now = (float)((double)most / 127.0);
     if (now < SCALE8_MIN) now = 0;
-    if (__any(!fine) || now > SCALE8_MAX || !(was >= 0 && was <= SCALE8_MAX)) now = NAN;
+    if (__any(!fine) || now > SCALE8_MAX || was != was) now = NAN;
     else now = fmaxf(now, was);
     if (lane == 0) *sp = now;
     const double inv = now > 0 ? 1.0 / (double)now : 0.0;

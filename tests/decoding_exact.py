@@ -56,7 +56,8 @@ class SharedPool(D.Pool):
 
 
 def append(codes, scale, table, page, block, first, x):
-    """serving8_ref.append with quotients that are rounded once, and scales as the header reads them.  Quotients of f64 numbers of at most 32 bits are next to a
+    """serving8_ref.append with quotients that are rounded once, and scales as the header reads them: from 0 to 2^-60 up
+    to it (0 being of zeros), negative and larger ones NaN.  Quotients of f64 numbers of at most 32 bits are next to a
     half only where they are one (they differ from it by 2^-34 at least), so f64 division finds every tie."""
     x = x.double()
     p, L = first, first + x.shape[0]
@@ -68,7 +69,7 @@ def append(codes, scale, table, page, block, first, x):
         if 0 <= pg < codes.shape[0]:
             for h in range(x.shape[1]):
                 was = float(scale[pg, nb, h]) if p > b0 else 0.0
-                was = math.nan if not 0 <= was <= MAX else was
+                was = math.nan if not 0 <= was <= MAX else max(was, MIN) if was > 0 else 0.0
                 now = float((y[:, h].abs().max() / 127).float())
                 now = 0.0 if now < MIN else now
                 now = math.nan if not bool(torch.isfinite(y[:, h]).all()) or now > MAX or was != was else max(now, was)

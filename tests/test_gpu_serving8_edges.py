@@ -1,4 +1,6 @@
-"""Pages in 8 bits on the GPU where append and attention can go wrong: values half way between two codes."""
+"""Pages in 8 bits on the GPU where append and attention can go wrong: values half way between two codes, scales
+that are none."""
+import math
 import random
 
 import pytest
@@ -74,4 +76,36 @@ def test_append_of_random_rows_to_the_bit(ops):
     b = R8.Batch8([(1, 20), (40, 90), (3, 3), (17, 33)], 2, 2, 128, page=64, block=32, dtype=F16, seed=33)
     for ty in (F32, F16, BF16):
         x = (torch.randn(b.rows, 4, 128, generator=torch.Generator().manual_seed(2)) * 40).round().to(ty)  # whole numbers: many ties
+        T8.same(*appended_like(ops, b, x, 2))
+
+
+@pytest.mark.parametrize("scale", [-1.0, -2.0 ** -70, 2.0 ** 51, math.inf, math.nan])
+def test_scales_that_are_none_are_nan_to_append_and_attention(ops, scale):
+    for lens in ([(1, 60)], [(2, 60)], [(50, 60)], [(40, 60)]):
+        for which in ("k_scale", "v_scale"):
+            b = R8.Batch8(lens, 8, 2, 128, page=32, block=16, dtype=BF16, seed=34)
+            getattr(b, which)[b.table[0, 0].long(), 1, 0] = scale  # positions 16..31 of head 0
+            out = T8.paged(ops, b)
+            sees = torch.arange(lens[0][1] - lens[0][0], lens[0][1]) >= 16
+            assert bool(out[sees][:, :4].isnan().all()) and not bool(out[:, 4:].isnan().any()) and not bool(out[~sees].isnan().any())
+    b = R8.Batch8([(3, 20)], 2, 2, 128, page=32, block=32, dtype=F16, seed=35)
+    b.k_scale[:] = b.v_scale[:] = scale
+    x = torch.randn(3, 4, 128, generator=torch.Generator().manual_seed(3))
+    got, want = appended_like(ops, b, x, 2)
+    T8.same(got, want)
+    assert bool(got[2][int(b.table[0, 0])].isnan().all())
+
+
+@pytest.mark.parametrize("tiny", [2.0 ** -62, 2.0 ** -70, 2.0 ** -100])
+def test_scales_that_are_too_small_count_as_the_smallest(ops, tiny):
+    for lens in ([(1, 40)], [(50, 60)]):
+        b = R8.Batch8(lens, 4, 2, 64, page=64, block=64, dtype=BF16, seed=36)
+        b.v_scale[:] = tiny
+        out = T8.paged(ops, b)
+        b.v_scale[:] = X.MIN
+        assert torch.equal(out, T8.paged(ops, b)) and bool((out != 0).any())
+    for top in (2.0 ** -50, 2.0 ** -52, 2.0 ** -57, 0.0):
+        b = R8.Batch8([(1, 20), (2, 9)], 2, 2, 64, page=32, block=32, dtype=F16, seed=37)
+        b.k_scale[:] = b.v_scale[:] = tiny
+        x = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(4)).clamp(-2, 2) * top
         T8.same(*appended_like(ops, b, x, 2))
