@@ -353,8 +353,7 @@ int32_t rie_hip_k_token_logprobs(int32_t ty, const void *logits, int32_t n, int3
  * of its token (rows outside the sequences are neither read nor written).  Any 32-bit position;
  * angles keep their digits.  n_q heads of q and n_k of k, of src_ty to dst_ty (f32, f16 or bf16,
  * rounded to nearest once); q_out may be q and k_out k, of the same strides and type, and outputs
- * overlap nothing else.  head_dim: 2
- * to 1024; rows of any alignment of their type (16-byte aligned ones, with dims a multiple of 16
+ * that overlap one another or other rows are refused.  head_dim: 2 to 1024; rows of any alignment of their type (16-byte aligned ones, with dims a multiple of 16
  * and head_dim of 8, are read faster).  Strides up to 2^40. */
 typedef struct rie_hip_rotary {
     int32_t n_rows, head_dim, dims, n_q, n_k, interleaved, src_ty, dst_ty;

@@ -117,6 +117,7 @@ int32_t rie_hip_k_rotary(const rie_hip_rotary *x, const rie_hip_seqs *seqs, void
         const int es = bytes_of(a.src_ty), ed = bytes_of(a.dst_ty);
         a.in_place = true;
         a.wide = a.dims % 16 == 0 && a.hd % 8 == 0;
+        std::array<RowsAt, 2> in_at{}, out_at{};  // of q, of k
         const auto rows = [&](int heads, const void *in, int64_t row, int64_t head, void *out, int64_t o_row, int64_t o_head, const char *what) {
             row = used(x->n_rows, row);
             head = used(heads, head);
@@ -128,6 +129,10 @@ int32_t rie_hip_k_rotary(const rie_hip_rotary *x, const rie_hip_seqs *seqs, void
             const bool place = in == out;
             if (place && (row != o_row || head != o_head || a.src_ty != a.dst_ty)) throw bad(std::string(what) + ": rows that are turned in place keep their type and strides");
             a.in_place = a.in_place && place;
+            const int i = what[0] == 'k';
+            in_at[i] = RowsAt{in, x->n_rows, row * es, heads, head * es, (int64_t)a.hd * es};
+            out_at[i] = RowsAt{out, x->n_rows, o_row * ed, heads, o_head * ed, (int64_t)a.hd * ed};
+            if (!place && rows_overlap(in_at[i], out_at[i])) throw bad(std::string(what) + " and " + what + "_out share memory");
             a.wide = a.wide && aligned16(in, row, head, es) && aligned16(out, o_row, o_head, ed);
             return std::array<int64_t, 4>{row * es, head * es, o_row * ed, o_head * ed};
         };
@@ -142,6 +147,11 @@ int32_t rie_hip_k_rotary(const rie_hip_rotary *x, const rie_hip_seqs *seqs, void
             a.k = (const uint8_t *)x->k;
             a.k_out = (uint8_t *)x->k_out;
             a.k_row = s[0], a.k_head = s[1], a.ko_row = s[2], a.ko_head = s[3];
+        }
+        if (a.n_q && a.n_k) {
+            if (rows_overlap(out_at[0], out_at[1])) throw bad("q_out and k_out share memory");
+            if (!a.in_place && rows_overlap(out_at[0], in_at[1])) throw bad("q_out and k share memory");
+            if (!a.in_place && rows_overlap(out_at[1], in_at[0])) throw bad("k_out and q share memory");
         }
         const OnDevice dev((hipStream_t)stream);
         dev.check(a.freqs, "freqs");

@@ -5,6 +5,7 @@
 // the same functions compile for the host, where tests check them.
 #pragma once
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 
@@ -83,6 +84,53 @@ constexpr int FEW_ROWS = 32;
 inline int few_row_blocks(bool paged, int max_new, int G) {
     const int64_t rows = (int64_t)max_new * G;
     return !paged || rows > FEW_ROWS ? 0 : rows <= 16 ? 1 : 2;
+}
+
+// Values in memory: `width` bytes each at p + i row + j head, i < n and j < heads (strides in bytes, not negative)
+struct RowsAt {
+    const void *p;
+    int64_t n, row, heads, head, width;
+};
+// Whether two of them share a byte.  What decides is whether Σ k s, over the strides s and the
+// differences k of the indexes, comes within the widths of the bases' distance: found from the
+// largest stride on, of which only few k leave a distance that the others can make up.  For strides
+// so crooked that this takes many steps the answer is yes.
+inline bool rows_overlap(const RowsAt &a, const RowsAt &b) {
+    typedef __int128 wide;
+    struct Term {
+        int64_t lo, hi, s;
+    } t[4];
+    int n = 0;
+    auto add = [&](int64_t na, int64_t sa, int64_t nb, int64_t sb) {
+        if (sa == sb && sa) {
+            if (na > 1 || nb > 1) t[n++] = Term{1 - na, nb - 1, sa};
+            return;
+        }
+        if (na > 1 && sa) t[n++] = Term{1 - na, 0, sa};
+        if (nb > 1 && sb) t[n++] = Term{0, nb - 1, sb};
+    };
+    add(a.n, a.row, b.n, b.row);
+    add(a.heads, a.head, b.heads, b.head);
+    std::sort(t, t + n, [](const Term &x, const Term &y) { return x.s > y.s; });
+    wide least[5], most[5];  // sums of the terms from i on
+    least[n] = most[n] = 0;
+    for (int i = n - 1; i >= 0; i--) {
+        least[i] = least[i + 1] + (wide)t[i].lo * t[i].s;
+        most[i] = most[i + 1] + (wide)t[i].hi * t[i].s;
+    }
+    int steps = 1 << 14;
+    auto met = [&](auto &&self, int i, wide d) -> bool {  // b - a is d so far
+        if (d + least[i] >= a.width || d + most[i] <= -b.width) return false;
+        if (i == n) return true;
+        // d + k s + (what the others make) has to come between -b.width and a.width
+        auto down = [](wide x, int64_t s) { return x >= 0 ? x / s : -((-x + s - 1) / s); };
+        const wide from = -down(-(1 - b.width - d - most[i + 1]), t[i].s), to = down(a.width - 1 - d - least[i + 1], t[i].s);
+        const int64_t k1 = to < t[i].hi ? (int64_t)to : t[i].hi;
+        for (int64_t k = from > t[i].lo ? (int64_t)from : t[i].lo; k <= k1; k++)
+            if (--steps < 0 || self(self, i + 1, d + (wide)k * t[i].s)) return true;
+        return false;
+    };
+    return met(met, 0, (wide)(intptr_t)b.p - (intptr_t)a.p);
 }
 
 // How a launch divides the positions of a block: every split takes C tiles, S at most.
