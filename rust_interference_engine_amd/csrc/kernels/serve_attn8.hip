@@ -111,7 +111,7 @@ __device__ __forceinline__ int few8_per(int total, int P) { return imax((total +
 // begins: of a piece, whether it has the sequence's first step
 template <int HD>
 __device__ __forceinline__ int64_t few8_part(const Few8Cut &cut, int kvh, int piece, bool begins, int R) {
-    return (((int64_t)kvh * cut.P + piece) * (cut.S ? 1 : 2) + (cut.S ? 0 : begins)) * (R * (HD + 2));
+    return (((int64_t)kvh * cut.P + piece) * (cut.S ? 1 : 2) + (cut.S ? 0 : begins)) * part_floats(R, HD);
 }
 
 // A wave's values in LDS: it copies 1 KB at a time, RPI whole rows, by 16-byte chunk, then row
@@ -1405,7 +1405,7 @@ void launch_append(const PagedAppend8Args &x, int grid, hipStream_t st) {
 size_t serve_attn8_ws(const ServeAttnArgs &a) {
     if (!few8(a)) return tile8_ws(a).bytes;
     const Few8Cut cut = few8_cut(a);
-    return cut.S == 1 ? 0 : (size_t)cut.P * a.n_kv * (cut.S ? 1 : 2) * few8_rows_most(a) * (a.hd + 2) * sizeof(float);
+    return cut.S == 1 ? 0 : (size_t)cut.P * a.n_kv * (cut.S ? 1 : 2) * part_floats(few8_rows_most(a), a.hd) * sizeof(float);
 }
 
 void launch_serve_attn8(ServeAttn8Args x, void *ws, hipStream_t st) {

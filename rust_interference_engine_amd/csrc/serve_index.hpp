@@ -133,6 +133,10 @@ inline bool rows_overlap(const RowsAt &a, const RowsAt &b) {
     return met(met, 0, (wide)(intptr_t)b.p - (intptr_t)a.p);
 }
 
+// Floats of a partial result of R rows of hd values, and each row's maximum and sum behind them all: whole
+// 16-byte vectors, also of odd numbers of rows
+RIE_HD int part_floats(int R, int hd) { return (R * (hd + 2) + 3) & ~3; }
+
 // How a launch divides the positions of a block: every split takes C tiles, S at most.
 struct SplitPlan {
     int C, S;
