@@ -1289,7 +1289,7 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     }
 }
 
-int tile8_waves(const ServeAttnArgs &a) { return a.hd <= 128 && (int64_t)a.b.max_new * a.G > 128 ? 8 : 4; }
+int tile8_waves(const ServeAttnArgs &a) { return tile8_wave_count(a.b.n_rows, a.b.n_seq, a.b.max_new, a.G, a.n_kv, a.hd); }
 int tile8_m(const ServeAttnArgs &a) { return 32 * tile8_waves(a); }
 int tile8_kt(int hd) { return hd <= 128 ? TILE8_KT<128> : TILE8_KT<256>; }
 

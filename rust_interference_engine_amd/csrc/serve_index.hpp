@@ -133,6 +133,12 @@ inline bool rows_overlap(const RowsAt &a, const RowsAt &b) {
     return met(met, 0, (wide)(intptr_t)b.p - (intptr_t)a.p);
 }
 
+// Waves of a workgroup of the tile kernel over 8-bit pages, 32 query rows each: 8 where there are so
+// many rows, but not of so many blocks that a workgroup for each would make 2^32 threads
+inline int tile8_wave_count(int n_rows, int n_seq, int max_new, int G, int n_kv, int hd) {
+    return hd <= 128 && (int64_t)max_new * G > 128 && block_count(n_rows, n_seq, G, 256) * n_kv < 1 << 23 ? 8 : 4;
+}
+
 // Floats of a partial result of R rows of hd values, and each row's maximum and sum behind them all: whole
 // 16-byte vectors, also of odd numbers of rows
 RIE_HD int part_floats(int R, int hd) { return (R * (hd + 2) + 3) & ~3; }

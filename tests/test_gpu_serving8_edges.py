@@ -1,5 +1,5 @@
 """Pages in 8 bits on the GPU where append and attention can go wrong: values half way between two codes, scales
-that are none."""
+that are none, millions of sequences."""
 import math
 import random
 
@@ -109,3 +109,18 @@ def test_scales_that_are_too_small_count_as_the_smallest(ops, tiny):
         b.k_scale[:] = b.v_scale[:] = tiny
         x = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(4)).clamp(-2, 2) * top
         T8.same(*appended_like(ops, b, x, 2))
+
+
+def test_chunks_among_millions_of_sequences(ops):
+    """more blocks of rows than workgroups of 512 threads can be launched for; all but a few sequences are empty"""
+    n_seq, KV, hd, page = (1 << 23) + 5, 1, 64, 128
+    some = {0: (70, 90), 1: (1, 5), 1 << 22: (3, 100), n_seq - 1: (9, 9)}
+    b = R8.Batch8([some[i] for i in some], 2 * KV, KV, hd, page=page, block=64, dtype=F16, seed=51)
+    at = torch.tensor(list(some))
+    new, lens, table = torch.zeros(n_seq, dtype=torch.int32), torch.zeros(n_seq, dtype=torch.int32), torch.full((n_seq, 1), -1, dtype=torch.int32)
+    new[at], lens[at], table[at] = torch.tensor([n for n, _ in some.values()], dtype=torch.int32), b.L, b.table[:, :1]
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)]).int()
+    kv = ops.PagedKv(b.paged(b.k_pages.to(GPU)), b.paged(b.v_pages.to(GPU)), table.to(GPU), k_scale=b.k_scale.to(GPU), v_scale=b.v_scale.to(GPU))
+    out = torch.full((b.rows, 2 * KV, hd), 7.0, dtype=F16, device=GPU)
+    ops.PagedAttention(kv, ops.Seqs(starts.to(GPU), lens.to(GPU), max_new=70, max_len=128), b.q.to(GPU), out)()
+    T8.check(b, out.cpu())
