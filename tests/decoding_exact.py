@@ -80,3 +80,23 @@ def append(codes, scale, table, page, block, first, x):
                 at = slice(slot + p - b0, slot + e - b0)
                 codes[pg, at, h] = (y[:, h] / now).round().to(torch.int8) if now > 0 else 0
         p = e
+
+
+def few_tolerance(o, a, q, k, scale, v_scale, n, dtype, size, softcap=0.0):
+    """|error| of attention over 8-bit pages with at most 32 query rows to a KV head, whose output o (exact) alone is
+    rounded (u |o|); a = Σ w|v|, size: the largest Σ|q k| scale, v_scale: the values' scales.
+
+    Scores are sums of whole numbers, exact but for the queries': half a unit of 2^-21 of their largest value's power of
+    two, so at most 2^-22 of that value.  Of an exponent in log2 units, at most E = size log2 e + |log2 of a scale| + 14,
+    8 roundings of 2^-24 (three factors, two parts of the sum, the sum with log2 of the scale, that logarithm, the
+    difference from the maximum); a softcap's tanh 2^-22 of the cap; the exponential 2^-23.  All of these enter a
+    probability, above and below.  p · s_v is two f16 numbers, in error by 2^-22, or, below f16's normal numbers, by 2^-25
+    where the largest of the wave is 2^6 or more: of n positions n 2^-31 of the largest scale times 127.  Sums of n f32
+    terms, matrix sums being cut off."""
+    u = torch.finfo(dtype).eps / 2
+    k1 = float(k.abs().sum(-1).max()) if k.numel() else 0.0
+    q1 = float(q.double().abs().max()) if q.numel() else 0.0
+    s = v_scale.double().clamp(MIN)
+    E = size / math.log(2) + float(s.log2().abs().max()) + 14
+    p = 2.0 ** -22 * q1 * k1 * scale + math.log(2) * 8 * 2.0 ** -24 * E + softcap * 2.0 ** -21 + 2.0 ** -23
+    return u * o.abs() + (2.0 ** -22 + 2 * p + 2 * (n + 16) * 2.0 ** -23) * a + n * 2.0 ** -31 * 127 * float(s.max()) + 1e-30

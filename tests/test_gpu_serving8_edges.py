@@ -1,5 +1,5 @@
 """Pages in 8 bits on the GPU where append and attention can go wrong: values half way between two codes, scales
-that are none, millions of sequences."""
+that are none, millions of sequences; what is rounded and what is not."""
 import math
 import random
 
@@ -9,6 +9,7 @@ torch = pytest.importorskip("torch")
 
 import decoding_exact as X  # noqa: E402
 import serving8_ref as R8  # noqa: E402
+import serving_ref as S  # noqa: E402
 import test_gpu_serving8 as T8  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -124,3 +125,51 @@ def test_chunks_among_millions_of_sequences(ops):
     out = torch.full((b.rows, 2 * KV, hd), 7.0, dtype=F16, device=GPU)
     ops.PagedAttention(kv, ops.Seqs(starts.to(GPU), lens.to(GPU), max_new=70, max_len=128), b.q.to(GPU), out)()
     T8.check(b, out.cpu())
+
+
+# ---- what is rounded: of few rows the output alone ----
+
+def check_few(b, out, window=0, softcap=0.0, scale=None):
+    scale = 1 / math.sqrt(b.hd) if scale is None else scale
+    for i, (n, L) in enumerate(b.lens):
+        r = int(b.starts[i])
+        q = b.q[r:r + n]
+        k, v = b.values(b.k_pages, b.k_scale, i), b.values(b.v_pages, b.v_scale, i)
+        o, a, size = S.attend(q, k, v, L - n, scale, window, softcap)
+        if n:
+            tol = X.few_tolerance(o, a, q, k, scale, b.v_scale, L, b.dtype, size, softcap)
+            err = (out[r:r + n].double() - o).abs()
+            assert bool((err <= tol).all()), (i, n, L, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("H,KV,hd,page,block", T8.SHAPES + [(14, 2, 64, 16, 16), (3, 1, 256, 64, 16), (32, 1, 128, 16, 16)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (40, 0.0), (0, 5.0)])
+def test_few_rows_round_their_output_only(ops, H, KV, hd, page, block, window, softcap):
+    lens = [(1, 1), (1, 17), (1, 33), (1, 500), (0, 64), (1, 129)]
+    b = R8.Batch8(lens, H, KV, hd, page=page, block=block, seed=41)
+    check_few(b, T8.paged(ops, b, window, softcap), window, softcap)
+
+
+@pytest.mark.parametrize("lens", [[(3, 300), (2, 9), (4, 40)], [(1, 5000)], [(4, 4097)], [(1, 3000), (2, 800), (1, 1700), (4, 20)], [(1, 900 + 7 * i) for i in range(66)]])
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 128), (12, 4, 64), (6, 3, 96), (4, 1, 256)])
+def test_few_rows_in_splits_and_pieces_round_their_output_only(ops, lens, H, KV, hd):
+    b = R8.Batch8(lens, H, KV, hd, page=64, block=32, seed=42)
+    check_few(b, T8.paged(ops, b))
+
+
+def cancelling(new, seed):
+    """two positions of nearly one weight whose values cancel: what is left is the probabilities' rounding"""
+    b = R8.Batch8([(new, 64 + i) for i in range(8)], 16, 4, 128, page=64, block=64, seed=seed)
+    b.q *= 0.05
+    b.v_scale[:] = 1.0
+    for i, (n, L) in enumerate(b.lens):
+        t = b.table[i, 0].long()
+        v = b.paged(b.v_pages)
+        v[t, 1:64:2] = -v[t, 0:64:2]
+    return b
+
+
+@pytest.mark.parametrize("new", [1, 5])
+def test_values_that_cancel(ops, new):
+    b = cancelling(new, 43)
+    check_few(b, T8.paged(ops, b))
