@@ -11,7 +11,8 @@
 // so only those are read again.  The workgroup of a request that is done last merges its rows.
 //
 // Beams are compared by sums in f64: in f32 the candidates of two beams would be equal to the last
-// bit too often, and their order that of the roundings.  ln Σ is f64 of an f32 sum (2^-22 of it).
+// bit too often, and their order that of the roundings.  ln Σ is f64 of an f32 sum
+// (off by under 2^-22 of it in all rows measured; of 192 of 128256 logits by 3 · 2^-24).
 //
 // Bound: HBM, rows · V values, for the first launch, latency for the second.  192 rows of 128256
 // bf16 logits, 16 wanted: 12.1 us (4.1 TB/s) + 14.7 us, of which 2.5 us wait for the groups'

@@ -64,10 +64,12 @@ constexpr float P_SHIFT8 = 6.0f;  // p · s_v is 2^(exponent − m + P_SHIFT8): 
 // instructions as they are; values are read transposed, 8 positions of a dim to a lane, and made
 // f16 there, 10 vector instructions for 8 values.
 //
-// Bound: HBM while all workgroups stream (6.4 TB/s by timestamps), and their beginning: starts,
-// page ids, scales and the first tile lie behind one another.  48 tokens over up to 4000
-// positions, 32/8 heads of 128 (149 MB) 34 us (4.4 TB/s) and 6 for the join, 1 over 100003
-// positions, 32/4 of 128 (103 MB) 21.8 (4.7 TB/s) and 5.2.
+// Bound: HBM while all workgroups stream, and their beginning: starts, page ids, scales and the
+// first tile lie behind one another.  48 tokens over up to 4000 positions, 32/8 heads of 128
+// (149 MB) 34 us (4.4 TB/s, where a copy reaches 5.2) and 6 for the join, 1 over 100003 positions,
+// 32/4 of 128 (103 MB) 21.5 (4.8 TB/s) and 5.  With two blocks of 16 rows (5 tokens of 16 sequences
+// over 4000 positions, 32/8 of 128) 47 for the call, where 1 token takes 31: twice the products, at
+// half as many waves.
 constexpr int FEW8_KT = 32, FEW8_STEP = 4 * FEW8_KT;          // positions of a wave's tile and of a step
 constexpr int FEW8_LEAST = 2, FEW8_BEGIN = 1, FEW8_SEQS = 64;  // steps that a piece is worth, those that a sequence's beginning takes; sequences that are cut in pieces
 // of a SIMD: with splits as many as registers allow, with pieces two, which have all that they need
@@ -87,7 +89,11 @@ constexpr int few8_waves(int hd, int nb, bool pieces) {
 // faster in splits (100003 positions 27.8, in pieces 29.7), which take nothing to find, and so are
 // sequences that pieces hold several of, whose beginnings then lie behind one another (500 of up
 // to 1500, 32/4 heads of 128, 168 us; whole 87).  Pieces for one workgroup to a CU: 53 for 43; for
-// four, which spill registers, 52.
+// four, which spill registers, 52.  The limit of 64 is that of a wave's lanes.  At it, pieces, splits
+// of twelve steps and of two: 64 of up to 4000, 32/8 of 128, 57.6, 68.4 and 60.5 us, 64 of up to 1500
+// 33.0, 28.3 and 33.4.  Behind it, splits of twelve and of two: 65 of up to 4000 64.0 and 50.8, 100 of
+// them 98.6 and 94.9, 100 of up to 1500 37.4 and 44.5, 300 of them 103.6 and 119, 200 of up to 3000,
+// 15/5 of 64, 48.0 and 46.9.
 struct Few8Cut {
     int P, S, C;
 };
@@ -131,6 +137,7 @@ __global__ __launch_bounds__(256, few8_waves(HD, NB, PIECES)) void attn8_few_ker
     using Lds = Value8Lds<HD>;
     const ServeAttnArgs &a = x.a;
     constexpr int KT = FEW8_KT, RPI = Lds::RPI, NLD = KT / RPI, DB = HD / 16;
+    // a sum (of 96 dims) formed by products of 64 and of 32 dims in turn had other bits from call to call
     constexpr int K64 = HD % 64 ? 0 : HD / 64, K32 = HD % 64 ? HD / 32 : 0, KS = K64 + K32;  // products of 64 or of 32 dims
     constexpr int VB = NLD * Lds::BLOCK, OB = 16 * NB * HD * 4;  // a wave's values, and its outputs at the end
     constexpr int WB = VB > OB ? VB : OB;
@@ -541,9 +548,11 @@ __global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, Few8Cut
 // to registers a tile ahead, each wave's 16 (8) rows, and are made f16 on their way to LDS (5
 // vector instructions for 4 values), in the place of a tile that has been read by then.
 //
-// Bound: a SIMD's matrix and vector instructions, which hardly overlap: of a wave's tile of 64
-// positions, head size 128, 1024 cycles are matrix products and about 1100 vector work (exponentials
-// alone 512, codes 160).  Eight waves to a tile (256 rows) where there are so many, since then
+// Bound: a SIMD's matrix and vector instructions, which hardly overlap, and a fifth of the time neither:
+// of a wave's tile of 64 positions, head size 128, 1024 cycles are matrix products, and 316 vector
+// instructions take about 1400 (exponentials alone 512, codes 160).  Counters, 13 sequences as below:
+// the matrix units are busy for 32 % of the SIMDs' cycles, vector instructions issue in 48 %; both waves
+// of a SIMD come to the same phase behind each barrier.  Eight waves to a tile (256 rows) where there are so many, since then
 // each makes half as many codes: 13 sequences as below, both under a profiler, 215 us with four
 // and 200 with eight.
 template <int HD>
@@ -958,8 +967,8 @@ __device__ __forceinline__ void tile8_piece(const ServeAttn8Args &xa, uint8_t *s
 // cuts fall.  A workgroup goes through the blocks of its piece; one that it has all of goes to the
 // outputs, and at most two (its first, its last) to partial results, which tile8_join_kernel adds
 // up.  With a workgroup for each block, the longest sequence's ran on while the others' were done:
-// chunks of 13 sequences up to 8200 258 us; in pieces 185, of which 175 the tiles (at the 2.1 GHz
-// that the card keeps with all matrix units busy), 5 the plan and 8 the join.
+// chunks of 13 sequences up to 8200 258 us; in pieces 183 (kernels alone, under a profiler: 183 the
+// tiles, at a lower clock, 6.5 the plan and 11.4 the join).
 struct Tile8Plan {
     int64_t total;  // what the tiles of all blocks take
     int n, pad;     // blocks
@@ -1161,8 +1170,8 @@ __global__ __launch_bounds__(256) void tile8_join_kernel(ServeAttnArgs a, int KT
 //
 // Bound: loads behind one another (the sequence, the rows, the page and scale meanwhile), and for
 // long prompts the second reading of blocks over 16 positions, from L2.  61 tokens for 4 heads of
-// 128 4.0 us; 2854 rows for 8 heads, f32, blocks of 32 (29 MB) 10.9 us.  32 rows kept in registers
-// 4.8 and 10.0: steps of single tokens are what a server makes most of.
+// 128 4.4 us; 2854 rows for 8 heads, f32, blocks of 32 (29 MB) 11.0 us.  32 rows kept in registers
+// 0.8 more and 0.9 less: steps of single tokens are what a server makes most of.
 template <int SRC>  // ggml type
 __device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
     if constexpr (SRC == T_F32) {

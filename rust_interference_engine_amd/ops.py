@@ -299,8 +299,8 @@ def rotary_frequencies(dims: int, base: float = 10000.0, *, factors=None, linear
     """The angles per position of ``dims`` / 2 pairs, base^(-2i / dims), as f64 on the host, and the factor of the
     rotated values.  For contexts beyond those trained on: ``factors`` divides each pair's angle by its own number (as
     ``rope_freqs.weight`` does), ``linear`` all of them by one; ``parts`` = (factor, original context) divides the
-    slow ones by factor and leaves the fast ones, with a ramp between those that turn once and 32 times within the
-    original context, and multiplies the rotated values by 0.1 ln(factor) + 1 (YaRN, arXiv 2309.00071)."""
+    slow ones by factor and leaves the fast ones, with a ramp, linear in the pair's number, between those that turn
+    once and 32 times within the original context, and multiplies the rotated values by 0.1 ln(factor) + 1 (YaRN, arXiv 2309.00071)."""
     _need(dims >= 2 and dims % 2 == 0, f"dims has to be even and positive, got {dims}")
     _need(base > 0 and linear > 0, "base and linear have to be positive")
     f = base ** (-2 * torch.arange(dims // 2, dtype=torch.float64) / dims) / linear
@@ -451,7 +451,8 @@ class PageReserve(_Op):
 class PageFork(_Op):
     """Row i of the pool becomes what row ``src[i]`` (int32 [sequences], on the GPU) was, all at
     once: full pages are shared, a partial last one is copied for all but one of the rows that
-    take it, in the pages of all ``caches`` [pages, ...].  A row whose src is none becomes empty."""
+    take it, and for that one too where a row beside them holds it, in the pages of all ``caches``
+    [pages, ...].  A row whose src is none becomes empty."""
 
     def __init__(self, pool: PagePool, src: torch.Tensor, caches=()):
         _ints(src, "src", 1)
