@@ -1170,7 +1170,7 @@ __global__ __launch_bounds__(256) void tile8_join_kernel(ServeAttnArgs a, int KT
 //
 // Bound: loads behind one another (the sequence, the rows, the page and scale meanwhile), and for
 // long prompts the second reading of blocks over 16 positions, from L2.  61 tokens for 4 heads of
-// 128 4.4 us; 2854 rows for 8 heads, f32, blocks of 32 (29 MB) 11.0 us.  32 rows kept in registers
+// 128 4.3 us; 2854 rows for 8 heads, f32, blocks of 32 (29 MB) 11.0 us.  32 rows kept in registers
 // 0.8 more and 0.9 less: steps of single tokens are what a server makes most of.
 template <int SRC>  // ggml type
 __device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
@@ -1188,15 +1188,16 @@ __device__ __forceinline__ void load8(const uint8_t *p, float (&v)[8]) {
     }
 }
 
-// 8 codes x / s, to the nearest whole number, ties to even; inv: 1 / s in f64.  In f32 a quotient is
-// off by under 2^-15 (three roundings of numbers up to 128), so what is 2^-14 or more away from half
-// way between two numbers goes the right way.  The others are formed in f64 (prompts 12.2 us with all
-// of them so): x and s have at most 32 bits, so a quotient that is not half way itself is 2^-34 of
-// its size away, and x · inv, good to 2^-52, goes the right way.  One that is may go either way; what
-// is left then is s / 2 exactly, in the fma as in truth.
+// 8 codes x / s, to the nearest whole number, ties to even.  In f32, by the hardware's inverse, a quotient
+// is off by under 2^-15 (of numbers up to 127.5: two roundings and one unit of the inverse, 2^-22 in
+// all), so what is 2^-14 or more away from half way between two numbers goes the right way.  The
+// others are formed in f64 (prompts 12.2 us with all of them so): x and s have at most 32 bits, so a
+// quotient that is not half way itself is 2^-34 of its size away, and x · (1 / s), good to 2^-52, goes
+// the right way.  One that is may go either way; what is left then is s / 2 exactly, in the fma as
+// in truth.
 template <class F>
-__device__ __forceinline__ u32x2 codes8(F x, double inv, float s) {
-    const float inv_f = (float)inv;
+__device__ __forceinline__ u32x2 codes8(F x, float s) {
+    const float inv_f = __builtin_amdgcn_rcpf(s);
     int c[8];
     bool near = false;
 #pragma unroll
@@ -1206,6 +1207,7 @@ __device__ __forceinline__ u32x2 codes8(F x, double inv, float s) {
         c[e] = (int)q;
     }
     if (near) {
+        const double inv = 1.0 / (double)s;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const double y = x(e), q = rint(y * inv), left = fma(-q, (double)s, y);
@@ -1278,13 +1280,12 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
     if (__any(!fine) || now > SCALE8_MAX || was != was) now = NAN;
     else now = fmaxf(now, was);
     if (lane == 0) *sp = now;
-    const double inv = now > 0 ? 1.0 / (double)now : 0.0;
     if (first > b0 && now > was) {  // codes of earlier positions
         for (int q = r; q < first - b0; q += RP) {
             if (!on) break;
             u32x2 *p = (u32x2 *)(dst + q * row + ch * 8);
             const u32x2 y = *p;
-            *p = codes8([&](int e) { return (double)(int8_t)(y[e / 4] >> e % 4 * 8) * (double)was; }, inv, now);
+            *p = codes8([&](int e) { return (double)(int8_t)(y[e / 4] >> e % 4 * 8) * (double)was; }, now);
         }
     }
     for (int r0 = 0; r0 < n; r0 += ROWS) {
@@ -1293,7 +1294,7 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8Args x) 
         for (int i = 0; i < NP; i++) {
             const int q = r0 + i * RP + r;
             if (!(on && i * RP + r < ROWS && q < n)) continue;
-            *(u32x2 *)(dst + (first - b0 + q) * row + ch * 8) = inv > 0 ? codes8([&](int e) { return v[i][e]; }, inv, now) : u32x2{0, 0};
+            *(u32x2 *)(dst + (first - b0 + q) * row + ch * 8) = now > 0 ? codes8([&](int e) { return v[i][e]; }, now) : u32x2{0, 0};
         }
     }
 }
