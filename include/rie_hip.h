@@ -353,8 +353,9 @@ int32_t rie_hip_k_token_logprobs(int32_t ty, const void *logits, int32_t n, int3
  * of its token (rows outside the sequences are neither read nor written).  Any 32-bit position;
  * angles keep their digits.  n_q heads of q and n_k of k, of src_ty to dst_ty (f32, f16 or bf16,
  * rounded to nearest once); q_out may be q and k_out k, of the same strides and type, and outputs
- * that overlap one another or other rows are refused.  head_dim: 2 to 1024; rows of any alignment of their type (16-byte aligned ones, with dims a multiple of 16
- * and head_dim of 8, are read faster).  Strides up to 2^40. */
+ * that otherwise share memory with one another or with q or k are refused.  head_dim: 2 to 1024;
+ * rows of any alignment of their type (16-byte aligned ones, with dims a multiple of 16 and head_dim
+ * of 8, are read faster).  Strides up to 2^40. */
 typedef struct rie_hip_rotary {
     int32_t n_rows, head_dim, dims, n_q, n_k, interleaved, src_ty, dst_ty;
     float magnitude;
@@ -419,14 +420,14 @@ int32_t rie_hip_k_page_reserve(const rie_hip_pool *pool, void *ws, size_t ws_byt
  * call).  Where refs says that the partial page has more than one holder before the call (a row was
  * cut back into pages that it shared), nobody keeps it and all get new ones, and of the pages
  * behind, those before the first such one stay: after a fork no row holds a page from its last
- * position's on that another row holds too.
- * Pages that no row holds any more become free. */
+ * position's on that another row holds too.  Pages that no row holds any more become free. */
 int32_t rie_hip_k_page_fork(const rie_hip_pool *pool, const int32_t *src, const rie_hip_page_buf *bufs, int32_t n_bufs, void *ws,
                             size_t ws_bytes, void *stream, char *err, size_t err_len);
 /* Rows with which[i] != 0 give up their pages and positions. */
 int32_t rie_hip_k_page_free(const rie_hip_pool *pool, const int32_t *which, void *stream, char *err, size_t err_len);
 /* With n pages in use: those numbered n and up move, in order, to the free ones below n, in the
- * tables, in refs and in the n_bufs caches, so that pages from n on are free. */
+ * tables, in refs and in the n_bufs caches, so that pages from n on are free.  (A program that
+ * counts pages in refs which no row holds finds them by the same rule, from refs before the call.) */
 int32_t rie_hip_k_page_compact(const rie_hip_pool *pool, const rie_hip_page_buf *bufs, int32_t n_bufs, void *ws, size_t ws_bytes,
                                void *stream, char *err, size_t err_len);
 /* Page src[i] of every cache to page dst[i], i < n; pairs with a number outside 0..n_pages-1 are

@@ -552,9 +552,9 @@ __global__ __launch_bounds__(256) void few8_join_kernel(ServeAttnArgs a, Few8Cut
 // of a wave's tile of 64 positions, head size 128, 1024 cycles are matrix products, and 316 vector
 // instructions take about 1400 (exponentials alone 512, codes 160).  Counters, 13 sequences as below:
 // the matrix units are busy for 32 % of the SIMDs' cycles, vector instructions issue in 48 %; both waves
-// of a SIMD come to the same phase behind each barrier.  Eight waves to a tile (256 rows) where there are so many, since then
-// each makes half as many codes: 13 sequences as below, both under a profiler, 215 us with four
-// and 200 with eight.
+// of a SIMD come to the same phase behind each barrier.  Eight waves to a tile (256 rows) where there
+// are so many, since then each makes half as many codes: 13 sequences as below, both under a profiler,
+// 215 us with four and 200 with eight.
 template <int HD>
 constexpr int TILE8_KT = HD <= 128 ? 64 : 32;
 
